@@ -1,0 +1,61 @@
+// What the operator kernels share: element types, wave reductions, launch and error helpers.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../../include/operators/atlas_ops.h"
+
+namespace atlas_ops {
+
+typedef int64_t i64;
+typedef uint64_t u64;
+typedef uint16_t bf16_t;
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+inline int fail(char* err, size_t cap, int code, const char* fmt, ...) {
+    if (err && cap) {
+        va_list args;
+        va_start(args, fmt);
+        vsnprintf(err, cap, fmt, args);
+        va_end(args);
+    }
+    return code;
+}
+
+// The status of the launches just made (no wait).
+inline int launched(char* err, size_t cap, const char* what) {
+    const hipError_t status = hipGetLastError();
+    return status == hipSuccess ? 0 : fail(err, cap, 4, "%s: %s", what, hipGetErrorString(status));
+}
+
+inline bool known_type(int type) { return type == ATLAS_OPS_F32 || type == ATLAS_OPS_BF16; }
+
+inline i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16_t v) { return __uint_as_float((uint32_t)v << 16); }
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+// Round to nearest even; a NaN keeps a payload bit (adding the rounding term could carry it away).
+template <>
+__device__ __forceinline__ bf16_t from_float<bf16_t>(float v) {
+    const uint32_t bits = __float_as_uint(v);
+    if ((bits & 0x7FFFFFFFu) > 0x7F800000u) return (bf16_t)((bits >> 16) | 0x40u);
+    return (bf16_t)((bits + 0x7FFFu + ((bits >> 16) & 1u)) >> 16);
+}
+
+// Sum over groups of LANES neighbouring lanes (a power of two up to 64); every lane gets it.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+}  // namespace atlas_ops

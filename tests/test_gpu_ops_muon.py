@@ -1,0 +1,162 @@
+"""The orthogonalised update on the GPU against the float64 reference (oracle/ops_oracle.py), which takes
+it through the singular values.
+
+Tolerances.  Rounding the iterates to 22 bits (and float32 sums) perturbs X by about 2^-23 |X|_F spread
+over all directions at each of the steps; a perturbation of a weak direction grows by up to 3.4 a step,
+485 over five, relative to its own start at |X|_F / sqrt(m).  The sum of the steps' perturbations grown to
+the end, 2^-23 (1 + 3.4 + ... + 3.4^5) = 8.2e-5 of |X_0|_F = 1, is a bound on the error's Frobenius norm where
+every direction is weak throughout; results have Frobenius norm sqrt(m), so 1e-4 sqrt(rank) bounds the
+error of low-rank matrices too.  Matrices of full rank whose singular values reach one are held to 2e-5
+of the result's norm.  bfloat16 results: half an ulp, 2^-9, on top.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from atlas_hip import ops
+from oracle import ops_oracle as oo
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def numpy(t):
+    return t.double().cpu().numpy()
+
+
+def make(shape, dtype=F32, seed=0, scale=1.0):
+    return (scale * torch.randn(shape, generator=torch.Generator().manual_seed(seed))).to(dtype).cuda()
+
+
+def error(got, want):
+    return float(np.linalg.norm(numpy(got) - want) / np.linalg.norm(want))
+
+
+SHAPES = [(1, 1), (1, 50), (50, 1), (16, 16), (20, 256), (256, 20), (63, 65), (64, 64), (65, 130), (129, 127), (256, 256),
+          (700, 256), (333, 1000), (3, 40, 70), (5, 70, 40), (2, 1, 1), (130, 128, 9)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_orthogonalize_matches_the_reference(shape, dtype):
+    print(f"case: orthogonalize {shape} {dtype}", flush=True)
+    m = make(shape, dtype, seed=sum(shape), scale=3e-3)
+    got = ops.orthogonalize(m)
+    assert got.dtype == dtype and got.shape == m.shape
+    assert error(got, oo.orthogonalize(numpy(m))) <= 2e-5 + (2 ** -8 if dtype == BF16 else 0)
+    assert torch.equal(got, ops.orthogonalize(m))
+
+
+def test_large_tiles():
+    """A smaller side of 1920 and more takes the tiles of 128; ragged, both orientations."""
+    print("case: orthogonalize 128-tiles", flush=True)
+    for shape in ((1990, 2050), (2050, 1990)):
+        m = make(shape, seed=4)
+        got = ops.orthogonalize(m)
+        x = m.double()
+        a, b, c = ops.COEFFICIENTS
+        x = x / (x.norm() + 1e-7)
+        for _ in range(5):
+            g = x @ x.mT.contiguous()
+            x = a * x + (b * g + c * (g @ g)) @ x
+        assert float((got.double() - x).norm() / x.norm()) <= 2e-5
+
+
+@pytest.mark.parametrize("rank", [1, 4])
+def test_low_rank(rank):
+    print(f"case: orthogonalize rank {rank}", flush=True)
+    m = make((200, rank), seed=1) @ make((rank, 300), seed=2)
+    got, want = ops.orthogonalize(m), oo.orthogonalize(numpy(m))
+    # the float32 input has a rounding noise of its own, which the iteration raises: part of the input
+    assert np.linalg.norm(numpy(got) - want) <= 1e-4 * math.sqrt(rank) * 10
+
+
+def test_a_wide_range_of_magnitudes():
+    """Norms that overflow or vanish in a float32 sum of squares, and singular values over six decades."""
+    print("case: orthogonalize magnitudes", flush=True)
+    m = make((48, 80))
+    want = oo.orthogonalize(numpy(m), eps=0.0)
+    for scale in (1e30, 1e-30, 2.0 ** 120):
+        got = ops.orthogonalize(m * scale, eps=0.0)
+        assert error(got, oo.orthogonalize(numpy(m * scale), eps=0.0)) <= 2e-5
+        assert error(got, want) <= 1e-4
+    decades = m * torch.logspace(0, -6, 48, device="cuda")[:, None]
+    want = oo.orthogonalize(numpy(decades))
+    # against the largest term, as weak directions stay weak
+    assert np.abs(numpy(ops.orthogonalize(decades)) - want).max() <= 2e-4
+
+
+def test_steps_coefficients_and_special_values():
+    print("case: orthogonalize options", flush=True)
+    m = make((60, 90), seed=3)
+    for steps, coefficients in ((1, ops.COEFFICIENTS), (3, (2.0, -1.5, 0.5)), (12, (1.875, -1.25, 0.375))):
+        got = ops.orthogonalize(m, steps=steps, coefficients=coefficients)
+        assert error(got, oo.orthogonalize(numpy(m), steps=steps, coefficients=coefficients)) <= 2e-5
+    assert (ops.orthogonalize(torch.zeros(30, 40, device="cuda")) == 0).all()
+    bad = make((2, 30, 40))
+    bad[1, 3, 4] = float("nan")
+    got = ops.orthogonalize(bad)
+    assert torch.isfinite(got[0]).all() and torch.isnan(got[1]).all()
+    assert ops.orthogonalize(torch.empty(0, 4, device="cuda")).shape == (0, 4)
+    assert ops.orthogonalize(torch.empty(3, 0, 4, device="cuda")).shape == (3, 0, 4)
+
+
+def test_strides():
+    print("case: orthogonalize strides", flush=True)
+    base = make((4, 60, 90))
+    for view in (base[::2], base[:, 3:50:2, 5:77], base.transpose(0, 1), base.transpose(1, 2), base[1].T,
+                 base[0:1].expand(3, 60, 90)):
+        assert torch.equal(ops.orthogonalize(view), ops.orthogonalize(view.contiguous()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", [(256, 256), (700, 256), (256, 20), (3, 33, 47)])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_update_matches_the_reference(shape, dtype, nesterov):
+    print(f"case: muon {shape} {dtype} {nesterov}", flush=True)
+    weight, gradient, momentum = make(shape, seed=1), make(shape, dtype, seed=2), make(shape, seed=3)
+    options = dict(learning_rate=0.05, factor=0.9, weight_decay=0.1, nesterov=nesterov)
+    w, m = numpy(weight), numpy(momentum)
+    for _ in range(3):
+        w, m = oo.muon(w, numpy(gradient), m, **options)
+        assert ops.muon_update(weight, gradient, momentum, **options) is None
+    assert error(momentum, m) <= 2e-7          # three roundings of a sum of two terms
+    assert error(weight, w) <= 1e-5            # three updates of at most 2e-5 each times the rate, and float32
+    w, m = oo.muon(w, numpy(gradient), m, **options, scale=0.2)
+    ops.muon_update(weight, gradient, momentum, **options, scale=0.2)
+    assert error(weight, w) <= 1e-5
+
+
+def test_update_bumps_versions_and_refuses():
+    print("case: muon refusals", flush=True)
+    w, g, m = make((30, 40)), make((30, 40), seed=1), make((30, 40), seed=2)
+    before = w._version, m._version, g._version
+    ops.muon_update(w, g, m, learning_rate=0.1)
+    assert (w._version, m._version, g._version) == (before[0] + 1, before[1] + 1, before[2])
+    for call in (lambda: ops.muon_update(w.T, g.T, m.T, learning_rate=0.1),
+                 lambda: ops.muon_update(w, g[:29], m, learning_rate=0.1),
+                 lambda: ops.muon_update(w, g, m.bfloat16(), learning_rate=0.1),
+                 lambda: ops.muon_update(w.bfloat16(), g, m, learning_rate=0.1),
+                 lambda: ops.muon_update(w, g.half(), m, learning_rate=0.1),
+                 lambda: ops.muon_update(w, g, w, learning_rate=0.1), lambda: ops.muon_update(w, m, m, learning_rate=0.1),
+                 lambda: ops.muon_update(w[0], g[0], m[0], learning_rate=0.1),
+                 lambda: ops.muon_update(w, g, m, learning_rate=0.1, steps=0),
+                 lambda: ops.orthogonalize(w, steps=65), lambda: ops.orthogonalize(w, coefficients=(1.0, 2.0)),
+                 lambda: ops.orthogonalize(w.half()), lambda: ops.orthogonalize(w.clone().requires_grad_())):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_another_stream():
+    print("case: muon stream", flush=True)
+    m = make((300, 400))
+    want = ops.orthogonalize(m)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = ops.orthogonalize(m)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got, want)
