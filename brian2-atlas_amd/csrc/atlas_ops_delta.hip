@@ -9,8 +9,8 @@
 //   S' = g_C S + K^T (rest B E)    rest_i = exp(G_C - G_i)
 // so that a chunk costs matrix products and one triangular inverse T = (I + M B)^-1, which no
 // state enters: `prepare` inverts for all chunks at once, `scan_forward` carries the states through the
-// chunks, and `outputs` takes every chunk's outputs at once.  The columns of S do not touch each other,
-// so a wave of the scan owns 16 of them.
+// chunks, and `outputs` takes every chunk's outputs at once.  The columns of S do not touch each other:
+// each workgroup of the scan has 16 of them.
 //
 // Backwards, with P = scale (lower part of D o Q K^T):
 //   dV' = P^T dO + rest K dS',  Y = T^T B dV',  dV = Y,  dS = g_C dS' + scale Q^T g dO - K^T g Y
@@ -196,348 +196,591 @@ __global__ void __launch_bounds__(256) step_kernel(Delta d, T* __restrict__ out,
 }
 
 // ------------------------------------------------------------------ what the chunk kernels share
-// Float32 MFMA blocks of 16 x 16 with 4 sum indices: lane l gives A[l % 16][l / 16] and B[l / 16][l % 16]
-// and receives rows 4 (l / 16) + j, column l % 16.  The sum may take its indices in any order that A and B
-// share, so a block of results is the B operand of a following product as it is: register j holds
-// the indices 4 (l / 16) + j of 16, and A gives the same ones (one 16-byte read of a row).
-__device__ __forceinline__ float4_t mfma(float a, float b, float4_t c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-// c += A B over 16 sum indices, `a` and `b` in the order above.
-__device__ __forceinline__ float4_t mfma16(float4_t a, float4_t b, float4_t c) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = mfma(a[j], b[j], c);
-    return c;
-}
+// Products run on bfloat16 MFMA blocks of 16 x 16 with 32 sum indices, at float32's accuracy: a float
+// is the sum of three bfloat16 pieces (to 2^-24), a product takes the pieces' products down to that
+// size, three where one side is bfloat16 already and six where neither is, summed in float32.  Float32
+// MFMA would take 16 times the cycles of one such product.
+//
+// Lane l gives 8 values of row l % 16 of A, 8 of column l % 16 of B, and receives rows 4 (l / 16) + j of
+// column l % 16.  The sum may take its indices in any order that A and B share: here lane group g = l / 16
+// holds the indices 4 g + j and 16 + 4 g + j of 32, so that two blocks of results on top of each other are, without
+// any exchange, the B operand of a product that sums over their rows, and the A operand of one whose rows
+// are their columns.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
 constexpr float4_t ZERO = {0.0f, 0.0f, 0.0f, 0.0f};
 
-struct Lane {
-    int col, quad;  // l % 16, 4 (l / 16)
-    __device__ __forceinline__ Lane() : col(threadIdx.x % 16), quad(threadIdx.x % 64 / 16 * 4) {}
-    // operand from rows: row `col` of the block at `m`, columns quad ..
-    __device__ __forceinline__ float4_t row(const float* m, int pitch) const {
-        return *(const float4_t*)(m + col * pitch + quad);
-    }
-    // operand from columns: column `col` of the block at `m`, rows quad ..
-    __device__ __forceinline__ float4_t column(const float* m, int pitch) const {
-        float4_t v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = m[(quad + j) * pitch + col];
-        return v;
-    }
+// N pieces of 8 values, the largest first.
+template <int N>
+struct Pieces {
+    bf16x8 p[N];
 };
 
-// A product with a triangular matrix adds zeros times the terms it masks, which a NaN or an infinity
-// there turns into NaNs of earlier tokens.  So where a wave finds any among the 64 tokens of its columns
-// (one FMA per value says so), it takes them out before the product and marks the rows from the first
-// on as NaN after it: a token's fault reaches its own and later tokens only.
-struct Faults {
-    int first;
-    __device__ __forceinline__ Faults(const Lane& l, float4_t (&v)[4]) : first(C) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fmaf(v[i][e], 0.0f, sum);
-        if (__ballot(sum != sum)) {
-#pragma unroll
-            for (int i = 3; i >= 0; --i)
-#pragma unroll
-                for (int e = 3; e >= 0; --e)
-                    if (!(fabsf(v[i][e]) < INFINITY)) {
-                        v[i][e] = 0.0f;
-                        first = 16 * i + l.quad + e;
-                    }
-            first = min(first, __shfl_xor(first, 16, 64));
-            first = min(first, __shfl_xor(first, 32, 64));
-        }
-    }
-    __device__ __forceinline__ float mark(int row, float v) const { return row < first ? v : NAN; }
+// N pieces of 4 values: half an operand.
+template <int N>
+struct Halves {
+    bf16x4 p[N];
 };
 
-// A chunk's decays: the running sums in 64 bits, as differences of large sums lose what a small
-// decay adds; kept as a float and its remainder.
-struct Gates {
-    float sum[C], remainder[C], since[C], rest[C], beta[C];
-
-    // By the workgroup's first wave; the caller synchronises.
-    __device__ __forceinline__ void load(const Delta& d, i64 b, i64 h, i64 n, i64 length) {
-        if (threadIdx.x >= 64) return;
-        const int i = threadIdx.x;
-        const i64 t = n * C + i;
-        double g = t < length ? (double)d.log_decay(b, t, h) : 0.0;
-#pragma unroll
-        for (int s = 1; s < 64; s *= 2) {
-            const double below = __shfl_up(g, s, 64);
-            if (i >= s) g += below;
-        }
-        const double last = __shfl(g, 63, 64);
-        sum[i] = (float)g;
-        remainder[i] = (float)(g - (double)sum[i]);
-        since[i] = expf((float)g);
-        rest[i] = expf((float)(last - g));
-        beta[i] = t < length ? d.rate(b, t, h) : 0.0f;
-    }
-    __device__ __forceinline__ float decay(int i, int j) const {
-        return expf((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
-    }
-};
-
-// A chunk's keys or queries as floats in LDS, zero beyond the key width and the sequence.
-template <typename T, int DK>
-__device__ __forceinline__ void load_chunk(float* lds, const Tensor& x, i64 b, i64 h, i64 n, i64 length, int width) {
-    constexpr int UNITS = DK / 4;
-#pragma unroll 4
-    for (int u = threadIdx.x; u < C * UNITS; u += 256) {
-        const int i = u / UNITS, c = u % UNITS * 4;
-        const i64 t = n * C + i;
-        float4_t v = ZERO;
-        if (t < length && c < width) v = load4(x.at<T>(b, t, h), c, width);
-        *(float4_t*)(lds + i * (DK + 4) + c) = v;
-    }
+__device__ __forceinline__ float4_t widen(bf16x4 v) {
+    const uint2_t bits = __builtin_bit_cast(uint2_t, v);
+    return float4_t{__uint_as_float(bits[0] << 16), __uint_as_float(bits[0] & 0xFFFF0000u),
+                    __uint_as_float(bits[1] << 16), __uint_as_float(bits[1] & 0xFFFF0000u)};
 }
 
-// Workspace positions of head (b, h), chunk n, in floats.
+template <int N>
+__device__ __forceinline__ Halves<N> split(float4_t v) {
+    Halves<N> h;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        h.p[i] = __builtin_convertvector(v, bf16x4);
+        if (i + 1 < N) v -= widen(h.p[i]);
+    }
+    return h;
+}
+
+template <int N>
+__device__ __forceinline__ Pieces<N> join(const Halves<N>& a, const Halves<N>& b) {
+    Pieces<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.p[i] = __builtin_shufflevector(a.p[i], b.p[i], 0, 1, 2, 3, 4, 5, 6, 7);
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ Pieces<N> split(float4_t a, float4_t b) {
+    return join(split<N>(a), split<N>(b));
+}
+
+// c + A B: the products of pieces whose order together is below three (below two where no side has
+// three), the smallest first.
+template <int NA, int NB>
+__device__ __forceinline__ float4_t mma(const Pieces<NA>& a, const Pieces<NB>& b, float4_t c) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB)
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[order - i], c, 0, 0, 0);
+    return c;
+}
+
+struct Lane {
+    int id, col, quad;  // l, l % 16, 4 (l / 16)
+    __device__ __forceinline__ Lane() : id(threadIdx.x % 64), col(threadIdx.x % 16), quad(threadIdx.x % 64 / 16 * 4) {}
+};
+
+// Operands in memory: N pieces, 16 bytes per lane each.
+template <int N>
+__device__ __forceinline__ Pieces<N> fetch(const bf16_t* p, i64 operand, const Lane& l) {
+    Pieces<N> r;
+#pragma unroll
+    for (int i = 0; i < N; ++i) r.p[i] = *(const bf16x8*)(p + ((operand * N + i) * 64 + l.id) * 8);
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ void put(bf16_t* p, i64 operand, const Lane& l, const Pieces<N>& v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *(bf16x8*)(p + ((operand * N + i) * 64 + l.id) * 8) = v.p[i];
+}
+
+// Half `half` of an operand: its indices 16 half ...
+template <int N>
+__device__ __forceinline__ void put_half(bf16_t* p, i64 operand, int half, const Lane& l, const Halves<N>& v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) *(bf16x4*)(p + ((operand * N + i) * 64 + l.id) * 8 + 4 * half) = v.p[i];
+}
+
+// 32 columns from c0 of a row, in the order above.
+template <typename T, int N>
+__device__ __forceinline__ Pieces<N> row_operand(const T* row, int c0, int width, bool live, const Lane& l) {
+    const float4_t a = live ? load4(row, c0 + l.quad, width) : ZERO;
+    const float4_t b = live ? load4(row, c0 + 16 + l.quad, width) : ZERO;
+    return split<N>(a, b);
+}
+
+// Rows quad .. quad + 3 of column l % 16 of a row-major block.
+__device__ __forceinline__ float4_t column(const float* m, i64 pitch, const Lane& l) {
+    float4_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = m[(l.quad + j) * pitch + l.col];
+    return v;
+}
+
+__device__ __forceinline__ void put_column(float* m, i64 pitch, const Lane& l, float4_t v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[(l.quad + j) * pitch + l.col] = v[j];
+}
+
+// Workgroup barrier for LDS alone: loads and stores of global memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A product with a triangular matrix adds zeros times the terms it masks, which a NaN or an infinity
+// there turns into NaNs of earlier tokens.  So where a wave finds any among its tokens (one FMA per value
+// says so), it takes them out before the product, and the rows from the column's first on are NaN after
+// it: a token's fault reaches its own and later tokens only.  Returns the column's first row of the
+// `count` blocks at `row`, C if there is none.
+template <int COUNT>
+__device__ __forceinline__ int take_faults(float4_t (&v)[COUNT], int row, const Lane& l) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fmaf(v[i][e], 0.0f, sum);
+    int first = C;
+    if (__ballot(sum != sum)) {
+#pragma unroll
+        for (int i = COUNT - 1; i >= 0; --i)
+#pragma unroll
+            for (int e = 3; e >= 0; --e)
+                if (!(fabsf(v[i][e]) < INFINITY)) {
+                    v[i][e] = 0.0f;
+                    first = row + 16 * i + l.quad + e;
+                }
+        first = min(first, __shfl_xor(first, 16, 64));
+        first = min(first, __shfl_xor(first, 32, 64));
+    }
+    return first;
+}
+
+// Of a triangle of 4 x 4 blocks, the operands that are not zero: row block i, 32 sum indices kb.
+__device__ __forceinline__ constexpr int lower(int i, int kb) { return i < 2 ? i : 2 * (i - 1) + kb; }
+__device__ __forceinline__ constexpr int upper(int i, int kb) { return i < 2 ? 2 * i + kb : i + 2; }
+constexpr int TRIANGLE = 6;
+
+// A chunk's decays.  The running sums are taken in 64 bits, as differences of large sums lose what a
+// small decay adds, and kept as a float and its remainder.
+enum Gate { SUM, REMAINDER, SINCE, REST, RATE, WRITE, GATES };  // WRITE = REST RATE
+
+// The workspace: operands of chunk n of key head (b, hk) or value head (b, h), and what the scans leave.
 struct Tape {
-    float *inverse, *scores, *errors, *states;
+    bf16_t *keys, *keys_t, *queries_t;       // rows are tokens; rows are key indices, sums over tokens
+    bf16_t *inverse, *inverse_t, *scores_t;  // T; T^T and P^T
+    float *gates, *errors, *states;          // E and S as rows of `padded` values
+
+    __device__ __forceinline__ i64 shared_chunk(const Delta& d, i64 b, i64 hk, i64 n) const {
+        return (b * d.heads + hk) * d.chunks + n;
+    }
     __device__ __forceinline__ i64 chunk(const Delta& d, i64 b, i64 h, i64 n) const {
         return (b * d.value_heads + h) * d.chunks + n;
     }
+    __device__ __forceinline__ const float* gate(i64 chunk, Gate which) const {
+        return gates + (chunk * GATES + which) * C;
+    }
 };
 
-// ------------------------------------------------------------------ T = (I + M B)^-1 of every chunk
+__device__ __forceinline__ float decay(const float* sum, const float* remainder, int i, int j) {
+    return expf((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
+}
+
+// ------------------------------------------------------------------ operands and T = (I + M B)^-1
+// One workgroup per chunk and key head: the keys (and, to train, queries) as operands, then for each
+// value head that shares them the gates and the inverse, 16 x 16 blocks by forward substitution, joined in
+// pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) prepare(Delta d, Tape tape) {
-    constexpr int P = DK + 4;
-    __shared__ __attribute__((aligned(16))) float k[C * P], low[C * CP], inv[C * CP];
-    __shared__ Gates gates;
+__global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, KB = DK / 32;
+    __shared__ __attribute__((aligned(16))) bf16_t rows[4 * KB * N * 512];
+    __shared__ __attribute__((aligned(16))) float low[C * CP], inv[C * CP];
+    __shared__ float gates[GATES][C];
     __shared__ int faulty;  // the first row with a NaN or an infinity; it and those after it become NaN
-    const i64 n = blockIdx.x, h = blockIdx.y, b = blockIdx.z, length = d.length(b);
+    const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
+    const i64 shared = tape.shared_chunk(d, b, hk, n);
     const int wave = threadIdx.x / 64;
     const Lane l;
-    if (threadIdx.x == 0) faulty = C;
-    gates.load(d, b, h, n, length);
-    load_chunk<T, DK>(k, d.k, b, h / d.group, n, length, d.key);
-    for (int e = threadIdx.x; e < C * CP; e += 256) inv[e] = 0.0f;
-    __syncthreads();
-    for (int j = 0; j <= wave; ++j) {
-        float4_t acc = ZERO;
-#pragma unroll 8
-        for (int f = 0; f < DK / 16; ++f)
-            acc = mfma16(l.row(k + 16 * wave * P + 16 * f, P), l.row(k + 16 * j * P + 16 * f, P), acc);
+    bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
+    const i64 t = n * C + 16 * wave + l.col;
+    Pieces<N> own[KB];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r = 16 * wave + l.quad + e, c = 16 * j + l.col;
-            float v = r > c ? acc[e] * gates.decay(r, c) * gates.beta[c] : 0.0f;
-            if (!(fabsf(v) < INFINITY)) {
-                atomicMin(&faulty, r);
-                v = 0.0f;
+    for (int kb = 0; kb < KB; ++kb) {
+        own[kb] = row_operand<T, N>(d.k.at<T>(b, t, hk), 32 * kb, d.key, t < length, l);
+        put<N>(rows, wave * KB + kb, l, own[kb]);
+        put<N>(keys, wave * KB + kb, l, own[kb]);
+    }
+    for (int what = 0; what < 1 + (train != 0); ++what) {
+        const Tensor& x = what ? d.q : d.k;
+        bf16_t* to = (what ? tape.queries_t : tape.keys_t) + shared * (4 * KB * N * 512);
+        for (int u = wave; u < 4 * KB; u += 4) {  // row block u / 2, tokens 32 (u % 2) ..
+            const int c = u / 2 * 16 + l.col;
+            float4_t v[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const i64 at = n * C + u % 2 * 32 + half * 16 + l.quad + e;
+                    v[half][e] = at < length && c < d.key ? to_float(x.at<T>(b, at, hk)[c]) : 0.0f;
+                }
+            put<N>(to, u, l, split<N>(v[0], v[1]));
+        }
+    }
+    __syncthreads();
+    float4_t kk[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        kk[j] = ZERO;
+        if (j <= wave) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) kk[j] = mma<N, N>(own[kb], fetch<N>(rows, j * KB + kb, l), kk[j]);
+        }
+    }
+    for (int member = 0; member < d.group; ++member) {
+        const i64 h = hk * d.group + member, chunk = tape.chunk(d, b, h, n);
+        __syncthreads();  // the member before is written out
+        if (threadIdx.x == 0) faulty = C;
+        if (threadIdx.x < 64) {
+            const int i = threadIdx.x;
+            const i64 at = n * C + i;
+            double g = at < length ? (double)d.log_decay(b, at, h) : 0.0;
+#pragma unroll
+            for (int s = 1; s < 64; s *= 2) {
+                const double below = __shfl_up(g, s, 64);
+                if (i >= s) g += below;
             }
-            low[r * CP + c] = v;
+            const double last = __shfl(g, 63, 64);
+            float v[GATES];
+            v[SUM] = (float)g;
+            v[REMAINDER] = (float)(g - (double)v[SUM]);
+            v[SINCE] = expf((float)g);
+            v[REST] = expf((float)(last - g));
+            v[RATE] = at < length ? d.rate(b, at, h) : 0.0f;
+            v[WRITE] = v[REST] * v[RATE];
+#pragma unroll
+            for (int w = 0; w < GATES; ++w) {
+                gates[w][i] = v[w];
+                tape.gates[(chunk * GATES + w) * C + i] = v[w];
+            }
         }
-    }
-    __syncthreads();
-    // the diagonal blocks' inverses by forward substitution, a column per lane
-    if (threadIdx.x % 64 < 16) {
-        const float* m = low + 16 * wave * (CP + 1);
-        float x[16];
+        for (int e = threadIdx.x; e < C * CP; e += 256) inv[e] = 0.0f;
+        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == l.col ? 1.0f : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) continue;
 #pragma unroll
-            for (int j = 0; j < i; ++j) v -= m[i * CP + j] * x[j];
-            x[i] = v;
-            inv[(16 * wave + i) * CP + 16 * wave + l.col] = v;
+            for (int e = 0; e < 4; ++e) {
+                const int r = 16 * wave + l.quad + e, c = 16 * j + l.col;
+                float v = r > c ? kk[j][e] * decay(gates[SUM], gates[REMAINDER], r, c) * gates[RATE][c] : 0.0f;
+                if (!(fabsf(v) < INFINITY)) {
+                    atomicMin(&faulty, r);
+                    v = 0.0f;
+                }
+                low[r * CP + c] = v;
+            }
         }
-    }
-    __syncthreads();
-    // the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below: blocks of 16, then of 32
-    if (wave < 2) {
-        float* corner = inv + (32 * wave + 16) * CP + 32 * wave;
-        const float4_t x = mfma16(l.row(low + (32 * wave + 16) * CP + 32 * wave, CP),
-                                  l.column(inv + 32 * wave * (CP + 1), CP), ZERO);
-        const float4_t y = mfma16(l.row(corner + 16, CP), x, ZERO);
+        __syncthreads();
+        if (l.id < 16) {  // a column per lane
+            const float* m = low + 16 * wave * (CP + 1);
+            float x[16];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) corner[(l.quad + e) * CP + l.col] = -y[e];
-    }
-    __syncthreads();
-    if (wave < 2) {  // column block `wave` of the lower left 32 x 32
-        float4_t x[2], y[2];
+            for (int i = 0; i < 16; ++i) {
+                float v = i == l.col ? 1.0f : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x[i] = ZERO;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                x[i] = mfma16(l.row(low + (32 + 16 * i) * CP + 16 * j, CP), l.column(inv + 16 * j * CP + 16 * wave, CP), x[i]);
+                for (int j = 0; j < i; ++j) v -= m[i * CP + j] * x[j];
+                x[i] = v;
+                inv[(16 * wave + i) * CP + 16 * wave + l.col] = v;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            y[i] = ZERO;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) y[i] = mfma16(l.row(inv + (32 + 16 * i) * CP + 32 + 16 * j, CP), x[j], y[i]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) inv[(32 + 16 * i + l.quad + e) * CP + 16 * wave + l.col] = -y[i][e];
+        __syncthreads();
+        // operands out of LDS: row l % 16 of a block, and the block's columns; indices 16 .. 31 of the sum
+        // are zero where a block stands alone
+        auto rows_of = [&](const float* m, bool both) {
+            const float4_t a = *(const float4_t*)(m + l.col * CP + l.quad);
+            return split<3>(a, both ? *(const float4_t*)(m + l.col * CP + 16 + l.quad) : ZERO);
+        };
+        if (wave < 2) {
+            float* corner = inv + (32 * wave + 16) * CP + 32 * wave;
+            const float4_t x = mma<3, 3>(rows_of(low + (32 * wave + 16) * CP + 32 * wave, false),
+                                         split<3>(column(inv + 32 * wave * (CP + 1), CP, l), ZERO), ZERO);
+            const float4_t y = mma<3, 3>(rows_of(corner + 16, false), split<3>(x, ZERO), ZERO);
+            put_column(corner, CP, l, -y);
         }
-    }
-    __syncthreads();
-    float* to = tape.inverse + tape.chunk(d, b, h, n) * C * C;
-    for (int u = threadIdx.x; u < C * C / 4; u += 256) {
-        const float4_t row = *(const float4_t*)(inv + u / 16 * CP + u % 16 * 4);
-        *(float4_t*)(to + 4 * u) = u / 16 < faulty ? row : float4_t{NAN, NAN, NAN, NAN};
+        __syncthreads();
+        if (wave < 2) {  // column block `wave` of the lower left 32 x 32
+            const float* a = inv + 16 * wave;
+            const Pieces<3> above = split<3>(column(a, CP, l), column(a + 16 * CP, CP, l));
+            float4_t x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[i] = mma<3, 3>(rows_of(low + (32 + 16 * i) * CP, true), above, ZERO);
+            const Pieces<3> below = split<3>(x[0], x[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                put_column(inv + (32 + 16 * i) * CP + 16 * wave, CP, l, -mma<3, 3>(rows_of(inv + (32 + 16 * i) * CP + 32, true), below, ZERO));
+        }
+        __syncthreads();
+        const int bad = faulty;
+        const float4_t nans = {NAN, NAN, NAN, NAN};
+        for (int u = wave; u < TRIANGLE; u += 4) {
+            const int i = u < 2 ? u : 1 + u / 2, kb = u < 2 ? 0 : u % 2;
+            const float* m = inv + (16 * i + l.col) * CP + 32 * kb + l.quad;
+            const bool fine = 16 * i + l.col < bad;
+            put<3>(tape.inverse + chunk * (TRIANGLE * 3 * 512), u, l,
+                   split<3>(fine ? *(const float4_t*)m : nans, fine ? *(const float4_t*)(m + 16) : nans));
+        }
+        if (!train) continue;
+        for (int u = wave; u < TRIANGLE; u += 4) {
+            const int i = u < 4 ? u / 2 : u - 2, kb = u < 4 ? u % 2 : 1;
+            const float* m = inv + 32 * kb * CP + 16 * i;
+            float4_t v[2] = {column(m, CP, l), column(m + 16 * CP, CP, l)};
+            if (bad < C) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (32 * kb + 16 * half + l.quad + e >= bad) v[half][e] = NAN;
+            }
+            put<3>(tape.inverse_t + chunk * (TRIANGLE * 3 * 512), u, l, split<3>(v[0], v[1]));
+        }
     }
 }
 
 // ------------------------------------------------------------------ the states through the chunks
+// A workgroup carries 16 columns of one head's state, each of its DK / 32 waves 32 rows of them in registers.
+// A chunk takes three exchanges through LDS: the waves' partial sums of K S (each then adds those of its own
+// tokens), R for T R, and rest B E for the state.  What bounds it is that chain, so a chunk's operands are
+// fetched while the chunk before it runs.
+//
+// Workgroups of one head run on one XCD (they share its operands in the L2): workgroups go to the 8 XCDs
+// in turn, so head 8 k + x takes the workgroups with index % 8 = x.
+constexpr int XCDS = 8;
+
+struct Place {
+    i64 b, h;
+    int column;
+    bool any;
+    __device__ __forceinline__ Place(const Delta& d) {
+        const int slices = (int)(d.padded / 16);
+        const i64 slot = blockIdx.x / XCDS, head = slot / slices * XCDS + blockIdx.x % XCDS;
+        column = (int)(slot % slices) * 16;
+        any = head < d.batch * d.value_heads;
+        b = head / d.value_heads;
+        h = head % d.value_heads;
+    }
+};
+
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) scan_forward(Delta d, Tape tape, float* __restrict__ final_state) {
-    constexpr int P = DK + 4, F = DK / 16;
-    __shared__ __attribute__((aligned(16))) float k[C * P], inv[C * CP];
-    __shared__ Gates gates;
-    const i64 h = blockIdx.y, b = blockIdx.z, length = d.length(b);
+__global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float* __restrict__ final_state) {
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
+    __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
+    __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
+    __shared__ int first[4][16];
+    const Place at(d);
+    if (!at.any) return;
+    const i64 b = at.b, h = at.h, length = d.length(b);
     const int wave = threadIdx.x / 64;
     const Lane l;
-    const int first = blockIdx.x * 64 + 16 * wave, col = first + l.col;
-    const bool works = first < d.padded, live = col < d.value;
-    float4_t s[F];
+    const int col = at.column + l.col;
+    const bool live = col < d.value;
+    const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+    const i64 base = (b * d.value_heads + h) * d.key * d.value + col;
+    float4_t s[2];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = 16 * f + l.quad + e;
-            s[f][e] = d.state && r < d.key && live
-                          ? d.state[((b * d.value_heads + h) * d.key + r) * d.value + col] : 0.0f;
+            const int r = 32 * wave + 16 * f + l.quad + e;
+            s[f][e] = d.state && r < d.key && live ? d.state[base + (i64)r * d.value] : 0.0f;
         }
+    Pieces<N> k[4], kt[2][2];
+    Pieces<3> inverse[OWN][2];
+    float4_t v[OWN], since[OWN], write[OWN];
+    float fade = 1.0f;
+    auto fetch_keys = [&](i64 n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = fetch<N>(tape.keys + (shared0 + n) * (4 * WAVES * N * 512), i * WAVES + wave, l);
+    };
+    auto fetch_tokens = [&](i64 n) {
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int i = wave * OWN + o;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb <= i) inverse[o][kb] = fetch<3>(tape.inverse + (chunk0 + n) * (TRIANGLE * 3 * 512), lower(i, kb), l);
+            since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
+            write[o] = *(const float4_t*)(tape.gate(chunk0 + n, WRITE) + 16 * i + l.quad);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const i64 t = n * C + 16 * i + l.quad + e;
+                v[o][e] = t < length && live ? to_float(d.v.at<T>(b, t, h)[col]) : 0.0f;
+            }
+        }
+    };
+    auto fetch_writes = [&](i64 n) {
+        fade = tape.gate(chunk0 + n, SINCE)[C - 1];
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                kt[f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
+    };
+    fetch_keys(0);
+    fetch_tokens(0);
+    fetch_writes(0);
     for (i64 n = 0; n < d.chunks; ++n) {
-        const i64 chunk = tape.chunk(d, b, h, n);
-        __syncthreads();  // the previous chunk's LDS is read
-        gates.load(d, b, h, n, length);
-        load_chunk<T, DK>(k, d.k, b, h / d.group, n, length, d.key);
-        for (int u = threadIdx.x; u < C * C / 4; u += 256)
-            *(float4_t*)(inv + u / 16 * CP + u % 16 * 4) = *(const float4_t*)(tape.inverse + chunk * C * C + 4 * u);
-        __syncthreads();
-        if (!works) continue;
+        const i64 next = n + 1 < d.chunks ? n + 1 : n;
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+        for (int f = 0; f < 2; ++f)
+            put_column(tape.states + ((chunk0 + n) * DK + 32 * wave + 16 * f) * d.padded + at.column, d.padded, l, s[f]);
+        const Pieces<3> state = split<3>(s[0], s[1]);
+        float4_t sums[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                tape.states[(chunk * DK + 16 * f + l.quad + e) * d.padded + col] = s[f][e];
-        // R = V - g K S, then E = T R
-        float4_t r[4];
+        for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[i], state, ZERO);
+        fetch_keys(next);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4_t acc = ZERO;
+        for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
+        lds_barrier();
+        // R = V - g K S of the wave's own tokens
+        float4_t r[OWN];
 #pragma unroll
-            for (int f = 0; f < F; ++f) acc = mfma16(l.row(k + 16 * i * P + 16 * f, P), s[f], acc);
+        for (int o = 0; o < OWN; ++o) {
+            float4_t sum = *(const float4_t*)part[0][wave * OWN + o][l.id];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * i + l.quad + e;
-                const i64 t = n * C + row;
-                const float v = t < length && live ? to_float(d.v.at<T>(b, t, h)[col]) : 0.0f;
-                r[i][e] = v - gates.since[row] * acc[e];
-            }
+            for (int w = 1; w < WAVES; ++w) sum += *(const float4_t*)part[w][wave * OWN + o][l.id];
+            r[o] = v[o] - since[o] * sum;
         }
-        const Faults faults(l, r);
-        float4_t w[4];
+        int fault = take_faults(r, 16 * wave * OWN, l);
+        if (l.id < 16) first[wave][l.id] = fault;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4_t acc = ZERO;
+        for (int o = 0; o < OWN; ++o) put_half<3>(seen, (wave * OWN + o) / 2, (wave * OWN + o) % 2, l, split<3>(r[o]));
+        lds_barrier();
+        fault = C;
 #pragma unroll
-            for (int j = 0; j <= i; ++j) acc = mfma16(l.row(inv + 16 * i * CP + 16 * j, CP), r[j], acc);
+        for (int w = 0; w < WAVES; ++w) fault = min(fault, first[w][l.col]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * i + l.quad + e;
-                acc[e] = faults.mark(row, acc[e]);
-                tape.errors[(chunk * C + row) * d.padded + col] = acc[e];
-                w[i][e] = acc[e] * gates.rest[row] * gates.beta[row];
-            }
+        for (int o = 0; o < OWN; ++o) {
+            const int i = wave * OWN + o;
+            float4_t e = ZERO;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb <= i) e = mma<3, 3>(inverse[o][kb], fetch<3>(seen, kb, l), e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = 16 * i + l.quad + j < fault ? e[j] : NAN;
+            put_column(tape.errors + ((chunk0 + n) * C + 16 * i) * d.padded + at.column, d.padded, l, e);
+            put_half<3>(written, i / 2, i % 2, l, split<3>(e * write[o]));
         }
-        const float fade = gates.since[C - 1];
+        fetch_tokens(next);
+        lds_barrier();
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            s[f] *= fade;
+        for (int f = 0; f < 2; ++f) s[f] *= fade;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[f] = mfma16(l.column(k + 16 * i * P + 16 * f, P), w[i], s[f]);
+        for (int kb = 0; kb < 2; ++kb) {
+            const Pieces<3> w = fetch<3>(written, kb, l);
+#pragma unroll
+            for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][kb], w, s[f]);
         }
+        fetch_writes(next);
     }
-    if (!works || !live) return;
+    if (!live) return;
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = 16 * f + l.quad + e;
-            if (r < d.key) final_state[((b * d.value_heads + h) * d.key + r) * d.value + col] = s[f][e];
+            const int r = 32 * wave + 16 * f + l.quad + e;
+            if (r < d.key) final_state[base + (i64)r * d.value] = s[f][e];
         }
 }
 
 // ------------------------------------------------------------------ every chunk's outputs
+// Wave w takes the scores of tokens 16 w .. 16 w + 15 (as P^T, whose blocks are P's operands), then every
+// fourth block of 16 value columns for all tokens.  bfloat16 outputs are rounded to 2^-9, so two pieces
+// (2^-16) of the states, scores and errors do for them.
 template <typename T, int DK>
 __global__ void __launch_bounds__(256) outputs(Delta d, Tape tape, T* __restrict__ out) {
-    constexpr int P = DK + 4, F = DK / 16;
-    __shared__ __attribute__((aligned(16))) float q[C * P], k[C * P], scores[C * CP];
-    __shared__ Gates gates;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = sizeof(T) == 2 ? 2 : 3, KB = DK / 32;
+    __shared__ __attribute__((aligned(16))) bf16_t queries[4 * KB * N * 512], scores[TRIANGLE * M * 512];
+    __shared__ __attribute__((aligned(16))) float gates[GATES][C];
     const i64 n = blockIdx.x, h = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const i64 chunk = tape.chunk(d, b, h, n);
+    const i64 chunk = tape.chunk(d, b, h, n), shared = tape.shared_chunk(d, b, h / d.group, n);
     const int wave = threadIdx.x / 64;
     const Lane l;
-    gates.load(d, b, h, n, length);
-    load_chunk<T, DK>(q, d.q, b, h / d.group, n, length, d.key);
-    load_chunk<T, DK>(k, d.k, b, h / d.group, n, length, d.key);
-    __syncthreads();
+    for (int u = threadIdx.x; u < GATES * C; u += 256) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
+    Pieces<N> own[KB];
+    const i64 t = n * C + 16 * wave + l.col;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+        own[kb] = row_operand<T, N>(d.q.at<T>(b, t, h / d.group), 32 * kb, d.key, t < length, l);
+        put<N>(queries, wave * KB + kb, l, own[kb]);
+    }
+    const bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
+    float4_t p[4], pt[4];
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float4_t acc = ZERO;
-        if (j <= wave) {
-#pragma unroll 8
-            for (int f = 0; f < F; ++f)
-                acc = mfma16(l.row(q + 16 * wave * P + 16 * f, P), l.row(k + 16 * j * P + 16 * f, P), acc);
+        p[j] = pt[j] = ZERO;
+        if (j > wave) continue;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const Pieces<N> k = fetch<N>(keys, j * KB + kb, l);
+            pt[j] = mma<N, N>(k, own[kb], pt[j]);
+            if (tape.scores_t) p[j] = mma<N, N>(own[kb], k, p[j]);
         }
+    }
+    __syncthreads();
+    const int i0 = 16 * wave;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = 16 * wave + l.quad + e, c = 16 * j + l.col;
-            const float p = r >= c ? d.scale * acc[e] * gates.decay(r, c) : 0.0f;
-            scores[r * CP + c] = p;
-            if (tape.scores) tape.scores[chunk * C * C + r * C + c] = p;
+            const int i = i0 + l.col, k = 16 * j + l.quad + e;
+            pt[j][e] = i >= k ? d.scale * pt[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
+        }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+        if (2 * kb <= wave) put<M>(scores, lower(wave, kb), l, split<M>(pt[2 * kb], pt[2 * kb + 1]));
+    if (tape.scores_t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > (wave | 1)) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = i0 + l.quad + e, k = 16 * j + l.col;
+                p[j][e] = i >= k ? d.scale * p[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
+            }
+            put_half<3>(tape.scores_t + chunk * (TRIANGLE * 3 * 512), upper(j, wave / 2), wave % 2, l, split<3>(p[j]));
         }
     }
     __syncthreads();
     for (int first = 16 * wave; first < d.padded; first += 64) {
-        const int col = first + l.col;
-        float4_t acc[4] = {ZERO, ZERO, ZERO, ZERO};
+        const float* states = tape.states + chunk * DK * d.padded + first;
+        const float* errors = tape.errors + chunk * C * d.padded + first;
+        float4_t w[4], acc[4] = {ZERO, ZERO, ZERO, ZERO};
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            float4_t s;
+        for (int j = 0; j < 4; ++j)
+            w[j] = column(errors + 16 * j * d.padded, d.padded, l) * *(const float4_t*)(gates[RATE] + 16 * j + l.quad);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = tape.states[(chunk * DK + 16 * f + l.quad + e) * d.padded + col];
+        for (int kb = 0; kb < KB; ++kb) {
+            const Pieces<M> s = split<M>(column(states + 32 * kb * d.padded, d.padded, l),
+                                         column(states + (32 * kb + 16) * d.padded, d.padded, l));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = mfma16(l.row(q + 16 * i * P + 16 * f, P), s, acc[i]);
+            for (int i = 0; i < 4; ++i) acc[i] = mma<N, M>(fetch<N>(queries, i * KB + kb, l), s, acc[i]);
         }
+        const int fault = take_faults(w, 0, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) acc[i] *= d.scale * *(const float4_t*)(gates[SINCE] + 16 * i + l.quad);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[i][e] *= d.scale * gates.since[16 * i + l.quad + e];
-        float4_t w[4];
+        for (int kb = 0; kb < 2; ++kb) {
+            const Pieces<M> e = split<M>(w[2 * kb], w[2 * kb + 1]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * j + l.quad + e;
-                w[j][e] = gates.beta[row] * tape.errors[(chunk * C + row) * d.padded + col];
-            }
-        const Faults faults(l, w);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = j; i < 4; ++i) acc[i] = mfma16(l.row(scores + 16 * i * CP + 16 * j, CP), w[j], acc[i]);
+            for (int i = 2 * kb; i < 4; ++i) acc[i] = mma<M, M>(fetch<M>(scores, lower(i, kb), l), e, acc[i]);
+        }
+        const int col = first + l.col;
         if (col >= d.value) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const i64 t = n * C + 16 * i + l.quad + e;
-                if (t < d.time)
-                    out[((b * d.time + t) * d.value_heads + h) * d.value + col] =
-                        from_float<T>(t < length ? faults.mark(16 * i + l.quad + e, acc[i][e]) : 0.0f);
+                const int row = 16 * i + l.quad + e;
+                const i64 at = n * C + row;
+                if (at < d.time)
+                    out[((b * d.time + at) * d.value_heads + h) * d.value + col] =
+                        from_float<T>(at >= length ? 0.0f : row < fault ? acc[i][e] : NAN);
             }
     }
 }
@@ -550,244 +793,312 @@ struct Back {
     float *states;            // dS' of every chunk
 };
 
+// As scan_forward, from the last chunk to the first: the waves' partial sums of K dS', then B dV' for
+// T^T B dV', then Y for the state's gradient.
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) scan_backward(Delta d, Tape tape, Back back, T* __restrict__ dv,
-                                                     float* __restrict__ dstate) {
-    constexpr int P = DK + 4, F = DK / 16;
-    __shared__ __attribute__((aligned(16))) float k[C * P], q[C * P], inv[C * CP], scores[C * CP];
-    __shared__ Gates gates;
-    const i64 h = blockIdx.y, b = blockIdx.z, length = d.length(b);
+__global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back back, T* __restrict__ dv,
+                                                        float* __restrict__ dstate) {
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
+    __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
+    __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
+    const Place at(d);
+    if (!at.any) return;
+    const i64 b = at.b, h = at.h, length = d.length(b);
     const int wave = threadIdx.x / 64;
     const Lane l;
-    const int first = blockIdx.x * 64 + 16 * wave, col = first + l.col;
-    const bool works = first < d.padded, live = col < d.value;
-    float4_t s[F];
+    const int col = at.column + l.col;
+    const bool live = col < d.value;
+    const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+    const i64 base = (b * d.value_heads + h) * d.key * d.value + col;
+    float4_t s[2];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = 16 * f + l.quad + e;
-            s[f][e] = back.grad_state && r < d.key && live
-                          ? back.grad_state[((b * d.value_heads + h) * d.key + r) * d.value + col] : 0.0f;
+            const int r = 32 * wave + 16 * f + l.quad + e;
+            s[f][e] = back.grad_state && r < d.key && live ? back.grad_state[base + (i64)r * d.value] : 0.0f;
         }
-    for (i64 n = d.chunks; n-- > 0;) {
-        const i64 chunk = tape.chunk(d, b, h, n);
-        __syncthreads();
-        gates.load(d, b, h, n, length);
-        load_chunk<T, DK>(k, d.k, b, h / d.group, n, length, d.key);
-        load_chunk<T, DK>(q, d.q, b, h / d.group, n, length, d.key);
-        for (int u = threadIdx.x; u < C * C / 4; u += 256) {
-            *(float4_t*)(inv + u / 16 * CP + u % 16 * 4) = *(const float4_t*)(tape.inverse + chunk * C * C + 4 * u);
-            *(float4_t*)(scores + u / 16 * CP + u % 16 * 4) = *(const float4_t*)(tape.scores + chunk * C * C + 4 * u);
-        }
-        __syncthreads();
-        if (!works) continue;
-        float4_t o[4], u[4];
+    Pieces<N> k[4], kt[2][2], qt[2][2];
+    Pieces<3> inverse[OWN][2], scores[OWN][2];
+    float4_t o[4], all_since[4], since[OWN], rest[OWN], rate[OWN];
+    float fade = 1.0f;
+    auto fetch_keys = [&](i64 n) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) k[i] = fetch<N>(tape.keys + (shared0 + n) * (4 * WAVES * N * 512), i * WAVES + wave, l);
+    };
+    auto fetch_tokens = [&](i64 n) {
+#pragma unroll
+        for (int w = 0; w < OWN; ++w) {
+            const int i = wave * OWN + w;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb + 1 >= i) {
+                    inverse[w][kb] = fetch<3>(tape.inverse_t + (chunk0 + n) * (TRIANGLE * 3 * 512), upper(i, kb), l);
+                    scores[w][kb] = fetch<3>(tape.scores_t + (chunk0 + n) * (TRIANGLE * 3 * 512), upper(i, kb), l);
+                }
+            since[w] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
+            rest[w] = *(const float4_t*)(tape.gate(chunk0 + n, REST) + 16 * i + l.quad);
+            rate[w] = *(const float4_t*)(tape.gate(chunk0 + n, RATE) + 16 * i + l.quad);
+        }
+    };
+    auto fetch_writes = [&](i64 n) {
+        fade = tape.gate(chunk0 + n, SINCE)[C - 1];
+#pragma unroll
+        for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                kt[f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
+                qt[f][kb] = fetch<N>(tape.queries_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            all_since[i] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const i64 t = n * C + 16 * i + l.quad + e;
                 o[i][e] = t < length && live ? to_float(back.grad.at<T>(b, t, h)[col]) : 0.0f;
             }
-#pragma unroll
-        for (int f = 0; f < F; ++f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                back.states[(chunk * DK + 16 * f + l.quad + e) * d.padded + col] = s[f][e];
-        // B dV' = B (P^T dO + rest K dS')
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4_t acc = ZERO;
-#pragma unroll
-            for (int f = 0; f < F; ++f) acc = mfma16(l.row(k + 16 * i * P + 16 * f, P), s[f], acc);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] *= gates.rest[16 * i + l.quad + e];
-#pragma unroll
-            for (int j = i; j < 4; ++j) acc = mfma16(l.column(scores + 16 * j * CP + 16 * i, CP), o[j], acc);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u[i][e] = acc[e] * gates.beta[16 * i + l.quad + e];
         }
-        const float fade = gates.since[C - 1];
+    };
+    fetch_keys(d.chunks - 1);
+    fetch_tokens(d.chunks - 1);
+    fetch_writes(d.chunks - 1);
+    for (i64 n = d.chunks; n-- > 0;) {
+        const i64 next = n > 0 ? n - 1 : 0;
 #pragma unroll
-        for (int f = 0; f < F; ++f) s[f] *= fade;
-        // Y = T^T B dV', and both products into dS
+        for (int f = 0; f < 2; ++f)
+            put_column(back.states + ((chunk0 + n) * DK + 32 * wave + 16 * f) * d.padded + at.column, d.padded, l, s[f]);
+        const Pieces<3> state = split<3>(s[0], s[1]);
+        float4_t sums[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float4_t acc = ZERO;
+        for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[i], state, ZERO);
+        fetch_keys(next);
 #pragma unroll
-            for (int j = i; j < 4; ++j) acc = mfma16(l.column(inv + 16 * j * CP + 16 * i, CP), u[j], acc);
+        for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
+        lds_barrier();
+        const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
+#pragma unroll
+        for (int w = 0; w < OWN; ++w) {
+            const int i = wave * OWN + w;
+            float4_t sum = *(const float4_t*)part[0][i][l.id];
+#pragma unroll
+            for (int from = 1; from < WAVES; ++from) sum += *(const float4_t*)part[from][i][l.id];
+            sum *= rest[w];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb + 1 >= i) sum = mma<3, N>(scores[w][kb], grads[kb], sum);
+            put_half<3>(seen, i / 2, i % 2, l, split<3>(sum * rate[w]));
+        }
+        lds_barrier();
+#pragma unroll
+        for (int w = 0; w < OWN; ++w) {
+            const int i = wave * OWN + w;
+            float4_t y = ZERO;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb + 1 >= i) y = mma<3, 3>(inverse[w][kb], fetch<3>(seen, kb, l), y);
+            put_half<3>(written, i / 2, i % 2, l, split<3>(y * -since[w]));
+            put_column(back.residuals + ((chunk0 + n) * C + 16 * i) * d.padded + at.column, d.padded, l, y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int row = 16 * i + l.quad + e;
-                const i64 t = n * C + row;
-                back.residuals[(chunk * C + row) * d.padded + col] = acc[e];
+                const i64 t = n * C + 16 * i + l.quad + e;
                 if (t < d.time && live)
-                    dv[((b * d.time + t) * d.value_heads + h) * d.value + col] = from_float<T>(t < length ? acc[e] : 0.0f);
-                acc[e] *= -gates.since[row];
-                o[i][e] *= d.scale * gates.since[row];
-            }
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                s[f] = mfma16(l.column(k + 16 * i * P + 16 * f, P), acc, s[f]);
-                s[f] = mfma16(l.column(q + 16 * i * P + 16 * f, P), o[i], s[f]);
+                    dv[((b * d.time + t) * d.value_heads + h) * d.value + col] = from_float<T>(t < length ? y[e] : 0.0f);
             }
         }
-    }
-    if (!dstate || !works || !live) return;
+        fetch_tokens(next);
+        Pieces<3> reads[2];
 #pragma unroll
-    for (int f = 0; f < F; ++f)
+        for (int kb = 0; kb < 2; ++kb)
+            reads[kb] = split<3>(o[2 * kb] * all_since[2 * kb] * d.scale, o[2 * kb + 1] * all_since[2 * kb + 1] * d.scale);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            s[f] *= fade;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[f] = mma<N, 3>(qt[f][kb], reads[kb], s[f]);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const Pieces<3> w = fetch<3>(written, kb, l);
+#pragma unroll
+            for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][kb], w, s[f]);
+        }
+        fetch_writes(next);
+    }
+    if (!dstate || !live) return;
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = 16 * f + l.quad + e;
-            if (r < d.key) dstate[((b * d.value_heads + h) * d.key + r) * d.value + col] = s[f][e];
+            const int r = 32 * wave + 16 * f + l.quad + e;
+            if (r < d.key) dstate[base + (i64)r * d.value] = s[f][e];
         }
 }
 
 // ------------------------------------------------------------------ every chunk's gradients
 // One workgroup per chunk and key head; it visits the value heads that share the key head one after the
-// other, so their sums into dq and dk need no atomics.  Wave w holds the tokens 16 w .. 16 w + 15.
+// other, so their sums into dq and dk need no atomics.  Eight waves: wave w holds the tokens 16 (w % 4) ..
+// of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
 template <typename T, int DK>
-__global__ void __launch_bounds__(256) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
+__global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
                                                  void* __restrict__ ddecay, void* __restrict__ dbeta) {
-    constexpr int P = DK + 4, F = DK / 16;
-    __shared__ __attribute__((aligned(16))) float q[C * P], k[C * P], d1[C * CP], d2[C * CP];
-    __shared__ float line[C], part[4];
-    __shared__ Gates gates;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, F = DK / 32;
+    __shared__ __attribute__((aligned(16))) float d1[C * CP], d2[C * CP];
+    __shared__ __attribute__((aligned(16))) float gates[GATES][C];
+    __shared__ float lines[2][2][C], part[8];
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const int wave = threadIdx.x / 64, token = 16 * wave;
+    const int wave = threadIdx.x / 64, block = wave % 4, half = wave / 4, token = 16 * block, key0 = half * F;
     const Lane l;
-    load_chunk<T, DK>(q, d.q, b, hk, n, length, d.key);
-    load_chunk<T, DK>(k, d.k, b, hk, n, length, d.key);
+    const i64 shared = tape.shared_chunk(d, b, hk, n);
+    const bf16_t* keys_t = tape.keys_t + shared * (C * DK * N);
+    const bf16_t* queries_t = tape.queries_t + shared * (C * DK * N);
     float4_t gq[F], gk[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) gq[f] = gk[f] = ZERO;
+    // rows of 32 values from column c, in the common order of the sum
+    auto values = [&](const float* row, int c) {
+        return split<3>(*(const float4_t*)(row + c + l.quad), c + 16 < d.padded ? *(const float4_t*)(row + c + 16 + l.quad) : ZERO);
+    };
     for (int member = 0; member < d.group; ++member) {
         const i64 h = hk * d.group + member, chunk = tape.chunk(d, b, h, n);
         __syncthreads();
-        gates.load(d, b, h, n, length);
-        __syncthreads();
-        float4_t reads[F], backs[F], writes[F], oe[4], ye[4];  // dO S^T, Y S^T, E dS'^T, dO E^T, Y E^T
+        for (int u = threadIdx.x; u < GATES * C; u += 512) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
+        float4_t reads[F], backs[F], writes[F], pairs[4];  // dO S^T, Y S^T, E dS'^T, dO E^T or Y E^T
 #pragma unroll
         for (int f = 0; f < F; ++f) reads[f] = backs[f] = writes[f] = ZERO;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) oe[j] = ye[j] = ZERO;
+        for (int j = 0; j < 4; ++j) pairs[j] = ZERO;
         float carried = 0.0f;  // this wave's share of <dS', S>
         const float* errors = tape.errors + chunk * C * d.padded;
         const float* residuals = back.residuals + chunk * C * d.padded;
         const i64 t = n * C + token + l.col;
-        for (int c = 0; c < d.padded; c += 16) {
-            float4_t o = ZERO;
-            if (t < length) o = load4(back.grad.at<T>(b, t, h), c + l.quad, d.value);
-            const float4_t y = *(const float4_t*)(residuals + (token + l.col) * d.padded + c + l.quad);
-            const float4_t e = *(const float4_t*)(errors + (token + l.col) * d.padded + c + l.quad);
+        for (int c = 0; c < d.padded; c += 32) {
+            const bool both = c + 16 < d.padded;
+            const Pieces<N> o = row_operand<T, N>(back.grad.at<T>(b, t, h), c, d.value, t < length, l);
+            const Pieces<3> y = values(residuals + (token + l.col) * d.padded, c);
+            const Pieces<3> e = values(errors + (token + l.col) * d.padded, c);
 #pragma unroll
             for (int f = 0; f < F; ++f) {
-                const i64 at = (chunk * DK + 16 * f + l.col) * d.padded + c + l.quad;
-                const float4_t s = *(const float4_t*)(tape.states + at), ds = *(const float4_t*)(back.states + at);
-                reads[f] = mfma16(o, s, reads[f]);
-                backs[f] = mfma16(y, s, backs[f]);
-                writes[f] = mfma16(e, ds, writes[f]);
-                if (f % 4 == wave) carried += (s[0] * ds[0] + s[1] * ds[1]) + (s[2] * ds[2] + s[3] * ds[3]);
+                const i64 at = (chunk * DK + 16 * (key0 + f) + l.col) * d.padded + c + l.quad;
+                const float *sp = tape.states + at, *dp = back.states + at;
+                const float4_t s0 = *(const float4_t*)sp, s1 = both ? *(const float4_t*)(sp + 16) : ZERO;
+                const float4_t g0 = *(const float4_t*)dp, g1 = both ? *(const float4_t*)(dp + 16) : ZERO;
+                if (f == block) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) carried += s0[i] * g0[i] + s1[i] * g1[i];
+                }
+                const Pieces<3> s = split<3>(s0, s1);
+                reads[f] = mma<N, 3>(o, s, reads[f]);
+                backs[f] = mma<3, 3>(y, s, backs[f]);
+                writes[f] = mma<3, 3>(e, split<3>(g0, g1), writes[f]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (j > wave) continue;
-                const float4_t other = *(const float4_t*)(errors + (16 * j + l.col) * d.padded + c + l.quad);
-                oe[j] = mfma16(o, other, oe[j]);
-                ye[j] = mfma16(y, other, ye[j]);
+                if (j > block) continue;
+                const Pieces<3> other = values(errors + (16 * j + l.col) * d.padded, c);
+                pairs[j] = half ? mma<3, 3>(y, other, pairs[j]) : mma<N, 3>(o, other, pairs[j]);
             }
         }
-        carried = lane_sum<64>(carried);
-        if (threadIdx.x % 64 == 0) part[wave] = carried;
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = token + l.quad + e, c = 16 * j + l.col;
-                const float decay = r >= c ? gates.decay(r, c) : 0.0f;
-                d1[r * CP + c] = r >= c ? d.scale * decay * oe[j][e] : 0.0f;
-                d2[r * CP + c] = r > c ? -decay * ye[j][e] : 0.0f;
+                const float a = r >= c ? decay(gates[SUM], gates[REMAINDER], r, c) : 0.0f;
+                if (half) d2[r * CP + c] = r > c ? -a * pairs[j][e] : 0.0f;
+                else d1[r * CP + c] = r >= c ? d.scale * a * pairs[j][e] : 0.0f;
             }
         __syncthreads();
-        float4_t written = ZERO;  // per row, k . rest B E dS'^T: its sum and <dS', S> make <dS', S'>
+        // the wave's own rows of the keys and queries, from the operands that hold them
+        auto own = [&](const bf16_t* from, int f) {
+            float4_t v = ZERO;
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+            for (int i = N - 1; i >= 0; --i)
+                v += widen(*(const bf16x4*)(from + (((i64)(2 * (key0 + f) + block / 2) * N + i) * 64 + l.id) * 8 + block % 2 * 4));
+            return v;
+        };
+        const float4_t since = *(const float4_t*)(gates[SINCE] + token + l.quad);
+        const float4_t rest = *(const float4_t*)(gates[REST] + token + l.quad);
+        const float4_t rate = *(const float4_t*)(gates[RATE] + token + l.quad);
+        float4_t written = ZERO;  // k . rest B E dS'^T by row: its sum and g_C <dS', S> make <dS', S'>
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = token + l.quad + e;
-                reads[f][e] *= d.scale * gates.since[r];
-                backs[f][e] *= -gates.since[r];
-                writes[f][e] *= gates.rest[r];
-                written[e] += k[r * P + 16 * f + l.col] * writes[f][e] * gates.beta[r];
-            }
-        for (int j = 0; j <= wave; ++j) {
-            const float4_t a1 = l.row(d1 + token * CP + 16 * j, CP), a2 = l.row(d2 + token * CP + 16 * j, CP);
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                float4_t kj = l.column(k + 16 * j * P + 16 * f, P);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kj[e] *= gates.beta[16 * j + l.quad + e];
-                reads[f] = mfma16(a1, kj, reads[f]);
-                backs[f] = mfma16(a2, kj, backs[f]);
-            }
+        for (int f = 0; f < F; ++f) {
+            reads[f] *= since * d.scale;
+            backs[f] *= -since;
+            writes[f] *= rest;
+            written += own(keys_t, f) * writes[f] * rate;
         }
-        for (int j = wave; j < 4; ++j) {
-            const float4_t a1 = l.column(d1 + 16 * j * CP + token, CP), a2 = l.column(d2 + 16 * j * CP + token, CP);
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-                writes[f] = mfma16(a1, l.column(q + 16 * j * P + 16 * f, P), writes[f]);
-                writes[f] = mfma16(a2, l.column(k + 16 * j * P + 16 * f, P), writes[f]);
+        for (int kb = 0; kb < 2; ++kb) {
+            if (2 * kb <= block) {  // sums over the tokens up to the wave's
+                Pieces<3> a[2];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const float* m = (w ? d2 : d1) + (token + l.col) * CP + 32 * kb + l.quad;
+                    const float* by = gates[RATE] + 32 * kb + l.quad;
+                    a[w] = split<3>(*(const float4_t*)m * *(const float4_t*)by, *(const float4_t*)(m + 16) * *(const float4_t*)(by + 16));
+                }
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    const Pieces<N> k = fetch<N>(keys_t, 2 * (key0 + f) + kb, l);
+                    reads[f] = mma<3, N>(a[0], k, reads[f]);
+                    backs[f] = mma<3, N>(a[1], k, backs[f]);
+                }
+            }
+            if (2 * kb + 1 >= block) {  // and over those from the wave's on
+                Pieces<3> a[2];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const float* m = (w ? d2 : d1) + 32 * kb * CP + token;
+                    a[w] = split<3>(column(m, CP, l), column(m + 16 * CP, CP, l));
+                }
+#pragma unroll
+                for (int f = 0; f < F; ++f) {
+                    writes[f] = mma<3, N>(a[0], fetch<N>(queries_t, 2 * (key0 + f) + kb, l), writes[f]);
+                    writes[f] = mma<3, N>(a[1], fetch<N>(keys_t, 2 * (key0 + f) + kb, l), writes[f]);
+                }
             }
         }
         float4_t db = ZERO, dg = ZERO;
 #pragma unroll
-        for (int f = 0; f < F; ++f)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = token + l.quad + e;
-                const float kv = k[r * P + 16 * f + l.col], qv = q[r * P + 16 * f + l.col];
-                db[e] += kv * writes[f][e];
-                dg[e] += qv * reads[f][e] + kv * backs[f][e];
-                gq[f][e] += reads[f][e];
-                gk[f][e] += backs[f][e] + gates.beta[r] * writes[f][e];
-            }
-        float ends = 0.0f;
+        for (int f = 0; f < F; ++f) {
+            const float4_t k = own(keys_t, f), q = own(queries_t, f);
+            db += k * writes[f];
+            dg += q * reads[f] + k * backs[f];
+            gq[f] += reads[f];
+            gk[f] += backs[f] + rate * writes[f];
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int r = token + l.quad + e;
             db[e] = lane_sum<16>(db[e]);
-            dg[e] = lane_sum<16>(dg[e]) - gates.beta[r] * db[e];
-            ends += written[e];
-            const i64 at = n * C + r;
+            dg[e] = lane_sum<16>(dg[e]);
             if (l.col == 0) {
-                line[r] = dg[e];
-                if (at < d.time) {
-                    const i64 to = (b * d.time + at) * d.value_heads + h;
-                    const float v = at < length ? db[e] : 0.0f;
-                    if (d.beta_bf16) ((bf16_t*)dbeta)[to] = from_float<bf16_t>(v);
-                    else ((float*)dbeta)[to] = v;
-                }
+                lines[half][0][token + l.quad + e] = db[e];
+                lines[half][1][token + l.quad + e] = dg[e];
             }
         }
-        ends = lane_sum<64>(ends);
-        if (threadIdx.x % 64 == 0) part[wave] = gates.since[C - 1] * part[wave] + ends;
+        const float ends = lane_sum<64>((written[0] + written[1]) + (written[2] + written[3]) + gates[SINCE][C - 1] * carried);
+        if (l.id == 0) part[wave] = ends;
         __syncthreads();
-        if (ddecay && threadIdx.x < 64) {
+        if (threadIdx.x < 64) {
             const int i = threadIdx.x;
-            float v = line[i];
-            if (i == C - 1) v += (part[0] + part[1]) + (part[2] + part[3]);
+            const i64 at = n * C + i, to = (b * d.time + at) * d.value_heads + h;
+            const float rates = lines[0][0][i] + lines[1][0][i];
+            float v = lines[0][1][i] + lines[1][1][i] - gates[RATE][i] * rates;
+            if (i == C - 1) v += ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
 #pragma unroll
             for (int s = 1; s < 64; s *= 2) {
                 const float above = __shfl_down(v, s, 64);
                 if (i + s < 64) v += above;
             }
-            const i64 at = n * C + i;
             if (at < d.time) {
-                const i64 to = (b * d.time + at) * d.value_heads + h;
-                if (at >= length) v = 0.0f;
-                if (d.decay_bf16) ((bf16_t*)ddecay)[to] = from_float<bf16_t>(v);
-                else ((float*)ddecay)[to] = v;
+                const bool live = at < length;
+                if (d.beta_bf16) ((bf16_t*)dbeta)[to] = from_float<bf16_t>(live ? rates : 0.0f);
+                else ((float*)dbeta)[to] = live ? rates : 0.0f;
+                if (ddecay && d.decay_bf16) ((bf16_t*)ddecay)[to] = from_float<bf16_t>(live ? v : 0.0f);
+                else if (ddecay) ((float*)ddecay)[to] = live ? v : 0.0f;
             }
         }
     }
@@ -796,7 +1107,7 @@ __global__ void __launch_bounds__(256) gradients(Delta d, Tape tape, Back back, 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const i64 t = n * C + token + l.quad + e;
-            const int c = 16 * f + l.col;
+            const int c = 16 * (key0 + f) + l.col;
             if (t >= d.time || c >= d.key) continue;
             const i64 to = ((b * d.time + t) * d.heads + hk) * d.key + c;
             dq[to] = from_float<T>(t < length ? gq[f][e] : 0.0f);
@@ -813,6 +1124,8 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
         return fail(err, cap, 7, "every size must be positive");
     if (a->key < 1 || a->key > MAX_KEY) return fail(err, cap, 7, "key must be 1 to %d", MAX_KEY);
     if (a->value_heads % a->heads) return fail(err, cap, 7, "value_heads must be a multiple of heads");
+    if (ceil_div(a->value, 16) * (a->batch * a->value_heads + XCDS) > 0x7FFFFFFF)
+        return fail(err, cap, 7, "batch x value_heads x value is out of range");
     if (a->batch > 65535 || a->value_heads > 65535 || a->time > 0x7FFFFFFF - C || a->value > (1 << 20))
         return fail(err, cap, 7, "batch and value_heads must be at most 65535, time below 2^31 - 64, value at most 2^20");
     if (!known_type(a->type) || !known_type(a->log_decay_type) || !known_type(a->beta_type))
@@ -837,29 +1150,42 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
 
 int key_width(const Delta& d) { return d.key <= 64 ? 64 : 128; }
 
-i64 carve(const Delta& d, int train, char* base, Tape* tape) {
-    const i64 chunks = d.batch * d.value_heads * d.chunks;
+// Carves the workspace (256-byte pieces); the operands of the backward pass only to train.
+i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
+    const i64 chunks = d.batch * d.value_heads * d.chunks, shared = d.batch * d.heads * d.chunks;
+    const i64 pieces = type == ATLAS_OPS_BF16 ? 1 : 3;
     i64 at = 0;
-    auto floats = [&](i64 n) {
-        float* p = (float*)(base + at);
-        at += n * (i64)sizeof(float);
-        return p;
+    auto take = [&](auto*& p, i64 bytes, bool wanted = true) {
+        p = wanted ? (std::decay_t<decltype(p)>)(base + at) : nullptr;
+        if (wanted) at += ceil_div(bytes, 256) * 256;
     };
     Tape t{};
-    t.inverse = floats(chunks * C * C);
-    t.errors = floats(chunks * C * d.padded);
-    t.states = floats(chunks * key_width(d) * d.padded);
-    if (train) t.scores = floats(chunks * C * C);
+    take(t.keys, shared * C * key_width(d) * pieces * 2);
+    take(t.keys_t, shared * C * key_width(d) * pieces * 2);
+    take(t.queries_t, shared * C * key_width(d) * pieces * 2, train);
+    take(t.inverse, chunks * TRIANGLE * 3 * 1024);
+    take(t.inverse_t, chunks * TRIANGLE * 3 * 1024, train);
+    take(t.scores_t, chunks * TRIANGLE * 3 * 1024, train);
+    take(t.gates, chunks * GATES * C * 4);
+    take(t.errors, chunks * C * d.padded * 4);
+    take(t.states, chunks * key_width(d) * d.padded * 4);
     if (tape) *tape = t;
     return at;
 }
 
 template <typename F>
 void with_kernel(const Delta& d, int type, F&& f) {
-    const auto narrow = std::integral_constant<int, 64>{};
-    const auto wide = std::integral_constant<int, 128>{};
-    if (type == ATLAS_OPS_F32) key_width(d) == 64 ? f(0.0f, narrow) : f(0.0f, wide);
-    else key_width(d) == 64 ? f(bf16_t{}, narrow) : f(bf16_t{}, wide);
+    auto by_width = [&](auto t) {
+        if (key_width(d) == 64) f(t, std::integral_constant<int, 64>{});
+        else f(t, std::integral_constant<int, 128>{});
+    };
+    if (type == ATLAS_OPS_F32) by_width(0.0f);
+    else by_width(bf16_t{});
+}
+
+// Workgroups of a scan: 16 columns each, whole groups of 8 heads (Place).
+dim3 scan_grid(const Delta& d) {
+    return dim3((unsigned)(ceil_div(d.batch * d.value_heads, XCDS) * XCDS * (d.padded / 16)));
 }
 
 }  // namespace
@@ -893,7 +1219,7 @@ int atlas_ops_delta_step(const AtlasDelta* a, void* out, float* final_state, voi
 
 int64_t atlas_ops_delta_workspace(const AtlasDelta* a, int train) {
     Delta d;
-    return check(a, d, nullptr, 0) ? 0 : carve(d, train, nullptr, nullptr);
+    return check(a, d, nullptr, 0) ? 0 : carve(d, a->type, train, nullptr, nullptr);
 }
 
 int atlas_ops_delta_forward(const AtlasDelta* a, int train, void* out, float* final_state, void* workspace, void* stream,
@@ -903,14 +1229,14 @@ int atlas_ops_delta_forward(const AtlasDelta* a, int train, void* out, float* fi
         if (int rc = check(a, d, err, cap)) return rc;
         if (!out || !final_state || !workspace) return fail(err, cap, 7, "null argument");
         Tape tape;
-        carve(d, train, (char*)workspace, &tape);
+        carve(d, a->type, train, (char*)workspace, &tape);
         hipStream_t st = (hipStream_t)stream;
         const dim3 all((unsigned)d.chunks, (unsigned)d.value_heads, (unsigned)d.batch);
-        const dim3 columns((unsigned)ceil_div(d.value, 64), (unsigned)d.value_heads, (unsigned)d.batch);
+        const dim3 keys((unsigned)d.chunks, (unsigned)d.heads, (unsigned)d.batch);
         with_kernel(d, a->type, [&](auto t, auto width) {
             using T = decltype(t);
-            prepare<T, width()><<<all, 256, 0, st>>>(d, tape);
-            scan_forward<T, width()><<<columns, 256, 0, st>>>(d, tape, final_state);
+            prepare<T, width()><<<keys, 256, 0, st>>>(d, tape, train);
+            scan_forward<T, width()><<<scan_grid(d), 2 * width(), 0, st>>>(d, tape, final_state);
             outputs<T, width()><<<all, 256, 0, st>>>(d, tape, (T*)out);
         });
         return launched(err, cap, "delta_forward");
@@ -935,17 +1261,16 @@ int atlas_ops_delta_backward(const AtlasDelta* a, const void* tape_memory, const
         if (!tape_memory || !grad_out || !grad_out_stride || !dq || !dk || !dv || !dbeta || !workspace)
             return fail(err, cap, 7, "null argument");
         Tape tape;
-        carve(d, 1, (char*)tape_memory, &tape);
+        carve(d, a->type, 1, (char*)tape_memory, &tape);
         float* floats = (float*)workspace;
         const Back back{tensor(grad_out, grad_out_stride), grad_state, floats,
                         floats + d.batch * d.value_heads * d.chunks * C * d.padded};
         hipStream_t st = (hipStream_t)stream;
-        const dim3 columns((unsigned)ceil_div(d.value, 64), (unsigned)d.value_heads, (unsigned)d.batch);
         const dim3 all((unsigned)d.chunks, (unsigned)d.heads, (unsigned)d.batch);
         with_kernel(d, a->type, [&](auto t, auto width) {
             using T = decltype(t);
-            scan_backward<T, width()><<<columns, 256, 0, st>>>(d, tape, back, (T*)dv, dstate);
-            gradients<T, width()><<<all, 256, 0, st>>>(d, tape, back, (T*)dq, (T*)dk, dlog_decay, dbeta);
+            scan_backward<T, width()><<<scan_grid(d), 2 * width(), 0, st>>>(d, tape, back, (T*)dv, dstate);
+            gradients<T, width()><<<all, 512, 0, st>>>(d, tape, back, (T*)dq, (T*)dk, dlog_decay, dbeta);
         });
         return launched(err, cap, "delta_backward");
     } catch (...) {
