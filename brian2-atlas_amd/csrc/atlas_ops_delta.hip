@@ -48,7 +48,7 @@ struct Delta {
     const int32_t* lengths;
     i64 batch, time, heads, value_heads;
     int key, value, group, decay_bf16, beta_bf16;
-    i64 chunks, padded;  // padded: value in whole blocks of 16
+    i64 chunks, padded;  // padded: value in whole operands of 32
     float scale;
 
     __device__ __forceinline__ i64 length(i64 b) const {
@@ -297,13 +297,66 @@ __device__ __forceinline__ void put_half(bf16_t* p, i64 operand, int half, const
     for (int i = 0; i < N; ++i) *(bf16x4*)(p + ((operand * N + i) * 64 + l.id) * 8 + 4 * half) = v.p[i];
 }
 
-// 32 columns from c0 of a row, in the order above.
-template <typename T, int N>
-__device__ __forceinline__ Pieces<N> row_operand(const T* row, int c0, int width, bool live, const Lane& l) {
-    const float4_t a = live ? load4(row, c0 + l.quad, width) : ZERO;
-    const float4_t b = live ? load4(row, c0 + 16 + l.quad, width) : ZERO;
-    return split<N>(a, b);
+// Loads of the caller's tensors have no branches around them (a load behind a branch is waited for there):
+// they go to a row and column that exist, and what lies outside is replaced by zero afterwards.  Only
+// where a width is no multiple of 32 do four values come one by one.
+__device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.time ? t : d.time - 1; }
+
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+
+template <typename T>
+__device__ __forceinline__ float4_t to_float4(const Four<T>& raw, bool live) {
+    float4_t v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = live ? to_float(raw.v[e]) : 0.0f;
+    return v;
 }
+
+// COUNT operands of 32 columns each from column c0 of a row, in the order above.
+template <typename T, int N, int COUNT>
+__device__ __forceinline__ void row_operands(Pieces<N> (&out)[COUNT], const T* row, int c0, int width, bool live, const Lane& l) {
+    float4_t v[COUNT][2];
+    if (width % 32 == 0) {
+        Four<T> raw[COUNT][2];
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int c = c0 + 32 * i + 16 * half + l.quad;
+                raw[i][half] = *(const Four<T>*)(row + (c < width ? c : 0));
+            }
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) v[i][half] = to_float4(raw[i][half], live && c0 + 32 * i + 16 * half < width);
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                v[i][half] = live ? load4(row, c0 + 32 * i + 16 * half + l.quad, width) : ZERO;
+    }
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) out[i] = split<N>(v[i][0], v[i][1]);
+}
+
+// The values of four tokens from t0 in one column, as loaded and as floats.
+template <typename T>
+struct Tokens {
+    T raw[4];
+    __device__ __forceinline__ void load(const Delta& d, const Tensor& x, i64 b, i64 h, i64 t0, int col, int width) {
+        const T* p = x.at<T>(b, 0, h) + (col < width ? col : width - 1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[e] = p[existing(t0 + e, d) * x.time];
+    }
+    __device__ __forceinline__ float4_t floats(i64 t0, i64 length, bool live) const {
+        float4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = live && t0 + e < length ? to_float(raw[e]) : 0.0f;
+        return v;
+    }
+};
 
 // Rows quad .. quad + 3 of column l % 16 of a row-major block.
 __device__ __forceinline__ float4_t column(const float* m, i64 pitch, const Lane& l) {
@@ -401,26 +454,29 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
     bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
     const i64 t = n * C + 16 * wave + l.col;
     Pieces<N> own[KB];
+    row_operands<T, N, KB>(own, d.k.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-        own[kb] = row_operand<T, N>(d.k.at<T>(b, t, hk), 32 * kb, d.key, t < length, l);
         put<N>(rows, wave * KB + kb, l, own[kb]);
         put<N>(keys, wave * KB + kb, l, own[kb]);
     }
     for (int what = 0; what < 1 + (train != 0); ++what) {
         const Tensor& x = what ? d.q : d.k;
         bf16_t* to = (what ? tape.queries_t : tape.keys_t) + shared * (4 * KB * N * 512);
-        for (int u = wave; u < 4 * KB; u += 4) {  // row block u / 2, tokens 32 (u % 2) ..
-            const int c = u / 2 * 16 + l.col;
-            float4_t v[2];
+        Tokens<T> v[KB][2];  // operand u: row block u / 2, tokens 32 (u % 2) ..
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+            const int u = wave + 4 * i;
 #pragma unroll
             for (int half = 0; half < 2; ++half)
+                v[i][half].load(d, x, b, hk, n * C + u % 2 * 32 + half * 16 + l.quad, u / 2 * 16 + l.col, d.key);
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const i64 at = n * C + u % 2 * 32 + half * 16 + l.quad + e;
-                    v[half][e] = at < length && c < d.key ? to_float(x.at<T>(b, at, hk)[c]) : 0.0f;
-                }
-            put<N>(to, u, l, split<N>(v[0], v[1]));
+        for (int i = 0; i < KB; ++i) {
+            const int u = wave + 4 * i;
+            const i64 t0 = n * C + u % 2 * 32 + l.quad;
+            const bool live = u / 2 * 16 + l.col < d.key;
+            put<N>(to, u, l, split<N>(v[i][0].floats(t0, length, live), v[i][1].floats(t0 + 16, length, live)));
         }
     }
     __syncthreads();
@@ -591,7 +647,8 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
         }
     Pieces<N> k[4], kt[2][2];
     Pieces<3> inverse[OWN][2];
-    float4_t v[OWN], since[OWN], write[OWN];
+    Tokens<T> v[OWN];
+    float4_t since[OWN], write[OWN];
     float fade = 1.0f;
     auto fetch_keys = [&](i64 n) {
 #pragma unroll
@@ -606,11 +663,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
                 if (2 * kb <= i) inverse[o][kb] = fetch<3>(tape.inverse + (chunk0 + n) * (TRIANGLE * 3 * 512), lower(i, kb), l);
             since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
             write[o] = *(const float4_t*)(tape.gate(chunk0 + n, WRITE) + 16 * i + l.quad);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const i64 t = n * C + 16 * i + l.quad + e;
-                v[o][e] = t < length && live ? to_float(d.v.at<T>(b, t, h)[col]) : 0.0f;
-            }
+            v[o].load(d, d.v, b, h, n * C + 16 * i + l.quad, col, d.value);
         }
     };
     auto fetch_writes = [&](i64 n) {
@@ -644,7 +697,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
             float4_t sum = *(const float4_t*)part[0][wave * OWN + o][l.id];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) sum += *(const float4_t*)part[w][wave * OWN + o][l.id];
-            r[o] = v[o] - since[o] * sum;
+            r[o] = v[o].floats(n * C + 16 * (wave * OWN + o) + l.quad, length, live) - since[o] * sum;
         }
         int fault = take_faults(r, 16 * wave * OWN, l);
         if (l.id < 16) first[wave][l.id] = fault;
@@ -704,9 +757,9 @@ __global__ void __launch_bounds__(256) outputs(Delta d, Tape tape, T* __restrict
     for (int u = threadIdx.x; u < GATES * C; u += 256) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
     Pieces<N> own[KB];
     const i64 t = n * C + 16 * wave + l.col;
+    row_operands<T, N, KB>(own, d.q.at<T>(b, existing(t, d), h / d.group), 0, d.key, t < length, l);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-        own[kb] = row_operand<T, N>(d.q.at<T>(b, t, h / d.group), 32 * kb, d.key, t < length, l);
         put<N>(queries, wave * KB + kb, l, own[kb]);
     }
     const bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
@@ -820,7 +873,8 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
         }
     Pieces<N> k[4], kt[2][2], qt[2][2];
     Pieces<3> inverse[OWN][2], scores[OWN][2];
-    float4_t o[4], all_since[4], since[OWN], rest[OWN], rate[OWN];
+    Tokens<T> go[4];
+    float4_t all_since[4], since[OWN], rest[OWN], rate[OWN];
     float fade = 1.0f;
     auto fetch_keys = [&](i64 n) {
 #pragma unroll
@@ -853,11 +907,7 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             all_since[i] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const i64 t = n * C + 16 * i + l.quad + e;
-                o[i][e] = t < length && live ? to_float(back.grad.at<T>(b, t, h)[col]) : 0.0f;
-            }
+            go[i].load(d, back.grad, b, h, n * C + 16 * i + l.quad, col, d.value);
         }
     };
     fetch_keys(d.chunks - 1);
@@ -876,6 +926,9 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
+        float4_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = go[i].floats(n * C + 16 * i + l.quad, length, live);
         const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
@@ -958,7 +1011,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
     for (int f = 0; f < F; ++f) gq[f] = gk[f] = ZERO;
     // rows of 32 values from column c, in the common order of the sum
     auto values = [&](const float* row, int c) {
-        return split<3>(*(const float4_t*)(row + c + l.quad), c + 16 < d.padded ? *(const float4_t*)(row + c + 16 + l.quad) : ZERO);
+        return split<3>(*(const float4_t*)(row + c + l.quad), *(const float4_t*)(row + c + 16 + l.quad));
     };
     for (int member = 0; member < d.group; ++member) {
         const i64 h = hk * d.group + member, chunk = tape.chunk(d, b, h, n);
@@ -974,16 +1027,17 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
         const float* residuals = back.residuals + chunk * C * d.padded;
         const i64 t = n * C + token + l.col;
         for (int c = 0; c < d.padded; c += 32) {
-            const bool both = c + 16 < d.padded;
-            const Pieces<N> o = row_operand<T, N>(back.grad.at<T>(b, t, h), c, d.value, t < length, l);
+            Pieces<N> os[1];
+            row_operands<T, N, 1>(os, back.grad.at<T>(b, existing(t, d), h), c, d.value, t < length, l);
+            const Pieces<N>& o = os[0];
             const Pieces<3> y = values(residuals + (token + l.col) * d.padded, c);
             const Pieces<3> e = values(errors + (token + l.col) * d.padded, c);
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 const i64 at = (chunk * DK + 16 * (key0 + f) + l.col) * d.padded + c + l.quad;
                 const float *sp = tape.states + at, *dp = back.states + at;
-                const float4_t s0 = *(const float4_t*)sp, s1 = both ? *(const float4_t*)(sp + 16) : ZERO;
-                const float4_t g0 = *(const float4_t*)dp, g1 = both ? *(const float4_t*)(dp + 16) : ZERO;
+                const float4_t s0 = *(const float4_t*)sp, s1 = *(const float4_t*)(sp + 16);
+                const float4_t g0 = *(const float4_t*)dp, g1 = *(const float4_t*)(dp + 16);
                 if (f == block) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) carried += s0[i] * g0[i] + s1[i] * g1[i];
@@ -1124,7 +1178,7 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
         return fail(err, cap, 7, "every size must be positive");
     if (a->key < 1 || a->key > MAX_KEY) return fail(err, cap, 7, "key must be 1 to %d", MAX_KEY);
     if (a->value_heads % a->heads) return fail(err, cap, 7, "value_heads must be a multiple of heads");
-    if (ceil_div(a->value, 16) * (a->batch * a->value_heads + XCDS) > 0x7FFFFFFF)
+    if (ceil_div(a->value, 32) * 2 * (a->batch * a->value_heads + XCDS) > 0x7FFFFFFF)
         return fail(err, cap, 7, "batch x value_heads x value is out of range");
     if (a->batch > 65535 || a->value_heads > 65535 || a->time > 0x7FFFFFFF - C || a->value > (1 << 20))
         return fail(err, cap, 7, "batch and value_heads must be at most 65535, time below 2^31 - 64, value at most 2^20");
@@ -1143,7 +1197,7 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
     d.key = (int)a->key, d.value = (int)a->value, d.group = (int)(a->value_heads / a->heads);
     d.decay_bf16 = a->log_decay_type == ATLAS_OPS_BF16, d.beta_bf16 = a->beta_type == ATLAS_OPS_BF16;
     d.chunks = ceil_div(a->time, C);
-    d.padded = ceil_div(a->value, 16) * 16;
+    d.padded = ceil_div(a->value, 32) * 32;
     d.scale = a->scale;
     return 0;
 }
