@@ -270,6 +270,20 @@ __device__ __forceinline__ float4_t mma(const Pieces<NA>& a, const Pieces<NB>& b
     return c;
 }
 
+// c + A B in two chains, the smaller products apart from the larger: half the latency of mma.
+template <int NA, int NB>
+__device__ __forceinline__ void mma2(const Pieces<NA>& a, const Pieces<NB>& b, float4_t& large, float4_t& small) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB) {
+                float4_t& c = order == ORDERS - 1 ? small : large;
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[order - i], c, 0, 0, 0);
+            }
+}
+
 struct Lane {
     int id, col, quad;  // l, l % 16, 4 (l / 16)
     __device__ __forceinline__ Lane() : id(threadIdx.x % 64), col(threadIdx.x % 16), quad(threadIdx.x % 64 / 16 * 4) {}
@@ -299,7 +313,7 @@ __device__ __forceinline__ void put_half(bf16_t* p, i64 operand, int half, const
 
 // Loads of the caller's tensors have no branches around them (a load behind a branch is waited for there):
 // they go to a row and column that exist, and what lies outside is replaced by zero afterwards.  Only
-// where a width is no multiple of 32 do four values come one by one.
+// where a width is no multiple of 4 do four values come one by one.
 __device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.time ? t : d.time - 1; }
 
 template <typename T>
@@ -317,7 +331,7 @@ __device__ __forceinline__ float4_t to_float4(const Four<T>& raw, bool live) {
 template <typename T, int N, int COUNT>
 __device__ __forceinline__ void row_operands(Pieces<N> (&out)[COUNT], const T* row, int c0, int width, bool live, const Lane& l) {
     float4_t v[COUNT][2];
-    if (width % 32 == 0) {
+    if (width % 4 == 0) {
         Four<T> raw[COUNT][2];
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
@@ -329,7 +343,7 @@ __device__ __forceinline__ void row_operands(Pieces<N> (&out)[COUNT], const T* r
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) v[i][half] = to_float4(raw[i][half], live && c0 + 32 * i + 16 * half < width);
+            for (int half = 0; half < 2; ++half) v[i][half] = to_float4(raw[i][half], live && c0 + 32 * i + 16 * half + l.quad < width);
     } else {
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
@@ -369,6 +383,16 @@ __device__ __forceinline__ float4_t column(const float* m, i64 pitch, const Lane
 __device__ __forceinline__ void put_column(float* m, i64 pitch, const Lane& l, float4_t v) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) m[(l.quad + j) * pitch + l.col] = v[j];
+}
+
+// Matrices of floats between the kernels lie as 16 x 16 blocks of results, 16 bytes per lane: block
+// (r, c) of a matrix of `blocks` block columns.
+__device__ __forceinline__ float4_t block(const float* m, i64 r, i64 c, i64 blocks, const Lane& l) {
+    return *(const float4_t*)(m + ((r * blocks + c) * 64 + l.id) * 4);
+}
+
+__device__ __forceinline__ void put_block(float* m, i64 r, i64 c, i64 blocks, const Lane& l, float4_t v) {
+    *(float4_t*)(m + ((r * blocks + c) * 64 + l.id) * 4) = v;
 }
 
 // Workgroup barrier for LDS alone: loads and stores of global memory stay in flight across it.
@@ -418,8 +442,9 @@ enum Gate { SUM, REMAINDER, SINCE, REST, RATE, WRITE, GATES };  // WRITE = REST 
 // The workspace: operands of chunk n of key head (b, hk) or value head (b, h), and what the scans leave.
 struct Tape {
     bf16_t *keys, *keys_t, *queries_t;       // rows are tokens; rows are key indices, sums over tokens
-    bf16_t *inverse, *inverse_t, *scores_t;  // T; T^T and P^T
-    float *gates, *errors, *states;          // E and S as rows of `padded` values
+    bf16_t *inverse, *scores;                // T and P
+    bf16_t *inverse_t, *scores_t;            // T^T and P^T
+    float *gates, *errors, *states;          // E and S in blocks
 
     __device__ __forceinline__ i64 shared_chunk(const Delta& d, i64 b, i64 hk, i64 n) const {
         return (b * d.heads + hk) * d.chunks + n;
@@ -436,13 +461,17 @@ __device__ __forceinline__ float decay(const float* sum, const float* remainder,
     return expf((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
 }
 
+// Pieces of what only the outputs see: bfloat16 outputs are rounded to 2^-9, so two (2^-16) do for them.
+template <typename T>
+constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
+
 // ------------------------------------------------------------------ operands and T = (I + M B)^-1
 // One workgroup per chunk and key head: the keys (and, to train, queries) as operands, then for each
-// value head that shares them the gates and the inverse, 16 x 16 blocks by forward substitution, joined in
+// value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
 // pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.
 template <typename T, int DK>
 __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, KB = DK / 32;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
     __shared__ __attribute__((aligned(16))) bf16_t rows[4 * KB * N * 512];
     __shared__ __attribute__((aligned(16))) float low[C * CP], inv[C * CP];
     __shared__ float gates[GATES][C];
@@ -453,8 +482,9 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
     const Lane l;
     bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
     const i64 t = n * C + 16 * wave + l.col;
-    Pieces<N> own[KB];
+    Pieces<N> own[KB], query[KB];
     row_operands<T, N, KB>(own, d.k.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
+    row_operands<T, N, KB>(query, d.q.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         put<N>(rows, wave * KB + kb, l, own[kb]);
@@ -480,13 +510,17 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
         }
     }
     __syncthreads();
-    float4_t kk[4];
+    float4_t kk[4], kq[4], qk[4];  // K K^T, K Q^T (whose blocks are operands of P) and Q K^T (of P^T)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        kk[j] = ZERO;
-        if (j <= wave) {
+        kk[j] = kq[j] = qk[j] = ZERO;
+        if (j > wave) continue;
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) kk[j] = mma<N, N>(own[kb], fetch<N>(rows, j * KB + kb, l), kk[j]);
+        for (int kb = 0; kb < KB; ++kb) {
+            const Pieces<N> other = fetch<N>(rows, j * KB + kb, l);
+            kk[j] = mma<N, N>(own[kb], other, kk[j]);
+            kq[j] = mma<N, N>(other, query[kb], kq[j]);
+            if (train) qk[j] = mma<N, N>(query[kb], other, qk[j]);
         }
     }
     for (int member = 0; member < d.group; ++member) {
@@ -530,6 +564,34 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
                     v = 0.0f;
                 }
                 low[r * CP + c] = v;
+            }
+        }
+        {
+            float4_t p[4] = {ZERO, ZERO, ZERO, ZERO};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > wave) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * wave + l.col, k = 16 * j + l.quad + e;
+                    p[j][e] = i >= k ? d.scale * kq[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb <= wave) put<M>(tape.scores + chunk * (TRIANGLE * M * 512), lower(wave, kb), l, split<M>(p[2 * kb], p[2 * kb + 1]));
+        }
+        if (train) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j > (wave | 1)) continue;
+                float4_t p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * wave + l.quad + e, k = 16 * j + l.col;
+                    p[e] = i >= k ? d.scale * qk[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
+                }
+                put_half<3>(tape.scores_t + chunk * (TRIANGLE * 3 * 512), upper(j, wave / 2), wave % 2, l, split<3>(p));
             }
         }
         __syncthreads();
@@ -680,8 +742,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
     for (i64 n = 0; n < d.chunks; ++n) {
         const i64 next = n + 1 < d.chunks ? n + 1 : n;
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
-            put_column(tape.states + ((chunk0 + n) * DK + 32 * wave + 16 * f) * d.padded + at.column, d.padded, l, s[f]);
+        for (int f = 0; f < 2; ++f) put_block(tape.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
         const Pieces<3> state = split<3>(s[0], s[1]);
         float4_t sums[4];
 #pragma unroll
@@ -710,25 +771,26 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
 #pragma unroll
         for (int o = 0; o < OWN; ++o) {
             const int i = wave * OWN + o;
-            float4_t e = ZERO;
+            float4_t large[2] = {ZERO, ZERO}, small[2] = {ZERO, ZERO};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb <= i) e = mma<3, 3>(inverse[o][kb], fetch<3>(seen, kb, l), e);
+                if (2 * kb <= i) mma2<3, 3>(inverse[o][kb], fetch<3>(seen, kb, l), large[kb], small[kb]);
+            float4_t e = (large[0] + large[1]) + (small[0] + small[1]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) e[j] = 16 * i + l.quad + j < fault ? e[j] : NAN;
-            put_column(tape.errors + ((chunk0 + n) * C + 16 * i) * d.padded + at.column, d.padded, l, e);
             put_half<3>(written, i / 2, i % 2, l, split<3>(e * write[o]));
+            put_block(tape.errors, (chunk0 + n) * 4 + i, at.column / 16, d.padded / 16, l, e);
         }
         fetch_tokens(next);
-        lds_barrier();
 #pragma unroll
         for (int f = 0; f < 2; ++f) s[f] *= fade;
+        lds_barrier();
+        float4_t other[2] = {ZERO, ZERO};
+        const Pieces<3> w[2] = {fetch<3>(written, 0, l), fetch<3>(written, 1, l)};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const Pieces<3> w = fetch<3>(written, kb, l);
+        for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][0], w[0], s[f]);
 #pragma unroll
-            for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][kb], w, s[f]);
-        }
+        for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[f][1], w[1], other[f]);
         fetch_writes(next);
     }
     if (!live) return;
@@ -742,98 +804,68 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
 }
 
 // ------------------------------------------------------------------ every chunk's outputs
-// Wave w takes the scores of tokens 16 w .. 16 w + 15 (as P^T, whose blocks are P's operands), then every
-// fourth block of 16 value columns for all tokens.  bfloat16 outputs are rounded to 2^-9, so two pieces
-// (2^-16) of the states, scores and errors do for them.
+// Each wave takes every fourth block of 16 value columns for the chunk's 64 tokens; it reads the states and
+// errors, the most of the traffic, once, and fetches a block's while it works on the one before.
 template <typename T, int DK>
 __global__ void __launch_bounds__(256) outputs(Delta d, Tape tape, T* __restrict__ out) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = sizeof(T) == 2 ? 2 : 3, KB = DK / 32;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
     __shared__ __attribute__((aligned(16))) bf16_t queries[4 * KB * N * 512], scores[TRIANGLE * M * 512];
-    __shared__ __attribute__((aligned(16))) float gates[GATES][C];
+    __shared__ __attribute__((aligned(16))) float gates[2][C];
     const i64 n = blockIdx.x, h = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const i64 chunk = tape.chunk(d, b, h, n), shared = tape.shared_chunk(d, b, h / d.group, n);
-    const int wave = threadIdx.x / 64;
+    const i64 chunk = tape.chunk(d, b, h, n);
+    const int wave = threadIdx.x / 64, blocks = (int)(d.padded / 16);
     const Lane l;
-    for (int u = threadIdx.x; u < GATES * C; u += 256) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
-    Pieces<N> own[KB];
-    const i64 t = n * C + 16 * wave + l.col;
-    row_operands<T, N, KB>(own, d.q.at<T>(b, existing(t, d), h / d.group), 0, d.key, t < length, l);
+    float4_t s[2 * KB], e[4];
+    auto fetch_block = [&](int c) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-        put<N>(queries, wave * KB + kb, l, own[kb]);
-    }
-    const bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
-    float4_t p[4], pt[4];
+        for (int r = 0; r < 2 * KB; ++r) s[r] = block(tape.states, chunk * (2 * KB) + r, c, blocks, l);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        p[j] = pt[j] = ZERO;
-        if (j > wave) continue;
+        for (int r = 0; r < 4; ++r) e[r] = block(tape.errors, chunk * 4 + r, c, blocks, l);
+    };
+    if (wave < blocks) fetch_block(wave);
+    {
+        const i64 t = n * C + 16 * wave + l.col;
+        Pieces<N> own[KB];
+        row_operands<T, N, KB>(own, d.q.at<T>(b, existing(t, d), h / d.group), 0, d.key, t < length, l);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            const Pieces<N> k = fetch<N>(keys, j * KB + kb, l);
-            pt[j] = mma<N, N>(k, own[kb], pt[j]);
-            if (tape.scores_t) p[j] = mma<N, N>(own[kb], k, p[j]);
-        }
+        for (int kb = 0; kb < KB; ++kb) put<N>(queries, wave * KB + kb, l, own[kb]);
+        for (int u = threadIdx.x; u < TRIANGLE * M * 64; u += 256)
+            *(bf16x8*)(scores + u * 8) = *(const bf16x8*)(tape.scores + chunk * (TRIANGLE * M * 512) + u * 8);
+        if (threadIdx.x < 2 * C) gates[wave][l.id] = tape.gate(chunk, wave ? RATE : SINCE)[l.id];
     }
     __syncthreads();
-    const int i0 = 16 * wave;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = i0 + l.col, k = 16 * j + l.quad + e;
-            pt[j][e] = i >= k ? d.scale * pt[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
-        }
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-        if (2 * kb <= wave) put<M>(scores, lower(wave, kb), l, split<M>(pt[2 * kb], pt[2 * kb + 1]));
-    if (tape.scores_t) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > (wave | 1)) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = i0 + l.quad + e, k = 16 * j + l.col;
-                p[j][e] = i >= k ? d.scale * p[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
-            }
-            put_half<3>(tape.scores_t + chunk * (TRIANGLE * 3 * 512), upper(j, wave / 2), wave % 2, l, split<3>(p[j]));
-        }
-    }
-    __syncthreads();
-    for (int first = 16 * wave; first < d.padded; first += 64) {
-        const float* states = tape.states + chunk * DK * d.padded + first;
-        const float* errors = tape.errors + chunk * C * d.padded + first;
+    for (int c = wave; c < blocks; c += 4) {
         float4_t w[4], acc[4] = {ZERO, ZERO, ZERO, ZERO};
+        Pieces<M> state[KB];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            w[j] = column(errors + 16 * j * d.padded, d.padded, l) * *(const float4_t*)(gates[RATE] + 16 * j + l.quad);
+        for (int kb = 0; kb < KB; ++kb) state[kb] = split<M>(s[2 * kb], s[2 * kb + 1]);
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            const Pieces<M> s = split<M>(column(states + 32 * kb * d.padded, d.padded, l),
-                                         column(states + (32 * kb + 16) * d.padded, d.padded, l));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = mma<N, M>(fetch<N>(queries, i * KB + kb, l), s, acc[i]);
-        }
+        for (int j = 0; j < 4; ++j) w[j] = e[j] * *(const float4_t*)(gates[1] + 16 * j + l.quad);
+        if (c + 4 < blocks) fetch_block(c + 4);
         const int fault = take_faults(w, 0, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= d.scale * *(const float4_t*)(gates[SINCE] + 16 * i + l.quad);
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = mma<N, M>(fetch<N>(queries, i * KB + kb, l), state[kb], acc[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= d.scale * *(const float4_t*)(gates[0] + 16 * i + l.quad);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const Pieces<M> e = split<M>(w[2 * kb], w[2 * kb + 1]);
+            const Pieces<M> error = split<M>(w[2 * kb], w[2 * kb + 1]);
 #pragma unroll
-            for (int i = 2 * kb; i < 4; ++i) acc[i] = mma<M, M>(fetch<M>(scores, lower(i, kb), l), e, acc[i]);
+            for (int i = 2 * kb; i < 4; ++i) acc[i] = mma<M, M>(fetch<M>(scores, lower(i, kb), l), error, acc[i]);
         }
-        const int col = first + l.col;
+        const int col = 16 * c + l.col;
         if (col >= d.value) continue;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = 16 * i + l.quad + e;
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * i + l.quad + j;
                 const i64 at = n * C + row;
                 if (at < d.time)
                     out[((b * d.time + at) * d.value_heads + h) * d.value + col] =
-                        from_float<T>(at >= length ? 0.0f : row < fault ? acc[i][e] : NAN);
+                        from_float<T>(at >= length ? 0.0f : row < fault ? acc[i][j] : NAN);
             }
     }
 }
@@ -916,8 +948,19 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
     for (i64 n = d.chunks; n-- > 0;) {
         const i64 next = n > 0 ? n - 1 : 0;
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
-            put_column(back.states + ((chunk0 + n) * DK + 32 * wave + 16 * f) * d.padded + at.column, d.padded, l, s[f]);
+        for (int f = 0; f < 2; ++f) put_block(back.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
+        // what does not need the state: P^T dO of the wave's own tokens
+        float4_t o[4], direct[OWN];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = go[i].floats(n * C + 16 * i + l.quad, length, live);
+        const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
+#pragma unroll
+        for (int w = 0; w < OWN; ++w) {
+            direct[w] = ZERO;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                if (2 * kb + 1 >= wave * OWN + w) direct[w] = mma<3, N>(scores[w][kb], grads[kb], direct[w]);
+        }
         const Pieces<3> state = split<3>(s[0], s[1]);
         float4_t sums[4];
 #pragma unroll
@@ -926,32 +969,25 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
-        float4_t o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = go[i].floats(n * C + 16 * i + l.quad, length, live);
-        const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
             const int i = wave * OWN + w;
             float4_t sum = *(const float4_t*)part[0][i][l.id];
 #pragma unroll
             for (int from = 1; from < WAVES; ++from) sum += *(const float4_t*)part[from][i][l.id];
-            sum *= rest[w];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb + 1 >= i) sum = mma<3, N>(scores[w][kb], grads[kb], sum);
-            put_half<3>(seen, i / 2, i % 2, l, split<3>(sum * rate[w]));
+            put_half<3>(seen, i / 2, i % 2, l, split<3>((direct[w] + sum * rest[w]) * rate[w]));
         }
         lds_barrier();
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
             const int i = wave * OWN + w;
-            float4_t y = ZERO;
+            float4_t large[2] = {ZERO, ZERO}, small[2] = {ZERO, ZERO};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb + 1 >= i) y = mma<3, 3>(inverse[w][kb], fetch<3>(seen, kb, l), y);
+                if (2 * kb + 1 >= i) mma2<3, 3>(inverse[w][kb], fetch<3>(seen, kb, l), large[kb], small[kb]);
+            const float4_t y = (large[0] + large[1]) + (small[0] + small[1]);
             put_half<3>(written, i / 2, i % 2, l, split<3>(y * -since[w]));
-            put_column(back.residuals + ((chunk0 + n) * C + 16 * i) * d.padded + at.column, d.padded, l, y);
+            put_block(back.residuals, (chunk0 + n) * 4 + i, at.column / 16, d.padded / 16, l, y);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const i64 t = n * C + 16 * i + l.quad + e;
@@ -971,12 +1007,12 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
             for (int kb = 0; kb < 2; ++kb) s[f] = mma<N, 3>(qt[f][kb], reads[kb], s[f]);
         }
         lds_barrier();
+        float4_t other[2] = {ZERO, ZERO};
+        const Pieces<3> w[2] = {fetch<3>(written, 0, l), fetch<3>(written, 1, l)};
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const Pieces<3> w = fetch<3>(written, kb, l);
+        for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][0], w[0], s[f]);
 #pragma unroll
-            for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][kb], w, s[f]);
-        }
+        for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[f][1], w[1], other[f]);
         fetch_writes(next);
     }
     if (!dstate || !live) return;
@@ -990,6 +1026,11 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 }
 
 // ------------------------------------------------------------------ every chunk's gradients
+// Five of the products sum over the value columns, while the scans leave S, dS', E and Y as blocks whose
+// lanes are those columns.  A block's transpose is its product with the identity, which MFMA takes
+// exactly for bfloat16 pieces: so 32 columns at a time are split into pieces once for the workgroup, turned,
+// and kept in LDS as operands for all its waves.
+//
 // One workgroup per chunk and key head; it visits the value heads that share the key head one after the
 // other, so their sums into dq and dk need no atomics.  Eight waves: wave w holds the tokens 16 (w % 4) ..
 // of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
@@ -997,63 +1038,99 @@ template <typename T, int DK>
 __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
                                                  void* __restrict__ ddecay, void* __restrict__ dbeta) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, F = DK / 32;
-    __shared__ __attribute__((aligned(16))) float d1[C * CP], d2[C * CP];
+    constexpr int STATES = DK / 16 * 3 * 512, TOKENS = 4 * 3 * 512;
+    // S, dS', E and Y of 32 columns; afterwards D1 and D2
+    __shared__ __attribute__((aligned(16))) bf16_t stage[2 * STATES + 2 * TOKENS];
     __shared__ __attribute__((aligned(16))) float gates[GATES][C];
     __shared__ float lines[2][2][C], part[8];
+    bf16_t *s_stage = stage, *g_stage = stage + STATES, *e_stage = stage + 2 * STATES, *y_stage = e_stage + TOKENS;
+    float *d1 = (float*)stage, *d2 = d1 + C * CP;
+    static_assert(2 * C * CP * sizeof(float) <= sizeof(stage), "D1 and D2 take the stage's place");
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const int wave = threadIdx.x / 64, block = wave % 4, half = wave / 4, token = 16 * block, key0 = half * F;
+    const int wave = threadIdx.x / 64, tb = wave % 4, half = wave / 4, token = 16 * tb, key0 = half * F;
+    const int columns = (int)(d.padded / 16);
     const Lane l;
     const i64 shared = tape.shared_chunk(d, b, hk, n);
     const bf16_t* keys_t = tape.keys_t + shared * (C * DK * N);
     const bf16_t* queries_t = tape.queries_t + shared * (C * DK * N);
+    // the identity as operand: indices 16 half .. of 32 against 16 columns
+    bf16x8 unit[2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        unit[0][j] = j < 4 && l.quad + j == l.col ? (__bf16)1.0f : (__bf16)0.0f;
+        unit[1][j] = j >= 4 && l.quad + j - 4 == l.col ? (__bf16)1.0f : (__bf16)0.0f;
+    }
+    // blocks (2 pair, c) and (2 pair + 1, c), turned, as half c % 2 of operands 2 pair and 2 pair + 1
+    auto turn = [&](bf16_t* to, int pair, int c, float4_t a, float4_t b2) {
+        const Pieces<3> pieces = split<3>(a, b2);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            Halves<3> turned;
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                turned.p[i] = __builtin_convertvector(__builtin_amdgcn_mfma_f32_16x16x32_bf16(pieces.p[i], unit[which], ZERO, 0, 0, 0), bf16x4);
+            put_half<3>(to, 2 * pair + which, c, l, turned);
+        }
+    };
     float4_t gq[F], gk[F];
 #pragma unroll
     for (int f = 0; f < F; ++f) gq[f] = gk[f] = ZERO;
-    // rows of 32 values from column c, in the common order of the sum
-    auto values = [&](const float* row, int c) {
-        return split<3>(*(const float4_t*)(row + c + l.quad), *(const float4_t*)(row + c + 16 + l.quad));
-    };
     for (int member = 0; member < d.group; ++member) {
         const i64 h = hk * d.group + member, chunk = tape.chunk(d, b, h, n);
-        __syncthreads();
-        for (int u = threadIdx.x; u < GATES * C; u += 512) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
         float4_t reads[F], backs[F], writes[F], pairs[4];  // dO S^T, Y S^T, E dS'^T, dO E^T or Y E^T
 #pragma unroll
         for (int f = 0; f < F; ++f) reads[f] = backs[f] = writes[f] = ZERO;
 #pragma unroll
         for (int j = 0; j < 4; ++j) pairs[j] = ZERO;
         float carried = 0.0f;  // this wave's share of <dS', S>
-        const float* errors = tape.errors + chunk * C * d.padded;
-        const float* residuals = back.residuals + chunk * C * d.padded;
         const i64 t = n * C + token + l.col;
-        for (int c = 0; c < d.padded; c += 32) {
-            Pieces<N> os[1];
-            row_operands<T, N, 1>(os, back.grad.at<T>(b, existing(t, d), h), c, d.value, t < length, l);
-            const Pieces<N>& o = os[0];
-            const Pieces<3> y = values(residuals + (token + l.col) * d.padded, c);
-            const Pieces<3> e = values(errors + (token + l.col) * d.padded, c);
+        const T* grad = back.grad.at<T>(b, existing(t, d), h);
+        // a stage's blocks: DK / 32 x 2 pairs of S and of dS', 2 x 2 of E and of Y
+        constexpr int UNITS = DK / 16;
+        float4_t sv[2], gv[2], tv[2];
+        Pieces<N> next[1];
+        auto fetch_stage = [&](int c) {
+            const int u = wave % UNITS, r = u / 2 * 2;
+            const float* tokens = (wave < 4 ? tape.errors : back.residuals);
+            const int v = wave % 4, q = v / 2 * 2;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                sv[i] = block(tape.states, chunk * (DK / 16) + r + i, c + u % 2, columns, l);
+                gv[i] = block(back.states, chunk * (DK / 16) + r + i, c + u % 2, columns, l);
+                tv[i] = block(tokens, chunk * 4 + q + i, c + v % 2, columns, l);
+            }
+            row_operands<T, N, 1>(next, grad, 16 * c, d.value, t < length, l);
+        };
+        fetch_stage(0);
+        for (int c = 0; c < columns; c += 2) {
+            __syncthreads();  // the stage before is read
+            if (wave < UNITS) {
+                const int u = wave;
+                turn(s_stage, u / 2, u % 2, sv[0], sv[1]);
+                turn(g_stage, u / 2, u % 2, gv[0], gv[1]);
+                const float4_t dot = sv[0] * gv[0] + sv[1] * gv[1];
+                carried += (dot[0] + dot[1]) + (dot[2] + dot[3]);
+            }
+            turn(wave < 4 ? e_stage : y_stage, wave % 4 / 2, wave % 2, tv[0], tv[1]);
+            const Pieces<N> o = next[0];
+            if (c + 2 < columns) fetch_stage(c + 2);
+            __syncthreads();
+            const Pieces<3> y = fetch<3>(y_stage, tb, l), e = fetch<3>(e_stage, tb, l);
 #pragma unroll
             for (int f = 0; f < F; ++f) {
-                const i64 at = (chunk * DK + 16 * (key0 + f) + l.col) * d.padded + c + l.quad;
-                const float *sp = tape.states + at, *dp = back.states + at;
-                const float4_t s0 = *(const float4_t*)sp, s1 = *(const float4_t*)(sp + 16);
-                const float4_t g0 = *(const float4_t*)dp, g1 = *(const float4_t*)(dp + 16);
-                if (f == block) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) carried += s0[i] * g0[i] + s1[i] * g1[i];
-                }
-                const Pieces<3> s = split<3>(s0, s1);
+                const Pieces<3> s = fetch<3>(s_stage, key0 + f, l);
                 reads[f] = mma<N, 3>(o, s, reads[f]);
                 backs[f] = mma<3, 3>(y, s, backs[f]);
-                writes[f] = mma<3, 3>(e, split<3>(g0, g1), writes[f]);
+                writes[f] = mma<3, 3>(e, fetch<3>(g_stage, key0 + f, l), writes[f]);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (j > block) continue;
-                const Pieces<3> other = values(errors + (16 * j + l.col) * d.padded, c);
+                if (j > tb) continue;
+                const Pieces<3> other = fetch<3>(e_stage, j, l);
                 pairs[j] = half ? mma<3, 3>(y, other, pairs[j]) : mma<N, 3>(o, other, pairs[j]);
             }
         }
+        for (int u = threadIdx.x; u < GATES * C; u += 512) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1070,7 +1147,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             float4_t v = ZERO;
 #pragma unroll
             for (int i = N - 1; i >= 0; --i)
-                v += widen(*(const bf16x4*)(from + (((i64)(2 * (key0 + f) + block / 2) * N + i) * 64 + l.id) * 8 + block % 2 * 4));
+                v += widen(*(const bf16x4*)(from + (((i64)(2 * (key0 + f) + tb / 2) * N + i) * 64 + l.id) * 8 + tb % 2 * 4));
             return v;
         };
         const float4_t since = *(const float4_t*)(gates[SINCE] + token + l.quad);
@@ -1086,7 +1163,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
         }
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            if (2 * kb <= block) {  // sums over the tokens up to the wave's
+            if (2 * kb <= tb) {  // sums over the tokens up to the wave's
                 Pieces<3> a[2];
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -1101,7 +1178,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
                     backs[f] = mma<3, N>(a[1], k, backs[f]);
                 }
             }
-            if (2 * kb + 1 >= block) {  // and over those from the wave's on
+            if (2 * kb + 1 >= tb) {  // and over those from the wave's on
                 Pieces<3> a[2];
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
@@ -1218,6 +1295,7 @@ i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
     take(t.keys_t, shared * C * key_width(d) * pieces * 2);
     take(t.queries_t, shared * C * key_width(d) * pieces * 2, train);
     take(t.inverse, chunks * TRIANGLE * 3 * 1024);
+    take(t.scores, chunks * TRIANGLE * (type == ATLAS_OPS_BF16 ? 2 : 3) * 1024);
     take(t.inverse_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.scores_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.gates, chunks * GATES * C * 4);
