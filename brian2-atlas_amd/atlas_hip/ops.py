@@ -74,7 +74,7 @@ def _call(device: int, entry, *args) -> None:
         buffer = ctypes.create_string_buffer(512)
         buffer, address = _local.error = (buffer, ctypes.addressof(buffer))
     stream = torch._C._cuda_getCurrentRawStream(device)
-    if torch.cuda.current_device() == device:
+    if torch._C._cuda_getDevice() == device:
         rc = entry(*args, stream, address, 512)
     else:
         with torch.cuda.device(device):
@@ -99,7 +99,17 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
     return index
 
 
-_F32 = {torch.float32: 0}
+_F32, _I32 = {torch.float32: 0}, {torch.int32: 0}
+_SAME = {t: {t: 0} for t in TYPES}
+
+
+def _empty(t):
+    """A contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _workspace(size: int, like):
+    return torch.empty(size, dtype=torch.uint8, device=like.device)
 
 
 # ------------------------------------------------------------------------------ layer normalisation
@@ -125,13 +135,26 @@ def _rows(x):
     return _rows(x.contiguous())
 
 
-def _norm_weights(x, weight, bias, device):
-    types = {torch.float32: 0, x.dtype: TYPES[x.dtype]}
+_NORM_WEIGHTS = {torch.float32: {torch.float32: 0}, torch.bfloat16: TYPES}
+
+
+def _norm_weights(x, width, weight, bias, device):
+    """weight and bias, contiguous, and the code of their type."""
+    types, code = _NORM_WEIGHTS[x.dtype], 0
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
-            _tensor(t, name, device, types, x.shape[-1:])
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must have the same type")
+            _tensor(t, name, device, types)
+            if t.dim() != 1 or t.shape[0] != width:
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(width,)}")
+            code = types[t.dtype]
+    if weight is not None:
+        if bias is not None and weight.dtype != bias.dtype:
+            raise ValueError("weight and bias must have the same type")
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return weight, bias, code
 
 
 def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, statistics: bool = False):
@@ -140,24 +163,20 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, statistics: bool
     x: float32 or bfloat16; weight and bias: float32 or x's type.  Returns y, contiguous and of x's type; with
     ``statistics`` (y, mean, rstd), which ``layer_norm_backward`` takes, as float32 of x's leading shape."""
     device = _tensor(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
         raise ValueError("x needs a last axis to normalise")
-    _norm_weights(x, weight, bias, device)
-    lead, width = x.shape[:-1], x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    weight, bias, code = _norm_weights(x, width, weight, bias, device)
+    y = _empty(x)
     mean = rstd = None
     if statistics:
-        mean, rstd = torch.empty((2, *lead), dtype=torch.float32, device=x.device)
+        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind()
     rows = x.numel() // width
     if rows:
         packed, keep = _rows(x)
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        given = weight if weight is not None else bias
         _call(device, library().atlas_ops_layer_norm, packed, rows, width, TYPES[x.dtype],
-              None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
-              0 if given is None else TYPES[given.dtype], eps, y.data_ptr(),
-              mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None)
+              None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), code, eps,
+              y.data_ptr(), mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None)
     return (y, mean, rstd) if statistics else y
 
 
@@ -167,27 +186,28 @@ def layer_norm_backward(grad, x, weight, mean, rstd, *, sums: bool = True):
     weight may be None (all ones; dweight and dbias are then float32).  Without ``sums`` dweight and dbias are
     None.  The sums over the rows are taken in float32 in a fixed order: the same bits on every run."""
     device = _tensor(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
         raise ValueError("x needs a last axis to normalise")
-    _tensor(grad, "grad", device, {x.dtype: 0}, x.shape)
-    _norm_weights(x, weight, None, device)
-    lead, width = x.shape[:-1], x.shape[-1]
+    _tensor(grad, "grad", device, _SAME[x.dtype], x.shape)
+    wtype = torch.float32 if weight is None else weight.dtype
+    weight, _, code = _norm_weights(x, width, weight, None, device)
+    lead = x.shape[:-1]
     _tensor(mean, "mean", device, _F32, lead)
     _tensor(rstd, "rstd", device, _F32, lead)
     rows, type_ = x.numel() // width, TYPES[x.dtype]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    wtype = torch.float32 if weight is None else weight.dtype
+    dx = _empty(x)
     dweight = dbias = workspace = None
     lib = library()
     if sums:
-        dweight, dbias = torch.empty((2, width), dtype=wtype, device=x.device)
-        workspace = torch.empty(lib.atlas_ops_layer_norm_workspace(rows, width, type_), dtype=torch.uint8, device=x.device)
+        dweight, dbias = torch.empty((2, width), dtype=wtype, device=x.device).unbind()
+        workspace = _workspace(lib.atlas_ops_layer_norm_workspace(rows, width, type_), x)
     if rows or sums:
         packed_grad, keep_grad = _rows(grad) if rows else (None, None)
         packed, keep = _rows(x) if rows else (None, None)
-        weight, mean, rstd = (None if t is None else t.contiguous() for t in (weight, mean, rstd))
+        mean, rstd = mean.contiguous(), rstd.contiguous()
         _call(device, lib.atlas_ops_layer_norm_backward, packed_grad, packed, rows, width, type_,
-              None if weight is None else weight.data_ptr(), TYPES[wtype], mean.data_ptr(), rstd.data_ptr(),
+              None if weight is None else weight.data_ptr(), code, mean.data_ptr(), rstd.data_ptr(),
               dx.data_ptr(), dweight.data_ptr() if sums else None, dbias.data_ptr() if sums else None,
               workspace.data_ptr() if sums else None)
     return dx, dweight, dbias
@@ -211,8 +231,7 @@ def _orthogonalize(device, source, shape, *, momentum, factor, nesterov, steps, 
     if source.stride(-1) != 1:
         source = source.contiguous()
     lib = library()
-    workspace = torch.empty(lib.atlas_ops_orthogonalize_workspace(batch, rows, columns), dtype=torch.uint8,
-                            device=source.device)
+    workspace = _workspace(lib.atlas_ops_orthogonalize_workspace(batch, rows, columns), source)
     packed = _ORTHOGONAL.pack(source.data_ptr(), batch, rows, columns, source.stride(0) if source.dim() == 3 else 0,
                               source.stride(-2), 0 if momentum is None else momentum.data_ptr(),
                               0 if out is None else out.data_ptr(), 0 if weight is None else weight.data_ptr(),
@@ -230,7 +249,7 @@ def orthogonalize(matrix, *, steps: int = 5, coefficients=COEFFICIENTS, eps: flo
     is contiguous and of the matrix's type."""
     device = _tensor(matrix, "matrix")
     shape = _matrix(matrix, "matrix")
-    out = torch.empty(matrix.shape, dtype=matrix.dtype, device=matrix.device)
+    out = _empty(matrix)
     if out.numel():
         _orthogonalize(device, matrix, shape, momentum=None, factor=0.0, nesterov=False, steps=steps,
                        coefficients=coefficients, eps=eps, out=out)
@@ -278,22 +297,21 @@ class _Problem:
 
     def __init__(self, q, k, v, log_decay, beta, state, lengths, scale, time_axis: bool):
         device = _tensor(q, "q")
-        names = "(batch, time, heads, width)" if time_axis else "(batch, heads, width)"
-        if q.dim() != 3 + time_axis or v.dim() != q.dim():
-            raise ValueError(f"q, k and v must be {names}")
-        same = {q.dtype: 0}
-        _tensor(k, "k", device, same, q.shape)
+        shape, out = q.shape, v.shape
+        if len(shape) != 3 + time_axis or len(out) != len(shape):
+            raise ValueError(f"q, k and v must be {'(batch, time, heads, width)' if time_axis else '(batch, heads, width)'}")
+        same = _SAME[q.dtype]
+        _tensor(k, "k", device, same, shape)
         _tensor(v, "v", device, same)
-        lead = q.shape[:-2]
-        heads, key = q.shape[-2:]
-        value_heads, value = v.shape[-2:]
-        if v.shape[:-2] != lead:
-            raise ValueError(f"v has leading shape {tuple(v.shape[:-2])}, q {tuple(lead)}")
+        *lead, heads, key = shape
+        *given, value_heads, value = out
+        if given != lead:
+            raise ValueError(f"v has leading shape {tuple(given)}, q {tuple(lead)}")
         if heads < 1 or value_heads < 1 or value_heads % heads:
             raise ValueError("the heads of v must be a multiple of those of q and k")
         if not 1 <= key <= MAX_KEY or value < 1:
             raise ValueError(f"the width of q and k must be 1 to {MAX_KEY}, that of v positive")
-        gates = (*lead, value_heads)
+        gates = out[:-1]
         if log_decay is not None:
             _tensor(log_decay, "log_decay", device, TYPES, gates)
         _tensor(beta, "beta", device, TYPES, gates)
@@ -301,13 +319,13 @@ class _Problem:
         if state is not None:
             _tensor(state, "state", device, _F32, (batch, value_heads, key, value))
         if lengths is not None:
-            _tensor(lengths, "lengths", device, {torch.int32: 0}, (batch,))
+            _tensor(lengths, "lengths", device, _I32, (batch,))
             lengths = lengths.contiguous()
         q, k, v = _last(q), _last(k), _last(v)
 
         def strides(t):
             s = t.stride()
-            return (s[0], s[1], s[2]) if time_axis else (s[0], 0, s[1])
+            return s[:3] if time_axis else (s[0], 0, s[1])
 
         self.device, self.batch, self.time, self.heads, self.value_heads = device, batch, time, heads, value_heads
         self.key, self.value, self.type = key, value, q.dtype
@@ -331,7 +349,7 @@ def delta_rule_step(q, k, v, log_decay, beta, state, *, scale: float | None = No
     p = _Problem(q, k, v, log_decay, beta, state, None, scale, False)
     if not state.is_contiguous():
         raise ValueError("state is updated in place and must be contiguous")
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _empty(v)
     if p.batch:
         _call(p.device, library().atlas_ops_delta_step, p.packed, out.data_ptr(), state.data_ptr())
         torch.autograd.graph.increment_version(state)
@@ -368,7 +386,7 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, lengths=None, scale: flo
     if state is not None and isinstance(state, torch.Tensor):
         state = state.contiguous()
     p = _Problem(q, k, v, log_decay, beta, state, lengths, scale, True)
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _empty(v)
     shape = (p.batch, p.value_heads, p.key, p.value)
     memory = None
     if not p.batch or not p.time:
@@ -379,7 +397,7 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, lengths=None, scale: flo
         if p.time <= SHORT and not tape:
             _call(p.device, lib.atlas_ops_delta_step, p.packed, out.data_ptr(), final.data_ptr())
         else:
-            memory = torch.empty(lib.atlas_ops_delta_workspace(p.packed, tape), dtype=torch.uint8, device=v.device)
+            memory = _workspace(lib.atlas_ops_delta_workspace(p.packed, tape), v)
             _call(p.device, lib.atlas_ops_delta_forward, p.packed, tape, out.data_ptr(), final.data_ptr(),
                   memory.data_ptr())
     if tape:
@@ -393,14 +411,14 @@ def delta_rule_backward(grad_out, grad_state, tape: DeltaTape) -> dict:
     was not given.  Heads of q and k that value heads share get the sum.  The same bits on every run."""
     p = tape.problem
     q, k, v, log_decay, beta, state, lengths = p.tensors
-    _tensor(grad_out, "grad_out", p.device, {p.type: 0}, v.shape)
+    _tensor(grad_out, "grad_out", p.device, _SAME[p.type], v.shape)
     if grad_state is not None:
         _tensor(grad_state, "grad_state", p.device, _F32, (p.batch, p.value_heads, p.key, p.value))
         grad_state = grad_state.contiguous()
     grad_out = _last(grad_out)
 
     def like(t):
-        return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        return None if t is None else _empty(t)
 
     grads = {"q": like(q), "k": like(k), "v": like(v), "log_decay": like(log_decay), "beta": like(beta),
              "state": like(state)}
@@ -415,7 +433,7 @@ def delta_rule_backward(grad_out, grad_state, tape: DeltaTape) -> dict:
             if t is not None:
                 t.record_stream(stream)
     lib = library()
-    workspace = torch.empty(lib.atlas_ops_delta_backward_workspace(p.packed), dtype=torch.uint8, device=v.device)
+    workspace = _workspace(lib.atlas_ops_delta_backward_workspace(p.packed), v)
     _call(p.device, lib.atlas_ops_delta_backward, p.packed, tape.memory.data_ptr(), grad_out.data_ptr(),
           struct.pack("@3q", *grad_out.stride()[:3]), None if grad_state is None else grad_state.data_ptr(),
           *(None if grads[n] is None else grads[n].data_ptr() for n in ("q", "k", "v", "log_decay", "beta", "state")),

@@ -42,13 +42,9 @@ template <typename T>
 __device__ __forceinline__ T from_float(float v);
 template <>
 __device__ __forceinline__ float from_float<float>(float v) { return v; }
-// Round to nearest even; a NaN keeps a payload bit (adding the rounding term could carry it away).
+// Round to nearest even, a NaN stays one: gfx950 converts two values per instruction.
 template <>
-__device__ __forceinline__ bf16_t from_float<bf16_t>(float v) {
-    const uint32_t bits = __float_as_uint(v);
-    if ((bits & 0x7FFFFFFFu) > 0x7F800000u) return (bf16_t)((bits >> 16) | 0x40u);
-    return (bf16_t)((bits + 0x7FFFu + ((bits >> 16) & 1u)) >> 16);
-}
+__device__ __forceinline__ bf16_t from_float<bf16_t>(float v) { return __builtin_bit_cast(bf16_t, (__bf16)v); }
 
 // Sum over groups of LANES neighbouring lanes (a power of two up to 64); every lane gets it.
 template <int LANES>
