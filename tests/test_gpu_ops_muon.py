@@ -50,19 +50,24 @@ def test_orthogonalize_matches_the_reference(shape, dtype):
     assert torch.equal(got, ops.orthogonalize(m))
 
 
-def test_large_tiles():
-    """A smaller side of 1920 and more takes the tiles of 128; ragged, both orientations."""
-    print("case: orthogonalize 128-tiles", flush=True)
-    for shape in ((1990, 2050), (2050, 1990)):
-        m = make(shape, seed=4)
-        got = ops.orthogonalize(m)
-        x = m.double()
-        a, b, c = ops.COEFFICIENTS
-        x = x / (x.norm() + 1e-7)
-        for _ in range(5):
+@pytest.mark.parametrize("shape", [(1990, 2050), (2050, 1990), (1990, 4100), (4100, 1990), (9, 700, 1300)])
+def test_large_tiles(shape):
+    """Sizes of the 64-tiles and of the 256 x 128 ones with split sums, ragged, both orientations, in a batch."""
+    print(f"case: orthogonalize large {shape}", flush=True)
+    m = make(shape, seed=4)
+    got = ops.orthogonalize(m)
+    x = m.double()
+    a, b, c = ops.COEFFICIENTS
+    x = x / (torch.linalg.norm(x, dim=(-2, -1), keepdim=True) + 1e-7)
+    for _ in range(5):
+        if x.shape[-2] <= x.shape[-1]:
             g = x @ x.mT.contiguous()
             x = a * x + (b * g + c * (g @ g)) @ x
-        assert float((got.double() - x).norm() / x.norm()) <= 2e-5
+        else:
+            g = x.mT.contiguous() @ x
+            x = a * x + x @ (b * g + c * (g @ g))
+    assert float((got.double() - x).norm() / x.norm()) <= 2e-5
+    assert torch.equal(got, ops.orthogonalize(m))
 
 
 @pytest.mark.parametrize("rank", [1, 4])
