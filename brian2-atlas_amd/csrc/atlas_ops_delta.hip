@@ -8,9 +8,9 @@
 //   out = scale (g Q S + (lower part of D o Q K^T) B E)
 //   S' = g_C S + K^T (rest B E)    rest_i = exp(G_C - G_i)
 // so that a chunk costs matrix products and one triangular inverse T = (I + M B)^-1, which no
-// state enters: `prepare` inverts for all chunks at once, `scan_forward` carries the states through the
-// chunks, and `outputs` takes every chunk's outputs at once.  The columns of S do not touch each other:
-// each workgroup of the scan has 16 of them.
+// state enters: `prepare` inverts for all chunks at once, and `scan_forward` carries the states through the
+// chunks and takes the outputs on the way.  The columns of S do not touch each other: each workgroup of the
+// scan has 16 of them.
 //
 // Backwards, with P = scale (lower part of D o Q K^T):
 //   dV' = P^T dO + rest K dS',  Y = T^T B dV',  dV = Y,  dS = g_C dS' + scale Q^T g dO - K^T g Y
@@ -23,6 +23,7 @@
 // as every factor exp(G_i) comes with q_i or the k_i that reads, and every exp(-G_i) with the k_i that
 // writes; dlog_decay sums dG from the token to the chunk's end.
 #include <algorithm>
+#include <type_traits>
 
 #include "device/atlas_ops.h"
 
@@ -56,31 +57,18 @@ struct Delta {
         const i64 n = lengths[b];
         return n < 0 ? 0 : n < time ? n : time;
     }
+    // A gate of either type, with loads that stand behind no branch.
+    __device__ static __forceinline__ float gate(const Tensor& x, int bf16, i64 b, i64 t, i64 h) {
+        const uint16_t* p = (const uint16_t*)x.data + ((b * x.batch + t * x.time + h * x.head) << (bf16 ? 0 : 1));
+        const uint32_t low = p[0], high = p[bf16 ? 0 : 1];
+        return __uint_as_float(bf16 ? low << 16 : high << 16 | low);
+    }
     __device__ __forceinline__ float log_decay(i64 b, i64 t, i64 h) const {
-        if (!decay.data) return 0.0f;
-        const float g = decay_bf16 ? to_float(*decay.at<bf16_t>(b, t, h)) : *decay.at<float>(b, t, h);
-        return g < LOWEST ? LOWEST : g;  // a NaN stays one
+        const float g = gate(decay.data ? decay : beta, decay.data ? decay_bf16 : beta_bf16, b, t, h);
+        return !decay.data ? 0.0f : g < LOWEST ? LOWEST : g;  // a NaN stays one
     }
-    __device__ __forceinline__ float rate(i64 b, i64 t, i64 h) const {
-        return beta_bf16 ? to_float(*beta.at<bf16_t>(b, t, h)) : *beta.at<float>(b, t, h);
-    }
+    __device__ __forceinline__ float rate(i64 b, i64 t, i64 h) const { return gate(beta, beta_bf16, b, t, h); }
 };
-
-// Four values from column c of a row of `width`, zeros beyond it.  No alignment is needed.
-template <typename T>
-__device__ __forceinline__ float4_t load4(const T* row, int c, int width) {
-    float4_t v;
-    if (c + 4 <= width) {
-        struct __attribute__((packed, aligned(sizeof(T)))) { T v[4]; } raw;
-        __builtin_memcpy(&raw, row + c, sizeof(raw));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = to_float(raw.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = c + i < width ? to_float(row[c + i]) : 0.0f;
-    }
-    return v;
-}
 
 // ------------------------------------------------------------------ token by token
 // A workgroup holds 32 columns of one head's state in registers: row groups of 32 / VEC lanes, each lane
@@ -311,48 +299,70 @@ __device__ __forceinline__ void put_half(bf16_t* p, i64 operand, int half, const
     for (int i = 0; i < N; ++i) *(bf16x4*)(p + ((operand * N + i) * 64 + l.id) * 8 + 4 * half) = v.p[i];
 }
 
-// Loads of the caller's tensors have no branches around them (a load behind a branch is waited for there):
-// they go to a row and column that exist, and what lies outside is replaced by zero afterwards.  Only
-// where a width is no multiple of 4 do four values come one by one.
+// Loads of the caller's tensors stand behind no branch (there each would be waited for before the next): they go
+// to a row and column that exist, and what lies outside is replaced by zero afterwards.
 __device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.time ? t : d.time - 1; }
 
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+// 32 columns of a row from column c0, as loaded and as an operand in the order above, zeros beyond the row's
+// width.  WIDE: rows of four values or more, read four at a time without alignment; where the row ends among
+// them its last four are read and shifted down.
+template <typename T, bool WIDE>
+struct Row {
+    struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
+    Four raw[2];
 
-template <typename T>
-__device__ __forceinline__ float4_t to_float4(const Four<T>& raw, bool live) {
-    float4_t v;
+    __device__ __forceinline__ void load(const T* row, int c0, int width, const Lane& l) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = live ? to_float(raw.v[e]) : 0.0f;
-    return v;
-}
+        for (int half = 0; half < 2; ++half) {
+            const int c = c0 + 16 * half + l.quad;
+            if constexpr (WIDE) {
+                raw[half] = *(const Four*)(row + min(c, width - 4));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raw[half].v[e] = row[min(c + e, width - 1)];
+            }
+        }
+    }
 
-// COUNT operands of 32 columns each from column c0 of a row, in the order above.
-template <typename T, int N, int COUNT>
-__device__ __forceinline__ void row_operands(Pieces<N> (&out)[COUNT], const T* row, int c0, int width, bool live, const Lane& l) {
-    float4_t v[COUNT][2];
-    if (width % 4 == 0) {
-        Four<T> raw[COUNT][2];
-#pragma unroll
-        for (int i = 0; i < COUNT; ++i)
+    template <int N>
+    __device__ __forceinline__ Pieces<N> operand(int c0, int width, bool live, const Lane& l) const {
+        if constexpr (WIDE && sizeof(T) == 2) {
+            uint64_t bits[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int c = c0 + 32 * i + 16 * half + l.quad;
-                raw[i][half] = *(const Four<T>*)(row + (c < width ? c : 0));
+                const int c = c0 + 16 * half + l.quad, gone = c - min(c, width - 4);
+                bits[half] = live && gone < 4 ? __builtin_bit_cast(uint64_t, raw[half]) >> (16 * gone) : 0;
             }
+            return Pieces<N>{{__builtin_bit_cast(bf16x8, bits)}};
+        } else {
+            float4_t v[2];
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i)
+            for (int half = 0; half < 2; ++half) {
+                const int c = c0 + 16 * half + l.quad, gone = WIDE ? c - min(c, width - 4) : 0;
+                float x[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) v[i][half] = to_float4(raw[i][half], live && c0 + 32 * i + 16 * half + l.quad < width);
-    } else {
+                for (int e = 0; e < 4; ++e) x[e] = to_float(raw[half].v[e]);
+                if constexpr (WIDE) {
+                    const bool one = gone & 1, two = gone & 2;
+                    x[0] = one ? x[1] : x[0], x[1] = one ? x[2] : x[1], x[2] = one ? x[3] : x[2];
+                    x[0] = two ? x[2] : x[0], x[1] = two ? x[3] : x[1];
+                }
 #pragma unroll
-        for (int i = 0; i < COUNT; ++i)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                v[i][half] = live ? load4(row, c0 + 32 * i + 16 * half + l.quad, width) : ZERO;
+                for (int e = 0; e < 4; ++e) v[half][e] = live && c + e < width ? x[e] : 0.0f;
+            }
+            return split<N>(v[0], v[1]);
+        }
     }
+};
+
+// COUNT operands of a row at once.
+template <typename T, bool WIDE, int N, int COUNT>
+__device__ __forceinline__ void row_operands(Pieces<N> (&out)[COUNT], const T* row, int c0, int width, bool live, const Lane& l) {
+    Row<T, WIDE> raw[COUNT];
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) out[i] = split<N>(v[i][0], v[i][1]);
+    for (int i = 0; i < COUNT; ++i) raw[i].load(row, c0 + 32 * i, width, l);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) out[i] = raw[i].template operand<N>(c0 + 32 * i, width, live, l);
 }
 
 // The values of four tokens from t0 in one column, as loaded and as floats.
@@ -395,11 +405,17 @@ __device__ __forceinline__ void put_block(float* m, i64 r, i64 c, i64 blocks, co
     *(float4_t*)(m + ((r * blocks + c) * 64 + l.id) * 4) = v;
 }
 
+// Keeps what stands before it before it.  A scan's loads return in the order of their issue, so one that the
+// scheduler moves behind others is waited for together with them.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 // Workgroup barrier for LDS alone: loads and stores of global memory stay in flight across it.
 __device__ __forceinline__ void lds_barrier() {
+    in_order();
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    in_order();
 }
 
 // A product with a triangular matrix adds zeros times the terms it masks, which a NaN or an infinity
@@ -436,7 +452,8 @@ __device__ __forceinline__ constexpr int upper(int i, int kb) { return i < 2 ? 2
 constexpr int TRIANGLE = 6;
 
 // A chunk's decays.  The running sums are taken in 64 bits, as differences of large sums lose what a
-// small decay adds, and kept as a float and its remainder.
+// small decay adds, and kept in powers of two as a float and its remainder: exp(G_i - G_j) is then one
+// hardware exp2 of an accurate difference.
 enum Gate { SUM, REMAINDER, SINCE, REST, RATE, WRITE, GATES };  // WRITE = REST RATE
 
 // The workspace: operands of chunk n of key head (b, hk) or value head (b, h), and what the scans leave.
@@ -458,7 +475,7 @@ struct Tape {
 };
 
 __device__ __forceinline__ float decay(const float* sum, const float* remainder, int i, int j) {
-    return expf((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
+    return __builtin_amdgcn_exp2f((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
 }
 
 // Pieces of what only the outputs see: bfloat16 outputs are rounded to 2^-9, so two (2^-16) do for them.
@@ -469,22 +486,30 @@ constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
 // One workgroup per chunk and key head: the keys (and, to train, queries) as operands, then for each
 // value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
 // pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.
-template <typename T, int DK>
+template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
     __shared__ __attribute__((aligned(16))) bf16_t rows[4 * KB * N * 512];
     __shared__ __attribute__((aligned(16))) float low[C * CP], inv[C * CP];
-    __shared__ float gates[GATES][C];
+    __shared__ __attribute__((aligned(16))) float gates[GATES][C];
     __shared__ int faulty;  // the first row with a NaN or an infinity; it and those after it become NaN
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
     const i64 shared = tape.shared_chunk(d, b, hk, n);
     const int wave = threadIdx.x / 64;
     const Lane l;
     bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
+    // the first wave's gates, a value head ahead
+    const i64 gate_time = n * C + l.id;
+    float next_decay = 0.0f, next_rate = 0.0f;
+    auto fetch_gates = [&](i64 h) {
+        next_decay = d.log_decay(b, existing(gate_time, d), h);
+        next_rate = d.rate(b, existing(gate_time, d), h);
+    };
+    fetch_gates(hk * d.group);
     const i64 t = n * C + 16 * wave + l.col;
     Pieces<N> own[KB], query[KB];
-    row_operands<T, N, KB>(own, d.k.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
-    row_operands<T, N, KB>(query, d.q.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
+    row_operands<T, WIDE, N, KB>(own, d.k.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
+    row_operands<T, WIDE, N, KB>(query, d.q.at<T>(b, existing(t, d), hk), 0, d.key, t < length, l);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
         put<N>(rows, wave * KB + kb, l, own[kb]);
@@ -510,7 +535,7 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
         }
     }
     __syncthreads();
-    float4_t kk[4], kq[4], qk[4];  // K K^T, K Q^T (whose blocks are operands of P) and Q K^T (of P^T)
+    float4_t kk[4], kq[4], qk[4];  // K K^T and K Q^T (rows are the earlier tokens: operands of P), Q K^T (of P^T)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         kk[j] = kq[j] = qk[j] = ZERO;
@@ -518,7 +543,7 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             const Pieces<N> other = fetch<N>(rows, j * KB + kb, l);
-            kk[j] = mma<N, N>(own[kb], other, kk[j]);
+            kk[j] = mma<N, N>(other, own[kb], kk[j]);
             kq[j] = mma<N, N>(other, query[kb], kq[j]);
             if (train) qk[j] = mma<N, N>(query[kb], other, qk[j]);
         }
@@ -529,8 +554,9 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
         if (threadIdx.x == 0) faulty = C;
         if (threadIdx.x < 64) {
             const int i = threadIdx.x;
-            const i64 at = n * C + i;
-            double g = at < length ? (double)d.log_decay(b, at, h) : 0.0;
+            double g = gate_time < length ? (double)next_decay * 1.4426950408889634 : 0.0;
+            const float own_rate = gate_time < length ? next_rate : 0.0f;
+            if (member + 1 < d.group) fetch_gates(h + 1);
 #pragma unroll
             for (int s = 1; s < 64; s *= 2) {
                 const double below = __shfl_up(g, s, 64);
@@ -540,9 +566,9 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
             float v[GATES];
             v[SUM] = (float)g;
             v[REMAINDER] = (float)(g - (double)v[SUM]);
-            v[SINCE] = expf((float)g);
-            v[REST] = expf((float)(last - g));
-            v[RATE] = at < length ? d.rate(b, at, h) : 0.0f;
+            v[SINCE] = __builtin_amdgcn_exp2f((float)g);
+            v[REST] = __builtin_amdgcn_exp2f((float)(last - g));
+            v[RATE] = own_rate;
             v[WRITE] = v[REST] * v[RATE];
 #pragma unroll
             for (int w = 0; w < GATES; ++w) {
@@ -552,30 +578,28 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
         }
         for (int e = threadIdx.x; e < C * CP; e += 256) inv[e] = 0.0f;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > wave) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 16 * wave + l.quad + e, c = 16 * j + l.col;
-                float v = r > c ? kk[j][e] * decay(gates[SUM], gates[REMAINDER], r, c) * gates[RATE][c] : 0.0f;
-                if (!(fabsf(v) < INFINITY)) {
-                    atomicMin(&faulty, r);
-                    v = 0.0f;
-                }
-                low[r * CP + c] = v;
-            }
-        }
         {
             float4_t p[4] = {ZERO, ZERO, ZERO, ZERO};
+            const int i = 16 * wave + l.col;
+            const float sum = gates[SUM][i], remainder = gates[REMAINDER][i];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j > wave) continue;
+                const int k0 = 16 * j + l.quad;
+                const float4_t sums = *(const float4_t*)(gates[SUM] + k0), remainders = *(const float4_t*)(gates[REMAINDER] + k0);
+                const float4_t rates = *(const float4_t*)(gates[RATE] + k0);
+                float4_t m;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 16 * wave + l.col, k = 16 * j + l.quad + e;
-                    p[j][e] = i >= k ? d.scale * kq[j][e] * decay(gates[SUM], gates[REMAINDER], i, k) : 0.0f;
+                    const float fade = __builtin_amdgcn_exp2f((sum - sums[e]) + (remainder - remainders[e]));
+                    p[j][e] = i >= k0 + e ? d.scale * kq[j][e] * fade : 0.0f;
+                    m[e] = i > k0 + e ? kk[j][e] * fade * rates[e] : 0.0f;
+                    if (!(fabsf(m[e]) < INFINITY)) {
+                        atomicMin(&faulty, i);
+                        m[e] = 0.0f;
+                    }
                 }
+                *(float4_t*)(low + i * CP + k0) = m;
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
@@ -660,11 +684,12 @@ __global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
     }
 }
 
-// ------------------------------------------------------------------ the states through the chunks
-// A workgroup carries 16 columns of one head's state, each of its DK / 32 waves 32 rows of them in registers.
-// A chunk takes three exchanges through LDS: the waves' partial sums of K S (each then adds those of its own
-// tokens), R for T R, and rest B E for the state.  What bounds it is that chain, so a chunk's operands are
-// fetched while the chunk before it runs.
+// ------------------------------------------------------------------ the states through the chunks, and the outputs
+// A workgroup carries 16 columns of one head's state.  Its first DK / 32 waves hold 32 rows of them each in
+// registers and take a chunk in three exchanges through LDS: their partial sums of K S (each then adds those
+// of its own tokens), R for T R, and rest B E for the state.  That chain bounds the scan, so a chunk's operands
+// are fetched while the chunk before it runs, and as many waves again take the outputs of the chunk before from
+// the states and errors that the first leave in LDS: in inference neither goes to memory.
 //
 // Workgroups of one head run on one XCD (they share its operands in the L2): workgroups go to the 8 XCDs
 // in turn, so head 8 k + x takes the workgroups with index % 8 = x.
@@ -676,28 +701,117 @@ struct Place {
     bool any;
     __device__ __forceinline__ Place(const Delta& d) {
         const int slices = (int)(d.padded / 16);
-        const i64 slot = blockIdx.x / XCDS, head = slot / slices * XCDS + blockIdx.x % XCDS;
-        column = (int)(slot % slices) * 16;
+        const int slot = (int)blockIdx.x / XCDS, head = slot / slices * XCDS + (int)blockIdx.x % XCDS;
+        column = slot % slices * 16;
         any = head < d.batch * d.value_heads;
-        b = head / d.value_heads;
-        h = head % d.value_heads;
+        b = head / (int)d.value_heads;
+        h = head % (int)d.value_heads;
     }
 };
 
-template <typename T, int DK>
-__global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float* __restrict__ final_state) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
+template <typename T, int DK, bool WIDE, bool TRAIN>
+__global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __restrict__ out, float* __restrict__ final_state) {
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
     __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
-    __shared__ int first[4][16];
+    // of two chunks in turn: S and B E as operands, and the first faulty row of each column
+    __shared__ __attribute__((aligned(16))) bf16_t held[2][WAVES * M * 512], errors[2][2 * M * 512];
+    __shared__ int first[4][16], blame[2][4][16];
     const Place at(d);
     if (!at.any) return;
     const i64 b = at.b, h = at.h, length = d.length(b);
-    const int wave = threadIdx.x / 64;
+    const int wave = threadIdx.x / 64 % WAVES;
     const Lane l;
     const int col = at.column + l.col;
     const bool live = col < d.value;
     const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+
+    if (threadIdx.x >= 64 * WAVES) {  // the outputs of tokens 16 OWN wave ..
+        Row<T, WIDE> q[OWN][WAVES];
+        Pieces<M> scores[OWN][2];
+        float4_t since[OWN];
+        // each is fetched for the next chunk as soon as this one's is used
+        const T* rows = d.q.at<T>(b, 0, h / d.group);
+        auto fetch_queries = [&](i64 n) {
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) {
+                const T* row = rows + existing(n * C + 16 * (wave * OWN + o) + l.col, d) * d.q.time;
+#pragma unroll
+                for (int kb = 0; kb < WAVES; ++kb) q[o][kb].load(row, 32 * kb, d.key, l);
+            }
+        };
+        auto fetch_scores = [&](i64 n) {
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) {
+                const int i = wave * OWN + o;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    scores[o][kb] = fetch<M>(tape.scores + (chunk0 + n) * (TRIANGLE * M * 512), lower(i, min(kb, i / 2)), l);
+                since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
+            }
+        };
+        // Chunk n, with `more` a part of it between each two barriers of chunk n + 1; `whole`: every token and column exists.
+        // Neither is asked within the loop, as a load or store behind a branch makes later waits wait for all before it.
+        auto chunk = [&](i64 n, auto more, auto whole) {
+            const int turn = (int)(n & 1);
+            float4_t acc[OWN][2];
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) acc[o][0] = acc[o][1] = ZERO;
+#pragma unroll
+            for (int kb = 0; kb < WAVES; ++kb) {
+                const Pieces<M> s = fetch<M>(held[turn], kb, l);
+#pragma unroll
+                for (int o = 0; o < OWN; ++o) acc[o][kb % 2] = mma<N, M>(q[o][kb].template operand<N>(32 * kb, d.key, true, l), s, acc[o][kb % 2]);
+            }
+            if constexpr (more()) {
+                fetch_queries(n + 1);
+                in_order();
+                lds_barrier();
+            }
+            const Pieces<M> e[2] = {fetch<M>(errors[turn], 0, l), fetch<M>(errors[turn], 1, l)};
+#pragma unroll
+            for (int o = 0; o < OWN; ++o) {
+                acc[o][0] = (acc[o][0] + acc[o][1]) * since[o] * d.scale;
+                acc[o][1] = ZERO;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    if (2 * kb <= wave * OWN + o) acc[o][kb] = mma<M, M>(scores[o][kb], e[kb], acc[o][kb]);
+                acc[o][0] += acc[o][1];
+            }
+            int fault = C;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) fault = min(fault, blame[turn][w][l.col]);
+            if constexpr (more()) {
+                fetch_scores(n + 1);
+                in_order();
+                lds_barrier();
+            }
+            T* to = out + ((b * d.time + n * C) * d.value_heads + h) * d.value + col;
+#pragma unroll
+            for (int o = 0; o < OWN; ++o)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = 16 * (wave * OWN + o) + l.quad + j;
+                    const i64 t = n * C + row;
+                    if (whole() || (t < d.time && live))
+                        to[row * d.value_heads * d.value] = from_float<T>(t >= length ? 0.0f : row < fault ? acc[o][0][j] : NAN);
+                }
+            if constexpr (more()) lds_barrier();
+        };
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        fetch_queries(0);
+        fetch_scores(0);
+        for (int i = 0; i < 3; ++i) lds_barrier();
+        const i64 last = d.chunks - 1;
+        if (at.column + 16 <= d.value)
+            for (i64 n = 0; n < last; ++n) chunk(n, yes, yes);
+        else
+            for (i64 n = 0; n < last; ++n) chunk(n, yes, no);
+        chunk(last, no, no);
+        return;
+    }
+
     const i64 base = (b * d.value_heads + h) * d.key * d.value + col;
     float4_t s[2];
 #pragma unroll
@@ -710,7 +824,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
     Pieces<N> k[4], kt[2][2];
     Pieces<3> inverse[OWN][2];
     Tokens<T> v[OWN];
-    float4_t since[OWN], write[OWN];
+    float4_t since[OWN], write[OWN], rate[OWN];
     float fade = 1.0f;
     auto fetch_keys = [&](i64 n) {
 #pragma unroll
@@ -722,9 +836,10 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
             const int i = wave * OWN + o;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb <= i) inverse[o][kb] = fetch<3>(tape.inverse + (chunk0 + n) * (TRIANGLE * 3 * 512), lower(i, kb), l);
+                inverse[o][kb] = fetch<3>(tape.inverse + (chunk0 + n) * (TRIANGLE * 3 * 512), lower(i, min(kb, i / 2)), l);
             since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
             write[o] = *(const float4_t*)(tape.gate(chunk0 + n, WRITE) + 16 * i + l.quad);
+            rate[o] = *(const float4_t*)(tape.gate(chunk0 + n, RATE) + 16 * i + l.quad);
             v[o].load(d, d.v, b, h, n * C + 16 * i + l.quad, col, d.value);
         }
     };
@@ -741,16 +856,24 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
     fetch_writes(0);
     for (i64 n = 0; n < d.chunks; ++n) {
         const i64 next = n + 1 < d.chunks ? n + 1 : n;
-#pragma unroll
-        for (int f = 0; f < 2; ++f) put_block(tape.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
+        const int turn = (int)(n & 1);
         const Pieces<3> state = split<3>(s[0], s[1]);
         float4_t sums[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[i], state, ZERO);
-        fetch_keys(next);
+        Pieces<M> shown;
+#pragma unroll
+        for (int i = 0; i < M; ++i) shown.p[i] = state.p[i];
+        put<M>(held[turn], wave, l, shown);
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
+        fetch_keys(next);
+        in_order();
+        if constexpr (TRAIN) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f) put_block(tape.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
+        }
         // R = V - g K S of the wave's own tokens
         float4_t r[OWN];
 #pragma unroll
@@ -768,6 +891,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
         fault = C;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) fault = min(fault, first[w][l.col]);
+        float4_t e[OWN];
 #pragma unroll
         for (int o = 0; o < OWN; ++o) {
             const int i = wave * OWN + o;
@@ -775,16 +899,22 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb <= i) mma2<3, 3>(inverse[o][kb], fetch<3>(seen, kb, l), large[kb], small[kb]);
-            float4_t e = (large[0] + large[1]) + (small[0] + small[1]);
+            e[o] = (large[0] + large[1]) + (small[0] + small[1]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = 16 * i + l.quad + j < fault ? e[j] : NAN;
-            put_half<3>(written, i / 2, i % 2, l, split<3>(e * write[o]));
-            put_block(tape.errors, (chunk0 + n) * 4 + i, at.column / 16, d.padded / 16, l, e);
+            for (int j = 0; j < 4; ++j) e[o][j] = 16 * i + l.quad + j < fault ? e[o][j] : NAN;
+            put_half<3>(written, i / 2, i % 2, l, split<3>(e[o] * write[o]));
+            if constexpr (TRAIN) put_block(tape.errors, (chunk0 + n) * 4 + i, at.column / 16, d.padded / 16, l, e[o]);
+            e[o] *= rate[o];
         }
-        fetch_tokens(next);
+        fault = take_faults(e, 16 * wave * OWN, l);
+        if (l.id < 16) blame[turn][wave][l.id] = fault;
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) put_half<M>(errors[turn], (wave * OWN + o) / 2, (wave * OWN + o) % 2, l, split<M>(e[o]));
 #pragma unroll
         for (int f = 0; f < 2; ++f) s[f] *= fade;
         lds_barrier();
+        fetch_tokens(next);
+        in_order();
         float4_t other[2] = {ZERO, ZERO};
         const Pieces<3> w[2] = {fetch<3>(written, 0, l), fetch<3>(written, 1, l)};
 #pragma unroll
@@ -792,6 +922,7 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
 #pragma unroll
         for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[f][1], w[1], other[f]);
         fetch_writes(next);
+        in_order();
     }
     if (!live) return;
 #pragma unroll
@@ -803,73 +934,6 @@ __global__ void __launch_bounds__(DK * 2) scan_forward(Delta d, Tape tape, float
         }
 }
 
-// ------------------------------------------------------------------ every chunk's outputs
-// Each wave takes every fourth block of 16 value columns for the chunk's 64 tokens; it reads the states and
-// errors, the most of the traffic, once, and fetches a block's while it works on the one before.
-template <typename T, int DK>
-__global__ void __launch_bounds__(256) outputs(Delta d, Tape tape, T* __restrict__ out) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
-    __shared__ __attribute__((aligned(16))) bf16_t queries[4 * KB * N * 512], scores[TRIANGLE * M * 512];
-    __shared__ __attribute__((aligned(16))) float gates[2][C];
-    const i64 n = blockIdx.x, h = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const i64 chunk = tape.chunk(d, b, h, n);
-    const int wave = threadIdx.x / 64, blocks = (int)(d.padded / 16);
-    const Lane l;
-    float4_t s[2 * KB], e[4];
-    auto fetch_block = [&](int c) {
-#pragma unroll
-        for (int r = 0; r < 2 * KB; ++r) s[r] = block(tape.states, chunk * (2 * KB) + r, c, blocks, l);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) e[r] = block(tape.errors, chunk * 4 + r, c, blocks, l);
-    };
-    if (wave < blocks) fetch_block(wave);
-    {
-        const i64 t = n * C + 16 * wave + l.col;
-        Pieces<N> own[KB];
-        row_operands<T, N, KB>(own, d.q.at<T>(b, existing(t, d), h / d.group), 0, d.key, t < length, l);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) put<N>(queries, wave * KB + kb, l, own[kb]);
-        for (int u = threadIdx.x; u < TRIANGLE * M * 64; u += 256)
-            *(bf16x8*)(scores + u * 8) = *(const bf16x8*)(tape.scores + chunk * (TRIANGLE * M * 512) + u * 8);
-        if (threadIdx.x < 2 * C) gates[wave][l.id] = tape.gate(chunk, wave ? RATE : SINCE)[l.id];
-    }
-    __syncthreads();
-    for (int c = wave; c < blocks; c += 4) {
-        float4_t w[4], acc[4] = {ZERO, ZERO, ZERO, ZERO};
-        Pieces<M> state[KB];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) state[kb] = split<M>(s[2 * kb], s[2 * kb + 1]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = e[j] * *(const float4_t*)(gates[1] + 16 * j + l.quad);
-        if (c + 4 < blocks) fetch_block(c + 4);
-        const int fault = take_faults(w, 0, l);
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = mma<N, M>(fetch<N>(queries, i * KB + kb, l), state[kb], acc[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= d.scale * *(const float4_t*)(gates[0] + 16 * i + l.quad);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const Pieces<M> error = split<M>(w[2 * kb], w[2 * kb + 1]);
-#pragma unroll
-            for (int i = 2 * kb; i < 4; ++i) acc[i] = mma<M, M>(fetch<M>(scores, lower(i, kb), l), error, acc[i]);
-        }
-        const int col = 16 * c + l.col;
-        if (col >= d.value) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = 16 * i + l.quad + j;
-                const i64 at = n * C + row;
-                if (at < d.time)
-                    out[((b * d.time + at) * d.value_heads + h) * d.value + col] =
-                        from_float<T>(at >= length ? 0.0f : row < fault ? acc[i][j] : NAN);
-            }
-    }
-}
-
 // ------------------------------------------------------------------ the states' gradients backwards
 struct Back {
     Tensor grad;              // of out
@@ -878,22 +942,96 @@ struct Back {
     float *states;            // dS' of every chunk
 };
 
-// As scan_forward, from the last chunk to the first: the waves' partial sums of K dS', then B dV' for
-// T^T B dV', then Y for the state's gradient.
+// As scan_forward, from the last chunk to the first: the first waves' partial sums of K dS', then B dV' for
+// T^T B dV', then Y for the state's gradient.  What needs no state, P^T dO and scale Q^T g dO, the other waves
+// leave in LDS a chunk ahead.
 template <typename T, int DK>
-__global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back back, T* __restrict__ dv,
-                                                        float* __restrict__ dstate) {
+__global__ void __launch_bounds__(DK * 4) scan_backward(Delta d, Tape tape, Back back, float* __restrict__ dstate) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
     __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
+    __shared__ __attribute__((aligned(16))) float direct[2][4][64][4], reads[2][DK / 16][64][4];  // of two chunks in turn
     const Place at(d);
     if (!at.any) return;
     const i64 b = at.b, h = at.h, length = d.length(b);
-    const int wave = threadIdx.x / 64;
+    const int wave = threadIdx.x / 64 % WAVES;
     const Lane l;
     const int col = at.column + l.col;
     const bool live = col < d.value;
     const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+
+    if (threadIdx.x >= 64 * WAVES) {
+        Tokens<T> go[4];
+        float4_t since[4];
+        Pieces<N> qt[2][2];
+        Pieces<3> scores[OWN][2];
+        auto fetch_grads = [&](i64 n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) go[i].load(d, back.grad, b, h, n * C + 16 * i + l.quad, col, d.value);
+        };
+        auto fetch_scores = [&](i64 n) {
+#pragma unroll
+            for (int w = 0; w < OWN; ++w)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    scores[w][kb] = fetch<3>(tape.scores_t + (chunk0 + n) * (TRIANGLE * 3 * 512),
+                                             upper(wave * OWN + w, max(kb, (wave * OWN + w) / 2)), l);
+        };
+        auto fetch_queries = [&](i64 n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) since[i] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    qt[f][kb] = fetch<N>(tape.queries_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
+        };
+        fetch_grads(d.chunks - 1);
+        fetch_scores(d.chunks - 1);
+        fetch_queries(d.chunks - 1);
+        // chunk n, but for the last chunk while the first waves are at n + 1
+        auto chunk = [&](i64 n, auto beside) {
+            const int turn = (int)(n & 1);
+            const i64 next = n > 0 ? n - 1 : 0;
+            float4_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = go[i].floats(n * C + 16 * i + l.quad, length, live);
+            fetch_grads(next);
+            in_order();
+            const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
+#pragma unroll
+            for (int w = 0; w < OWN; ++w) {
+                float4_t acc[2] = {ZERO, ZERO};
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    if (2 * kb + 1 >= wave * OWN + w) acc[kb] = mma<3, N>(scores[w][kb], grads[kb], acc[kb]);
+                *(float4_t*)direct[turn][wave * OWN + w][l.id] = acc[0] + acc[1];
+            }
+            fetch_scores(next);
+            in_order();
+            if constexpr (beside()) lds_barrier();
+            float4_t acc[2] = {ZERO, ZERO};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const Pieces<3> g = split<3>(o[2 * kb] * since[2 * kb] * d.scale, o[2 * kb + 1] * since[2 * kb + 1] * d.scale);
+#pragma unroll
+                for (int f = 0; f < 2; ++f) acc[f] = mma<N, 3>(qt[f][kb], g, acc[f]);
+            }
+            fetch_queries(next);
+            in_order();
+            if constexpr (beside()) lds_barrier();
+#pragma unroll
+            for (int f = 0; f < 2; ++f) *(float4_t*)reads[turn][2 * wave + f][l.id] = acc[f];
+            lds_barrier();
+        };
+        chunk(d.chunks - 1, std::false_type{});
+        for (i64 n = d.chunks - 1; n-- > 0;) chunk(n, std::true_type{});
+        lds_barrier();  // those of chunk 0
+        lds_barrier();
+        lds_barrier();
+        return;
+    }
+
     const i64 base = (b * d.value_heads + h) * d.key * d.value + col;
     float4_t s[2];
 #pragma unroll
@@ -903,10 +1041,9 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
             const int r = 32 * wave + 16 * f + l.quad + e;
             s[f][e] = back.grad_state && r < d.key && live ? back.grad_state[base + (i64)r * d.value] : 0.0f;
         }
-    Pieces<N> k[4], kt[2][2], qt[2][2];
-    Pieces<3> inverse[OWN][2], scores[OWN][2];
-    Tokens<T> go[4];
-    float4_t all_since[4], since[OWN], rest[OWN], rate[OWN];
+    Pieces<N> k[4], kt[2][2];
+    Pieces<3> inverse[OWN][2];
+    float4_t since[OWN], rest[OWN], rate[OWN];
     float fade = 1.0f;
     auto fetch_keys = [&](i64 n) {
 #pragma unroll
@@ -918,10 +1055,7 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
             const int i = wave * OWN + w;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb + 1 >= i) {
-                    inverse[w][kb] = fetch<3>(tape.inverse_t + (chunk0 + n) * (TRIANGLE * 3 * 512), upper(i, kb), l);
-                    scores[w][kb] = fetch<3>(tape.scores_t + (chunk0 + n) * (TRIANGLE * 3 * 512), upper(i, kb), l);
-                }
+                inverse[w][kb] = fetch<3>(tape.inverse_t + (chunk0 + n) * (TRIANGLE * 3 * 512), upper(i, max(kb, i / 2)), l);
             since[w] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
             rest[w] = *(const float4_t*)(tape.gate(chunk0 + n, REST) + 16 * i + l.quad);
             rate[w] = *(const float4_t*)(tape.gate(chunk0 + n, RATE) + 16 * i + l.quad);
@@ -932,52 +1066,37 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+            for (int kb = 0; kb < 2; ++kb)
                 kt[f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
-                qt[f][kb] = fetch<N>(tape.queries_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            all_since[i] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
-            go[i].load(d, back.grad, b, h, n * C + 16 * i + l.quad, col, d.value);
-        }
     };
     fetch_keys(d.chunks - 1);
     fetch_tokens(d.chunks - 1);
     fetch_writes(d.chunks - 1);
+    lds_barrier();  // the last chunk's P^T dO and Q^T g dO
     for (i64 n = d.chunks; n-- > 0;) {
         const i64 next = n > 0 ? n - 1 : 0;
-#pragma unroll
-        for (int f = 0; f < 2; ++f) put_block(back.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
-        // what does not need the state: P^T dO of the wave's own tokens
-        float4_t o[4], direct[OWN];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = go[i].floats(n * C + 16 * i + l.quad, length, live);
-        const Pieces<N> grads[2] = {split<N>(o[0], o[1]), split<N>(o[2], o[3])};
-#pragma unroll
-        for (int w = 0; w < OWN; ++w) {
-            direct[w] = ZERO;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb + 1 >= wave * OWN + w) direct[w] = mma<3, N>(scores[w][kb], grads[kb], direct[w]);
-        }
+        const int turn = (int)(n & 1);
         const Pieces<3> state = split<3>(s[0], s[1]);
         float4_t sums[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[i], state, ZERO);
-        fetch_keys(next);
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
+        fetch_keys(next);
+        in_order();
+#pragma unroll
+        for (int f = 0; f < 2; ++f) put_block(back.states, (chunk0 + n) * (DK / 16) + 2 * wave + f, at.column / 16, d.padded / 16, l, s[f]);
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
             const int i = wave * OWN + w;
             float4_t sum = *(const float4_t*)part[0][i][l.id];
 #pragma unroll
             for (int from = 1; from < WAVES; ++from) sum += *(const float4_t*)part[from][i][l.id];
-            put_half<3>(seen, i / 2, i % 2, l, split<3>((direct[w] + sum * rest[w]) * rate[w]));
+            put_half<3>(seen, i / 2, i % 2, l, split<3>((*(const float4_t*)direct[turn][i][l.id] + sum * rest[w]) * rate[w]));
         }
         lds_barrier();
+        float4_t y[OWN];
 #pragma unroll
         for (int w = 0; w < OWN; ++w) {
             const int i = wave * OWN + w;
@@ -985,28 +1104,14 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
                 if (2 * kb + 1 >= i) mma2<3, 3>(inverse[w][kb], fetch<3>(seen, kb, l), large[kb], small[kb]);
-            const float4_t y = (large[0] + large[1]) + (small[0] + small[1]);
-            put_half<3>(written, i / 2, i % 2, l, split<3>(y * -since[w]));
-            put_block(back.residuals, (chunk0 + n) * 4 + i, at.column / 16, d.padded / 16, l, y);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const i64 t = n * C + 16 * i + l.quad + e;
-                if (t < d.time && live)
-                    dv[((b * d.time + t) * d.value_heads + h) * d.value + col] = from_float<T>(t < length ? y[e] : 0.0f);
-            }
+            y[w] = (large[0] + large[1]) + (small[0] + small[1]);
+            put_half<3>(written, i / 2, i % 2, l, split<3>(y[w] * -since[w]));
         }
-        fetch_tokens(next);
-        Pieces<3> reads[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-            reads[kb] = split<3>(o[2 * kb] * all_since[2 * kb] * d.scale, o[2 * kb + 1] * all_since[2 * kb + 1] * d.scale);
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            s[f] *= fade;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) s[f] = mma<N, 3>(qt[f][kb], reads[kb], s[f]);
-        }
+        for (int f = 0; f < 2; ++f) s[f] = s[f] * fade + *(const float4_t*)reads[turn][2 * wave + f][l.id];
         lds_barrier();
+        fetch_tokens(next);
+        in_order();
         float4_t other[2] = {ZERO, ZERO};
         const Pieces<3> w[2] = {fetch<3>(written, 0, l), fetch<3>(written, 1, l)};
 #pragma unroll
@@ -1014,6 +1119,9 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 #pragma unroll
         for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[f][1], w[1], other[f]);
         fetch_writes(next);
+        in_order();
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) put_block(back.residuals, (chunk0 + n) * 4 + wave * OWN + o, at.column / 16, d.padded / 16, l, y[o]);
     }
     if (!dstate || !live) return;
 #pragma unroll
@@ -1034,9 +1142,9 @@ __global__ void __launch_bounds__(DK * 2) scan_backward(Delta d, Tape tape, Back
 // One workgroup per chunk and key head; it visits the value heads that share the key head one after the
 // other, so their sums into dq and dk need no atomics.  Eight waves: wave w holds the tokens 16 (w % 4) ..
 // of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
-template <typename T, int DK>
+template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
-                                                 void* __restrict__ ddecay, void* __restrict__ dbeta) {
+                                                 T* __restrict__ dv, void* __restrict__ ddecay, void* __restrict__ dbeta) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, F = DK / 32;
     constexpr int STATES = DK / 16 * 3 * 512, TOKENS = 4 * 3 * 512;
     // S, dS', E and Y of 32 columns; afterwards D1 and D2
@@ -1088,7 +1196,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
         // a stage's blocks: DK / 32 x 2 pairs of S and of dS', 2 x 2 of E and of Y
         constexpr int UNITS = DK / 16;
         float4_t sv[2], gv[2], tv[2];
-        Pieces<N> next[1];
+        Row<T, WIDE> next;
         auto fetch_stage = [&](int c) {
             const int u = wave % UNITS, r = u / 2 * 2;
             const float* tokens = (wave < 4 ? tape.errors : back.residuals);
@@ -1099,7 +1207,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
                 gv[i] = block(back.states, chunk * (DK / 16) + r + i, c + u % 2, columns, l);
                 tv[i] = block(tokens, chunk * 4 + q + i, c + v % 2, columns, l);
             }
-            row_operands<T, N, 1>(next, grad, 16 * c, d.value, t < length, l);
+            next.load(grad, 16 * c, d.value, l);
         };
         fetch_stage(0);
         for (int c = 0; c < columns; c += 2) {
@@ -1112,7 +1220,20 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
                 carried += (dot[0] + dot[1]) + (dot[2] + dot[3]);
             }
             turn(wave < 4 ? e_stage : y_stage, wave % 4 / 2, wave % 2, tv[0], tv[1]);
-            const Pieces<N> o = next[0];
+            if (wave >= 4) {  // Y is the gradient of v
+                const int col = (c + wave % 2) * 16 + l.col;
+                if (col < d.value) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const i64 at = n * C + 16 * (wave % 4 / 2 * 2 + i) + l.quad + e;
+                            if (at < d.time)
+                                dv[((b * d.time + at) * d.value_heads + h) * d.value + col] = from_float<T>(at < length ? tv[i][e] : 0.0f);
+                        }
+                }
+            }
+            const Pieces<N> o = next.template operand<N>(16 * c, d.value, t < length, l);
             if (c + 2 < columns) fetch_stage(c + 2);
             __syncthreads();
             const Pieces<3> y = fetch<3>(y_stage, tb, l), e = fetch<3>(e_stage, tb, l);
@@ -1281,7 +1402,7 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
 
 int key_width(const Delta& d) { return d.key <= 64 ? 64 : 128; }
 
-// Carves the workspace (256-byte pieces); the operands of the backward pass only to train.
+// Carves the workspace (256-byte pieces); what only the backward pass reads is there only to train.
 i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
     const i64 chunks = d.batch * d.value_heads * d.chunks, shared = d.batch * d.heads * d.chunks;
     const i64 pieces = type == ATLAS_OPS_BF16 ? 1 : 3;
@@ -1299,20 +1420,22 @@ i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
     take(t.inverse_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.scores_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.gates, chunks * GATES * C * 4);
-    take(t.errors, chunks * C * d.padded * 4);
-    take(t.states, chunks * key_width(d) * d.padded * 4);
+    take(t.errors, chunks * C * d.padded * 4, train);
+    take(t.states, chunks * key_width(d) * d.padded * 4, train);
     if (tape) *tape = t;
     return at;
 }
 
+// Calls f with the element type, the key width's instantiation and whether rows of `width` are wide ones.
 template <typename F>
-void with_kernel(const Delta& d, int type, F&& f) {
-    auto by_width = [&](auto t) {
-        if (key_width(d) == 64) f(t, std::integral_constant<int, 64>{});
-        else f(t, std::integral_constant<int, 128>{});
+void with_kernel(const Delta& d, int type, int width, F&& f) {
+    auto by_width = [&](auto t, auto wide) {
+        if (key_width(d) == 64) f(t, std::integral_constant<int, 64>{}, wide);
+        else f(t, std::integral_constant<int, 128>{}, wide);
     };
-    if (type == ATLAS_OPS_F32) by_width(0.0f);
-    else by_width(bf16_t{});
+    auto by_rows = [&](auto t) { width >= 4 ? by_width(t, std::true_type{}) : by_width(t, std::false_type{}); };
+    if (type == ATLAS_OPS_F32) by_rows(0.0f);
+    else by_rows(bf16_t{});
 }
 
 // Workgroups of a scan: 16 columns each, whole groups of 8 heads (Place).
@@ -1363,13 +1486,12 @@ int atlas_ops_delta_forward(const AtlasDelta* a, int train, void* out, float* fi
         Tape tape;
         carve(d, a->type, train, (char*)workspace, &tape);
         hipStream_t st = (hipStream_t)stream;
-        const dim3 all((unsigned)d.chunks, (unsigned)d.value_heads, (unsigned)d.batch);
         const dim3 keys((unsigned)d.chunks, (unsigned)d.heads, (unsigned)d.batch);
-        with_kernel(d, a->type, [&](auto t, auto width) {
+        with_kernel(d, a->type, d.key, [&](auto t, auto width, auto wide) {
             using T = decltype(t);
-            prepare<T, width()><<<keys, 256, 0, st>>>(d, tape, train);
-            scan_forward<T, width()><<<scan_grid(d), 2 * width(), 0, st>>>(d, tape, final_state);
-            outputs<T, width()><<<all, 256, 0, st>>>(d, tape, (T*)out);
+            prepare<T, width(), wide()><<<keys, 256, 0, st>>>(d, tape, train);
+            if (train) scan_forward<T, width(), wide(), true><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
+            else scan_forward<T, width(), wide(), false><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
         });
         return launched(err, cap, "delta_forward");
     } catch (...) {
@@ -1399,10 +1521,10 @@ int atlas_ops_delta_backward(const AtlasDelta* a, const void* tape_memory, const
                         floats + d.batch * d.value_heads * d.chunks * C * d.padded};
         hipStream_t st = (hipStream_t)stream;
         const dim3 all((unsigned)d.chunks, (unsigned)d.heads, (unsigned)d.batch);
-        with_kernel(d, a->type, [&](auto t, auto width) {
+        with_kernel(d, a->type, d.value, [&](auto t, auto width, auto wide) {
             using T = decltype(t);
-            scan_backward<T, width()><<<scan_grid(d), 2 * width(), 0, st>>>(d, tape, back, (T*)dv, dstate);
-            gradients<T, width()><<<all, 512, 0, st>>>(d, tape, back, (T*)dq, (T*)dk, dlog_decay, dbeta);
+            scan_backward<T, width()><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, back, dstate);
+            gradients<T, width(), wide()><<<all, 512, 0, st>>>(d, tape, back, (T*)dq, (T*)dk, (T*)dv, dlog_decay, dbeta);
         });
         return launched(err, cap, "delta_backward");
     } catch (...) {

@@ -46,11 +46,17 @@ __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ bf16_t from_float<bf16_t>(float v) { return __builtin_bit_cast(bf16_t, (__bf16)v); }
 
-// Sum over groups of LANES neighbouring lanes (a power of two up to 64); every lane gets it.
+// Sum over groups of LANES neighbouring lanes (16, 32 or 64); every lane gets it.  Within 16 lanes the values
+// rotate in the adder's own operand (DPP); only the steps beyond go through the LDS crossbar.
 template <int LANES>
 __device__ __forceinline__ float lane_sum(float v) {
+    static_assert(LANES == 16 || LANES == 32 || LANES == 64, "whole rows of 16 lanes");
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x124, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x122, 0xF, 0xF, false));
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x121, 0xF, 0xF, false));
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+    for (int d = 16; d < LANES; d *= 2) v += __shfl_xor(v, d, 64);
     return v;
 }
 
