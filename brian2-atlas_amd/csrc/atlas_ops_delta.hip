@@ -487,7 +487,7 @@ constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
 // value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
 // pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(256) prepare(Delta d, Tape tape, int train) {
+__global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
     __shared__ __attribute__((aligned(16))) bf16_t rows[4 * KB * N * 512];
     __shared__ __attribute__((aligned(16))) float low[C * CP], inv[C * CP];
@@ -710,7 +710,7 @@ struct Place {
 };
 
 template <typename T, int DK, bool WIDE, bool TRAIN>
-__global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __restrict__ out, float* __restrict__ final_state) {
+__global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T* __restrict__ out, float* __restrict__ final_state) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
     __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
@@ -821,14 +821,18 @@ __global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __
             const int r = 32 * wave + 16 * f + l.quad + e;
             s[f][e] = d.state && r < d.key && live ? d.state[base + (i64)r * d.value] : 0.0f;
         }
-    Pieces<N> k[4], kt[2][2];
+    // Chunks ahead that keys are fetched, or, where the operands of one chunk alone fill the registers, each of them
+    // only after those of the product before it are used (TIGHT).
+    constexpr bool TIGHT = DK == 64 && N == 3;
+    constexpr int DEPTH = DK == 128 && N == 1 ? 2 : 1;
+    Pieces<N> k[DEPTH][4], kt[DEPTH][2][2];
     Pieces<3> inverse[OWN][2];
     Tokens<T> v[OWN];
     float4_t since[OWN], write[OWN], rate[OWN];
-    float fade = 1.0f;
-    auto fetch_keys = [&](i64 n) {
+    float fade[DEPTH];
+    auto fetch_keys = [&](i64 n, int to) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = fetch<N>(tape.keys + (shared0 + n) * (4 * WAVES * N * 512), i * WAVES + wave, l);
+        for (int i = 0; i < 4; ++i) k[to][i] = fetch<N>(tape.keys + (shared0 + n) * (4 * WAVES * N * 512), i * WAVES + wave, l);
     };
     auto fetch_tokens = [&](i64 n) {
 #pragma unroll
@@ -843,24 +847,28 @@ __global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __
             v[o].load(d, d.v, b, h, n * C + 16 * i + l.quad, col, d.value);
         }
     };
-    auto fetch_writes = [&](i64 n) {
-        fade = tape.gate(chunk0 + n, SINCE)[C - 1];
+    auto fetch_writes = [&](i64 n, int to) {
+        fade[to] = tape.gate(chunk0 + n, SINCE)[C - 1];
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                kt[f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
+                kt[to][f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
     };
-    fetch_keys(0);
+    const i64 last = d.chunks - 1;
+#pragma unroll
+    for (int ahead = 0; ahead < DEPTH; ++ahead) {
+        fetch_keys(min((i64)ahead, last), ahead);
+        if constexpr (!TIGHT) fetch_writes(min((i64)ahead, last), ahead);
+    }
     fetch_tokens(0);
-    fetch_writes(0);
-    for (i64 n = 0; n < d.chunks; ++n) {
-        const i64 next = n + 1 < d.chunks ? n + 1 : n;
+    auto chunk = [&](i64 n, auto slot) {
+        const i64 next = min(n + 1, last), later = min(n + DEPTH, last);
         const int turn = (int)(n & 1);
         const Pieces<3> state = split<3>(s[0], s[1]);
         float4_t sums[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[i], state, ZERO);
+        for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[slot()][i], state, ZERO);
         Pieces<M> shown;
 #pragma unroll
         for (int i = 0; i < M; ++i) shown.p[i] = state.p[i];
@@ -868,7 +876,8 @@ __global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
-        fetch_keys(next);
+        if constexpr (TIGHT) fetch_writes(n, slot());
+        else fetch_keys(later, slot());
         in_order();
         if constexpr (TRAIN) {
 #pragma unroll
@@ -911,18 +920,32 @@ __global__ void __launch_bounds__(DK * 4) scan_forward(Delta d, Tape tape, T* __
 #pragma unroll
         for (int o = 0; o < OWN; ++o) put_half<M>(errors[turn], (wave * OWN + o) / 2, (wave * OWN + o) % 2, l, split<M>(e[o]));
 #pragma unroll
-        for (int f = 0; f < 2; ++f) s[f] *= fade;
+        for (int f = 0; f < 2; ++f) s[f] *= fade[slot()];
+        if constexpr (TIGHT) {
+            in_order();
+            fetch_keys(next, slot());
+        }
         lds_barrier();
-        fetch_tokens(next);
+        if constexpr (!TIGHT) fetch_tokens(next);
         in_order();
         float4_t other[2] = {ZERO, ZERO};
         const Pieces<3> w[2] = {fetch<3>(written, 0, l), fetch<3>(written, 1, l)};
 #pragma unroll
-        for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[f][0], w[0], s[f]);
+        for (int f = 0; f < 2; ++f) s[f] = mma<N, 3>(kt[slot()][f][0], w[0], s[f]);
 #pragma unroll
-        for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[f][1], w[1], other[f]);
-        fetch_writes(next);
+        for (int f = 0; f < 2; ++f) s[f] += mma<N, 3>(kt[slot()][f][1], w[1], other[f]);
+        if constexpr (TIGHT) fetch_tokens(next);
+        else fetch_writes(later, slot());
         in_order();
+    };
+    if constexpr (DEPTH == 2) {
+        for (i64 n = 0; n < last; n += 2) {
+            chunk(n, std::integral_constant<int, 0>{});
+            chunk(n + 1, std::integral_constant<int, 1>{});
+        }
+        if (last % 2 == 0) chunk(last, std::integral_constant<int, 0>{});
+    } else {
+        for (i64 n = 0; n <= last; ++n) chunk(n, std::integral_constant<int, 0>{});
     }
     if (!live) return;
 #pragma unroll
@@ -946,7 +969,7 @@ struct Back {
 // T^T B dV', then Y for the state's gradient.  What needs no state, P^T dO and scale Q^T g dO, the other waves
 // leave in LDS a chunk ahead.
 template <typename T, int DK>
-__global__ void __launch_bounds__(DK * 4) scan_backward(Delta d, Tape tape, Back back, float* __restrict__ dstate) {
+__global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, Back back, float* __restrict__ dstate) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
     __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
@@ -1143,7 +1166,7 @@ __global__ void __launch_bounds__(DK * 4) scan_backward(Delta d, Tape tape, Back
 // other, so their sums into dq and dk need no atomics.  Eight waves: wave w holds the tokens 16 (w % 4) ..
 // of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
+__global__ void __launch_bounds__(512, 2) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
                                                  T* __restrict__ dv, void* __restrict__ ddecay, void* __restrict__ dbeta) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, F = DK / 32;
     constexpr int STATES = DK / 16 * 3 * 512, TOKENS = 4 * 3 * 512;
@@ -1151,11 +1174,14 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
     __shared__ __attribute__((aligned(16))) bf16_t stage[2 * STATES + 2 * TOKENS];
     __shared__ __attribute__((aligned(16))) float gates[GATES][C];
     __shared__ float lines[2][2][C], part[8];
+    // dq and dk of the value heads so far, each wave's own blocks
+    __shared__ __attribute__((aligned(16))) float sums[DK == 64 ? 1 : 2][DK == 64 ? 4 : 8 * F * 64 * 4];
+    float4_t gq[F], gk[F];
     bf16_t *s_stage = stage, *g_stage = stage + STATES, *e_stage = stage + 2 * STATES, *y_stage = e_stage + TOKENS;
     float *d1 = (float*)stage, *d2 = d1 + C * CP;
     static_assert(2 * C * CP * sizeof(float) <= sizeof(stage), "D1 and D2 take the stage's place");
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
-    const int wave = threadIdx.x / 64, tb = wave % 4, half = wave / 4, token = 16 * tb, key0 = half * F;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), tb = wave % 4, half = wave / 4, token = 16 * tb, key0 = half * F;
     const int columns = (int)(d.padded / 16);
     const Lane l;
     const i64 shared = tape.shared_chunk(d, b, hk, n);
@@ -1180,9 +1206,6 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             put_half<3>(to, 2 * pair + which, c, l, turned);
         }
     };
-    float4_t gq[F], gk[F];
-#pragma unroll
-    for (int f = 0; f < F; ++f) gq[f] = gk[f] = ZERO;
     for (int member = 0; member < d.group; ++member) {
         const i64 h = hk * d.group + member, chunk = tape.chunk(d, b, h, n);
         float4_t reads[F], backs[F], writes[F], pairs[4];  // dO S^T, Y S^T, E dS'^T, dO E^T or Y E^T
@@ -1209,9 +1232,12 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             }
             next.load(grad, 16 * c, d.value, l);
         };
-        fetch_stage(0);
+        float gate = 0.0f;
+        if (threadIdx.x < GATES * C) gate = tape.gates[chunk * GATES * C + threadIdx.x];
         for (int c = 0; c < columns; c += 2) {
+            fetch_stage(c);
             __syncthreads();  // the stage before is read
+            if (c == 0 && threadIdx.x < GATES * C) gates[threadIdx.x / C][threadIdx.x % C] = gate;
             if (wave < UNITS) {
                 const int u = wave;
                 turn(s_stage, u / 2, u % 2, sv[0], sv[1]);
@@ -1234,7 +1260,6 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
                 }
             }
             const Pieces<N> o = next.template operand<N>(16 * c, d.value, t < length, l);
-            if (c + 2 < columns) fetch_stage(c + 2);
             __syncthreads();
             const Pieces<3> y = fetch<3>(y_stage, tb, l), e = fetch<3>(e_stage, tb, l);
 #pragma unroll
@@ -1243,15 +1268,16 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
                 reads[f] = mma<N, 3>(o, s, reads[f]);
                 backs[f] = mma<3, 3>(y, s, backs[f]);
                 writes[f] = mma<3, 3>(e, fetch<3>(g_stage, key0 + f, l), writes[f]);
+                in_order();
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j > tb) continue;
                 const Pieces<3> other = fetch<3>(e_stage, j, l);
                 pairs[j] = half ? mma<3, 3>(y, other, pairs[j]) : mma<N, 3>(o, other, pairs[j]);
+                in_order();
             }
         }
-        for (int u = threadIdx.x; u < GATES * C; u += 512) gates[u / C][u % C] = tape.gates[chunk * GATES * C + u];
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1282,7 +1308,7 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             writes[f] *= rest;
             written += own(keys_t, f) * writes[f] * rate;
         }
-#pragma unroll
+#pragma unroll 1
         for (int kb = 0; kb < 2; ++kb) {
             if (2 * kb <= tb) {  // sums over the tokens up to the wave's
                 Pieces<3> a[2];
@@ -1319,8 +1345,39 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             const float4_t k = own(keys_t, f), q = own(queries_t, f);
             db += k * writes[f];
             dg += q * reads[f] + k * backs[f];
-            gq[f] += reads[f];
-            gk[f] += backs[f] + rate * writes[f];
+            backs[f] += rate * writes[f];
+        }
+        if (d.group > 1) {
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                float4_t* sum[2];
+                if constexpr (DK == 64) {
+                    sum[0] = &gq[f];
+                    sum[1] = &gk[f];
+                } else {
+                    sum[0] = (float4_t*)sums[0] + (wave * F + f) * 64 + l.id;
+                    sum[1] = (float4_t*)sums[1] + (wave * F + f) * 64 + l.id;
+                }
+                if (member > 0) {
+                    reads[f] += *sum[0];
+                    backs[f] += *sum[1];
+                }
+                *sum[0] = reads[f];
+                *sum[1] = backs[f];
+            }
+        }
+        if (member + 1 == d.group) {
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const i64 at = n * C + token + l.quad + e;
+                    const int c = 16 * (key0 + f) + l.col;
+                    if (at >= d.time || c >= d.key) continue;
+                    const i64 to = ((b * d.time + at) * d.heads + hk) * d.key + c;
+                    dq[to] = from_float<T>(at < length ? reads[f][e] : 0.0f);
+                    dk[to] = from_float<T>(at < length ? backs[f][e] : 0.0f);
+                }
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1354,17 +1411,6 @@ __global__ void __launch_bounds__(512) gradients(Delta d, Tape tape, Back back, 
             }
         }
     }
-#pragma unroll
-    for (int f = 0; f < F; ++f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const i64 t = n * C + token + l.quad + e;
-            const int c = 16 * (key0 + f) + l.col;
-            if (t >= d.time || c >= d.key) continue;
-            const i64 to = ((b * d.time + t) * d.heads + hk) * d.key + c;
-            dq[to] = from_float<T>(t < length ? gq[f][e] : 0.0f);
-            dk[to] = from_float<T>(t < length ? gk[f][e] : 0.0f);
-        }
 }
 
 // ------------------------------------------------------------------ host
