@@ -58,16 +58,25 @@ struct Delta {
         return n < 0 ? 0 : n < time ? n : time;
     }
     // A gate of either type, with loads that stand behind no branch.
-    __device__ static __forceinline__ float gate(const Tensor& x, int bf16, i64 b, i64 t, i64 h) {
+    struct Gate { uint32_t low, high; };
+    __device__ static __forceinline__ Gate load(const Tensor& x, int bf16, i64 b, i64 t, i64 h) {
         const uint16_t* p = (const uint16_t*)x.data + ((b * x.batch + t * x.time + h * x.head) << (bf16 ? 0 : 1));
-        const uint32_t low = p[0], high = p[bf16 ? 0 : 1];
-        return __uint_as_float(bf16 ? low << 16 : high << 16 | low);
+        return {p[0], p[bf16 ? 0 : 1]};
     }
-    __device__ __forceinline__ float log_decay(i64 b, i64 t, i64 h) const {
-        const float g = gate(decay.data ? decay : beta, decay.data ? decay_bf16 : beta_bf16, b, t, h);
+    __device__ static __forceinline__ float value_of(Gate g, int bf16) {
+        return __uint_as_float(bf16 ? g.low << 16 : g.high << 16 | g.low);
+    }
+    __device__ __forceinline__ Gate load_decay(i64 b, i64 t, i64 h) const {
+        return load(decay.data ? decay : beta, decay.data ? decay_bf16 : beta_bf16, b, t, h);
+    }
+    __device__ __forceinline__ Gate load_rate(i64 b, i64 t, i64 h) const { return load(beta, beta_bf16, b, t, h); }
+    __device__ __forceinline__ float log_decay(Gate x) const {
+        const float g = value_of(x, decay_bf16);
         return !decay.data ? 0.0f : g < LOWEST ? LOWEST : g;  // a NaN stays one
     }
-    __device__ __forceinline__ float rate(i64 b, i64 t, i64 h) const { return gate(beta, beta_bf16, b, t, h); }
+    __device__ __forceinline__ float rate(Gate x) const { return value_of(x, beta_bf16); }
+    __device__ __forceinline__ float log_decay(i64 b, i64 t, i64 h) const { return log_decay(load_decay(b, t, h)); }
+    __device__ __forceinline__ float rate(i64 b, i64 t, i64 h) const { return rate(load_rate(b, t, h)); }
 };
 
 // ------------------------------------------------------------------ token by token
@@ -84,22 +93,40 @@ __global__ void __launch_bounds__(256) step_kernel(Delta d, T* __restrict__ out,
     const i64 b = blockIdx.z, h = blockIdx.y, hk = h / d.group;
     const int col = blockIdx.x * 32 + lane * VEC;
     const i64 base = (b * d.value_heads + h) * d.key * d.value;
+    // Nothing is loaded behind a branch, or each load would be waited for before the next: rows and columns that
+    // do not exist read the last, and their values become zeros.
+    T kt[PER], qt[PER], vt[VEC];
+    Delta::Gate decay, beta;
+    auto fetch = [&](i64 t) {
+        const T *qp = d.q.at<T>(b, t, hk), *kp = d.k.at<T>(b, t, hk), *vp = d.v.at<T>(b, t, h);
+        decay = d.load_decay(b, t, h), beta = d.load_rate(b, t, h);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) vt[c] = vp[min(col + c, (int)d.value - 1)];
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+            const int at = min(row + r * ROWS, d.key - 1);
+            kt[r] = kp[at];
+            qt[r] = qp[at];
+        }
+    };
     float s[PER][VEC];
+    const float* from = (d.state ? d.state : final_state) + base + min(col, (int)d.value - VEC);
 #pragma unroll
     for (int r = 0; r < PER; ++r) {
-        const int at = row + r * ROWS;
+        const float* p = from + (i64)min(row + r * ROWS, d.key - 1) * d.value;
+        if constexpr (VEC == 4) {  // value is a multiple of 4
+            const float4_t v = *(const float4_t*)p;
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) s[r][c] = 0.0f;
-        if (d.state && at < d.key && col < d.value) {
-            if constexpr (VEC == 4) {  // value is a multiple of 4
-                const float4_t v = *(const float4_t*)(d.state + base + (i64)at * d.value + col);
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) s[r][c] = v[c];
-            } else {
-                s[r][0] = d.state[base + (i64)at * d.value + col];
-            }
+            for (int c = 0; c < VEC; ++c) s[r][c] = v[c];
+        } else {
+            s[r][0] = *p;
         }
     }
+    fetch(0);
+#pragma unroll
+    for (int r = 0; r < PER; ++r)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) s[r][c] = d.state && row + r * ROWS < d.key && col < d.value ? s[r][c] : 0.0f;
     const i64 length = d.length(b);
     for (i64 t = 0; t < d.time; ++t) {
         T* o = out + ((b * d.time + t) * d.value_heads + h) * d.value;
@@ -109,20 +136,20 @@ __global__ void __launch_bounds__(256) step_kernel(Delta d, T* __restrict__ out,
                     if (col + c < d.value) o[col + c] = from_float<T>(0.0f);
             continue;
         }
-        const T *qp = d.q.at<T>(b, t, hk), *kp = d.k.at<T>(b, t, hk), *vp = d.v.at<T>(b, t, h);
-        const float a = expf(d.log_decay(b, t, h)), rate = d.rate(b, t, h);
+        const float a = expf(d.log_decay(decay)), rate = d.rate(beta);
         float v[VEC];
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) v[c] = col + c < d.value ? to_float(vp[col + c]) : 0.0f;
+        for (int c = 0; c < VEC; ++c) v[c] = col + c < d.value ? to_float(vt[c]) : 0.0f;
         float kr[PER], qr[PER], ks[VEC], qs[VEC], kq = 0.0f;
 #pragma unroll
         for (int c = 0; c < VEC; ++c) ks[c] = qs[c] = 0.0f;
 #pragma unroll
         for (int r = 0; r < PER; ++r) {
             const int at = row + r * ROWS;
-            kr[r] = at < d.key ? to_float(kp[at]) : 0.0f;
-            qr[r] = at < d.key ? to_float(qp[at]) : 0.0f;
+            kr[r] = at < d.key ? to_float(kt[r]) : 0.0f;
+            qr[r] = at < d.key ? to_float(qt[r]) : 0.0f;
         }
+        if (t + 1 < length) fetch(t + 1);
 #pragma unroll
         for (int r = 0; r < PER; ++r) {
             kq += kr[r] * qr[r];
