@@ -356,8 +356,11 @@ def delta_rule_step(q, k, v, log_decay, beta, state, *, scale: float | None = No
     return out
 
 
-# Sequences up to this length without a tape run token by token in one launch.
-SHORT = 16
+# Sequences up to this length without a tape run token by token in one launch: a token costs what the longest of
+# them takes alike, while the chunks' two kernels cost the same from one token to 64.  Measured against chunks, with
+# 16 heads of 128 x 128 in bfloat16: 16 sequences of 8 tokens 26 us to 48, of 16 tokens 46 to 48; one sequence
+# of 8 heads 16 us to 19 and 27 to 20; 256 sequences of 4 heads of 64 x 64 43 us to 59 and 80 to 59.
+SHORT = 12
 
 
 class DeltaTape:
