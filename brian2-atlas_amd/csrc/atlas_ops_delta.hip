@@ -485,7 +485,8 @@ enum Gate { SUM, REMAINDER, SINCE, REST, RATE, WRITE, GATES };  // WRITE = REST 
 
 // The workspace: operands of chunk n of key head (b, hk) or value head (b, h), and what the scans leave.
 struct Tape {
-    bf16_t *keys, *keys_t, *queries_t;       // rows are tokens; rows are key indices, sums over tokens
+    bf16_t *keys, *queries;                  // rows are tokens
+    bf16_t *keys_t, *queries_t;              // rows are key indices, sums over tokens
     bf16_t *inverse, *scores;                // T and P
     bf16_t *inverse_t, *scores_t;            // T^T and P^T
     float *gates, *errors, *states;          // E and S in blocks
@@ -524,7 +525,7 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
     const i64 shared = tape.shared_chunk(d, b, hk, n);
     const int wave = threadIdx.x / 64;
     const Lane l;
-    bf16_t* keys = tape.keys + shared * (4 * KB * N * 512);
+    bf16_t *keys = tape.keys + shared * (4 * KB * N * 512), *queries = tape.queries + shared * (4 * KB * N * 512);
     // the first wave's gates, a value head ahead
     const i64 gate_time = n * C + l.id;
     float next_decay = 0.0f, next_rate = 0.0f;
@@ -541,6 +542,7 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
     for (int kb = 0; kb < KB; ++kb) {
         put<N>(rows, wave * KB + kb, l, own[kb]);
         put<N>(keys, wave * KB + kb, l, own[kb]);
+        put<N>(queries, wave * KB + kb, l, query[kb]);
     }
     for (int what = 0; what < 1 + (train != 0); ++what) {
         const Tensor& x = what ? d.q : d.k;
@@ -736,7 +738,7 @@ struct Place {
     }
 };
 
-template <typename T, int DK, bool WIDE, bool TRAIN>
+template <typename T, int DK, bool TRAIN>
 __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T* __restrict__ out, float* __restrict__ final_state) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
@@ -754,18 +756,16 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
     const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
 
     if (threadIdx.x >= 64 * WAVES) {  // the outputs of tokens 16 OWN wave ..
-        Row<T, WIDE> q[OWN][WAVES];
+        Pieces<N> q[OWN][WAVES];
         Pieces<M> scores[OWN][2];
         float4_t since[OWN];
         // each is fetched for the next chunk as soon as this one's is used
-        const T* rows = d.q.at<T>(b, 0, h / d.group);
         auto fetch_queries = [&](i64 n) {
 #pragma unroll
-            for (int o = 0; o < OWN; ++o) {
-                const T* row = rows + existing(n * C + 16 * (wave * OWN + o) + l.col, d) * d.q.time;
+            for (int o = 0; o < OWN; ++o)
 #pragma unroll
-                for (int kb = 0; kb < WAVES; ++kb) q[o][kb].load(row, 32 * kb, d.key, l);
-            }
+                for (int kb = 0; kb < WAVES; ++kb)
+                    q[o][kb] = fetch<N>(tape.queries + (shared0 + n) * (4 * WAVES * N * 512), (wave * OWN + o) * WAVES + kb, l);
         };
         auto fetch_scores = [&](i64 n) {
 #pragma unroll
@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
             for (int kb = 0; kb < WAVES; ++kb) {
                 const Pieces<M> s = fetch<M>(held[turn], kb, l);
 #pragma unroll
-                for (int o = 0; o < OWN; ++o) acc[o][kb % 2] = mma<N, M>(q[o][kb].template operand<N>(32 * kb, d.key, true, l), s, acc[o][kb % 2]);
+                for (int o = 0; o < OWN; ++o) acc[o][kb % 2] = mma<N, M>(q[o][kb], s, acc[o][kb % 2]);
             }
             if constexpr (more()) {
                 fetch_queries(n + 1);
@@ -1486,6 +1486,7 @@ i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
     };
     Tape t{};
     take(t.keys, shared * C * key_width(d) * pieces * 2);
+    take(t.queries, shared * C * key_width(d) * pieces * 2);
     take(t.keys_t, shared * C * key_width(d) * pieces * 2);
     take(t.queries_t, shared * C * key_width(d) * pieces * 2, train);
     take(t.inverse, chunks * TRIANGLE * 3 * 1024);
@@ -1563,8 +1564,8 @@ int atlas_ops_delta_forward(const AtlasDelta* a, int train, void* out, float* fi
         with_kernel(d, a->type, d.key, [&](auto t, auto width, auto wide) {
             using T = decltype(t);
             prepare<T, width(), wide()><<<keys, 256, 0, st>>>(d, tape, train);
-            if (train) scan_forward<T, width(), wide(), true><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
-            else scan_forward<T, width(), wide(), false><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
+            if (train) scan_forward<T, width(), true><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
+            else scan_forward<T, width(), false><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
         });
         return launched(err, cap, "delta_forward");
     } catch (...) {
