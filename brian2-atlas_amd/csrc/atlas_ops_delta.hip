@@ -82,7 +82,8 @@ struct Delta {
 // ------------------------------------------------------------------ token by token
 // A workgroup holds 32 columns of one head's state in registers: row groups of 32 / VEC lanes, each lane
 // VEC neighbouring columns of every 8 VEC-th row.  One reduction per token: S^T k and S^T q of the
-// decayed state and k . q, as out = scale ((a S)^T q + beta e (k . q)).
+// decayed state and k . q, as out = scale ((a S)^T q + beta e (k . q)).  Memory bounds one token: the state is read
+// and written once, 64 x 8 heads of 128 x 128 in 13.4 us, 5.0 TB/s.  More tokens follow one another at 2 to 9 us each.
 constexpr int MAX_KEY = 128;
 
 template <typename T, int VEC>
@@ -332,7 +333,8 @@ __device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.ti
 
 // 32 columns of a row from column c0, as loaded and as an operand in the order above, zeros beyond the row's
 // width.  WIDE: rows of four values or more, read four at a time without alignment; where the row ends among
-// them its last four are read and shifted down.
+// them its last four are read and shifted down (prepare, 16384 tokens of 16 heads of 128: 98 us, a value at a time
+// 166; gradients, 2 x 4099: 337 and 356).
 template <typename T, bool WIDE>
 struct Row {
     struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
@@ -513,7 +515,10 @@ constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
 // ------------------------------------------------------------------ operands and T = (I + M B)^-1
 // One workgroup per chunk and key head: the keys (and, to train, queries) as operands, then for each
 // value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
-// pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.
+// pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.  Its steps wait for one another, so what counts is
+// how many workgroups a CU holds: 168 registers, three of them with bfloat16 (2 x 4099 tokens of 4 x 4 heads of
+// 128: 59 us with three, 82 with two; 16384 of 16 heads 114 us), two by their LDS with float32 (256 x 100 of 4 heads
+// of 64: 104 us).
 template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
@@ -720,6 +725,13 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
 // are fetched while the chunk before it runs, and as many waves again take the outputs of the chunk before from
 // the states and errors that the first leave in LDS: in inference neither goes to memory.
 //
+// Measured: 16384 tokens of 16 heads of 128, bfloat16, 256 chunks one after the other, 482 us or 1.9 us a chunk (a
+// kernel of its own for the outputs: 440 and 178 us, and the states written).  The three exchanges, their MFMA latencies
+// and the splits between them make 1.5 us of that; the rest is operands that arrive late and what the outputs take
+// of the load path (with queries loaded from the caller's rows, 8 bytes a lane, 577 us; a value at a time, 1207).
+// 256 x 100 of 4 heads of 64, float32: 160 us for 4096 workgroups of two chunks, bound by the operands that every 16
+// columns read anew from the L2.
+//
 // Workgroups of one head run on one XCD (they share its operands in the L2): workgroups go to the 8 XCDs
 // in turn, so head 8 k + x takes the workgroups with index % 8 = x.
 constexpr int XCDS = 8;
@@ -777,7 +789,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
                 since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
             }
         };
-        // Chunk n, with `more` a part of it between each two barriers of chunk n + 1; `whole`: every token and column exists.
+        // Chunk n, with `more` a part of it between each two barriers of chunk n + 1; `whole`: all tokens and columns exist.
         // Neither is asked within the loop, as a load or store behind a branch makes later waits wait for all before it.
         auto chunk = [&](i64 n, auto more, auto whole) {
             const int turn = (int)(n & 1);
@@ -848,8 +860,9 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
             const int r = 32 * wave + 16 * f + l.quad + e;
             s[f][e] = d.state && r < d.key && live ? d.state[base + (i64)r * d.value] : 0.0f;
         }
-    // Chunks ahead that keys are fetched, or, where the operands of one chunk alone fill the registers, each of them
-    // only after those of the product before it are used (TIGHT).
+    // Chunks ahead that keys are fetched (16384 tokens of 16 heads: 577 us with two, 641 with one); where
+    // the operands of one chunk alone fill the registers, each is fetched only after those of the product
+    // before it are used (TIGHT; 256 x 100 of 4 heads of 64, float32: 163 us, two workgroups per CU with spills 226).
     constexpr bool TIGHT = DK == 64 && N == 3;
     constexpr int DEPTH = DK == 128 && N == 1 ? 2 : 1;
     Pieces<N> k[DEPTH][4], kt[DEPTH][2][2];
@@ -994,7 +1007,9 @@ struct Back {
 
 // As scan_forward, from the last chunk to the first: the first waves' partial sums of K dS', then B dV' for
 // T^T B dV', then Y for the state's gradient.  What needs no state, P^T dO and scale Q^T g dO, the other waves
-// leave in LDS a chunk ahead.
+// leave in LDS a chunk ahead.  2 x 4099 of 16 heads of 128, bfloat16: 193 us, 2.9 us a chunk (262 with one set of waves
+// for both); fetching its keys two chunks ahead, as forwards, gains nothing here.  256 x 100 of 4 heads of 64,
+// float32: 124 us with two workgroups per CU (254 registers), 160 with one.
 template <typename T, int DK>
 __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, Back back, float* __restrict__ dstate) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
@@ -1192,6 +1207,11 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
 // One workgroup per chunk and key head; it visits the value heads that share the key head one after the
 // other, so their sums into dq and dk need no atomics.  Eight waves: wave w holds the tokens 16 (w % 4) ..
 // of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
+//
+// Bound by its chain of stages (loads, turns, barrier, products) with one workgroup per CU: 2 x 4099 of 4 x 4 heads of
+// 128, bfloat16, 343 us, about 270 TFLOP/s of MFMA, a quarter of the rate; 256 x 100 of 4 heads of 64, float32,
+// 165 us.  Fetching a stage ahead costs more in registers than it hides (365 and 203 us), and so does half the
+// registers for twice the workgroups where keys are 64 wide (285 us).
 template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(512, 2) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,
                                                  T* __restrict__ dv, void* __restrict__ ddecay, void* __restrict__ dbeta) {
@@ -1473,6 +1493,7 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
     return 0;
 }
 
+// Keys up to 64 take operands of half the width: 256 x 100 of 4 heads of 64, float32, 545 us, and 894 with those of 128.
 int key_width(const Delta& d) { return d.key <= 64 ? 64 : 128; }
 
 // Carves the workspace (256-byte pieces); what only the backward pass reads is there only to train.
@@ -1531,7 +1552,8 @@ int atlas_ops_delta_step(const AtlasDelta* a, void* out, float* final_state, voi
         if (!out || !final_state) return fail(err, cap, 7, "null argument");
         const dim3 grid((unsigned)ceil_div(d.value, 32), (unsigned)d.value_heads, (unsigned)d.batch);
         hipStream_t st = (hipStream_t)stream;
-        // 16-byte accesses of the state need its rows to start on 16 bytes
+        // 16-byte accesses of the state need its rows to start on 16 bytes (64 x 8 heads of 128 x 128: 13.3 us, with
+        // 4-byte ones 15.7)
         const bool wide = d.value % 4 == 0 && ((uintptr_t)d.state | (uintptr_t)final_state) % 16 == 0;
         if (a->type == ATLAS_OPS_F32) {
             if (wide) step_kernel<float, 4><<<grid, 256, 0, st>>>(d, (float*)out, final_state);
