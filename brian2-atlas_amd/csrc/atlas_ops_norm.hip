@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(256) norm_forward_long(Rows x, int width, cons
 // registers allow it (32768 x 4096 bfloat16: 298 us with two of 187 registers, 239 with three of 168;
 // four would spill, 667).  Now 224 us there, 3.6 TB/s of the two reads and the write; 25600 x 256 float32 18.1.
 template <typename T, typename W, int LANES, int CH>
-__global__ void __launch_bounds__(256, CH <= 2 ? 3 : CH == 4 ? 2 : 1) norm_backward(Rows grad, Rows x, i64 rows, int width,
+__global__ void __launch_bounds__(256, CH <= 2 ? 3 : 2) norm_backward(Rows grad, Rows x, i64 rows, int width,
                                                      const W* __restrict__ weight, const float* __restrict__ mean_in,
                                                      const float* __restrict__ rstd_in, T* __restrict__ dx,
                                                      float* __restrict__ partial) {
@@ -433,31 +433,35 @@ __global__ void __launch_bounds__(1024) norm_reduce(i64 blocks, i64 width, const
     }
 }
 
-// The layout of a row by its width: 16 lanes up to 16 units (16 rows per workgroup), a wave up to
-// 4 units per lane, a workgroup up to 4 (bfloat16) or 8 (float32) units per lane, else the long kernels.
+// The layout of a row by its units of 16 bytes.  16 lanes up to 16 units, 16 rows per workgroup (262144 x 64 float32:
+// forward 24 us, backward 41, and 79, 108 with a wave each).  A wave up to 4 units per lane forward (32768 x 2048
+// bfloat16 69 us, a workgroup 84), up to 2 backward, where a row's registers are twice as many (a workgroup 146 us,
+// a wave 209).  A workgroup up to 4 per lane, backward of bfloat16 up to 2: the registers of more cost the workgroups that hide
+// the loads, and reading the rows again from the caches is faster (4 against long: 8192 x 4096 float32 60 to 62 and 152
+// to 164 us; 8192 x 8192 bfloat16 71 to 79 and 314 to 228; 8 against long: 4096 x 8192 float32 99 to 77 and 213 to 168).
 struct Shape {
     int lanes, chunks;  // chunks 0: long rows
 };
 
-Shape shape_of(i64 width, int type) {
+Shape shape_of(i64 width, int type, bool backward) {
     const i64 units = ceil_div(width, type == ATLAS_OPS_F32 ? 4 : 8);
     if (units <= 16) return {16, 1};
     for (int c : {1, 2, 4})
-        if (units <= 64 * c) return {64, c};
-    for (int c : {2, 4, 8})
-        if (units <= 256 * c && (c < 8 || type == ATLAS_OPS_F32)) return {256, c};
+        if (units <= 64 * c && !(backward && c == 4)) return {64, c};
+    for (int c : {2, 4})
+        if (units <= 256 * c && !(backward && c == 4 && type == ATLAS_OPS_BF16)) return {256, c};
     return {256, 0};
 }
 
-template <typename T, typename F>
+template <typename T, bool BACKWARD, typename F>
 void with_shape(Shape s, F&& f) {
     if (s.lanes == 16) f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
     else if (s.lanes == 64 && s.chunks == 1) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
     else if (s.lanes == 64 && s.chunks == 2) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (s.lanes == 64) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
-    else if (s.chunks == 2) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else if (s.chunks == 4) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-    else if constexpr (sizeof(T) == 4) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+    else if (s.lanes == 64) {
+        if constexpr (!BACKWARD) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+    } else if (s.chunks == 2) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else if constexpr (!BACKWARD || sizeof(T) == 4) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
 }
 
 template <typename F>
@@ -474,7 +478,7 @@ constexpr i64 FORWARD_BLOCKS = 1024, BACKWARD_BLOCKS = 768;
 
 // Blocks of the backward pass's rows; the partials stay a small share of the traffic.
 i64 row_blocks(i64 rows, i64 width, int type) {
-    const Shape s = shape_of(width, type);
+    const Shape s = shape_of(width, type, true);
     if (s.chunks == 0) return std::min<i64>(rows, 64);
     return std::min<i64>(ceil_div(rows, 256 / s.lanes), BACKWARD_BLOCKS);
 }
@@ -504,7 +508,7 @@ int atlas_ops_layer_norm(const AtlasRows* x, int64_t rows, int64_t width, int ty
         if (int rc = check(x, rows, width, type, weight_type, err, cap)) return rc;
         if (!rows) return 0;
         if (!y || (mean == nullptr) != (rstd == nullptr)) return fail(err, cap, 7, "null output");
-        const Shape shape = shape_of(width, type);
+        const Shape shape = shape_of(width, type, false);
         const Rows in{x->data, x->inner, x->outer_stride, x->inner_stride};
         with_types(type, weight_type, [&](auto t, auto w) {
             using T = decltype(t);
@@ -514,7 +518,7 @@ int atlas_ops_layer_norm(const AtlasRows* x, int64_t rows, int64_t width, int ty
                     in, (int)width, (const W*)weight, (const W*)bias, eps, (T*)y, mean, rstd);
                 return;
             }
-            with_shape<T>(shape, [&](auto lanes, auto chunks) {
+            with_shape<T, false>(shape, [&](auto lanes, auto chunks) {
                 norm_forward<T, W, lanes(), chunks()>
                     <<<dim3((unsigned)std::min<i64>(ceil_div(rows, 256 / lanes()), FORWARD_BLOCKS)), 256, 0, (hipStream_t)stream>>>(
                         in, rows, (int)width, (const W*)weight, (const W*)bias, eps, (T*)y, mean, rstd);
@@ -529,7 +533,7 @@ int atlas_ops_layer_norm(const AtlasRows* x, int64_t rows, int64_t width, int ty
 int64_t atlas_ops_layer_norm_workspace(int64_t rows, int64_t width, int type) {
     if (rows < 1 || width < 1 || !known_type(type)) return 0;
     // the partial sums, and of long rows what their means left out
-    return (2 * row_blocks(rows, width, type) * width + (shape_of(width, type).chunks ? 0 : rows)) * (i64)sizeof(float);
+    return (2 * row_blocks(rows, width, type) * width + (shape_of(width, type, true).chunks ? 0 : rows)) * (i64)sizeof(float);
 }
 
 int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int64_t rows, int64_t width, int type,
@@ -546,7 +550,7 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
             using T = decltype(t);
             using W = decltype(w);
             if (rows) {
-                const Shape shape = shape_of(width, type);
+                const Shape shape = shape_of(width, type, true);
                 const Rows in{x->data, x->inner, x->outer_stride, x->inner_stride};
                 const Rows g{grad->data, grad->inner, grad->outer_stride, grad->inner_stride};
                 if (shape.chunks == 0) {
@@ -557,7 +561,7 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
                         norm_columns<T><<<dim3((unsigned)ceil_div(width, 256), (unsigned)blocks), 256, 0, st>>>(
                             g, in, rows, (int)width, mean, rstd, workspace + 2 * blocks * width, workspace);
                 } else {
-                    with_shape<T>(shape, [&](auto lanes, auto chunks) {
+                    with_shape<T, true>(shape, [&](auto lanes, auto chunks) {
                         const size_t lds = lanes() < 256 ? 256 * chunks() * Unit<T>::N * sizeof(float) : 0;
                         norm_backward<T, W, lanes(), chunks()><<<dim3((unsigned)blocks), 256, lds, st>>>(
                             g, in, rows, (int)width, (const W*)weight, mean, rstd, (T*)dx, sums ? workspace : nullptr);
