@@ -860,7 +860,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
             const int r = 32 * wave + 16 * f + l.quad + e;
             s[f][e] = d.state && r < d.key && live ? d.state[base + (i64)r * d.value] : 0.0f;
         }
-    // Chunks ahead that keys are fetched (16384 tokens of 16 heads: 577 us with two, 641 with one); where
+    // Chunks ahead that keys are fetched (16384 tokens of 16 heads: two take 65 us less than one); where
     // the operands of one chunk alone fill the registers, each is fetched only after those of the product
     // before it are used (TIGHT; 256 x 100 of 4 heads of 64, float32: 163 us, two workgroups per CU with spills 226).
     constexpr bool TIGHT = DK == 64 && N == 3;
