@@ -508,10 +508,6 @@ __device__ __forceinline__ float decay(const float* sum, const float* remainder,
     return __builtin_amdgcn_exp2f((sum[i] - sum[j]) + (remainder[i] - remainder[j]));
 }
 
-// Pieces of what only the outputs see: bfloat16 outputs are rounded to 2^-9, so two (2^-16) do for them.
-template <typename T>
-constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
-
 // ------------------------------------------------------------------ operands and T = (I + M B)^-1
 // One workgroup per chunk and key head: the keys (and, to train, queries) as operands, then for each
 // value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
@@ -521,7 +517,7 @@ constexpr int OUTPUT_PIECES = sizeof(T) == 2 ? 2 : 3;
 // of 64: 104 us).
 template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, KB = DK / 32;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, KB = DK / 32;
     __shared__ __attribute__((aligned(16))) bf16_t rows[4 * KB * N * 512];
     __shared__ __attribute__((aligned(16))) float low[C * CP], inv[C * CP];
     __shared__ __attribute__((aligned(16))) float gates[GATES][C];
@@ -637,7 +633,7 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                if (2 * kb <= wave) put<M>(tape.scores + chunk * (TRIANGLE * M * 512), lower(wave, kb), l, split<M>(p[2 * kb], p[2 * kb + 1]));
+                if (2 * kb <= wave) put<3>(tape.scores + chunk * (TRIANGLE * 3 * 512), lower(wave, kb), l, split<3>(p[2 * kb], p[2 * kb + 1]));
         }
         if (train) {
 #pragma unroll
@@ -752,11 +748,11 @@ struct Place {
 
 template <typename T, int DK, bool TRAIN>
 __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T* __restrict__ out, float* __restrict__ final_state) {
-    constexpr int N = sizeof(T) == 2 ? 1 : 3, M = OUTPUT_PIECES<T>, WAVES = DK / 32, OWN = 4 / WAVES;
+    constexpr int N = sizeof(T) == 2 ? 1 : 3, WAVES = DK / 32, OWN = 4 / WAVES;
     __shared__ __attribute__((aligned(16))) float part[WAVES][4][64][4];
     __shared__ __attribute__((aligned(16))) bf16_t seen[2 * 3 * 512], written[2 * 3 * 512];
     // of two chunks in turn: S and B E as operands, and the first faulty row of each column
-    __shared__ __attribute__((aligned(16))) bf16_t held[2][WAVES * M * 512], errors[2][2 * M * 512];
+    __shared__ __attribute__((aligned(16))) bf16_t held[2][WAVES * 3 * 512], errors[2][2 * 3 * 512];
     __shared__ int first[4][16], blame[2][4][16];
     const Place at(d);
     if (!at.any) return;
@@ -769,7 +765,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
 
     if (threadIdx.x >= 64 * WAVES) {  // the outputs of tokens 16 OWN wave ..
         Pieces<N> q[OWN][WAVES];
-        Pieces<M> scores[OWN][2];
+        Pieces<3> scores[OWN][2];
         float4_t since[OWN];
         // each is fetched for the next chunk as soon as this one's is used
         auto fetch_queries = [&](i64 n) {
@@ -785,7 +781,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
                 const int i = wave * OWN + o;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
-                    scores[o][kb] = fetch<M>(tape.scores + (chunk0 + n) * (TRIANGLE * M * 512), lower(i, min(kb, i / 2)), l);
+                    scores[o][kb] = fetch<3>(tape.scores + (chunk0 + n) * (TRIANGLE * 3 * 512), lower(i, min(kb, i / 2)), l);
                 since[o] = *(const float4_t*)(tape.gate(chunk0 + n, SINCE) + 16 * i + l.quad);
             }
         };
@@ -798,23 +794,23 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
             for (int o = 0; o < OWN; ++o) acc[o][0] = acc[o][1] = ZERO;
 #pragma unroll
             for (int kb = 0; kb < WAVES; ++kb) {
-                const Pieces<M> s = fetch<M>(held[turn], kb, l);
+                const Pieces<3> s = fetch<3>(held[turn], kb, l);
 #pragma unroll
-                for (int o = 0; o < OWN; ++o) acc[o][kb % 2] = mma<N, M>(q[o][kb], s, acc[o][kb % 2]);
+                for (int o = 0; o < OWN; ++o) acc[o][kb % 2] = mma<N, 3>(q[o][kb], s, acc[o][kb % 2]);
             }
             if constexpr (more()) {
                 fetch_queries(n + 1);
                 in_order();
                 lds_barrier();
             }
-            const Pieces<M> e[2] = {fetch<M>(errors[turn], 0, l), fetch<M>(errors[turn], 1, l)};
+            const Pieces<3> e[2] = {fetch<3>(errors[turn], 0, l), fetch<3>(errors[turn], 1, l)};
 #pragma unroll
             for (int o = 0; o < OWN; ++o) {
                 acc[o][0] = (acc[o][0] + acc[o][1]) * since[o] * d.scale;
                 acc[o][1] = ZERO;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
-                    if (2 * kb <= wave * OWN + o) acc[o][kb] = mma<M, M>(scores[o][kb], e[kb], acc[o][kb]);
+                    if (2 * kb <= wave * OWN + o) acc[o][kb] = mma<3, 3>(scores[o][kb], e[kb], acc[o][kb]);
                 acc[o][0] += acc[o][1];
             }
             int fault = C;
@@ -909,10 +905,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
         float4_t sums[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] = mma<N, 3>(k[slot()][i], state, ZERO);
-        Pieces<M> shown;
-#pragma unroll
-        for (int i = 0; i < M; ++i) shown.p[i] = state.p[i];
-        put<M>(held[turn], wave, l, shown);
+        put<3>(held[turn], wave, l, state);
 #pragma unroll
         for (int i = 0; i < 4; ++i) *(float4_t*)part[wave][i][l.id] = sums[i];
         lds_barrier();
@@ -958,7 +951,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
         fault = take_faults(e, 16 * wave * OWN, l);
         if (l.id < 16) blame[turn][wave][l.id] = fault;
 #pragma unroll
-        for (int o = 0; o < OWN; ++o) put_half<M>(errors[turn], (wave * OWN + o) / 2, (wave * OWN + o) % 2, l, split<M>(e[o]));
+        for (int o = 0; o < OWN; ++o) put_half<3>(errors[turn], (wave * OWN + o) / 2, (wave * OWN + o) % 2, l, split<3>(e[o]));
 #pragma unroll
         for (int f = 0; f < 2; ++f) s[f] *= fade[slot()];
         if constexpr (TIGHT) {
@@ -1511,7 +1504,7 @@ i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
     take(t.keys_t, shared * C * key_width(d) * pieces * 2);
     take(t.queries_t, shared * C * key_width(d) * pieces * 2, train);
     take(t.inverse, chunks * TRIANGLE * 3 * 1024);
-    take(t.scores, chunks * TRIANGLE * (type == ATLAS_OPS_BF16 ? 2 : 3) * 1024);
+    take(t.scores, chunks * TRIANGLE * 3 * 1024);
     take(t.inverse_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.scores_t, chunks * TRIANGLE * 3 * 1024, train);
     take(t.gates, chunks * GATES * C * 4);
