@@ -57,6 +57,9 @@ struct Delta {
         const i64 n = lengths[b];
         return n < 0 ? 0 : n < time ? n : time;
     }
+    // A sequence's chunks with a token.  No kernel visits the others: there a product of zeros would turn a NaN or an
+    // infinity of the state, which they leave as it is, into NaNs of its column.
+    __device__ __forceinline__ i64 used_chunks(i64 b) const { return (length(b) + C - 1) / C; }
     // A gate of either type, with loads that stand behind no branch.
     struct Gate { uint32_t low, high; };
     __device__ static __forceinline__ Gate load(const Tensor& x, int bf16, i64 b, i64 t, i64 h) {
@@ -523,6 +526,7 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
     __shared__ __attribute__((aligned(16))) float gates[GATES][C];
     __shared__ int faulty;  // the first row with a NaN or an infinity; it and those after it become NaN
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
+    if (n * C >= length) return;
     const i64 shared = tape.shared_chunk(d, b, hk, n);
     const int wave = threadIdx.x / 64;
     const Lane l;
@@ -762,6 +766,7 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
     const int col = at.column + l.col;
     const bool live = col < d.value;
     const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+    const i64 chunks = d.used_chunks(b), last = chunks - 1;
 
     if (threadIdx.x >= 64 * WAVES) {  // the outputs of tokens 16 OWN wave ..
         Pieces<N> q[OWN][WAVES];
@@ -835,15 +840,19 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
         };
         constexpr std::true_type yes{};
         constexpr std::false_type no{};
-        fetch_queries(0);
-        fetch_scores(0);
-        for (int i = 0; i < 3; ++i) lds_barrier();
-        const i64 last = d.chunks - 1;
-        if (at.column + 16 <= d.value)
-            for (i64 n = 0; n < last; ++n) chunk(n, yes, yes);
-        else
-            for (i64 n = 0; n < last; ++n) chunk(n, yes, no);
-        chunk(last, no, no);
+        if (chunks > 0) {
+            fetch_queries(0);
+            fetch_scores(0);
+            for (int i = 0; i < 3; ++i) lds_barrier();
+            if (at.column + 16 <= d.value)
+                for (i64 n = 0; n < last; ++n) chunk(n, yes, yes);
+            else
+                for (i64 n = 0; n < last; ++n) chunk(n, yes, no);
+            chunk(last, no, no);
+        }
+        if (live)
+            for (i64 t = chunks * C + 4 * wave + l.quad / 4; t < d.time; t += 4 * WAVES)
+                out[((b * d.time + t) * d.value_heads + h) * d.value + col] = from_float<T>(0.0f);
         return;
     }
 
@@ -891,13 +900,6 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
             for (int kb = 0; kb < 2; ++kb)
                 kt[to][f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
     };
-    const i64 last = d.chunks - 1;
-#pragma unroll
-    for (int ahead = 0; ahead < DEPTH; ++ahead) {
-        fetch_keys(min((i64)ahead, last), ahead);
-        if constexpr (!TIGHT) fetch_writes(min((i64)ahead, last), ahead);
-    }
-    fetch_tokens(0);
     auto chunk = [&](i64 n, auto slot) {
         const i64 next = min(n + 1, last), later = min(n + DEPTH, last);
         const int turn = (int)(n & 1);
@@ -971,14 +973,22 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
         else fetch_writes(later, slot());
         in_order();
     };
-    if constexpr (DEPTH == 2) {
-        for (i64 n = 0; n < last; n += 2) {
-            chunk(n, std::integral_constant<int, 0>{});
-            chunk(n + 1, std::integral_constant<int, 1>{});
+    if (chunks > 0) {
+#pragma unroll
+        for (int ahead = 0; ahead < DEPTH; ++ahead) {
+            fetch_keys(min((i64)ahead, last), ahead);
+            if constexpr (!TIGHT) fetch_writes(min((i64)ahead, last), ahead);
         }
-        if (last % 2 == 0) chunk(last, std::integral_constant<int, 0>{});
-    } else {
-        for (i64 n = 0; n <= last; ++n) chunk(n, std::integral_constant<int, 0>{});
+        fetch_tokens(0);
+        if constexpr (DEPTH == 2) {
+            for (i64 n = 0; n < last; n += 2) {
+                chunk(n, std::integral_constant<int, 0>{});
+                chunk(n + 1, std::integral_constant<int, 1>{});
+            }
+            if (last % 2 == 0) chunk(last, std::integral_constant<int, 0>{});
+        } else {
+            for (i64 n = 0; n <= last; ++n) chunk(n, std::integral_constant<int, 0>{});
+        }
     }
     if (!live) return;
 #pragma unroll
@@ -1017,8 +1027,10 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
     const int col = at.column + l.col;
     const bool live = col < d.value;
     const i64 chunk0 = tape.chunk(d, b, h, 0), shared0 = tape.shared_chunk(d, b, h / d.group, 0);
+    const i64 chunks = d.used_chunks(b);
 
     if (threadIdx.x >= 64 * WAVES) {
+        if (!chunks) return;
         Tokens<T> go[4];
         float4_t since[4];
         Pieces<N> qt[2][2];
@@ -1044,9 +1056,9 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
                 for (int kb = 0; kb < 2; ++kb)
                     qt[f][kb] = fetch<N>(tape.queries_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
         };
-        fetch_grads(d.chunks - 1);
-        fetch_scores(d.chunks - 1);
-        fetch_queries(d.chunks - 1);
+        fetch_grads(chunks - 1);
+        fetch_scores(chunks - 1);
+        fetch_queries(chunks - 1);
         // chunk n, but for the last chunk while the first waves are at n + 1
         auto chunk = [&](i64 n, auto beside) {
             const int turn = (int)(n & 1);
@@ -1082,8 +1094,8 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
             for (int f = 0; f < 2; ++f) *(float4_t*)reads[turn][2 * wave + f][l.id] = acc[f];
             lds_barrier();
         };
-        chunk(d.chunks - 1, std::false_type{});
-        for (i64 n = d.chunks - 1; n-- > 0;) chunk(n, std::true_type{});
+        chunk(chunks - 1, std::false_type{});
+        for (i64 n = chunks - 1; n-- > 0;) chunk(n, std::true_type{});
         lds_barrier();  // those of chunk 0
         lds_barrier();
         lds_barrier();
@@ -1127,11 +1139,13 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
             for (int kb = 0; kb < 2; ++kb)
                 kt[f][kb] = fetch<N>(tape.keys_t + (shared0 + n) * (4 * WAVES * N * 512), (2 * wave + f) * 2 + kb, l);
     };
-    fetch_keys(d.chunks - 1);
-    fetch_tokens(d.chunks - 1);
-    fetch_writes(d.chunks - 1);
-    lds_barrier();  // the last chunk's P^T dO and Q^T g dO
-    for (i64 n = d.chunks; n-- > 0;) {
+    if (chunks > 0) {
+        fetch_keys(chunks - 1);
+        fetch_tokens(chunks - 1);
+        fetch_writes(chunks - 1);
+        lds_barrier();  // the last chunk's P^T dO and Q^T g dO
+    }
+    for (i64 n = chunks; n-- > 0;) {
         const i64 next = n > 0 ? n - 1 : 0;
         const int turn = (int)(n & 1);
         const Pieces<3> state = split<3>(s[0], s[1]);
@@ -1222,6 +1236,23 @@ __global__ void __launch_bounds__(512, 2) gradients(Delta d, Tape tape, Back bac
     static_assert(2 * C * CP * sizeof(float) <= sizeof(stage), "D1 and D2 take the stage's place");
     const i64 n = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, length = d.length(b);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), tb = wave % 4, half = wave / 4, token = 16 * tb, key0 = half * F;
+    if (n * C >= length) {  // no gradient reaches an unused token
+        const i64 first = b * d.time + n * C, tokens = min((i64)C, d.time - n * C), spread = (i64)d.group * d.value;
+        for (i64 e = threadIdx.x; e < tokens * d.key; e += 512) {
+            const i64 to = ((first + e / d.key) * d.heads + hk) * d.key + e % d.key;
+            dq[to] = dk[to] = from_float<T>(0.0f);
+        }
+        for (i64 e = threadIdx.x; e < tokens * spread; e += 512)
+            dv[(first + e / spread) * d.value_heads * d.value + hk * spread + e % spread] = from_float<T>(0.0f);
+        for (i64 e = threadIdx.x; e < tokens * d.group; e += 512) {
+            const i64 to = (first + e / d.group) * d.value_heads + hk * d.group + e % d.group;
+            if (d.beta_bf16) ((bf16_t*)dbeta)[to] = 0;
+            else ((float*)dbeta)[to] = 0.0f;
+            if (ddecay && d.decay_bf16) ((bf16_t*)ddecay)[to] = 0;
+            else if (ddecay) ((float*)ddecay)[to] = 0.0f;
+        }
+        return;
+    }
     const int columns = (int)(d.padded / 16);
     const Lane l;
     const i64 shared = tape.shared_chunk(d, b, hk, n);

@@ -360,3 +360,39 @@ def test_bfloat16_outputs_are_rounded_once(key):
     for tape in (False, True):
         other = (ops.delta_rule(*args, tape=tape)[0] != want).double().mean()
         assert other <= 1e-3, float(other)
+
+
+def same(a, b):
+    """The same values, NaN where NaN is."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("key,time", [(24, 12), (24, 150), (64, 150), (100, 150), (100, 330)])
+def test_unused_tokens_leave_any_state_as_it_is(key, time, dtype):
+    """NaN and infinities in the state of a sequence without tokens, or that its last token left there, stay where
+    they are; backwards the same for the final state's gradient."""
+    print(f"case: delta rule unused {key} {time} {dtype}", flush=True)
+    case = make(3, time, 1, 2, key, 40, dtype, seed=17)
+    case["state"][0, 0, 3, 5], case["state"][0, 1, 1, 0] = float("nan"), float("inf")
+    case["v"][1, min(time, 64) - 1, 1, 7] = float("inf")
+    lengths = [0, min(time, 64), time]
+    device_lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    args = [case[n] for n in INPUTS]
+    for tape in (False, True):
+        out, final = ops.delta_rule(*args, lengths=device_lengths, tape=tape)[:2]
+        assert same(final[0], args[5][0]) and (out[0] == 0).all()
+        alone, left = ops.delta_rule(*(a[1:2] if a is args[5] else a[1:2, :lengths[1]] for a in args), tape=True)[:2]
+        if tape:  # without one, short sequences take another kernel
+            assert same(final[1], left[0]) and same(out[1, :lengths[1]], alone[0]) and (out[1, lengths[1]:] == 0).all()
+        assert torch.isfinite(final[2]).all()
+    case["v"][1, min(time, 64) - 1, 1, 7] = 1.0
+    case["state"][0] = 1.0
+    out, _, tape = ops.delta_rule(*args, lengths=device_lengths, tape=True)
+    go, gs = torch.ones_like(out), torch.ones_like(args[5])
+    want = ops.delta_rule_backward(go, gs, tape)
+    gs[0, 0, 3, 5], gs[0, 1, 1, 0] = float("nan"), float("inf")
+    grads = ops.delta_rule_backward(go, gs, tape)
+    assert same(grads["state"][0], gs[0])
+    for n in INPUTS[:5]:
+        assert (grads[n][0] == 0).all() and (grads[n][1, lengths[1]:] == 0).all() and torch.equal(grads[n], want[n]), n
