@@ -7,7 +7,8 @@ within a sequence (``delta_rule_step`` for one tick of a stream), and ``muon_upd
 matrices.  They take and return torch tensors on the GPU.  Each call enqueues hand-written kernels of
 libatlas_ops_hip.so on the current stream of the tensors' device and returns without waiting;
 workspaces come from torch's allocator.  Gradients are explicit calls, as the trainers' are: a tensor that
-autograd follows is refused unless gradients are disabled.  There is no CPU fallback.
+autograd follows is refused unless gradients are disabled, and so is a dual tensor of forward mode.  There is
+no CPU fallback.
 
 Invalid arguments raise ``ValueError``, a missing library ``NativeUnavailable``, a failed launch
 ``NativeError``.  Tensors may have any strides: what the kernels cannot address (a last axis that is
@@ -22,6 +23,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from .native import NativeError, NativeUnavailable
 
@@ -93,6 +95,9 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: gradients are explicit here, call under torch.no_grad()")
+    # a level is open only within forward_ad.dual_level(), and disabled within an autograd.Function
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent: forward-mode derivatives are not computed here")
     index = t.get_device()
     if device is not None and index != device:
         raise ValueError(f"{name} is on GPU {index}, expected {device}")
