@@ -95,6 +95,8 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: gradients are explicit here, call under torch.no_grad()")
+    if t.is_neg():
+        raise ValueError(f"{name} is a view that negates what its memory holds: pass {name}.resolve_neg()")
     # a level is open only within forward_ad.dual_level(), and disabled within an autograd.Function
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} has a tangent: forward-mode derivatives are not computed here")

@@ -42,3 +42,16 @@ def test_tangents_are_refused():
                 call()
         for call in calls(lambda t: t).values():
             call()
+
+
+def test_negated_views_are_refused():
+    """Imaginary parts of conjugates are views that negate when they are read: their memory holds the other sign."""
+    print("case: negated views", flush=True)
+    def negated(t):
+        view = torch.complex(t, -t).conj().imag
+        assert view.is_neg() and torch.equal(view.resolve_neg(), t)
+        return view
+
+    for name, call in calls(negated).items():
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
