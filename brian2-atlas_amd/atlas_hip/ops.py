@@ -35,6 +35,7 @@ EXPORTS = ["atlas_ops_layer_norm", "atlas_ops_layer_norm_workspace", "atlas_ops_
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_KEY = 128
+INVALID = 7  # the entry points' code of an invalid argument
 
 # the C structures of atlas_ops.h, packed as the ABI lays them out
 _ROWS = struct.Struct("@P3q")
@@ -82,7 +83,8 @@ def _call(device: int, entry, *args) -> None:
         with torch.cuda.device(device):
             rc = entry(*args, stream, address, 512)
     if rc:
-        raise NativeError(rc, buffer.value.decode(errors="replace"))
+        message = buffer.value.decode(errors="replace")
+        raise ValueError(message) if rc == INVALID else NativeError(rc, message)
 
 
 def _tensor(t, name: str, device=None, types=TYPES, shape=None):
@@ -228,23 +230,29 @@ def _matrix(t, name):
     return batch, t.shape[-2], t.shape[-1]
 
 
-def _orthogonalize(device, source, shape, *, momentum, factor, nesterov, steps, coefficients, eps, out=None,
-                   weight=None, keep=0.0, rate=0.0):
+def _orthogonalize(device, source, shape, *, momentum, factor, nesterov, steps, coefficients, eps, weight=None,
+                   keep=0.0, rate=0.0):
+    """Into weight, or a new tensor, which it returns."""
     if not isinstance(steps, int) or not 1 <= steps <= 64:
         raise ValueError("steps must be 1 to 64")
     if len(coefficients) != 3:
         raise ValueError("the iteration has three coefficients")
     batch, rows, columns = shape
+    lib = library()
+    size = lib.atlas_ops_orthogonalize_workspace(batch, rows, columns)
+    if not size:
+        raise ValueError(f"{batch} matrices of {rows} x {columns}: at most 65535, of 2^20 rows and columns, one side at most 16384")
+    out = _empty(source) if weight is None else None
     if source.stride(-1) != 1:
         source = source.contiguous()
-    lib = library()
-    workspace = _workspace(lib.atlas_ops_orthogonalize_workspace(batch, rows, columns), source)
+    workspace = _workspace(size, source)
     packed = _ORTHOGONAL.pack(source.data_ptr(), batch, rows, columns, source.stride(0) if source.dim() == 3 else 0,
                               source.stride(-2), 0 if momentum is None else momentum.data_ptr(),
                               0 if out is None else out.data_ptr(), 0 if weight is None else weight.data_ptr(),
-                              TYPES[source.dtype], 0 if out is None else TYPES[out.dtype], int(nesterov), steps,
+                              TYPES[source.dtype], TYPES[source.dtype], int(nesterov), steps,
                               factor, eps, keep, rate, *coefficients)
     _call(device, lib.atlas_ops_orthogonalize, packed, workspace.data_ptr())
+    return out
 
 
 def orthogonalize(matrix, *, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
@@ -253,14 +261,13 @@ def orthogonalize(matrix, *, steps: int = 5, coefficients=COEFFICIENTS, eps: flo
     ``X = matrix / (|matrix|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with
     ``A = X X^T`` and ``coefficients`` (a, b, c).  The default coefficients raise small singular values fast and
     leave the large ones between about 0.7 and 1.2.  Computed to float32's accuracy for either type; the result
-    is contiguous and of the matrix's type."""
+    is contiguous and of the matrix's type.  At most 65535 matrices, of 2^20 rows and columns, one side at most 16384."""
     device = _tensor(matrix, "matrix")
     shape = _matrix(matrix, "matrix")
-    out = _empty(matrix)
-    if out.numel():
-        _orthogonalize(device, matrix, shape, momentum=None, factor=0.0, nesterov=False, steps=steps,
-                       coefficients=coefficients, eps=eps, out=out)
-    return out
+    if not matrix.numel():
+        return _empty(matrix)
+    return _orthogonalize(device, matrix, shape, momentum=None, factor=0.0, nesterov=False, steps=steps,
+                          coefficients=coefficients, eps=eps)
 
 
 def muon_update(weight, gradient, momentum, *, learning_rate: float, factor: float = 0.95, weight_decay: float = 0.0,

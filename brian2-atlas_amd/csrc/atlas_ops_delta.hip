@@ -1487,14 +1487,18 @@ __global__ void __launch_bounds__(512, 2) gradients(Delta d, Tape tape, Back bac
 // ------------------------------------------------------------------ host
 Tensor tensor(const void* p, const int64_t* s) { return Tensor{p, s[0], s[1], s[2]}; }
 
-int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
+// Keys up to 64 take operands of half the width: 256 x 100 of 4 heads of 64, float32, 545 us, and 894 with those of 128.
+int key_width(const Delta& d) { return d.key <= 64 ? 64 : 128; }
+
+// Workgroups of a scan: 16 columns each, whole groups of 8 heads (Place).
+i64 scan_groups(const Delta& d) { return ceil_div(d.batch * d.value_heads, XCDS) * XCDS * (d.padded / 16); }
+
+int check(const AtlasDelta* a, Delta& d, char* err, size_t cap, bool in_chunks = true) {
     if (!a) return fail(err, cap, 7, "null argument");
     if (a->batch < 1 || a->time < 1 || a->heads < 1 || a->value_heads < 1 || a->value < 1)
         return fail(err, cap, 7, "every size must be positive");
     if (a->key < 1 || a->key > MAX_KEY) return fail(err, cap, 7, "key must be 1 to %d", MAX_KEY);
     if (a->value_heads % a->heads) return fail(err, cap, 7, "value_heads must be a multiple of heads");
-    if (ceil_div(a->value, 32) * 2 * (a->batch * a->value_heads + XCDS) > 0x7FFFFFFF)
-        return fail(err, cap, 7, "batch x value_heads x value is out of range");
     if (a->batch > 65535 || a->value_heads > 65535 || a->time > 0x7FFFFFFF - C || a->value > (1 << 20))
         return fail(err, cap, 7, "batch and value_heads must be at most 65535, time below 2^31 - 64, value at most 2^20");
     if (!known_type(a->type) || !known_type(a->log_decay_type) || !known_type(a->beta_type))
@@ -1514,11 +1518,11 @@ int check(const AtlasDelta* a, Delta& d, char* err, size_t cap) {
     d.chunks = ceil_div(a->time, C);
     d.padded = ceil_div(a->value, 32) * 32;
     d.scale = a->scale;
+    if (in_chunks && scan_groups(d) * 4 * key_width(d) >= THREADS)
+        return fail(err, cap, 7, "batch x value_heads x value is out of range");
+    if (in_chunks && d.chunks * 512 >= THREADS) return fail(err, cap, 7, "time must be at most 2^29 - 64");
     return 0;
 }
-
-// Keys up to 64 take operands of half the width: 256 x 100 of 4 heads of 64, float32, 545 us, and 894 with those of 128.
-int key_width(const Delta& d) { return d.key <= 64 ? 64 : 128; }
 
 // Carves the workspace (256-byte pieces); what only the backward pass reads is there only to train.
 i64 carve(const Delta& d, int type, int train, char* base, Tape* tape) {
@@ -1557,10 +1561,7 @@ void with_kernel(const Delta& d, int type, int width, F&& f) {
     else by_rows(bf16_t{});
 }
 
-// Workgroups of a scan: 16 columns each, whole groups of 8 heads (Place).
-dim3 scan_grid(const Delta& d) {
-    return dim3((unsigned)(ceil_div(d.batch * d.value_heads, XCDS) * XCDS * (d.padded / 16)));
-}
+dim3 scan_grid(const Delta& d) { return dim3((unsigned)scan_groups(d)); }
 
 }  // namespace
 }  // namespace atlas_ops
@@ -1572,7 +1573,7 @@ extern "C" {
 int atlas_ops_delta_step(const AtlasDelta* a, void* out, float* final_state, void* stream, char* err, size_t cap) {
     try {
         Delta d;
-        if (int rc = check(a, d, err, cap)) return rc;
+        if (int rc = check(a, d, err, cap, false)) return rc;
         if (!out || !final_state) return fail(err, cap, 7, "null argument");
         const dim3 grid((unsigned)ceil_div(d.value, 32), (unsigned)d.value_heads, (unsigned)d.batch);
         hipStream_t st = (hipStream_t)stream;

@@ -512,6 +512,13 @@ Buffers carve(const Sizes& s, i64 batch, char* base) {
     return w;
 }
 
+// The sizes that the products' grids and the 32-bit numbers of their tiles are made for.
+bool in_range(i64 batch, i64 rows, i64 columns) {
+    constexpr i64 LONG = 1 << 20, SHORT = 16384;
+    return batch >= 1 && batch <= 65535 && rows >= 1 && columns >= 1 && rows <= LONG && columns <= LONG &&
+           std::min(rows, columns) <= SHORT;
+}
+
 template <typename K, Product WHAT>
 i64 tiles_of(const Task& t) {
     return WHAT == GRAM || WHAT == POLY ? K::triangle(t.columns / K::COLUMNS) : (i64)(t.rows / K::ROWS) * (t.columns / K::COLUMNS);
@@ -554,20 +561,19 @@ using namespace atlas_ops;
 extern "C" {
 
 int64_t atlas_ops_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t columns) {
-    if (batch < 1 || rows < 1 || columns < 1) return 0;
+    if (!in_range(batch, rows, columns)) return 0;
     return carve(sizes_of(batch, rows, columns), batch, nullptr).bytes;
 }
 
 int atlas_ops_orthogonalize(const AtlasOrthogonal* o, void* workspace, void* stream, char* err, size_t cap) {
     try {
-        if (!o || !o->matrix || !workspace || (!o->out) == (!o->weight)) return fail(err, cap, 7, "null argument");
-        if (o->batch < 1 || o->batch > 65535 || o->rows < 1 || o->columns < 1 || o->rows > (1 << 20) ||
-            o->columns > (1 << 20))
-            return fail(err, cap, 7, "batch must be 1 to 65535, rows and columns 1 to 2^20");
+        if (!o) return fail(err, cap, 7, "null argument");
+        if (!in_range(o->batch, o->rows, o->columns))
+            return fail(err, cap, 7, "batch must be 1 to 65535, rows and columns 1 to 2^20 and one of them at most 16384");
+        if (!o->matrix || !workspace || (!o->out) == (!o->weight)) return fail(err, cap, 7, "null argument");
         if (o->steps < 1 || o->steps > 64) return fail(err, cap, 7, "steps must be 1 to 64");
         if (!known_type(o->type) || (o->out && !known_type(o->out_type))) return fail(err, cap, 7, "unknown type");
         const Sizes s = sizes_of(o->batch, o->rows, o->columns);
-        if (s.mp > 16384) return fail(err, cap, 7, "the smaller side must be at most 16384");
         const Buffers w = carve(s, o->batch, (char*)workspace);
         hipStream_t st = (hipStream_t)stream;
         const Source source{o->matrix, o->rows, o->columns, o->batch_stride, o->row_stride, o->momentum, o->factor, o->nesterov};

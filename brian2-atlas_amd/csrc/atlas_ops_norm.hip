@@ -483,13 +483,20 @@ i64 row_blocks(i64 rows, i64 width, int type) {
     return std::min<i64>(ceil_div(rows, 256 / s.lanes), BACKWARD_BLOCKS);
 }
 
+// A long row is a workgroup of its own.
+bool fits(i64 rows, i64 width, int type, bool backward) {
+    return shape_of(width, type, backward).chunks > 0 || rows * 256 < THREADS;
+}
+
 bool usable(const AtlasRows* r) { return r && r->data && r->inner > 0; }
 
-int check(const AtlasRows* x, i64 rows, i64 width, int type, int weight_type, char* err, size_t cap) {
+int check(const AtlasRows* x, i64 rows, i64 width, int type, int weight_type, bool backward, char* err, size_t cap) {
     if (rows < 0 || rows > 0x7FFFFFFF || width < 1 || width > 0x7FFF0000)
         return fail(err, cap, 7, "rows and width must be below 2^31, width positive");
     if (!known_type(type) || !known_type(weight_type) || (type == ATLAS_OPS_F32 && weight_type != ATLAS_OPS_F32))
         return fail(err, cap, 7, "weight must be float32 or have the rows' type");
+    if (!fits(rows, width, type, backward))
+        return fail(err, cap, 7, "rows of this width must be fewer than 2^24");
     if (rows && !usable(x)) return fail(err, cap, 7, "null rows");
     return 0;
 }
@@ -505,7 +512,7 @@ int atlas_ops_layer_norm(const AtlasRows* x, int64_t rows, int64_t width, int ty
                          int weight_type, float eps, void* y, float* mean, float* rstd, void* stream, char* err,
                          size_t cap) {
     try {
-        if (int rc = check(x, rows, width, type, weight_type, err, cap)) return rc;
+        if (int rc = check(x, rows, width, type, weight_type, false, err, cap)) return rc;
         if (!rows) return 0;
         if (!y || (mean == nullptr) != (rstd == nullptr)) return fail(err, cap, 7, "null output");
         const Shape shape = shape_of(width, type, false);
@@ -531,7 +538,7 @@ int atlas_ops_layer_norm(const AtlasRows* x, int64_t rows, int64_t width, int ty
 }
 
 int64_t atlas_ops_layer_norm_workspace(int64_t rows, int64_t width, int type) {
-    if (rows < 1 || width < 1 || !known_type(type)) return 0;
+    if (rows < 1 || width < 1 || !known_type(type) || !fits(rows, width, type, true)) return 0;
     // the partial sums, and of long rows what their means left out
     return (2 * row_blocks(rows, width, type) * width + (shape_of(width, type, true).chunks ? 0 : rows)) * (i64)sizeof(float);
 }
@@ -540,7 +547,7 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
                                   const void* weight, int weight_type, const float* mean, const float* rstd, void* dx,
                                   void* dweight, void* dbias, float* workspace, void* stream, char* err, size_t cap) {
     try {
-        if (int rc = check(x, rows, width, type, weight_type, err, cap)) return rc;
+        if (int rc = check(x, rows, width, type, weight_type, true, err, cap)) return rc;
         const bool sums = dweight || dbias;
         if (rows && (!usable(grad) || !mean || !rstd || !dx || (sums && !workspace)))
             return fail(err, cap, 7, "null argument");

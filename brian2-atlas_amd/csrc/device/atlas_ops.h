@@ -31,6 +31,8 @@ inline int launched(char* err, size_t cap, const char* what) {
     return status == hipSuccess ? 0 : fail(err, cap, 4, "%s: %s", what, hipGetErrorString(status));
 }
 
+constexpr i64 THREADS = (i64)1 << 32;  // a grid's threads along x stay below
+
 inline bool known_type(int type) { return type == ATLAS_OPS_F32 || type == ATLAS_OPS_BF16; }
 
 inline i64 ceil_div(i64 a, i64 b) { return (a + b - 1) / b; }

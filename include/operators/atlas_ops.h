@@ -7,7 +7,7 @@
  * allocated, kept between calls or read back.  `type` and the other element types are
  * ATLAS_OPS_F32 or ATLAS_OPS_BF16.  Strides count elements.  Return codes are those of the
  * training library: 0 ok, 4 launch failure, 7 invalid argument or host exception, with a message
- * in (error, capacity).
+ * in (error, capacity).  Sizes that a call refuses have a workspace of 0 bytes.
  */
 #ifndef ATLAS_OPS_H
 #define ATLAS_OPS_H
@@ -68,7 +68,8 @@ typedef struct {
     float coefficients[3];
 } AtlasOrthogonal;
 
-/* Bytes of workspace for a call of these sizes. */
+/* Bytes of workspace for a call of these sizes: batch 1 to 65535, rows and columns 1 to 2^20 and one of them at most
+ * 16384. */
 int64_t atlas_ops_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t columns);
 int atlas_ops_orthogonalize(const AtlasOrthogonal* problem, void* workspace, void* stream, char* error,
                             size_t capacity);
@@ -82,7 +83,8 @@ int atlas_ops_orthogonalize(const AtlasOrthogonal* problem, void* workspace, voi
  * those of (batch, time, head).  A log_decay below -120 counts as -120, whose exponential is zero in
  * float32: it empties the state.  state (f32, contiguous (batch, value_heads, key, value)) may be NULL
  * for zeros.  lengths (i32[batch], NULL for `time`): tokens from lengths[b] on leave the state as it is
- * and give zeros.  1 <= key <= 128.
+ * and give zeros.  1 <= key <= 128; batch and value_heads up to 65535, value up to 2^20.  In chunks also: time up
+ * to 2^29 - 64, batch x value_heads x value (to whole 8 heads and 32 values) below 2^27, with keys up to 64 below 2^28.
  */
 typedef struct {
     const void *q, *k, *v, *log_decay, *beta;

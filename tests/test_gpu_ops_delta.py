@@ -396,3 +396,13 @@ def test_unused_tokens_leave_any_state_as_it_is(key, time, dtype):
     assert same(grads["state"][0], gs[0])
     for n in INPUTS[:5]:
         assert (grads[n][0] == 0).all() and (grads[n][1, lengths[1]:] == 0).all() and torch.equal(grads[n], want[n]), n
+
+
+def test_sizes_beyond_the_limits_are_invalid_arguments():
+    print("case: delta rule limits", flush=True)
+    one = torch.ones(1, device="cuda")
+    q, v, gate = one.expand(65536, 13, 1, 1), one.expand(65536, 13, 1, 1), one.expand(65536, 13, 1)
+    with pytest.raises(ValueError, match="65535"):
+        ops.delta_rule(q, q, v, gate, gate)
+    with pytest.raises(ValueError, match="65535"):
+        ops.delta_rule_step(q[:, 0], q[:, 0], v[:, 0], gate[:, 0], gate[:, 0], torch.ones(65536, 1, 1, 1, device="cuda"))

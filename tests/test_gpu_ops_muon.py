@@ -165,3 +165,19 @@ def test_another_stream():
         got = ops.orthogonalize(m)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(got, want)
+
+
+def test_sizes_beyond_the_limits_are_invalid_arguments():
+    """Refused as such, and before anything is allocated for them."""
+    print("case: muon limits", flush=True)
+    one = torch.ones(1, device="cuda")
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for shape in ((16385, 16385), (2, (1 << 20) + 1), ((1 << 20) + 1, 2), (65536, 1, 1)):
+        with pytest.raises(ValueError, match="16384"):
+            ops.orthogonalize(one.expand(shape))
+    assert torch.cuda.max_memory_allocated() == before
+    weight, momentum = torch.ones(65536, 1, 1, device="cuda"), torch.ones(65536, 1, 1, device="cuda")
+    with pytest.raises(ValueError, match="16384"):
+        ops.muon_update(weight, one.expand(65536, 1, 1), momentum, learning_rate=0.1)
+    assert (weight == 1).all() and (momentum == 1).all()

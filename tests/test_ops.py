@@ -205,3 +205,45 @@ def test_workspace_sizes():
     assert lib.atlas_ops_delta_backward_workspace(packed) > 0
     assert lib.atlas_ops_layer_norm_workspace(1000, 256, 0) > 0 and lib.atlas_ops_layer_norm_workspace(0, 256, 0) == 0
     assert lib.atlas_ops_orthogonalize_workspace(1, 100, 50) > 0
+
+
+def test_the_abi_refuses_what_a_launch_could_not_take():
+    """A grid holds fewer than 2^32 threads along x: more is an invalid argument, not a failed launch.  A refused size
+    has no workspace, and is refused for its size before the workspace is asked for."""
+    lib = ops.library()
+    err = ctypes.create_string_buffer(256)
+    address = ctypes.addressof(err)
+    p = 4096  # never read: each call is refused
+
+    def refused(rc, text):
+        assert rc == 7 and text in err.value.decode(), (rc, err.value)
+
+    def delta(batch, time, value_heads, key, value):
+        return ops._DELTA.pack(p, p, p, p, p, *([4] * 15), 0, 0, batch, time, 1, value_heads, key, value, 0, 0, 0, 1.0)
+
+    # 65535 x 17 heads of 128 columns: 8 slices of 512 threads for each, of 256 with keys of 64; 2^29 + 1 tokens: more
+    # than 2^23 chunks of 512 threads
+    for packed, text in ((delta(65535, 64, 17, 128, 128), "value_heads x value"), (delta(65535, 64, 33, 64, 128), "value_heads x value"),
+                         (delta(1, (1 << 29) + 1, 1, 16, 16), "time")):
+        refused(lib.atlas_ops_delta_forward(packed, 0, p, p, p, None, address, 256), text)
+        refused(lib.atlas_ops_delta_backward(packed, p, p, ops.struct.pack("@3q", 4, 4, 4), p, p, p, p, p, p, p, p, None,
+                                             address, 256), text)
+        assert lib.atlas_ops_delta_workspace(packed, 0) == lib.atlas_ops_delta_workspace(packed, 1) == 0
+        assert lib.atlas_ops_delta_backward_workspace(packed) == 0
+    assert lib.atlas_ops_delta_workspace(delta(65535, 64, 16, 128, 128), 0) > 0
+    assert lib.atlas_ops_delta_workspace(delta(1, (1 << 29) - 64, 1, 16, 16), 0) > 0
+
+    rows = ops._ROWS.pack(p, 1 << 24, 0, 8)
+    assert lib.atlas_ops_layer_norm_workspace(1 << 24, 4100, 1) == 0
+    assert lib.atlas_ops_layer_norm_workspace((1 << 24) - 1, 4100, 1) > 0
+    for width, type_ in ((4100, 0), (8200, 1)):  # a workgroup for each row
+        refused(lib.atlas_ops_layer_norm(rows, 1 << 24, width, type_, None, None, 0, 1e-5, p, None, None, None, address, 256), "rows")
+        refused(lib.atlas_ops_layer_norm_backward(rows, rows, 1 << 24, width, type_, None, 0, p, p, p, p, p, p, None, address,
+                                                  256), "rows")
+    refused(lib.atlas_ops_layer_norm_backward(rows, rows, 1 << 24, 4100, 1, None, 0, p, p, p, p, p, p, None, address, 256), "rows")
+
+    for sizes in ((1, 17000, 17000), (1, 1 << 21, 4), (1, 4, 1 << 21), (70000, 4, 4)):
+        assert lib.atlas_ops_orthogonalize_workspace(*sizes) == 0
+        packed = ops._ORTHOGONAL.pack(p, *sizes, 16, 4, 0, p, 0, 0, 0, 1, 5, 0.9, 1e-7, 1.0, 0.1, 3.0, -4.0, 2.0)
+        refused(lib.atlas_ops_orthogonalize(packed, None, None, address, 256), "16384" if sizes[1] == 17000 else "batch")
+    assert lib.atlas_ops_orthogonalize_workspace(1, 16384, 1 << 20) > 0
