@@ -199,8 +199,8 @@ def layer_norm_backward(grad, x, weight, mean, rstd, *, sums: bool = True):
     if width < 1:
         raise ValueError("x needs a last axis to normalise")
     _tensor(grad, "grad", device, _SAME[x.dtype], x.shape)
-    wtype = torch.float32 if weight is None else weight.dtype
     weight, _, code = _norm_weights(x, width, weight, None, device)
+    wtype = torch.float32 if weight is None else weight.dtype
     lead = x.shape[:-1]
     _tensor(mean, "mean", device, _F32, lead)
     _tensor(rstd, "rstd", device, _F32, lead)
@@ -311,12 +311,12 @@ class _Problem:
 
     def __init__(self, q, k, v, log_decay, beta, state, lengths, scale, time_axis: bool):
         device = _tensor(q, "q")
+        same = _SAME[q.dtype]
+        _tensor(v, "v", device, same)
         shape, out = q.shape, v.shape
         if len(shape) != 3 + time_axis or len(out) != len(shape):
             raise ValueError(f"q, k and v must be {'(batch, time, heads, width)' if time_axis else '(batch, heads, width)'}")
-        same = _SAME[q.dtype]
         _tensor(k, "k", device, same, shape)
-        _tensor(v, "v", device, same)
         *lead, heads, key = shape
         *given, value_heads, value = out
         if given != lead:
@@ -426,6 +426,8 @@ def delta_rule_backward(grad_out, grad_state, tape: DeltaTape) -> dict:
     """The gradients of ``delta_rule`` from those of out (of its type) and of the final state (float32, or None
     for zeros): a dict with ``q, k, v, log_decay, beta, state``, each of its input's type, None for an input that
     was not given.  Heads of q and k that value heads share get the sum.  The same bits on every run."""
+    if not isinstance(tape, DeltaTape):
+        raise ValueError("tape must be the one that delta_rule returned")
     p = tape.problem
     q, k, v, log_decay, beta, state, lengths = p.tensors
     _tensor(grad_out, "grad_out", p.device, _SAME[p.type], v.shape)

@@ -55,3 +55,20 @@ def test_negated_views_are_refused():
     for name, call in calls(negated).items():
         with pytest.raises(ValueError, match="resolve_neg"):
             call()
+
+
+def test_what_is_no_tensor_is_refused():
+    print("case: no tensors", flush=True)
+    t = tensors()
+    x, k, gate = t["x"], t["k"], t["gate"]
+    _, mean, rstd = ops.layer_norm(x, statistics=True)
+    out = ops.delta_rule(k, k, k, gate, -gate)[0]
+    for call in (lambda: ops.layer_norm_backward(x, x, [1.0] * 32, mean, rstd), lambda: ops.layer_norm_backward(x, x, None, 0.0, 1.0),
+                 lambda: ops.delta_rule(k, k, None, gate, -gate), lambda: ops.delta_rule(None, k, k, gate, -gate),
+                 lambda: ops.delta_rule(k, k, k, gate, -gate, state=0.0), lambda: ops.delta_rule(k, k, k, gate, -gate, lengths=[1, 2]),
+                 lambda: ops.delta_rule_backward(out, None, None), lambda: ops.delta_rule_backward(out, None, (out, out)),
+                 lambda: ops.delta_rule_step(k[:, 0], k[:, 0], None, gate[:, 0], -gate[:, 0], torch.zeros(2, 1, 8, 8, device="cuda")),
+                 lambda: ops.layer_norm(None), lambda: ops.orthogonalize([[1.0]]),
+                 lambda: ops.muon_update(x, None, torch.zeros_like(x), learning_rate=0.1)):
+        with pytest.raises(ValueError):
+            call()
