@@ -112,6 +112,17 @@ _F32, _I32 = {torch.float32: 0}, {torch.int32: 0}
 _SAME = {t: {t: 0} for t in TYPES}
 
 
+def _span(t):
+    """From t's first element to its last, in elements."""
+    return 1 + sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+
+
+def _overlap(a, b):
+    """Whether the memory from a's first element to its last and that of b have bytes in common."""
+    start, other = a.data_ptr(), b.data_ptr()
+    return start < other + _span(b) * b.element_size() and other < start + _span(a) * a.element_size()
+
+
 def _empty(t):
     """A contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -279,7 +290,7 @@ def muon_update(weight, gradient, momentum, *, learning_rate: float, factor: flo
     ``weight <- (1 - learning_rate weight_decay) weight - learning_rate scale orthogonalize(u)``,
     u = ``gradient + factor momentum`` with ``nesterov``, else the momentum.  Weights are (source, target), as the
     trainers'; ``scale`` is by default ``sqrt(max(1, targets / sources))``.  weight and momentum: float32, contiguous;
-    gradient: float32 or bfloat16."""
+    gradient: float32 or bfloat16.  The three must not share memory."""
     device = _tensor(weight, "weight", types=_F32)
     shape = _matrix(weight, "weight")
     _tensor(momentum, "momentum", device, _F32, weight.shape)
@@ -289,8 +300,12 @@ def muon_update(weight, gradient, momentum, *, learning_rate: float, factor: flo
             raise ValueError(f"{name} is updated in place and must be contiguous")
     if not weight.numel():
         return
-    if len({weight.data_ptr(), momentum.data_ptr(), gradient.data_ptr()}) < 3:
+    if _overlap(weight, momentum):
         raise ValueError("weight, momentum and gradient must not share memory")
+    if _overlap(gradient, weight) or _overlap(gradient, momentum):
+        if _span(gradient) == gradient.numel():
+            raise ValueError("weight, momentum and gradient must not share memory")
+        gradient = gradient.contiguous()  # the others may lie in the gaps between its rows
     if scale is None:
         scale = math.sqrt(max(1.0, shape[2] / shape[1]))
     _orthogonalize(device, gradient, shape, momentum=momentum, factor=factor, nesterov=nesterov, steps=steps,
@@ -357,7 +372,8 @@ def delta_rule_step(q, k, v, log_decay, beta, state, *, scale: float | None = No
     """One tick of the gated delta rule for every stream of a batch; ``state`` is updated in place.
 
     As ``delta_rule`` without the time axis: q, k (batch, heads, key), v (batch, value heads, value), log_decay
-    and beta (batch, value heads), state float32 (batch, value heads, key, value), contiguous.  Returns out."""
+    and beta (batch, value heads), state float32 (batch, value heads, key, value), contiguous, of memory that the other
+    tensors have no part in.  Returns out."""
     if state is None:
         raise ValueError("a step needs a state to update")
     p = _Problem(q, k, v, log_decay, beta, state, None, scale, False)

@@ -55,7 +55,7 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
  * momentum + matrix and u = matrix + factor momentum (nesterov) or the momentum.  The result goes to
  * `out` (contiguous, out_type), or, where out is NULL, into weight (f32, contiguous):
  * weight <- keep weight - rate X.  Element (r, c) of matrix b is at b * batch_stride + r * row_stride + c.
- * Accuracy is float32's for either type.
+ * Accuracy is float32's for either type.  matrix, momentum, weight and out must not share memory.
  */
 typedef struct {
     const void* matrix;
@@ -97,7 +97,7 @@ typedef struct {
 } AtlasDelta;
 
 /* Token by token: out (contiguous, `type`) and the state after the last token.  final_state may be
- * `state` itself. */
+ * `state` itself, and shares no memory with the other inputs. */
 int atlas_ops_delta_step(const AtlasDelta* delta, void* out, float* final_state, void* stream, char* error,
                          size_t capacity);
 

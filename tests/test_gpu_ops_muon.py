@@ -181,3 +181,26 @@ def test_sizes_beyond_the_limits_are_invalid_arguments():
     with pytest.raises(ValueError, match="16384"):
         ops.muon_update(weight, one.expand(65536, 1, 1), momentum, learning_rate=0.1)
     assert (weight == 1).all() and (momentum == 1).all()
+
+
+def test_update_refuses_shared_memory():
+    """Also where only a part is shared; a gradient whose gaps hold the others is taken."""
+    print("case: muon shared memory", flush=True)
+    flat = torch.randn(5000, generator=torch.Generator().manual_seed(8)).cuda()
+    w, g, m = flat[:1200].view(30, 40), flat[1200:2400].view(30, 40), flat[2400:3600].view(30, 40)
+    part = flat[100:1300].view(30, 40)
+    halves = flat.bfloat16()
+    for call in (lambda: ops.muon_update(w, g, part, learning_rate=0.1), lambda: ops.muon_update(w, part, m, learning_rate=0.1),
+                 lambda: ops.muon_update(part, w.T.contiguous().T, w, learning_rate=0.1),
+                 lambda: ops.muon_update(w, flat[2399:3599].view(30, 40), m, learning_rate=0.1),
+                 lambda: ops.muon_update(w, flat[1100:2300].view(40, 30).T, m, learning_rate=0.1),
+                 lambda: ops.muon_update(halves.view(F32)[:1200].view(30, 40), halves[2399:3599].view(30, 40), m, learning_rate=0.1)):
+        with pytest.raises(ValueError, match="share memory"):
+            call()
+    wide = torch.randn(2, 2400, generator=torch.Generator().manual_seed(9)).cuda()
+    gradient = wide[:, :600].unflatten(1, (20, 30))              # 2 x 20 x 30, with 1800 values between the two
+    weight, momentum = wide[0, 600:1800].view(2, 20, 30), torch.zeros(2, 20, 30, device="cuda")
+    alone, other, copy = weight.clone(), momentum.clone(), gradient.clone()
+    ops.muon_update(alone, copy, other, learning_rate=0.1)
+    ops.muon_update(weight, gradient, momentum, learning_rate=0.1)
+    assert torch.equal(weight, alone) and torch.equal(momentum, other)
