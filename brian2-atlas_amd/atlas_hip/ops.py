@@ -272,7 +272,8 @@ def orthogonalize(matrix, *, steps: int = 5, coefficients=COEFFICIENTS, eps: flo
     ``X = matrix / (|matrix|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with
     ``A = X X^T`` and ``coefficients`` (a, b, c).  The default coefficients raise small singular values fast and
     leave the large ones between about 0.7 and 1.2.  Computed to float32's accuracy for either type; the result
-    is contiguous and of the matrix's type.  At most 65535 matrices, of 2^20 rows and columns, one side at most 16384."""
+    is contiguous and of the matrix's type.  Coefficients that could raise a matrix of the iteration beyond 4000 are
+    refused.  At most 65535 matrices, of 2^20 rows and columns, one side at most 16384."""
     device = _tensor(matrix, "matrix")
     shape = _matrix(matrix, "matrix")
     if not matrix.numel():

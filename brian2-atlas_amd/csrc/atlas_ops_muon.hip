@@ -8,8 +8,8 @@
 // Each step raises the small singular values by a factor of about a, so rounding in X or A grows by
 // a^steps (485 at the defaults) in the weakest directions: bfloat16 or float16 products lose them.  Every
 // matrix of the iteration is therefore held as two float16 planes, v = (hi + lo / 2048) / 16, 22
-// significant bits (the iterates' entries are below 1.5, so hi is normal down to 4e-6, and lo covers
-// what is below), in the 4 bytes that a float32 takes.  A product of two such matrices is three
+// significant bits (the iterates' entries are below 1.5 with the default coefficients; hi is normal down to
+// 4e-6, and lo covers what is below), in the 4 bytes that a float32 takes.  A product of two such matrices is three
 // float16 MFMAs, hi hi + (hi lo + lo hi) / 2048 with float32 sums; the dropped lo lo term is below
 // 2^-22.  That is float32's accuracy at 1/3 of the float16 rate instead of the float32 MFMA's 1/16.
 //
@@ -19,6 +19,7 @@
 // rows of a tile give to a stage of a product is one contiguous piece.  A and b A + c A A are symmetric: only
 // the tiles on and above the diagonal are computed, and written twice.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "device/atlas_ops.h"
@@ -512,6 +513,39 @@ Buffers carve(const Sizes& s, i64 batch, char* base) {
     return w;
 }
 
+// Whether the iteration's matrices stay within what the planes hold (65504 / SCALE = 4094) for every source.  An entry is at
+// most the largest singular value, which is |X|_F <= 1 at first.  With s up to `top`: X X^T has s^2, b A + c A A has
+// b u + c u^2 with u = s^2, the next X has a s + b s^3 + c s^5; each is largest at an end or where its derivative is zero.
+bool within_planes(int steps, const float* k) {
+    constexpr double LIMIT = 4000.0;
+    const double a = k[0], b = k[1], c = k[2];
+    double top = 1.0;
+    for (int i = 0; i < steps; ++i) {
+        const double end = top * top;
+        double poly = 0.0, next = 0.0;
+        auto poly_at = [&](double u) {
+            if (u >= 0.0 && u <= end) poly = std::max(poly, std::abs(u * (b + c * u)));
+        };
+        auto next_at = [&](double u) {
+            if (u >= 0.0 && u <= end) next = std::max(next, std::abs(std::sqrt(u) * (a + u * (b + c * u))));
+        };
+        poly_at(end);
+        next_at(end);
+        if (c != 0.0) {
+            poly_at(-b / (2.0 * c));
+            const double root = std::sqrt(9.0 * b * b - 20.0 * a * c);  // NaN where there is none: in no range
+            next_at((-3.0 * b + root) / (10.0 * c));
+            next_at((-3.0 * b - root) / (10.0 * c));
+        } else if (b != 0.0) {
+            next_at(-a / (3.0 * b));
+        }
+        // the last X goes to the caller as it is
+        if (!(end <= LIMIT && poly <= LIMIT && (i + 1 == steps || next <= LIMIT))) return false;
+        top = next;
+    }
+    return true;
+}
+
 // The sizes that the products' grids and the 32-bit numbers of their tiles are made for.
 bool in_range(i64 batch, i64 rows, i64 columns) {
     constexpr i64 LONG = 1 << 20, SHORT = 16384;
@@ -572,6 +606,10 @@ int atlas_ops_orthogonalize(const AtlasOrthogonal* o, void* workspace, void* str
             return fail(err, cap, 7, "batch must be 1 to 65535, rows and columns 1 to 2^20 and one of them at most 16384");
         if (!o->matrix || !workspace || (!o->out) == (!o->weight)) return fail(err, cap, 7, "null argument");
         if (o->steps < 1 || o->steps > 64) return fail(err, cap, 7, "steps must be 1 to 64");
+        for (const float k : o->coefficients)
+            if (!std::isfinite(k)) return fail(err, cap, 7, "the coefficients must be finite");
+        if (!within_planes(o->steps, o->coefficients))
+            return fail(err, cap, 7, "the coefficients raise the iteration's matrices beyond 4000");
         if (!known_type(o->type) || (o->out && !known_type(o->out_type))) return fail(err, cap, 7, "unknown type");
         const Sizes s = sizes_of(o->batch, o->rows, o->columns);
         const Buffers w = carve(s, o->batch, (char*)workspace);

@@ -55,7 +55,8 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
  * momentum + matrix and u = matrix + factor momentum (nesterov) or the momentum.  The result goes to
  * `out` (contiguous, out_type), or, where out is NULL, into weight (f32, contiguous):
  * weight <- keep weight - rate X.  Element (r, c) of matrix b is at b * batch_stride + r * row_stride + c.
- * Accuracy is float32's for either type.  matrix, momentum, weight and out must not share memory.
+ * Accuracy is float32's for either type.  The coefficients are finite and such that no X before the last, X X^T
+ * or b A + c A A passes 4000 for any matrix.  matrix, momentum, weight and out must not share memory.
  */
 typedef struct {
     const void* matrix;

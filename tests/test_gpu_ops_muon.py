@@ -204,3 +204,26 @@ def test_update_refuses_shared_memory():
     ops.muon_update(alone, copy, other, learning_rate=0.1)
     ops.muon_update(weight, gradient, momentum, learning_rate=0.1)
     assert torch.equal(weight, alone) and torch.equal(momentum, other)
+
+
+def test_coefficients_that_leave_the_range_are_refused():
+    """Iterates lie in float16 planes, up to 4094: coefficients that raise any matrix's singular values, at most one at
+    first, beyond that are refused, and those that stay below are held to 2e-5 of the result's norm; but where s grows
+    as s^5, a rounding of 2^-22 grows five times a step, to 2^-22 (1 + 5 + ... + 5^6) = 4.7e-3 after six."""
+    print("case: orthogonalize coefficients", flush=True)
+    for m in (torch.ones(1, 1, device="cuda"), make((20, 30), seed=4), make((40, 1), seed=1) @ make((1, 50), seed=2)):
+        for steps, coefficients, tol in ((2, (30.0, 0.0, 0.0), 2e-5), (1, (1e6, 0.0, 0.0), 2e-5), (1, (1.0, 2000.0, 1500.0), 2e-5),
+                                         (64, (1.5, -0.5, 0.0), 2e-5), (20, ops.COEFFICIENTS, 2e-5), (6, (1e-3, 0.0, 1.0), 4.7e-3)):
+            got, want = ops.orthogonalize(m, steps=steps, coefficients=coefficients), oo.orthogonalize(numpy(m), steps, coefficients)
+            if min(m.shape) == 1 or m.shape[0] < m.shape[1] == 30:
+                assert np.abs(numpy(got) - want).max() <= tol * max(1.0, np.linalg.norm(want)), (steps, coefficients)
+            else:  # what the product's rounding leaves beside its rank grows by up to 3.4 a step: no exact value
+                assert torch.isfinite(got).all()
+        for steps, coefficients in ((3, (30.0, 0.0, 0.0)), (2, (5000.0, 0.0, 0.0)), (1, (1.0, 2500.0, 2000.0)),
+                                    (9, (-2.0, -1.0, 0.0)), (5, (float("nan"), 0.0, 0.0)), (5, (1.0, 0.0, float("inf")))):
+            with pytest.raises(ValueError, match="coefficients"):
+                ops.orthogonalize(m, steps=steps, coefficients=coefficients)
+            weight, momentum = torch.ones_like(m), torch.ones_like(m)
+            with pytest.raises(ValueError, match="coefficients"):
+                ops.muon_update(weight, m, momentum, learning_rate=0.1, steps=steps, coefficients=coefficients)
+            assert (weight == 1).all() and (momentum == 1).all()

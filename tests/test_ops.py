@@ -247,3 +247,13 @@ def test_the_abi_refuses_what_a_launch_could_not_take():
         packed = ops._ORTHOGONAL.pack(p, *sizes, 16, 4, 0, p, 0, 0, 0, 1, 5, 0.9, 1e-7, 1.0, 0.1, 3.0, -4.0, 2.0)
         refused(lib.atlas_ops_orthogonalize(packed, None, None, address, 256), "16384" if sizes[1] == 17000 else "batch")
     assert lib.atlas_ops_orthogonalize_workspace(1, 16384, 1 << 20) > 0
+
+
+def test_the_abi_refuses_coefficients_beyond_the_planes():
+    lib = ops.library()
+    err = ctypes.create_string_buffer(256)
+    for steps, coefficients in ((3, (30.0, 0.0, 0.0)), (2, (5000.0, 0.0, 0.0)), (1, (1.0, 2500.0, 2000.0)), (9, (-2.0, -1.0, 0.0)),
+                                (5, (float("nan"), 0.0, 0.0)), (5, (1.0, 0.0, float("-inf")))):
+        packed = ops._ORTHOGONAL.pack(4096, 1, 4, 4, 16, 4, 0, 4096, 0, 0, 0, 1, steps, 0.9, 1e-7, 1.0, 0.1, *coefficients)
+        rc = lib.atlas_ops_orthogonalize(packed, 4096, None, ctypes.addressof(err), 256)  # the address is never read
+        assert rc == 7 and b"coefficients" in err.value, (steps, coefficients, err.value)
