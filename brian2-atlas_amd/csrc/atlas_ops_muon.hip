@@ -203,10 +203,11 @@ struct Task {
 };
 
 // How a product is cut: ROWS x COLUMNS of the result per workgroup, of which each of its WR x WC waves takes
-// an equal part in 16 x 16 blocks, DEPTH sum indices per stage, in one or two LDS buffers.
-template <int ROWS_, int COLUMNS_, int WR_, int WC_, int DEPTH_, int BUFFERS_>
+// an equal part in 16 x 16 blocks, DEPTH sum indices per stage.  SPLIT: a triangle's sums may be split.
+template <int ROWS_, int COLUMNS_, int WR_, int WC_, int DEPTH_, bool SPLIT_>
 struct Cut {
-    static constexpr int ROWS = ROWS_, COLUMNS = COLUMNS_, WR = WR_, WC = WC_, DEPTH = DEPTH_, BUFFERS = BUFFERS_;
+    static constexpr int ROWS = ROWS_, COLUMNS = COLUMNS_, WR = WR_, WC = WC_, DEPTH = DEPTH_;
+    static constexpr bool SPLIT = SPLIT_;
     static constexpr int THREADS = 64 * WR * WC, FR = ROWS / WR / 16, FC = COLUMNS / WC / 16;
     // Where 8 halves of a row lie in LDS.  A wave reads 16 rows at 4 neighbouring places each: with the
     // places exchanged by the row they hit every bank equally (padded rows of 80 or 144 bytes take twice the cycles).
@@ -312,18 +313,19 @@ __device__ __forceinline__ void finish(const Task& t, i64 b, int r, int c, float
 // and the launch.
 //
 // One tile of Left Right^T.  While a stage is multiplied out of LDS, the next comes from memory into registers,
-// and from there into the other buffer, or into the only one once every wave has left it.
+// and from there into the other buffer.
 template <typename K, Product WHAT>
 __global__ void __launch_bounds__(K::THREADS) ortho_product(Task t) {
-    constexpr int FR = K::FR, FC = K::FC, DEPTH = K::DEPTH, KB = DEPTH / 32, B = K::BUFFERS;
+    constexpr int FR = K::FR, FC = K::FC, DEPTH = K::DEPTH, KB = DEPTH / 32;
+    constexpr bool SPLIT = K::SPLIT && (WHAT == GRAM || WHAT == POLY);
     constexpr int STEP = K::THREADS / 4, LR = K::ROWS / STEP, LC = K::COLUMNS / STEP;  // rows per round of loads, rounds
-    __shared__ __attribute__((aligned(16))) half_t lds[B][2][(K::ROWS + K::COLUMNS) * DEPTH];
+    __shared__ __attribute__((aligned(16))) half_t lds[2][2][(K::ROWS + K::COLUMNS) * DEPTH];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, wi = wave / K::WC, wj = wave % K::WC;
     const i64 b = blockIdx.z;
     // read here: the compiler keeps a task's field that it finds behind a branch in LDS, addressed through the
     // dispatch packet in host memory, which every kernel then waits for (up to 7 us)
     const float product = t.product;
-    float* const partial = t.partial;
+    float* const partial = SPLIT ? t.partial : nullptr;
     int ti, tj;
     tile_of<K, WHAT>(blockIdx.x, t.rows, ti, tj);
     // four threads take the 64 bytes of a row
@@ -333,7 +335,8 @@ __global__ void __launch_bounds__(K::THREADS) ortho_product(Task t) {
     const half_t *left_hi = t.left.hi + left_at, *left_lo = t.left.lo + left_at;
     const half_t *right_hi = t.right.hi + right_at, *right_lo = t.right.lo + right_at;
     // the split's part, in columns of 32 sum indices
-    const int all = t.depth / 32, first = all * (int)blockIdx.y / t.splits, end = all * ((int)blockIdx.y + 1) / t.splits;
+    const int all = t.depth / 32;
+    const int first = SPLIT ? all * (int)blockIdx.y / t.splits : 0, end = SPLIT ? all * ((int)blockIdx.y + 1) / t.splits : all;
     half8_t next_left[2][KB][LR], next_right[2][KB][LC];
     auto fetch = [&](int k) {
 #pragma unroll
@@ -395,8 +398,7 @@ __global__ void __launch_bounds__(K::THREADS) ortho_product(Task t) {
         }
         if (k + KB >= end) break;
         // the other buffer was read in the stage before this one, which every wave has left
-        if constexpr (B == 1) lds_barrier();
-        buffer ^= B - 1;
+        buffer ^= 1;
         stage(buffer);
         fetch(k + 2 * KB);
         lds_barrier();
@@ -448,9 +450,9 @@ __global__ void __launch_bounds__(K::THREADS) ortho_join(Task t) {
 // 64 x 64, and of 32 x 32 below 192 of these, spread small matrices over the CUs, where a stage's way from memory
 // is what takes the time (all five steps, 64 / 32: 256 x 256 107 / 83 us, 768 x 768 218 / 176, 1024 x 1024 273 / 255;
 // 32 for up to 400 tiles costs 1536 x 1536 563 instead of 525).
-typedef Cut<256, 128, 4, 2, 32, 2> Large;
-typedef Cut<64, 64, 2, 2, 32, 2> Small;
-typedef Cut<32, 32, 2, 1, 64, 2> Tiny;
+typedef Cut<256, 128, 4, 2, 32, true> Large;
+typedef Cut<64, 64, 2, 2, 32, false> Small;
+typedef Cut<32, 32, 2, 1, 64, false> Tiny;
 constexpr i64 CUS = 256, FEW_TILES = 192;
 
 struct Sizes {
@@ -459,10 +461,9 @@ struct Sizes {
     int gram_splits, poly_splits;
 };
 
-template <typename K>
 int splits_of(i64 batch, i64 mp, i64 depth) {
     // a triangle of few tiles is split along the sum while that fills CUs; a part keeps 512 indices or more
-    const i64 tiles = batch * K::triangle(mp / K::COLUMNS);
+    const i64 tiles = batch * Large::triangle(mp / Large::COLUMNS);
     return (int)std::max<i64>(1, std::min(CUS / tiles, depth / 512));
 }
 
@@ -477,8 +478,8 @@ Sizes sizes_of(i64 batch, i64 rows, i64 columns) {
     const i64 side = s.large ? Large::ROWS : Small::ROWS;
     s.mp = ceil_div(s.m, side) * side;
     s.np = ceil_div(s.n, side) * side;
-    s.gram_splits = s.large ? splits_of<Large>(batch, s.mp, s.np) : 1;
-    s.poly_splits = s.large ? splits_of<Large>(batch, s.mp, s.mp) : 1;
+    s.gram_splits = s.large ? splits_of(batch, s.mp, s.np) : 1;
+    s.poly_splits = s.large ? splits_of(batch, s.mp, s.mp) : 1;
     return s;
 }
 
@@ -561,12 +562,12 @@ i64 tiles_of(const Task& t) {
 template <typename K, Product WHAT>
 void multiply(Task t, i64 batch, int splits, float* sums, hipStream_t st) {
     if constexpr (std::is_same_v<K, Small>)
-        if (batch * tiles_of<Small, WHAT>(t) < FEW_TILES) return multiply<Tiny, WHAT>(t, batch, splits, sums, st);
+        if (batch * tiles_of<Small, WHAT>(t) < FEW_TILES) return multiply<Tiny, WHAT>(t, batch, 1, nullptr, st);
     const i64 tiles = tiles_of<K, WHAT>(t);
     t.splits = splits;
     t.partial = splits > 1 ? sums : nullptr;
     ortho_product<K, WHAT><<<dim3((unsigned)tiles, (unsigned)splits, (unsigned)batch), K::THREADS, 0, st>>>(t);
-    if constexpr (std::is_same_v<K, Large> && (WHAT == GRAM || WHAT == POLY))
+    if constexpr (K::SPLIT && (WHAT == GRAM || WHAT == POLY))
         if (splits > 1) ortho_join<K, WHAT><<<dim3((unsigned)tiles, K::FR, (unsigned)batch), K::THREADS, 0, st>>>(t);
 }
 
