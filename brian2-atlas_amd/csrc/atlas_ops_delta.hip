@@ -1610,7 +1610,7 @@ int atlas_ops_delta_forward(const AtlasDelta* a, int train, void* out, float* fi
         const dim3 keys((unsigned)d.chunks, (unsigned)d.heads, (unsigned)d.batch);
         with_kernel(d, a->type, d.key, [&](auto t, auto width, auto wide) {
             using T = decltype(t);
-            prepare<T, width(), wide()><<<keys, 256, 0, st>>>(d, tape, train);
+            prepare<T, width(), wide() || width() == 128><<<keys, 256, 0, st>>>(d, tape, train);  // keys that wide fill four values
             if (train) scan_forward<T, width(), true><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
             else scan_forward<T, width(), false><<<scan_grid(d), 4 * width(), 0, st>>>(d, tape, (T*)out, final_state);
         });
