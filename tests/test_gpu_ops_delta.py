@@ -406,3 +406,14 @@ def test_sizes_beyond_the_limits_are_invalid_arguments():
         ops.delta_rule(q, q, v, gate, gate)
     with pytest.raises(ValueError, match="65535"):
         ops.delta_rule_step(q[:, 0], q[:, 0], v[:, 0], gate[:, 0], gate[:, 0], torch.ones(65536, 1, 1, 1, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("key,value,heads,value_heads,time,lengths", [
+    (128, 128, 1, 1, 129, None), (128, 128, 1, 2, 192, None), (128, 40, 2, 2, 200, [200, 65]), (128, 128, 1, 3, 300, [300, 190]),
+    (128, 17, 1, 1, 321, None), (96, 40, 1, 2, 129, [128, 129]), (96, 40, 2, 2, 192, None), (96, 72, 1, 2, 256, [64, 256]),
+    (96, 40, 1, 1, 300, None), (65, 33, 1, 4, 385, [385, 0])])
+def test_wide_keys_over_many_chunks(key, value, heads, value_heads, time, lengths, dtype):
+    """Odd and even numbers of chunks, from three on, of the kernels for keys above 64."""
+    print(f"case: delta rule wide {key} {value} {heads} {value_heads} {time} {lengths} {dtype}", flush=True)
+    check(make(2, time, heads, value_heads, key, value, dtype, seed=key + time), lengths)

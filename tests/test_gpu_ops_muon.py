@@ -227,3 +227,57 @@ def test_coefficients_that_leave_the_range_are_refused():
             with pytest.raises(ValueError, match="coefficients"):
                 ops.muon_update(weight, m, momentum, learning_rate=0.1, steps=steps, coefficients=coefficients)
             assert (weight == 1).all() and (momentum == 1).all()
+
+
+@pytest.mark.parametrize("shape", [(2050, 4100), (4100, 1990), (700, 1300)])
+def test_update_of_large_matrices(shape):
+    """The weight written out of the tiles of 256 x 128, both orientations, ragged, and of those of 64 x 64."""
+    print(f"case: muon large {shape}", flush=True)
+    weight, gradient, momentum = make(shape, seed=1), make(shape, seed=2), make(shape, seed=3)
+    options = dict(learning_rate=0.05, factor=0.9, weight_decay=0.1)
+    next_momentum = 0.9 * momentum.double() + gradient.double()
+    x = gradient.double() + 0.9 * next_momentum
+    x = x / (torch.linalg.norm(x) + 1e-7)
+    a, b, c = ops.COEFFICIENTS
+    for _ in range(5):
+        if shape[0] <= shape[1]:
+            g = x @ x.T.contiguous()
+            x = a * x + (b * g + c * (g @ g)) @ x
+        else:
+            g = x.T.contiguous() @ x
+            x = a * x + x @ (b * g + c * (g @ g))
+    rate = 0.05 * math.sqrt(max(1.0, shape[1] / shape[0]))
+    want = (1.0 - 0.05 * 0.1) * weight.double() - rate * x
+    start = weight.double()
+    ops.muon_update(weight, gradient, momentum, **options)
+    assert float((momentum.double() - next_momentum).norm() / next_momentum.norm()) <= 2e-7
+    # the step taken, to 2e-5 of it, and the weight's own rounding
+    bound = 2e-5 * float((want - start).norm()) + 2.0 ** -24 * float(want.norm())
+    assert float((weight.double() - want).norm()) <= bound
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_update_with_gradients_of_other_strides(dtype):
+    print(f"case: muon strides {dtype}", flush=True)
+    base = make((4, 60, 90), dtype, seed=5)
+    wide = make((130, 80), dtype, seed=6)
+    for gradient in (base.transpose(0, 1), base[:, 3:50:2, 5:77], base.transpose(1, 2), base[1].T, base[0:1].expand(3, 60, 90),
+                     wide[::2, 1:78], wide[5:6].expand(30, 80)):
+        results = []
+        for g in (gradient, gradient.contiguous()):
+            weight, momentum = make(g.shape, seed=1), make(g.shape, seed=2)
+            ops.muon_update(weight, g, momentum, learning_rate=0.1)
+            results.append((weight, momentum))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("rank", [1, 4])
+def test_exactly_low_rank(rank):
+    """Factors of small whole numbers: their product is exact in float32, so nothing but the iteration's own rounding
+    stands outside the rank, held to the bound above."""
+    print(f"case: orthogonalize exact rank {rank}", flush=True)
+    g = torch.Generator().manual_seed(7)
+    left, right = (torch.randint(-7, 8, s, generator=g).float() for s in ((200, rank), (rank, 300)))
+    m = (left @ right).cuda()
+    got, want = ops.orthogonalize(m), oo.orthogonalize(numpy(m))
+    assert np.linalg.norm(numpy(got) - want) <= 1e-4 * math.sqrt(rank)

@@ -177,3 +177,14 @@ def test_another_stream():
         got = ops.layer_norm(x)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width", [(33001, 20), (26001, 48), (9001, 300), (6001, 500), (9001, 1000), (2000, 1500),
+                                        (2600, 2000), (1700, 3000), (2200, 4000), (150, 6000), (150, 9000)])
+def test_several_rows_in_each_place(rows, width, dtype):
+    """More rows than the grid has places for, all of them different, in every layout of a row: the next row's fetch,
+    the shared sums and the column sums go round."""
+    print(f"case: layer norm rows {rows} x {width} {dtype}", flush=True)
+    x, grad = make((rows, width), dtype, 4), make((rows, width), dtype, 5, 0.1)
+    check(x, make(width, F32, 2, 1.0), make(width, F32, 3, 0.0), grad)

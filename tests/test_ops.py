@@ -2,6 +2,7 @@
 everything that needs no GPU.  The reference is pinned by torch autograd in float64 of separately written
 forwards and by central differences."""
 import ctypes
+import inspect
 import re
 from pathlib import Path
 
@@ -257,3 +258,21 @@ def test_the_abi_refuses_coefficients_beyond_the_planes():
         packed = ops._ORTHOGONAL.pack(4096, 1, 4, 4, 16, 4, 0, 4096, 0, 0, 0, 1, steps, 0.9, 1e-7, 1.0, 0.1, *coefficients)
         rc = lib.atlas_ops_orthogonalize(packed, 4096, None, ctypes.addressof(err), 256)  # the address is never read
         assert rc == 7 and b"coefficients" in err.value, (steps, coefficients, err.value)
+
+
+def test_a_decay_gradient_taken_too_early_is_caught(monkeypatch):
+    """The gradient of log_decay taken before the correction's own share has left the state's gradient: both the
+    comparison with autograd and that with differences have to see it."""
+    right = """                D = D - np.outer(kt, de)
+                g["log_decay"][b, t, h] = (D * faded).sum()
+"""
+    wrong = "".join(reversed(right.splitlines(keepends=True)))
+    source = inspect.getsource(oo.delta_rule_backward)
+    assert source.count(right) == 1
+    planted = {}
+    exec(source.replace(right, wrong), vars(oo), planted)
+    monkeypatch.setattr(oo, "delta_rule_backward", planted["delta_rule_backward"])
+    with pytest.raises(AssertionError, match="log_decay"):
+        test_delta_reference_matches_autograd()
+    with pytest.raises(AssertionError, match="log_decay"):
+        test_delta_reference_matches_differences(None)
