@@ -89,7 +89,8 @@ def _call(device: int, entry, *args) -> None:
 
 def _tensor(t, name: str, device=None, types=TYPES, shape=None):
     """The checks every tensor passes; returns its device's index."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0:
         raise ValueError(f"{name} must be a tensor on the GPU")
     if t.dtype not in types:
         raise ValueError(f"{name} is {t.dtype}, expected {' or '.join(str(x) for x in types)}")
@@ -99,10 +100,9 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
         raise ValueError(f"{name} requires a gradient: gradients are explicit here, call under torch.no_grad()")
     if t.is_neg():
         raise ValueError(f"{name} is a view that negates what its memory holds: pass {name}.resolve_neg()")
-    # a level is open only within forward_ad.dual_level(), and disabled within an autograd.Function
+    # forward mode: a level is open only within forward_ad.dual_level(), and disabled within an autograd.Function
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} has a tangent: forward-mode derivatives are not computed here")
-    index = t.get_device()
     if device is not None and index != device:
         raise ValueError(f"{name} is on GPU {index}, expected {device}")
     return index
@@ -133,12 +133,10 @@ def _workspace(size: int, like):
 
 
 # ------------------------------------------------------------------------------ layer normalisation
-def _rows(x):
+def _rows(x, rows, width):
     """x as rows of its last axis: the packed AtlasRows and the tensor it points into (a contiguous copy
     where the leading axes are not one or two strides)."""
-    width = x.shape[-1]
     if x.is_contiguous():
-        rows = x.numel() // width
         return _ROWS.pack(x.data_ptr(), rows, 0, width), x
     if width == 1 or x.stride(-1) == 1:
         axes = []  # (size, stride) from the innermost, neighbours joined
@@ -152,7 +150,7 @@ def _rows(x):
         if len(axes) <= 2:
             axes += [(1, 0)] * (2 - len(axes))
             return _ROWS.pack(x.data_ptr(), axes[0][0], axes[1][1], axes[0][1]), x
-    return _rows(x.contiguous())
+    return _rows(x.contiguous(), rows, width)
 
 
 _NORM_WEIGHTS = {torch.float32: {torch.float32: 0}, torch.bfloat16: TYPES}
@@ -164,7 +162,7 @@ def _norm_weights(x, width, weight, bias, device):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None:
             _tensor(t, name, device, types)
-            if t.dim() != 1 or t.shape[0] != width:
+            if t.dim() != 1 or t.numel() != width:
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(width,)}")
             code = types[t.dtype]
     if weight is not None:
@@ -193,7 +191,7 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, statistics: bool
         mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device).unbind()
     rows = x.numel() // width
     if rows:
-        packed, keep = _rows(x)
+        packed, keep = _rows(x, rows, width)
         _call(device, library().atlas_ops_layer_norm, packed, rows, width, TYPES[x.dtype],
               None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), code, eps,
               y.data_ptr(), mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None)
@@ -223,8 +221,8 @@ def layer_norm_backward(grad, x, weight, mean, rstd, *, sums: bool = True):
         dweight, dbias = torch.empty((2, width), dtype=wtype, device=x.device).unbind()
         workspace = _workspace(lib.atlas_ops_layer_norm_workspace(rows, width, type_), x)
     if rows or sums:
-        packed_grad, keep_grad = _rows(grad) if rows else (None, None)
-        packed, keep = _rows(x) if rows else (None, None)
+        packed_grad, keep_grad = _rows(grad, rows, width) if rows else (None, None)
+        packed, keep = _rows(x, rows, width) if rows else (None, None)
         mean, rstd = mean.contiguous(), rstd.contiguous()
         _call(device, lib.atlas_ops_layer_norm_backward, packed_grad, packed, rows, width, type_,
               None if weight is None else weight.data_ptr(), code, mean.data_ptr(), rstd.data_ptr(),
