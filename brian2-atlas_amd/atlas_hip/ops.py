@@ -412,7 +412,8 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, lengths=None, scale: flo
     head h uses the q and k of head ``h // (value heads / heads)``.  log_decay (None: no decay) and beta
     (batch, time, value heads): float32 or bfloat16; a log_decay of -inf empties the state.  state: float32 (batch,
     value heads, key, value).  lengths: int32 (batch,), tokens from a sequence's length on leave its state
-    unchanged and give zeros.  scale: by default ``1 / sqrt(key)``.
+    unchanged, whatever is in it, and give zeros.  scale: by default ``1 / sqrt(key)``.  A NaN or an infinity reaches its own
+    and later tokens only.  At most 65535 sequences and value heads, values up to 2^20 wide.
 
     Returns (out, final state); with ``tape`` (out, final state, tape), the tape for ``delta_rule_backward``."""
     if state is not None and isinstance(state, torch.Tensor):
@@ -440,7 +441,8 @@ def delta_rule(q, k, v, log_decay, beta, state=None, *, lengths=None, scale: flo
 def delta_rule_backward(grad_out, grad_state, tape: DeltaTape) -> dict:
     """The gradients of ``delta_rule`` from those of out (of its type) and of the final state (float32, or None
     for zeros): a dict with ``q, k, v, log_decay, beta, state``, each of its input's type, None for an input that
-    was not given.  Heads of q and k that value heads share get the sum.  The same bits on every run."""
+    was not given.  Heads of q and k that value heads share get the sum.  The same bits on every run.  A NaN or an infinity
+    of a used token may reach the gradients of every token of its sequence."""
     if not isinstance(tape, DeltaTape):
         raise ValueError("tape must be the one that delta_rule returned")
     p = tape.problem

@@ -336,8 +336,8 @@ __device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.ti
 
 // 32 columns of a row from column c0, as loaded and as an operand in the order above, zeros beyond the row's
 // width.  WIDE: rows of four values or more, read four at a time without alignment; where the row ends among
-// them its last four are read and shifted down (prepare, 16384 tokens of 16 heads of 128: 98 us, a value at a time
-// 166; gradients, 2 x 4099: 337 and 356).
+// them its last four are read and shifted down (a value at a time, prepare took 68 us more for 16384 tokens of 16 heads
+// of 128, gradients 19 us more for 2 x 4099).
 template <typename T, bool WIDE>
 struct Row {
     struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; };
@@ -516,8 +516,8 @@ __device__ __forceinline__ float decay(const float* sum, const float* remainder,
 // value head that shares them the gates, the scores and the inverse, 16 x 16 blocks by forward substitution, joined in
 // pairs: the inverse of [[a, 0], [m, c]] has -c^-1 m a^-1 below.  Its steps wait for one another, so what counts is
 // how many workgroups a CU holds: 168 registers, three of them with bfloat16 (2 x 4099 tokens of 4 x 4 heads of
-// 128: 59 us with three, 82 with two; 16384 of 16 heads 114 us), two by their LDS with float32 (256 x 100 of 4 heads
-// of 64: 104 us).
+// 128: 59 us with three, 82 with two; 16384 of 16 heads 119 us), two by their LDS with float32 (256 x 100 of 4 heads
+// of 64: 102 us).
 template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train) {
     constexpr int N = sizeof(T) == 2 ? 1 : 3, KB = DK / 32;
@@ -725,11 +725,11 @@ __global__ void __launch_bounds__(256, 3) prepare(Delta d, Tape tape, int train)
 // are fetched while the chunk before it runs, and as many waves again take the outputs of the chunk before from
 // the states and errors that the first leave in LDS: in inference neither goes to memory.
 //
-// Measured: 16384 tokens of 16 heads of 128, bfloat16, 256 chunks one after the other, 482 us or 1.9 us a chunk (a
+// Measured: 16384 tokens of 16 heads of 128, bfloat16, 256 chunks one after the other, 480 us or 1.9 us a chunk (a
 // kernel of its own for the outputs: 440 and 178 us, and the states written).  The three exchanges, their MFMA latencies
 // and the splits between them make 1.5 us of that; the rest is operands that arrive late and what the outputs take
 // of the load path (with queries loaded from the caller's rows, 8 bytes a lane, 577 us; a value at a time, 1207).
-// 256 x 100 of 4 heads of 64, float32: 160 us for 4096 workgroups of two chunks, bound by the operands that every 16
+// 256 x 100 of 4 heads of 64, float32: 157 us for 4096 workgroups of two chunks, bound by the operands that every 16
 // columns read anew from the L2.
 //
 // Workgroups of one head run on one XCD (they share its operands in the L2): workgroups go to the 8 XCDs
@@ -867,7 +867,8 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_forward(Delta d, Tape tape, T*
         }
     // Chunks ahead that keys are fetched (16384 tokens of 16 heads: two take 65 us less than one); where
     // the operands of one chunk alone fill the registers, each is fetched only after those of the product
-    // before it are used (TIGHT; 256 x 100 of 4 heads of 64, float32: 163 us, two workgroups per CU with spills 226).
+    // before it are used (TIGHT; 256 x 100 of 4 heads of 64, float32: 157 us with 45 to 47 registers spilled, otherwise 226
+    // with 52 to 64).
     constexpr bool TIGHT = DK == 64 && N == 3;
     constexpr int DEPTH = DK == 128 && N == 1 ? 2 : 1;
     Pieces<N> k[DEPTH][4], kt[DEPTH][2][2];
@@ -1216,8 +1217,9 @@ __global__ void __launch_bounds__(DK * 4, 2) scan_backward(Delta d, Tape tape, B
 // of half w / 4 of the key indices, and its half chooses which of the two C x C products it takes.
 //
 // Bound by its chain of stages (loads, turns, barrier, products) with one workgroup per CU: 2 x 4099 of 4 x 4 heads of
-// 128, bfloat16, 343 us, about 270 TFLOP/s of MFMA, a quarter of the rate; 256 x 100 of 4 heads of 64, float32,
-// 165 us.  Fetching a stage ahead costs more in registers than it hides (365 and 203 us), and so does half the
+// 128, bfloat16, 335 us, about 275 TFLOP/s of MFMA, a quarter of the rate; 256 x 100 of 4 heads of 64, float32,
+// 167 us.  Of its 244 to 256 registers 40 to 68 are spilled with keys above 64, 16 with bfloat16 values of fewer than four
+// columns, else none.  Fetching a stage ahead costs more in registers than it hides (365 and 203 us), and so does half the
 // registers for twice the workgroups where keys are 64 wide (285 us).
 template <typename T, int DK, bool WIDE>
 __global__ void __launch_bounds__(512, 2) gradients(Delta d, Tape tape, Back back, T* __restrict__ dq, T* __restrict__ dk,

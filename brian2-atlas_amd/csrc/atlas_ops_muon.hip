@@ -307,9 +307,9 @@ __device__ __forceinline__ void finish(const Task& t, i64 b, int r, int c, float
     }
 }
 
-// 4096 x 2048: (b A + c A A) X 123 us, 838 TFLOP/s of float16 MFMA (a large library product of that type: 1093), bound
-// by what an MFMA waits for its operands from LDS; X X^T 68 us and A A 39 us for their triangles, whose 72 tiles are
-// split in parts that ortho_join adds in 12 and 13 us.  256 x 256: 5 us each, the way of a few stages from memory
+// 4096 x 2048: (b A + c A A) X 120 us, 859 TFLOP/s of float16 MFMA (a large library product of that type: 1093), bound
+// by what an MFMA waits for its operands from LDS; X X^T 67 us and A A 38 us for their triangles, whose 72 tiles are
+// split in parts that ortho_join adds in 11 and 13 us.  256 x 256: 5 us each, the way of a few stages from memory
 // and the launch.
 //
 // One tile of Left Right^T.  While a stage is multiplied out of LDS, the next comes from memory into registers,
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(K::THREADS) ortho_join(Task t) {
 
 // Tiles of 256 x 128 on eight waves keep the MFMAs fed from LDS (each value read serves 64 products); those of
 // 64 x 64, and of 32 x 32 below 192 of these, spread small matrices over the CUs, where a stage's way from memory
-// is what takes the time (all five steps, 64 / 32: 256 x 256 107 / 83 us, 768 x 768 218 / 176, 1024 x 1024 273 / 255;
+// is what takes the time (all five steps, measured side by side, 64 / 32: 256 x 256 107 / 83 us, 768 x 768 218 / 176, 1024 x 1024 273 / 255;
 // 32 for up to 400 tiles costs 1536 x 1536 563 instead of 525).
 typedef Cut<256, 128, 4, 2, 32, true> Large;
 typedef Cut<64, 64, 2, 2, 32, false> Small;

@@ -246,8 +246,8 @@ __global__ void __launch_bounds__(256) norm_forward_long(Rows x, int width, cons
 // partial[b * 2 * width], of db right after them.
 //
 // A row's loads wait for the reduction of the row before; three workgroups per CU hide that where their
-// registers allow it (32768 x 4096 bfloat16: 298 us with two of 187 registers, 239 with three of 168;
-// four would spill, 667).  Now 224 us there, 3.6 TB/s of the two reads and the write; 25600 x 256 float32 18.1.
+// registers allow it (32768 x 4096 bfloat16: 298 us with two of 187 registers, 239 with three of 168 although 8 are
+// spilled, 19 with a bfloat16 weight; with four, 667).  Now 224 us there, 3.6 TB/s of the two reads and the write; 25600 x 256 float32 18.1.
 template <typename T, typename W, int LANES, int CH>
 __global__ void __launch_bounds__(256, CH <= 2 ? 3 : 2) norm_backward(Rows grad, Rows x, i64 rows, int width,
                                                      const W* __restrict__ weight, const float* __restrict__ mean_in,
@@ -436,7 +436,8 @@ __global__ void __launch_bounds__(1024) norm_reduce(i64 blocks, i64 width, const
 // The layout of a row by its units of 16 bytes.  16 lanes up to 16 units, 16 rows per workgroup (262144 x 64 float32:
 // forward 24 us, backward 41, and 79, 108 with a wave each).  A wave up to 4 units per lane forward (32768 x 2048
 // bfloat16 69 us, a workgroup 84), up to 2 backward, where a row's registers are twice as many (a workgroup 146 us,
-// a wave 209).  A workgroup up to 4 per lane, backward of bfloat16 up to 2: the registers of more cost the workgroups that hide
+// a wave 209; the bytes take 77, and half the units of that layout, of 512, lie beyond a row of 129 to 256 units).  A
+// workgroup up to 4 per lane, backward of bfloat16 up to 2: the registers of more cost the workgroups that hide
 // the loads, and reading the rows again from the caches is faster (4 against long: 8192 x 4096 float32 60 to 62 and 152
 // to 164 us; 8192 x 8192 bfloat16 71 to 79 and 314 to 228; 8 against long: 4096 x 8192 float32 99 to 77 and 213 to 168).
 struct Shape {

@@ -417,3 +417,19 @@ def test_wide_keys_over_many_chunks(key, value, heads, value_heads, time, length
     """Odd and even numbers of chunks, from three on, of the kernels for keys above 64."""
     print(f"case: delta rule wide {key} {value} {heads} {value_heads} {time} {lengths} {dtype}", flush=True)
     check(make(2, time, heads, value_heads, key, value, dtype, seed=key + time), lengths)
+
+
+def test_a_faulty_key_or_query_stays_behind_its_token():
+    """A query's fault reaches its own output alone, a key's its own and later tokens of its head."""
+    print("case: delta rule faulty keys", flush=True)
+    for fault in (float("nan"), float("inf")):
+        for tokens in (150, 10):
+            case = make(2, 150, 2, 4, 24, 40, seed=18)
+            case["q"][0, 5, 1, 2] = fault
+            case["k"][1, 5, 0, 3] = fault
+            out, state = ops.delta_rule(*(case[n] if n == "state" else case[n][:, :tokens] for n in INPUTS))
+            assert not torch.isfinite(out[0, 5, 2:]).any() and torch.isfinite(out[0, 5, :2]).all()
+            out[0, 5] = 0.0
+            assert torch.isfinite(out[0]).all() and torch.isfinite(state[0]).all()
+            assert torch.isfinite(out[1, :5]).all() and torch.isfinite(out[1, :, 2:]).all() and torch.isfinite(state[1, 2:]).all()
+            assert not torch.isfinite(out[1, 6:, :2]).any() and not torch.isfinite(state[1, :2]).all(dim=-2).any()
