@@ -25,7 +25,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "device/atlas_ops.h"
+#include "device/atlas_mma.h"
 
 namespace atlas_ops {
 namespace {
@@ -33,15 +33,6 @@ namespace {
 constexpr int C = 64;         // tokens per chunk
 constexpr int CP = C + 4;     // pitch of a C x C matrix in LDS
 constexpr float LOWEST = -120.0f;
-
-struct Tensor {
-    const void* data;
-    i64 batch, time, head;
-    template <typename T>
-    __device__ __forceinline__ const T* at(i64 b, i64 t, i64 h) const {
-        return (const T*)data + b * batch + t * time + h * head;
-    }
-};
 
 struct Delta {
     Tensor q, k, v, decay, beta;
@@ -215,121 +206,6 @@ __global__ void __launch_bounds__(256) step_kernel(Delta d, T* __restrict__ out,
 }
 
 // ------------------------------------------------------------------ what the chunk kernels share
-// Products run on bfloat16 MFMA blocks of 16 x 16 with 32 sum indices, at float32's accuracy: a float
-// is the sum of three bfloat16 pieces (to 2^-24), a product takes the pieces' products down to that
-// size, three where one side is bfloat16 already and six where neither is, summed in float32.  Float32
-// MFMA would take 16 times the cycles of one such product.
-//
-// Lane l gives 8 values of row l % 16 of A, 8 of column l % 16 of B, and receives rows 4 (l / 16) + j of
-// column l % 16.  The sum may take its indices in any order that A and B share: here lane group g = l / 16
-// holds the indices 4 g + j and 16 + 4 g + j of 32, so that two blocks of results on top of each other are, without
-// any exchange, the B operand of a product that sums over their rows, and the A operand of one whose rows
-// are their columns.
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float float8_t __attribute__((ext_vector_type(8)));
-typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
-
-constexpr float4_t ZERO = {0.0f, 0.0f, 0.0f, 0.0f};
-
-// N pieces of 8 values, the largest first.
-template <int N>
-struct Pieces {
-    bf16x8 p[N];
-};
-
-// N pieces of 4 values: half an operand.
-template <int N>
-struct Halves {
-    bf16x4 p[N];
-};
-
-__device__ __forceinline__ float4_t widen(bf16x4 v) {
-    const uint2_t bits = __builtin_bit_cast(uint2_t, v);
-    return float4_t{__uint_as_float(bits[0] << 16), __uint_as_float(bits[0] & 0xFFFF0000u),
-                    __uint_as_float(bits[1] << 16), __uint_as_float(bits[1] & 0xFFFF0000u)};
-}
-
-template <int N>
-__device__ __forceinline__ Halves<N> split(float4_t v) {
-    Halves<N> h;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        h.p[i] = __builtin_convertvector(v, bf16x4);
-        if (i + 1 < N) v -= widen(h.p[i]);
-    }
-    return h;
-}
-
-template <int N>
-__device__ __forceinline__ Pieces<N> join(const Halves<N>& a, const Halves<N>& b) {
-    Pieces<N> r;
-#pragma unroll
-    for (int i = 0; i < N; ++i) r.p[i] = __builtin_shufflevector(a.p[i], b.p[i], 0, 1, 2, 3, 4, 5, 6, 7);
-    return r;
-}
-
-template <int N>
-__device__ __forceinline__ Pieces<N> split(float4_t a, float4_t b) {
-    return join(split<N>(a), split<N>(b));
-}
-
-// c + A B: the products of pieces whose order together is below three (below two where no side has
-// three), the smallest first.
-template <int NA, int NB>
-__device__ __forceinline__ float4_t mma(const Pieces<NA>& a, const Pieces<NB>& b, float4_t c) {
-    constexpr int ORDERS = NA > NB ? NA : NB;
-#pragma unroll
-    for (int order = ORDERS - 1; order >= 0; --order)
-#pragma unroll
-        for (int i = 0; i <= order; ++i)
-            if (i < NA && order - i < NB)
-                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[order - i], c, 0, 0, 0);
-    return c;
-}
-
-// c + A B in two chains, the smaller products apart from the larger: half the latency of mma.
-template <int NA, int NB>
-__device__ __forceinline__ void mma2(const Pieces<NA>& a, const Pieces<NB>& b, float4_t& large, float4_t& small) {
-    constexpr int ORDERS = NA > NB ? NA : NB;
-#pragma unroll
-    for (int order = ORDERS - 1; order >= 0; --order)
-#pragma unroll
-        for (int i = 0; i <= order; ++i)
-            if (i < NA && order - i < NB) {
-                float4_t& c = order == ORDERS - 1 ? small : large;
-                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[order - i], c, 0, 0, 0);
-            }
-}
-
-struct Lane {
-    int id, col, quad;  // l, l % 16, 4 (l / 16)
-    __device__ __forceinline__ Lane() : id(threadIdx.x % 64), col(threadIdx.x % 16), quad(threadIdx.x % 64 / 16 * 4) {}
-};
-
-// Operands in memory: N pieces, 16 bytes per lane each.
-template <int N>
-__device__ __forceinline__ Pieces<N> fetch(const bf16_t* p, i64 operand, const Lane& l) {
-    Pieces<N> r;
-#pragma unroll
-    for (int i = 0; i < N; ++i) r.p[i] = *(const bf16x8*)(p + ((operand * N + i) * 64 + l.id) * 8);
-    return r;
-}
-
-template <int N>
-__device__ __forceinline__ void put(bf16_t* p, i64 operand, const Lane& l, const Pieces<N>& v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *(bf16x8*)(p + ((operand * N + i) * 64 + l.id) * 8) = v.p[i];
-}
-
-// Half `half` of an operand: its indices 16 half ...
-template <int N>
-__device__ __forceinline__ void put_half(bf16_t* p, i64 operand, int half, const Lane& l, const Halves<N>& v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) *(bf16x4*)(p + ((operand * N + i) * 64 + l.id) * 8 + 4 * half) = v.p[i];
-}
-
 // Loads of the caller's tensors stand behind no branch (there each would be waited for before the next): they go
 // to a row and column that exist, and what lies outside is replaced by zero afterwards.
 __device__ __forceinline__ i64 existing(i64 t, const Delta& d) { return t < d.time ? t : d.time - 1; }
@@ -435,19 +311,6 @@ __device__ __forceinline__ float4_t block(const float* m, i64 r, i64 c, i64 bloc
 
 __device__ __forceinline__ void put_block(float* m, i64 r, i64 c, i64 blocks, const Lane& l, float4_t v) {
     *(float4_t*)(m + ((r * blocks + c) * 64 + l.id) * 4) = v;
-}
-
-// Keeps what stands before it before it.  A scan's loads return in the order of their issue, so one that the
-// scheduler moves behind others is waited for together with them.
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
-
-// Workgroup barrier for LDS alone: loads and stores of global memory stay in flight across it.
-__device__ __forceinline__ void lds_barrier() {
-    in_order();
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    in_order();
 }
 
 // A product with a triangular matrix adds zeros times the terms it masks, which a NaN or an infinity
