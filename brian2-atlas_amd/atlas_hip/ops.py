@@ -1,10 +1,11 @@
-"""Operators of sequence layers on the MI355X: layer normalisation, the gated delta rule and the
-orthogonalised weight update.
+"""Operators of sequence layers on the MI355X: normalisation, layers of plastic synapses, the embedding of
+symbols, dropout and the orthogonalised weight update.
 
 Where ``rsnn`` trains one fixed recurrent network, these are the parts around a recurrent layer of
-one's own: ``layer_norm`` for its currents, ``delta_rule`` as a layer whose synapses decay and learn
-within a sequence (``delta_rule_step`` for one tick of a stream), and ``muon_update`` for its dense
-matrices.  They take and return torch tensors on the GPU.  Each call enqueues hand-written kernels of
+one's own: ``embedding`` for inputs that are symbols, ``layer_norm`` for its currents or ``rms_norm`` for a stream of
+several layers, ``delta_rule`` and ``linear_attention`` as layers whose synapses decay and learn within a sequence
+(``delta_rule_step`` and ``linear_attention_step`` for one tick of a stream), ``dropout``, and ``muon_update`` for its
+dense matrices.  They take and return torch tensors on the GPU.  Each call enqueues hand-written kernels of
 libatlas_ops_hip.so on the current stream of the tensors' device and returns without waiting;
 workspaces come from torch's allocator.  Gradients are explicit calls, as the trainers' are: a tensor that
 autograd follows is refused unless gradients are disabled, and so is a dual tensor of forward mode.  There is
@@ -31,7 +32,10 @@ LIBRARY = Path(__file__).resolve().parent.parent / "libatlas_ops_hip.so"
 EXPORTS = ["atlas_ops_layer_norm", "atlas_ops_layer_norm_workspace", "atlas_ops_layer_norm_backward",
            "atlas_ops_orthogonalize_workspace", "atlas_ops_orthogonalize", "atlas_ops_delta_step",
            "atlas_ops_delta_workspace", "atlas_ops_delta_forward", "atlas_ops_delta_backward_workspace",
-           "atlas_ops_delta_backward"]
+           "atlas_ops_delta_backward", "atlas_ops_rms_norm", "atlas_ops_rms_norm_workspace", "atlas_ops_rms_norm_backward",
+           "atlas_ops_embedding", "atlas_ops_embedding_workspace", "atlas_ops_embedding_backward", "atlas_ops_dropout",
+           "atlas_ops_linear_step", "atlas_ops_linear_workspace", "atlas_ops_linear_forward",
+           "atlas_ops_linear_backward_workspace", "atlas_ops_linear_backward"]
 TYPES = {torch.float32: 0, torch.bfloat16: 1}
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_KEY = 128
@@ -63,6 +67,19 @@ def library() -> ctypes.CDLL:
         lib.atlas_ops_delta_forward.argtypes = [text, i32, vp, vp, vp, vp, *err]
         lib.atlas_ops_delta_backward_workspace.argtypes = [text]
         lib.atlas_ops_delta_backward.argtypes = [text, vp, vp, text, vp, vp, vp, vp, vp, vp, vp, vp, vp, *err]
+        f64, u64 = ctypes.c_double, ctypes.c_uint64
+        lib.atlas_ops_rms_norm.argtypes = [text, text, i64, i64, i32, vp, i32, f32, vp, vp, vp, vp, vp, *err]
+        lib.atlas_ops_rms_norm_workspace.argtypes = [i64, i64, i32]
+        lib.atlas_ops_rms_norm_backward.argtypes = [text, text, text, i64, i64, i32, vp, i32, vp, vp, vp, vp, vp, *err]
+        lib.atlas_ops_embedding.argtypes = [vp, i64, i64, i64, i32, vp, i32, i64, f32, vp, vp, *err]
+        lib.atlas_ops_embedding_workspace.argtypes = [i64, i64, i64, i32]
+        lib.atlas_ops_embedding_backward.argtypes = [text, vp, i32, i64, i64, i64, i32, i32, f32, vp, vp, vp, *err]
+        lib.atlas_ops_dropout.argtypes = [vp, vp, i64, i32, f64, u64, u64, u64, vp, vp, vp, *err]
+        lib.atlas_ops_linear_step.argtypes = [text, vp, vp, vp, *err]
+        lib.atlas_ops_linear_workspace.argtypes = [text, i32]
+        lib.atlas_ops_linear_forward.argtypes = [text, i32, vp, vp, vp, vp, *err]
+        lib.atlas_ops_linear_backward_workspace.argtypes = [text]
+        lib.atlas_ops_linear_backward.argtypes = [text, vp, vp, text, vp, vp, vp, vp, vp, i32, vp, vp, vp, *err]
         for name in EXPORTS:
             getattr(lib, name).restype = i64 if name.endswith("_workspace") else i32
         _lib = lib
@@ -108,7 +125,7 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
     return index
 
 
-_F32, _I32 = {torch.float32: 0}, {torch.int32: 0}
+_F32, _I32, _I64 = {torch.float32: 0}, {torch.int32: 0}, {torch.int64: 0}
 _SAME = {t: {t: 0} for t in TYPES}
 
 
@@ -126,6 +143,10 @@ def _overlap(a, b):
 def _empty(t):
     """A contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _last(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _workspace(size: int, like):
@@ -231,6 +252,178 @@ def layer_norm_backward(grad, x, weight, mean, rstd, *, sums: bool = True):
     return dx, dweight, dbias
 
 
+# --------------------------------------------------------- root-mean-square norm of a stream
+def _rms_arguments(x, weight, residual):
+    """The device, width and rows of x and the checked weight with its type's code."""
+    device = _tensor(x, "x")
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
+        raise ValueError("x needs a last axis to normalise")
+    if residual is not None:
+        _tensor(residual, "residual", device, _SAME[x.dtype], x.shape)
+    weight, _, code = _norm_weights(x, width, weight, None, device)
+    return device, width, x.numel() // width, weight, code
+
+
+def _rms_forward(device, x, residual, rows, width, weight, code, eps, y, scale, total, rstd):
+    packed, keep = _rows(x, rows, width)
+    added, keep_added = (None, None) if residual is None else _rows(residual, rows, width)
+    _call(device, library().atlas_ops_rms_norm, packed, added, rows, width, TYPES[x.dtype],
+          None if weight is None else weight.data_ptr(), code, eps, y.data_ptr(), None if scale is None else scale.data_ptr(),
+          None if total is None else total.data_ptr(), None if rstd is None else rstd.data_ptr())
+
+
+def rms_norm(x, weight=None, residual=None, *, eps: float = 1e-5, statistics: bool = False):
+    """``total * rstd * weight`` over the last axis, ``total = x + residual`` (rounded to x's type; x alone without a
+    residual), ``rstd = 1 / sqrt(mean(total ** 2) + eps)``.
+
+    x: float32 or bfloat16; residual: of x's shape and type; weight: float32 or x's type.  Returns y, or (y, total) with a
+    residual, both contiguous and of x's type; ``statistics`` adds rstd at the end, float32 of x's leading shape, which
+    ``rms_norm_backward`` takes."""
+    device, width, rows, weight, code = _rms_arguments(x, weight, residual)
+    y = _empty(x)
+    total = None if residual is None else _empty(x)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if statistics else None
+    if rows:
+        _rms_forward(device, x, residual, rows, width, weight, code, eps, y, None, total, rstd)
+    if residual is None and not statistics:
+        return y
+    return (y, *(t for t in (total, rstd) if t is not None))
+
+
+def rms_norm_8bit(x, weight=None, residual=None, *, eps: float = 1e-5):
+    """``rms_norm`` for a product of 8 bits: (values, scale), or (values, scale, total) with a residual.
+
+    values: float8_e4m3fn, the norm's result over its row's scale, rounded once; scale: float32 of x's leading shape, the
+    row's largest magnitude / 448, at least 2^-126.  A NaN has no part in the scale; an infinity makes it infinite."""
+    device, width, rows, weight, code = _rms_arguments(x, weight, residual)
+    values = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    total = None if residual is None else _empty(x)
+    if rows:
+        _rms_forward(device, x, residual, rows, width, weight, code, eps, values, scale, total, None)
+    return (values, scale) if residual is None else (values, scale, total)
+
+
+def rms_norm_backward(grad, total, weight, rstd, *, grad_total=None, sums: bool = True):
+    """The gradients (dx, dweight) of ``rms_norm`` from that of y; dx is that of x and of the residual alike.
+
+    total: x + residual as returned (x without a residual); grad_total: the gradient of total from where the stream goes
+    on, added to dx.  weight may be None (all ones; dweight is then float32).  Without ``sums`` dweight is None.  The sums
+    over the rows are taken in float32 in a fixed order: the same bits on every run."""
+    device = _tensor(total, "total")
+    width = total.shape[-1] if total.dim() else 0
+    if width < 1:
+        raise ValueError("total needs a last axis to normalise")
+    same = _SAME[total.dtype]
+    _tensor(grad, "grad", device, same, total.shape)
+    if grad_total is not None:
+        _tensor(grad_total, "grad_total", device, same, total.shape)
+    weight, _, code = _norm_weights(total, width, weight, None, device)
+    _tensor(rstd, "rstd", device, _F32, total.shape[:-1])
+    rows, type_ = total.numel() // width, TYPES[total.dtype]
+    dx = _empty(total)
+    dweight = workspace = None
+    lib = library()
+    if sums:
+        dweight = torch.empty(width, dtype=torch.float32 if weight is None else weight.dtype, device=total.device)
+        workspace = _workspace(lib.atlas_ops_rms_norm_workspace(rows, width, type_), total)
+    if rows or sums:
+        packed_grad, keep_grad = _rows(grad, rows, width) if rows else (None, None)
+        packed, keep = _rows(total, rows, width) if rows else (None, None)
+        packed_stream, keep_stream = _rows(grad_total, rows, width) if rows and grad_total is not None else (None, None)
+        rstd = rstd.contiguous()
+        _call(device, lib.atlas_ops_rms_norm_backward, packed_grad, packed, packed_stream, rows, width, type_,
+              None if weight is None else weight.data_ptr(), code, rstd.data_ptr(), dx.data_ptr(),
+              dweight.data_ptr() if sums else None, workspace.data_ptr() if sums else None)
+    return dx, dweight
+
+
+# ------------------------------------------------------------------------- symbols
+_INTEGERS = {torch.int64: 1, torch.int32: 0}
+MAX_TOKENS, MAX_ROW = 1 << 27, 1 << 20
+
+
+def embedding(table, tokens, *, scale: float = 1.0):
+    """``scale * table[tokens]``: (*tokens' shape, width), contiguous and of the table's type.
+
+    table: (rows, width), float32 or bfloat16; tokens: int32 or int64 of any shape.  A token that is no row, as -1 in the
+    padding of a batch, gives zeros."""
+    device = _tensor(table, "table")
+    if table.dim() != 2 or table.shape[1] < 1:
+        raise ValueError("table must be (rows, width)")
+    _tensor(tokens, "tokens", device, _INTEGERS)
+    rows, width = table.shape
+    shape = (*tokens.shape, width)
+    if not rows:
+        return torch.zeros(shape, dtype=table.dtype, device=table.device)
+    out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    if tokens.numel():
+        table, tokens = _last(table), tokens.contiguous()
+        _call(device, library().atlas_ops_embedding, table.data_ptr(), rows, width, table.stride(0), TYPES[table.dtype],
+              tokens.data_ptr(), _INTEGERS[tokens.dtype], tokens.numel(), scale, out.data_ptr())
+    return out
+
+
+def embedding_backward(grad, tokens, rows: int, *, scale: float = 1.0, dtype=None):
+    """The gradient of ``embedding``'s table of ``rows`` rows from that of its result: (rows, width), of ``dtype`` (float32 or
+    bfloat16, by default grad's).
+
+    Row r is the sum of the gradients of its tokens, in their order and in float32, zeros without any; tokens that are no
+    row have no part.  The same bits on every run.  At most 2^27 tokens, rows below 2^31 - 1, width up to 2^20."""
+    device = _tensor(grad, "grad")
+    if not grad.dim() or grad.shape[-1] < 1:
+        raise ValueError("grad needs a last axis, that of the table")
+    _tensor(tokens, "tokens", device, _INTEGERS, grad.shape[:-1])
+    width, count = grad.shape[-1], tokens.numel()
+    dtype = grad.dtype if dtype is None else dtype
+    if dtype not in TYPES:
+        raise ValueError(f"dtype is {dtype}, expected {' or '.join(str(x) for x in TYPES)}")
+    if not isinstance(rows, int) or not 0 <= rows < (1 << 31) - 1 or count > MAX_TOKENS or width > MAX_ROW:
+        raise ValueError(f"a table of {rows} rows of {width} from {count} tokens: at most 2^27 tokens, rows below 2^31 - 1, width up to 2^20")
+    table = torch.empty((rows, width), dtype=dtype, device=grad.device)
+    if rows:
+        lib = library()
+        packed, keep = _rows(grad, count, width) if count else (None, None)
+        tokens = tokens.contiguous()
+        workspace = _workspace(lib.atlas_ops_embedding_workspace(count, rows, width, TYPES[grad.dtype]), grad)
+        _call(device, lib.atlas_ops_embedding_backward, packed, tokens.data_ptr(), _INTEGERS[tokens.dtype], count, rows, width,
+              TYPES[grad.dtype], TYPES[dtype], scale, table.data_ptr(), workspace.data_ptr())
+    return table
+
+
+def dropout(x, probability: float, seed: int, *, stream: int = 0, tick=0, residual=None):
+    """``residual + (x / (1 - probability) where it is kept, else 0)``, contiguous and of x's type; the same call on the
+    gradient of the result, without the residual, is the gradient of x.
+
+    The mask is not stored: it follows from the place of a value in x and from seed, stream (a layer's number) and tick (a
+    step's), whole numbers of 64 bits, by the simulator's counter generator (``splitmix64-counter-v1``), each draw of
+    which serves two neighbouring values, 32 bits each.  tick may be an int64 tensor of one value on the GPU, which is read
+    when the kernel runs: a captured graph draws anew where the tensor has been counted up.  probability: 0 or
+    more, below 1, resolved to 2^-32."""
+    device = _tensor(x, "x")
+    if not 0.0 <= probability < 1.0:
+        raise ValueError("probability must be 0 or more and below 1")
+    if residual is not None:
+        _tensor(residual, "residual", device, _SAME[x.dtype], x.shape)
+        residual = residual.contiguous()
+    at = None
+    if isinstance(tick, torch.Tensor):
+        _tensor(tick, "tick", device, _I64)
+        if tick.numel() != 1:
+            raise ValueError("tick must be one value")
+        at, tick = tick, 0
+    for name, n in (("seed", seed), ("stream", stream), ("tick", tick)):
+        if not isinstance(n, int) or not -(1 << 63) <= n < 1 << 64:
+            raise ValueError(f"{name} must be a whole number of 64 bits")
+    y = _empty(x)
+    if x.numel():
+        x = x.contiguous()
+        _call(device, library().atlas_ops_dropout, x.data_ptr(), None if residual is None else residual.data_ptr(), x.numel(),
+              TYPES[x.dtype], probability, seed, stream, tick, None if at is None else at.data_ptr(), y.data_ptr())
+    return y
+
+
 # --------------------------------------------------------------------- the orthogonalised update
 def _matrix(t, name):
     if t.dim() not in (2, 3):
@@ -314,16 +507,12 @@ def muon_update(weight, gradient, momentum, *, learning_rate: float, factor: flo
 
 
 # --------------------------------------------------------------------------- the gated delta rule
-def _last(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 class _Problem:
-    """The checked arguments of a delta rule: sizes, the packed AtlasDelta and the tensors behind it."""
+    """The checked arguments of a delta rule, or of linear attention: sizes, the packed AtlasDelta and the tensors behind it."""
 
     __slots__ = ("device", "batch", "time", "heads", "value_heads", "key", "value", "type", "packed", "tensors")
 
-    def __init__(self, q, k, v, log_decay, beta, state, lengths, scale, time_axis: bool):
+    def __init__(self, q, k, v, log_decay, beta, state, lengths, scale, time_axis: bool, linear: bool = False):
         device = _tensor(q, "q")
         same = _SAME[q.dtype]
         _tensor(v, "v", device, same)
@@ -339,10 +528,14 @@ class _Problem:
             raise ValueError("the heads of v must be a multiple of those of q and k")
         if not 1 <= key <= MAX_KEY or value < 1:
             raise ValueError(f"the width of q and k must be 1 to {MAX_KEY}, that of v positive")
+        if linear and value > MAX_KEY:
+            raise ValueError(f"the width of v must be 1 to {MAX_KEY}")
         gates = out[:-1]
+        shared = linear and isinstance(log_decay, torch.Tensor) and log_decay.dim() == 1
         if log_decay is not None:
-            _tensor(log_decay, "log_decay", device, TYPES, gates)
-        _tensor(beta, "beta", device, TYPES, gates)
+            _tensor(log_decay, "log_decay", device, TYPES, (value_heads,) if shared else gates)
+        if not linear:
+            _tensor(beta, "beta", device, TYPES, gates)
         batch, time = lead[0], lead[1] if time_axis else 1
         if state is not None:
             _tensor(state, "state", device, _F32, (batch, value_heads, key, value))
@@ -359,11 +552,12 @@ class _Problem:
         self.key, self.value, self.type = key, value, q.dtype
         self.tensors = (q, k, v, log_decay, beta, state, lengths)
         self.packed = _DELTA.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if log_decay is None else log_decay.data_ptr(), beta.data_ptr(),
-            *strides(q), *strides(k), *strides(v), *((0, 0, 0) if log_decay is None else strides(log_decay)),
-            *strides(beta), 0 if state is None else state.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if log_decay is None else log_decay.data_ptr(),
+            0 if linear else beta.data_ptr(), *strides(q), *strides(k), *strides(v),
+            *((0, 0, 0) if log_decay is None else (0, 0, log_decay.stride(0)) if shared else strides(log_decay)),
+            *((0, 0, 0) if linear else strides(beta)), 0 if state is None else state.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
             batch, time, heads, value_heads, key, value, TYPES[q.dtype],
-            0 if log_decay is None else TYPES[log_decay.dtype], TYPES[beta.dtype],
+            0 if log_decay is None else TYPES[log_decay.dtype], 0 if linear else TYPES[beta.dtype],
             1.0 / math.sqrt(key) if scale is None else scale)
 
 
@@ -474,4 +668,109 @@ def delta_rule_backward(grad_out, grad_state, tape: DeltaTape) -> dict:
           struct.pack("@3q", *grad_out.stride()[:3]), None if grad_state is None else grad_state.data_ptr(),
           *(None if grads[n] is None else grads[n].data_ptr() for n in ("q", "k", "v", "log_decay", "beta", "state")),
           workspace.data_ptr())
+    return grads
+
+
+# --------------------------------------------------------------------------------- linear attention
+def linear_attention_step(q, k, v, log_decay, state, *, scale: float | None = None):
+    """One tick of linear attention for every stream of a batch; ``state`` is updated in place.
+
+    As ``linear_attention`` without the time axis: q, k (batch, heads, key), v (batch, value heads, value), log_decay (batch,
+    value heads) or (value heads,), state float32 (batch, value heads, key, value), contiguous, of memory that the other
+    tensors have no part in.  Returns out."""
+    if state is None:
+        raise ValueError("a step needs a state to update")
+    p = _Problem(q, k, v, log_decay, None, state, None, scale, False, True)
+    if not state.is_contiguous():
+        raise ValueError("state is updated in place and must be contiguous")
+    out = _empty(v)
+    if p.batch:
+        _call(p.device, library().atlas_ops_linear_step, p.packed, out.data_ptr(), state.data_ptr())
+        torch.autograd.graph.increment_version(state)
+    return out
+
+
+# Sequences up to this length without a tape run token by token in one launch.
+SHORT_LINEAR = 12
+
+
+class LinearTape:
+    """What ``linear_attention_backward`` needs of a forward pass: its inputs and the segments' states.  The inputs must
+    not change before the backward pass has run."""
+
+    __slots__ = ("problem", "memory", "stream")
+
+    def __init__(self, problem, memory, stream):
+        self.problem, self.memory, self.stream = problem, memory, stream
+
+
+def linear_attention(q, k, v, log_decay=None, state=None, *, lengths=None, scale: float | None = None, tape: bool = False):
+    """Linear attention with a decay by head: a layer whose synapses grow by Hebb's rule and decay while it runs.
+
+    Every value head keeps a state S (key x value), at first ``state`` or zeros.  By token
+    ``S <- exp(log_decay) S + k v^T``, ``out = scale S^T q``.
+
+    q, k (batch, time, heads, key), v (batch, time, value heads, value): float32 or bfloat16, key and value up to 128; value
+    head h uses the q and k of head ``h // (value heads / heads)``.  log_decay (None: no decay): float32 or bfloat16, (batch,
+    time, value heads), or (value heads,) for a decay that every token of a head has; -inf empties the state.  state:
+    float32 (batch, value heads, key, value).  lengths: int32 (batch,), tokens from a sequence's length on leave its
+    state unchanged, whatever is in it, and give zeros.  scale: by default ``1 / sqrt(key)``.  A NaN or an infinity reaches
+    its own and later tokens only.  At most 65535 sequences and value heads, 2^29 tokens.
+
+    Returns (out, final state); with ``tape`` (out, final state, tape), the tape for ``linear_attention_backward``."""
+    if state is not None and isinstance(state, torch.Tensor):
+        state = state.contiguous()
+    p = _Problem(q, k, v, log_decay, None, state, lengths, scale, True, True)
+    out = _empty(v)
+    shape = (p.batch, p.value_heads, p.key, p.value)
+    memory = None
+    if not p.batch or not p.time:
+        final = torch.zeros(shape, dtype=torch.float32, device=v.device) if state is None else state.clone()
+    else:
+        final = torch.empty(shape, dtype=torch.float32, device=v.device)
+        lib = library()
+        if p.time <= SHORT_LINEAR and not tape:
+            _call(p.device, lib.atlas_ops_linear_step, p.packed, out.data_ptr(), final.data_ptr())
+        else:
+            memory = _workspace(lib.atlas_ops_linear_workspace(p.packed, tape), v)
+            _call(p.device, lib.atlas_ops_linear_forward, p.packed, tape, out.data_ptr(), final.data_ptr(), memory.data_ptr())
+    if tape:
+        return out, final, LinearTape(p, memory, torch._C._cuda_getCurrentRawStream(p.device))
+    return out, final
+
+
+def linear_attention_backward(grad_out, grad_state, tape: LinearTape) -> dict:
+    """The gradients of ``linear_attention`` from those of out (of its type) and of the final state (float32, or None for
+    zeros): a dict with ``q, k, v, log_decay, state``, each of its input's shape and type, None for an input that was
+    not given.  Heads of q and k that value heads share get the sum, a decay by head that of its tokens.  The same
+    bits on every run.  A NaN or an infinity of a used token may reach the gradients of every token of its sequence."""
+    if not isinstance(tape, LinearTape):
+        raise ValueError("tape must be the one that linear_attention returned")
+    p = tape.problem
+    q, k, v, log_decay, _, state, lengths = p.tensors
+    _tensor(grad_out, "grad_out", p.device, _SAME[p.type], v.shape)
+    if grad_state is not None:
+        _tensor(grad_state, "grad_state", p.device, _F32, (p.batch, p.value_heads, p.key, p.value))
+        grad_state = grad_state.contiguous()
+    grad_out = _last(grad_out)
+    grads = {name: None if t is None else _empty(t)
+             for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("state", state))}
+    if not p.batch or not p.time:
+        if log_decay is not None:
+            grads["log_decay"].zero_()
+        if state is not None:
+            grads["state"] = torch.zeros_like(state) if grad_state is None else grad_state.clone()
+        return grads
+    if torch._C._cuda_getCurrentRawStream(p.device) != tape.stream:
+        # this stream's kernels read the tape: its memory is not to be reused before they have
+        stream = torch.cuda.current_stream(p.device)
+        for t in (tape.memory, *p.tensors):
+            if t is not None:
+                t.record_stream(stream)
+    lib = library()
+    workspace = _workspace(lib.atlas_ops_linear_backward_workspace(p.packed), v)
+    dq, dk, dv, decay, dstate = (None if g is None else g.data_ptr() for g in grads.values())
+    _call(p.device, lib.atlas_ops_linear_backward, p.packed, tape.memory.data_ptr(), grad_out.data_ptr(),
+          struct.pack("@3q", *grad_out.stride()[:3]), None if grad_state is None else grad_state.data_ptr(), dq, dk, dv, decay,
+          int(log_decay is not None and log_decay.dim() == 1), dstate, workspace.data_ptr())
     return grads

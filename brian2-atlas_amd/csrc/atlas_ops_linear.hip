@@ -1,0 +1,972 @@
+// Linear attention with a decay by head: token by token for streaming, in chunks for sequences, and its
+// gradients.  Part of libatlas_ops_hip.so.
+//
+// By token: S <- a S + k v^T, out = scale S^T q: Hebb's rule with forgetting.  In a chunk that starts from S,
+// with G_i the sum of the log decays up to and with token i and g = exp(G):
+//   out_i = scale (g_i S^T q_i + sum_{j <= i} exp(G_i - G_j) (q_i . k_j) v_j)
+//   S'    = g_C S + sum_j exp(G_C - G_j) k_j v_j^T
+// One kernel, `scan`, does this for three tensors (queries, keys, values), forwards or backwards in time, and
+// the gradients are three more runs of it.  With T_t the gradient of the state after token t,
+//   T_t = a_{t+1} T_{t+1} + scale q_t dO_t^T   is the same recurrence backwards, and
+//   dQ_t = scale S_t dO_t       forwards:  queries dO, keys v, values k (the state S^T)
+//   dV_t = T_t^T k_t            backwards: queries k,  keys q, values dO
+//   dK_t = T_t v_t              backwards: queries v,  keys dO, values q (the state T^T)
+// The gradient of log a_t is L_t = <T_t, a_t S_{t-1}> with L_t = L_{t+1} + q_t . dQ_t - k_t . dK_t, whose dots
+// the runs take beside their outputs; `decay_gradients` sums them in 64 bits.
+//
+// Few sequences are split along time: `scan` first takes the sums of segments from an empty state, `join_states`
+// carries the states through them, and every segment then runs from its own.
+#include <algorithm>
+#include <type_traits>
+
+#include "device/atlas_mma.h"
+#include "device/atlas_rows.h"
+
+namespace atlas_ops {
+namespace {
+
+constexpr int MAX_WIDTH = 128;
+constexpr float LOWEST = -120.0f;  // the exponential is zero in float32
+
+// Log decays of (batch, time, value head), of any strides.
+struct Decays {
+    Tensor x;
+    int bf16;
+    struct Raw { uint16_t low, high; };
+    // with a load that stands behind no branch (of `other` where there are no decays)
+    __device__ __forceinline__ Raw load(const void* other, i64 b, i64 t, i64 h) const {
+        const uint16_t* p = x.data ? (const uint16_t*)x.data + ((b * x.batch + t * x.time + h * x.head) << (bf16 ? 0 : 1)) : (const uint16_t*)other;
+        return {p[0], p[x.data && !bf16 ? 1 : 0]};
+    }
+    __device__ __forceinline__ float value(Raw r) const {
+        const float g = __uint_as_float(bf16 ? (uint32_t)r.low << 16 : (uint32_t)r.high << 16 | r.low);
+        return !x.data ? 0.0f : g < LOWEST ? LOWEST : g;  // a NaN stays one
+    }
+};
+
+__device__ __forceinline__ i64 length_of(const int32_t* lengths, i64 time, i64 b) {
+    if (!lengths) return time;
+    const i64 n = lengths[b];
+    return n < 0 ? 0 : n < time ? n : time;
+}
+
+// ------------------------------------------------------------------ token by token
+struct Step {
+    Tensor q, k, v;
+    Decays decay;
+    const float* state;
+    const int32_t* lengths;
+    i64 time;
+    int value_heads, group, key, value;
+    float scale;
+};
+
+// A workgroup holds 32 columns of one head's state in registers: row groups of 32 / VEC lanes, each lane VEC
+// neighbouring columns of every 8 VEC-th row.  One reduction per token: S^T q of the new state.  Memory bounds one
+// token: the state is read and written once.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) step_kernel(Step d, T* __restrict__ out, float* final_state) {
+    constexpr int LANES = 32 / VEC, ROWS = 256 / LANES, PER = MAX_WIDTH / ROWS;
+    __shared__ float sums[2][4][32];
+    const int lane = threadIdx.x % LANES, row = threadIdx.x / LANES, wave = threadIdx.x / 64;
+    const i64 b = blockIdx.z, h = blockIdx.y, hk = h / d.group;
+    const int col = blockIdx.x * 32 + lane * VEC;
+    const i64 base = (b * d.value_heads + h) * d.key * d.value;
+    // Nothing is loaded behind a branch, or each load would be waited for before the next: rows and columns that
+    // do not exist read the last, and their values become zeros.
+    T kt[PER], qt[PER], vt[VEC];
+    Decays::Raw raw;
+    auto fetch = [&](i64 t) {
+        const T *qp = d.q.at<T>(b, t, hk), *kp = d.k.at<T>(b, t, hk), *vp = d.v.at<T>(b, t, h);
+        raw = d.decay.load(qp, b, t, h);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) vt[c] = vp[min(col + c, d.value - 1)];
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+            const int at = min(row + r * ROWS, d.key - 1);
+            kt[r] = kp[at];
+            qt[r] = qp[at];
+        }
+    };
+    float s[PER][VEC];
+    const float* from = (d.state ? d.state : final_state) + base + min(col, d.value - VEC);
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+        const float* p = from + (i64)min(row + r * ROWS, d.key - 1) * d.value;
+        if constexpr (VEC == 4) {  // value is a multiple of 4
+            const float4_t v = *(const float4_t*)p;
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) s[r][c] = v[c];
+        } else {
+            s[r][0] = *p;
+        }
+    }
+    fetch(0);
+#pragma unroll
+    for (int r = 0; r < PER; ++r)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) s[r][c] = d.state && row + r * ROWS < d.key && col < d.value ? s[r][c] : 0.0f;
+    const i64 length = length_of(d.lengths, d.time, b);
+    for (i64 t = 0; t < d.time; ++t) {
+        T* o = out + ((b * d.time + t) * d.value_heads + h) * d.value;
+        if (t >= length) {
+            if (row == 0)
+                for (int c = 0; c < VEC; ++c)
+                    if (col + c < d.value) o[col + c] = from_float<T>(0.0f);
+            continue;
+        }
+        const float a = expf(d.decay.value(raw));
+        float v[VEC], kr[PER], qr[PER], qs[VEC];
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+            v[c] = col + c < d.value ? to_float(vt[c]) : 0.0f;
+            qs[c] = 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < PER; ++r) {
+            const int at = row + r * ROWS;
+            kr[r] = at < d.key ? to_float(kt[r]) : 0.0f;
+            qr[r] = at < d.key ? to_float(qt[r]) : 0.0f;
+        }
+        if (t + 1 < length) fetch(t + 1);
+#pragma unroll
+        for (int r = 0; r < PER; ++r)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+                s[r][c] = a * s[r][c] + kr[r] * v[c];
+                qs[c] += s[r][c] * qr[r];
+            }
+#pragma unroll
+        for (int step = LANES; step < 64; step *= 2)
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) qs[c] += __shfl_xor(qs[c], step, 64);
+        const int turn = t & 1;  // the sums of the token before are read until the next barrier
+        if (threadIdx.x % 64 < LANES) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) sums[turn][wave][lane * VEC + c] = qs[c];
+        }
+        __syncthreads();
+        if (row == 0) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+                const int at = lane * VEC + c;
+                const float sum = (sums[turn][0][at] + sums[turn][1][at]) + (sums[turn][2][at] + sums[turn][3][at]);
+                if (col + c < d.value) o[col + c] = from_float<T>(d.scale * sum);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+        const int at = row + r * ROWS;
+        if (at >= d.key || col >= d.value) continue;
+        float* p = final_state + base + (i64)at * d.value + col;
+        if constexpr (VEC == 4) {
+            float4_t v;
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) v[c] = s[r][c];
+            *(float4_t*)p = v;
+        } else {
+            *p = s[r][0];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ chunks
+// One of the three tensors of a scan: value head h reads head h / group.
+struct Role {
+    Tensor x;
+    int group, width;
+};
+
+struct Scan {
+    Role q, k, v;                  // q and k of one width, v of the outputs'
+    Decays decay;
+    const int32_t* lengths;
+    i64 time;
+    int value_heads, chunks, per, segments;  // per: chunks of a segment
+    int first;                     // the segment of blockIdx.x = 0
+    int backwards;                 // in time: row r of a chunk is its token C - 1 - r, which decays by the token behind
+    float write, read;             // factors of k v^T and of the outputs
+    // the states at the segments' starts, [batch, value head, segment] (or without segments), of q's x v's widths,
+    // or `turned`; null: zeros
+    const float* start;
+    int start_segments, turned;
+    // outputs (null to take the segments' sums only)
+    void* out;                     // (batch, time, value_heads, v's width) contiguous
+    int out_f32;                   // float32 whatever T is
+    float *final_state, *copy;     // after the last segment; backwards also decayed by the first token; may be null
+    float *sums, *decays;          // [batch, value head, segment]: a segment's state from zeros, and its whole decay
+    const void* dot_with;          // (a Role) null, or what each output row is multiplied with
+    Role dot;
+    float* dots;                   // [batch, value head, time]
+};
+
+template <typename T>
+struct Cut {
+    static constexpr int N = sizeof(T) == 2 ? 1 : 3;  // bfloat16 pieces of a value
+    static constexpr int C = sizeof(T) == 2 ? 64 : 32;  // tokens per chunk
+    static constexpr int QB = C / 16, KB = C / 32;
+};
+
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+
+// Four values of column l % 16, rows quad .. quad + 3 from `at`, the address of row quad + l % 16 / 4, columns 4 (l % 4) ..:
+// the hardware turns 4 x 16 blocks for 16 lanes each.
+__device__ __forceinline__ bf16x4 turned_read(const bf16_t* at) {
+    typedef __attribute__((address_space(3))) bf16x4 lds;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds*)(at));
+}
+
+__device__ __forceinline__ bf16x8 both(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Workgroup: one segment of one value head.  Wave w holds the state's columns of its NB blocks of 16 in
+// registers, all DK rows.  NB = 2: block n of the wave has columns 32 w + 8 i + 4 n + j (i, j < 4) at lanes 4 i + j, so
+// that a lane's results are eight neighbours; NB = 1: 16 w + l.
+template <typename T, int DK, int NB, bool OUT>
+__global__ void __launch_bounds__(256, 2) scan(Scan d) {
+    constexpr int N = Cut<T>::N, C = Cut<T>::C, QB = Cut<T>::QB, KB = Cut<T>::KB, DV = 64 * NB;
+    constexpr int E = Unit<T>::N, PITCH = DK + 8, VPITCH = DV + (sizeof(T) == 2 ? 8 : 4);
+    constexpr int KU = C * DK / E / 256, VU = C * DV / E / 256;  // units of a chunk per thread
+    constexpr int SCORES = QB == 4 ? 6 : 2;                      // operands of 16 queries x 32 keys that are not zero
+    __shared__ __attribute__((aligned(16))) bf16_t qs[OUT ? N * C * PITCH : 8], ks[N * C * PITCH];
+    __shared__ __attribute__((aligned(16))) T vs[C * VPITCH];
+    __shared__ __attribute__((aligned(16))) bf16_t scores[OUT ? SCORES * 3 * 512 : 8];
+    __shared__ __attribute__((aligned(16))) float gate_sum[C], gate_rest[C], since[C], rest[C];
+    __shared__ float dot_part[OUT ? 4 : 1][C];
+    const Lane l;
+    const int wave = threadIdx.x / 64;
+    const int segment = d.first + blockIdx.x;
+    const i64 h = blockIdx.y, b = blockIdx.z, head = b * d.value_heads + h;
+    const i64 length = length_of(d.lengths, d.time, b);
+    const int low = segment * d.per, high = min(low + d.per, d.chunks);
+    const int used = (int)((length + C - 1) / C);  // chunks with a token
+    const int inner = d.q.width, outer = d.v.width;
+    const T *qp = d.q.x.at<T>(b, 0, h / d.q.group), *kp = d.k.x.at<T>(b, 0, h / d.k.group), *vp = d.v.x.at<T>(b, 0, h / d.v.group);
+    const int cell = 4 * NB * (l.col / 4) + l.col % 4;  // of block 0 within the wave's columns; block n: + 4 n
+    const int column = 16 * NB * wave + cell;
+
+    // the state: block r of rows 16 r .., block n of columns
+    float4_t s[DK / 16][NB];
+#pragma unroll
+    for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[r][n] = ZERO;
+    if (OUT && d.start) {
+        const float* from = d.start + (d.start_segments ? head * d.segments + segment : head) * inner * outer;
+#pragma unroll
+        for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = 16 * r + l.quad + j, col = column + 4 * n;
+                    const bool live = row < inner && col < outer;
+                    const float v = from[live ? d.turned ? (i64)col * inner + row : (i64)row * outer + col : 0];
+                    s[r][n][j] = live ? v : 0.0f;
+                }
+    }
+
+    Unit<T> qu[OUT ? KU : 1], ku[KU], vu[VU];
+    Decays::Raw raw;
+    auto token = [&](int chunk, int row) { return (i64)chunk * C + (d.backwards ? C - 1 - row : row); };
+    auto fetch = [&](int chunk) {
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int at = threadIdx.x + 256 * u, row = at / (DK / E), col = at % (DK / E) * E;
+            const i64 t = min(token(chunk, row), d.time - 1);
+            if constexpr (OUT) qu[u].load(qp + t * d.q.x.time, col, inner);
+            ku[u].load(kp + t * d.k.x.time, col, inner);
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int at = threadIdx.x + 256 * u, row = at / (DV / E), col = at % (DV / E) * E;
+            vu[u].load(vp + min(token(chunk, row), d.time - 1) * d.v.x.time, col, outer);
+        }
+        raw = d.decay.load(qp, b, min(token(chunk, l.id % C) + d.backwards, d.time - 1), h);
+    };
+    // splits a unit into the N planes of an LDS tile
+    auto place = [&](bf16_t* tile, const Unit<T>& u, int row, int col, bool live) {
+        bf16_t* p = tile + row * PITCH + col;
+        if constexpr (N == 1) {
+            u64* q = (u64*)p;
+            q[0] = live ? u.low : 0;
+            q[1] = live ? u.high : 0;
+        } else {
+            const float4_t v = {live ? u[0] : 0.0f, live ? u[1] : 0.0f, live ? u[2] : 0.0f, live ? u[3] : 0.0f};
+            const Halves<3> parts = split<3>(v);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) *(bf16x4*)(p + i * C * PITCH) = parts.p[i];
+        }
+    };
+    // an operand of rows block of a tile, 32 columns from c0
+    auto rows_operand = [&](const bf16_t* tile, int block, int c0) {
+        Pieces<N> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bf16_t* p = tile + i * C * PITCH + (16 * block + l.col) * PITCH + c0 + l.quad;
+            r.p[i] = both(*(const bf16x4*)p, *(const bf16x4*)(p + 16));
+        }
+        return r;
+    };
+
+    const int steps = high - low;
+    double whole = 0.0;  // log decay of the segment's chunks
+    if (low < used) fetch(d.backwards ? min(high, used) - 1 : low);
+    for (int step = 0; step < steps; ++step) {
+        const int chunk = d.backwards ? high - 1 - step : low + step;
+        if (chunk >= used) {  // no token: zeros
+            if constexpr (OUT) {
+                const i64 t0 = (i64)chunk * C;
+                const int rows = (int)min((i64)C, d.time - t0);
+                for (int at = threadIdx.x; at < rows * outer; at += 256) {
+                    const i64 o = ((b * d.time + t0 + at / outer) * d.value_heads + h) * outer + at % outer;
+                    if (d.out_f32) ((float*)d.out)[o] = 0.0f;
+                    else ((T*)d.out)[o] = from_float<T>(0.0f);
+                }
+                if (d.dots && (int)threadIdx.x < rows) d.dots[head * d.time + t0 + threadIdx.x] = 0.0f;
+            }
+            continue;
+        }
+        // ---- the chunk into LDS, its decays: G as a float and its remainder, in powers of two
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int at = threadIdx.x + 256 * u, row = at / (DK / E), col = at % (DK / E) * E;
+            const bool live = token(chunk, row) < length;
+            if constexpr (OUT) place(qs, qu[u], row, col, live);
+            place(ks, ku[u], row, col, live);
+        }
+#pragma unroll
+        for (int u = 0; u < VU; ++u) {
+            const int at = threadIdx.x + 256 * u, row = at / (DV / E), col = at % (DV / E) * E;
+            const bool live = token(chunk, row) < length;
+            u64* p = (u64*)(vs + row * VPITCH + col);
+            p[0] = live ? vu[u].low : 0;
+            p[1] = live ? vu[u].high : 0;
+        }
+        double total;
+        {
+            const int row = l.id % C;
+            const i64 t = token(chunk, row) + d.backwards;
+            double sum = t < length ? (double)d.decay.value(raw) * 1.4426950408889634 : 0.0;
+#pragma unroll
+            for (int k = 1; k < C; k *= 2) {
+                const double before = __shfl_up(sum, k, C);
+                if (row >= k) sum += before;
+            }
+            total = __shfl(sum, C - 1, 64);
+            if (wave == 0 && l.id < C) {
+                gate_sum[row] = (float)sum;
+                gate_rest[row] = (float)(sum - (double)(float)sum);
+                since[row] = __builtin_amdgcn_exp2f((float)sum);
+                rest[row] = __builtin_amdgcn_exp2f((float)(total - sum)) * d.write;
+            }
+            whole += total;
+        }
+        __syncthreads();
+        const int next = d.backwards ? chunk - 1 : chunk + 1;
+        if (d.backwards ? next >= low : next < min(high, used)) fetch(next);
+
+        // ---- the values as operands: columns of this wave, sums over tokens
+        float4_t v[KB][NB][2];
+        bf16x8 vb[KB][NB];  // N = 1
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if constexpr (N == 1) {
+                    const bf16_t* p = (const bf16_t*)vs + (32 * kb + l.quad + l.col / 4) * VPITCH + 16 * NB * wave + 4 * NB * (l.col % 4) + 4 * n;
+                    const bf16x4 a = turned_read(p), c = turned_read(p + 16 * VPITCH);
+                    vb[kb][n] = both(a, c);
+                    v[kb][n][0] = widen(a), v[kb][n][1] = widen(c);
+                } else {
+                    const float* p = (const float*)vs + (32 * kb + l.quad) * VPITCH + column + 4 * n;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[kb][n][0][j] = p[j * VPITCH], v[kb][n][1][j] = p[(16 + j) * VPITCH];
+                }
+            }
+
+        if constexpr (OUT) {
+            // ---- decayed scores of this wave's queries, turned: rows are keys
+            for (int qb = wave; qb < QB; qb += 4) {
+                float4_t p[QB];
+#pragma unroll
+                for (int kj = 0; kj < QB; ++kj) p[kj] = ZERO;
+#pragma unroll
+                for (int c = 0; c < DK / 32; ++c) {
+                    const Pieces<N> q = rows_operand(qs, qb, 32 * c);
+#pragma unroll
+                    for (int kj = 0; kj < QB; ++kj)
+                        if (kj <= qb) p[kj] = mma(rows_operand(ks, kj, 32 * c), q, p[kj]);
+                }
+                const int i = 16 * qb + l.col;
+                const float sum = gate_sum[i], remainder = gate_rest[i];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    if (2 * kb > qb) continue;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float4_t& x = p[2 * kb + half];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int at = 32 * kb + 16 * half + l.quad + j;
+                            const float decay = __builtin_amdgcn_exp2f((sum - gate_sum[at]) + (remainder - gate_rest[at])) * d.write;
+                            x[j] = at <= i ? x[j] * decay : 0.0f;
+                        }
+                    }
+                    const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kb) : qb;
+                    put<3>(scores, operand, l, split<3>(p[2 * kb], p[2 * kb + 1]));
+                }
+            }
+            // ---- what the state answers: rows are columns of the values, columns are queries
+            float4_t o[QB][NB];
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[qb][n] = ZERO;
+#pragma unroll
+            for (int c = 0; c < DK / 32; ++c) {
+                Pieces<3> state[NB];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) state[n] = split<3>(s[2 * c][n], s[2 * c + 1][n]);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    const Pieces<N> q = rows_operand(qs, qb, 32 * c);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[qb][n] = mma(state[n], q, o[qb][n]);
+                }
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                const float g = since[16 * qb + l.col];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[qb][n] *= g;
+            }
+            // ---- a NaN or an infinity among the values would reach the tokens before it through zeros of the scores:
+            // it is taken out, and the rows from its column's first on are NaN afterwards
+            float faulty = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) faulty = fmaf(v[kb][n][e / 4][e % 4], 0.0f, faulty);
+            const bool any = __ballot(faulty != faulty) != 0;
+            int worst[NB];  // the first faulty token of block n's column l % 16
+            Pieces<N> value[KB][NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                worst[n] = C;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    float4_t x[2] = {v[kb][n][0], v[kb][n][1]};
+                    if (any) {
+#pragma unroll
+                        for (int e = 7; e >= 0; --e)
+                            if (!(fabsf(x[e / 4][e % 4]) < INFINITY)) {
+                                x[e / 4][e % 4] = 0.0f;
+                                worst[n] = min(worst[n], 32 * kb + 16 * (e / 4) + l.quad + e % 4);
+                            }
+                    }
+                    if constexpr (N == 1) {
+                        value[kb][n].p[0] = vb[kb][n];
+                        if (any) value[kb][n] = split<1>(x[0], x[1]);
+                    } else {
+                        value[kb][n] = split<3>(x[0], x[1]);
+                    }
+                }
+                if (any) {
+                    worst[n] = min(worst[n], __shfl_xor(worst[n], 16, 64));
+                    worst[n] = min(worst[n], __shfl_xor(worst[n], 32, 64));
+                }
+            }
+            __syncthreads();  // the scores are there
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    if (2 * kb > qb) continue;
+                    const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kb) : qb;
+                    const Pieces<3> p = atlas_ops::fetch<3>(scores, operand, l);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[qb][n] = mma(value[kb][n], p, o[qb][n]);
+                }
+            if (any) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int first = __shfl(worst[n], l.quad + j, 64);  // of the results' row
+#pragma unroll
+                        for (int qb = 0; qb < QB; ++qb)
+                            if (16 * qb + l.col >= first) o[qb][n][j] = NAN;
+                    }
+            }
+            // ---- a lane's 4 NB neighbouring columns of one token
+            const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) {
+                const i64 t = token(chunk, 16 * qb + l.col);
+                float row[4 * NB];
+#pragma unroll
+                for (int e = 0; e < 4 * NB; ++e) row[e] = t < length ? d.read * o[qb][e / 4][e % 4] : 0.0f;
+                if (d.dots) {
+                    float dot = 0.0f;
+                    if (t < length && left > 0) {
+                        const T* x = d.dot.x.at<T>(b, t, h / d.dot.group) + c0;
+#pragma unroll
+                        for (int e = 0; e < 4 * NB; ++e) dot += e < left ? row[e] * to_float(x[e < left ? e : 0]) : 0.0f;
+                    }
+                    dot += __shfl_xor(dot, 16, 64);
+                    dot += __shfl_xor(dot, 32, 64);
+                    if (l.quad == 0) dot_part[wave][16 * qb + l.col] = dot;
+                }
+                if (t < d.time && left > 0) {
+                    const i64 at = ((b * d.time + t) * d.value_heads + h) * outer + c0;
+                    if (d.out_f32) store_unit<float, 4 * NB>((float*)d.out + at, left, row);
+                    else store_unit<T, 4 * NB>((T*)d.out + at, left, row);
+                }
+            }
+        }
+
+        // ---- the state behind the chunk
+        const float decayed = __builtin_amdgcn_exp2f((float)total);
+#pragma unroll
+        for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+            for (int n = 0; n < NB; ++n) s[r][n] *= decayed;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            Pieces<3> written[NB];
+            const float4_t ra = *(const float4_t*)(rest + 32 * kb + l.quad), rb = *(const float4_t*)(rest + 32 * kb + 16 + l.quad);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) written[n] = split<3>(v[kb][n][0] * ra, v[kb][n][1] * rb);
+#pragma unroll
+            for (int r = 0; r < DK / 16; ++r) {
+                Pieces<N> k;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const bf16_t* p = ks + i * C * PITCH + (32 * kb + l.quad + l.col / 4) * PITCH + 16 * r + 4 * (l.col % 4);
+                    k.p[i] = both(turned_read(p), turned_read(p + 16 * PITCH));
+                }
+#pragma unroll
+                for (int n = 0; n < NB; ++n) s[r][n] = mma(k, written[n], s[r][n]);
+            }
+        }
+        __syncthreads();  // the tiles are read, the dots written
+        if constexpr (OUT) {
+            const i64 t = token(chunk, threadIdx.x % C);
+            if (d.dots && threadIdx.x < C && t < d.time) {
+                const int r = threadIdx.x;
+                d.dots[head * d.time + t] = (dot_part[0][r] + dot_part[1][r]) + (dot_part[2][r] + dot_part[3][r]);
+            }
+        }
+    }
+
+    // ---- the state behind the segment
+    float *to = nullptr, *copy = nullptr;
+    float factor = 1.0f;
+    if constexpr (OUT) {
+        if (segment != (d.backwards ? 0 : d.segments - 1)) return;
+        if (d.final_state) to = d.final_state + head * inner * outer;
+        if (d.copy) copy = d.copy + head * inner * outer;
+        if (d.backwards && length > 0) factor = expf(d.decay.value(d.decay.load(qp, b, 0, h)));
+    } else {
+        to = d.sums + (head * d.segments + segment) * inner * outer;
+        if (threadIdx.x == 0) d.decays[head * d.segments + segment] = (float)exp2(whole);
+    }
+    if (!to) return;
+#pragma unroll
+    for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * r + l.quad + j, col = column + 4 * n;
+                if (row >= inner || col >= outer) continue;
+                to[(i64)row * outer + col] = factor * s[r][n][j];
+                if (copy) copy[(i64)row * outer + col] = factor * s[r][n][j];
+            }
+}
+
+// Turns the segments' sums into the states at their starts, in place.  backwards: the last segment's start is `start`.
+__global__ void __launch_bounds__(256) join_states(float* sums, const float* decays, const float* start, i64 cells, int segments, int backwards) {
+    const i64 cell = (i64)blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
+    if (cell >= cells) return;
+    float carry = start ? start[head * cells + cell] : 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < segments; ++i) {
+        const int segment = backwards ? segments - 1 - i : i;
+        float* p = sums + (head * segments + segment) * cells + cell;
+        const float own = i + 1 < segments ? *p : 0.0f, decay = i + 1 < segments ? decays[head * segments + segment] : 0.0f;
+        *p = carry;
+        carry = decay * carry + own;
+    }
+}
+
+// ------------------------------------------------------------------ gradients of the decays
+// A workgroup takes a segment: L behind its last token from the states there, then back through its tokens.
+struct DecayGradients {
+    Decays decay;
+    const void* other;                      // memory that may be read where there are no decays
+    const int32_t* lengths;
+    i64 time, tokens, cells;                // tokens of a segment; cells of a state
+    int value_heads, segments;
+    const float *starts, *last, *behind, *grad_state;  // S at the segments' starts, after the sequence; T behind the segments
+    const float *dq, *dk;                   // the dots, [batch, value head, time]
+    void* out;                              // (batch, time, value heads) of the decays' type, or null:
+    float* sums;                            // [batch, segment, value head] sums over the segment's tokens
+};
+
+__global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
+    __shared__ double parts[2][4];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, segment = blockIdx.x;
+    const i64 h = blockIdx.y, b = blockIdx.z, head = b * d.value_heads + h;
+    const i64 length = length_of(d.lengths, d.time, b), first = segment * d.tokens, end = min(first + d.tokens, d.time);
+    // <S, T> behind the segment: sums in 64 bits
+    const float* state = segment + 1 < d.segments ? d.starts + (head * d.segments + segment + 1) * d.cells : d.last + head * d.cells;
+    const float* grad = d.behind ? d.behind + (head * d.segments + segment) * d.cells : d.grad_state ? d.grad_state + head * d.cells : nullptr;
+    double carry = 0.0;
+    if (grad) {
+        for (i64 i = threadIdx.x; i < d.cells; i += 256) carry += (double)state[i] * (double)grad[i];
+#pragma unroll
+        for (int k = 32; k; k /= 2) carry += __shfl_xor(carry, k, 64);
+        if (lane == 0) parts[0][wave] = carry;
+        __syncthreads();
+        carry = (parts[0][0] + parts[0][1]) + (parts[0][2] + parts[0][3]);
+        if (end < length) carry *= exp((double)d.decay.value(d.decay.load(d.other, b, end, h)));
+    }
+    double sum = 0.0;
+    int turn = 1;
+    for (i64 base = end; base > first; base -= 256, turn ^= 1) {
+        const i64 t = base - 1 - threadIdx.x;
+        const bool live = t >= first && t < length;
+        const i64 at = head * d.time + (live ? t : first);
+        double x = live ? (double)d.dq[at] - (double)d.dk[at] : 0.0;
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) {
+            const double before = __shfl_up(x, k, 64);
+            if (lane >= k) x += before;
+        }
+        if (lane == 63) parts[turn][wave] = x;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) x += parts[turn][w];
+        x += carry;
+        carry += (parts[turn][0] + parts[turn][1]) + (parts[turn][2] + parts[turn][3]);
+        if (live) sum += x;
+        if (d.out && t >= first) {
+            const i64 o = (b * d.time + t) * d.value_heads + h;
+            const float value = live ? (float)x : 0.0f;
+            if (d.decay.bf16) ((bf16_t*)d.out)[o] = from_float<bf16_t>(value);
+            else ((float*)d.out)[o] = value;
+        }
+    }
+    if (!d.sums) return;
+#pragma unroll
+    for (int k = 32; k; k /= 2) sum += __shfl_xor(sum, k, 64);
+    __syncthreads();  // the last tiles' parts are read
+    if (lane == 0) parts[0][wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        d.sums[(b * d.segments + segment) * d.value_heads + h] = (float)((parts[0][0] + parts[0][1]) + (parts[0][2] + parts[0][3]));
+}
+
+// Sums over rows of (rows, columns): the gradient of a decay that all sequences share.
+__global__ void __launch_bounds__(256) head_sums(const float* __restrict__ sums, i64 rows, int columns, int bf16, void* out) {
+    __shared__ double parts[4];
+    const int column = blockIdx.x;
+    double sum = 0.0;
+    for (i64 r = threadIdx.x; r < rows; r += 256) sum += (double)sums[r * columns + column];
+#pragma unroll
+    for (int k = 32; k; k /= 2) sum += __shfl_xor(sum, k, 64);
+    if (threadIdx.x % 64 == 0) parts[threadIdx.x / 64] = sum;
+    __syncthreads();
+    if (threadIdx.x) return;
+    const float total = (float)((parts[0] + parts[1]) + (parts[2] + parts[3]));
+    if (bf16) ((bf16_t*)out)[column] = from_float<bf16_t>(total);
+    else ((float*)out)[column] = total;
+}
+
+// Heads of q and k that `group` value heads share: the sums of their gradients, rows of (value heads x width).
+template <typename T>
+__global__ void __launch_bounds__(256) group_sums(const float* __restrict__ parts, i64 count, int width, int group, T* __restrict__ out) {
+    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < count; i += (i64)gridDim.x * 256) {
+        const float* p = parts + i / width * group * width + i % width;
+        float sum = 0.0f;
+        for (int g = 0; g < group; ++g) sum += p[(i64)g * width];
+        out[i] = from_float<T>(sum);
+    }
+}
+
+// ------------------------------------------------------------------ plans
+template <typename F>
+void with_type(int type, F&& f) {
+    if (type == ATLAS_OPS_F32) f(0.0f);
+    else f(bf16_t{});
+}
+
+int chunk_of(int type) { return type == ATLAS_OPS_F32 ? Cut<float>::C : Cut<bf16_t>::C; }
+
+// Segments: as many as give every CU two workgroups, of at least two chunks each.
+struct Plan {
+    i64 chunks, heads;  // of a sequence; batch x value heads
+    int per, segments;
+    i64 state;          // floats of a state
+};
+
+Plan plan_of(const AtlasDelta& d) {
+    Plan p{};
+    p.chunks = ceil_div(d.time, chunk_of(d.type));
+    p.heads = d.batch * d.value_heads;
+    p.state = d.key * d.value;
+    const i64 wanted = std::max<i64>(1, std::min<i64>(512 / p.heads, p.chunks / 2));
+    p.per = (int)ceil_div(p.chunks, wanted);
+    p.segments = (int)ceil_div(p.chunks, p.per);
+    return p;
+}
+
+// The workspace of a forward pass, which a backward pass takes as its tape: the states at the segments' starts, the
+// decays of segments, and for a tape the final state.
+i64 forward_floats(const AtlasDelta& d, bool train) {
+    const Plan p = plan_of(d);
+    const i64 starts = p.segments > 1 ? p.heads * p.segments * (p.state + 1) : 0;
+    return starts + (train ? p.heads * p.state : 0);
+}
+
+// Of a backward pass: T behind the segments and their decays, the dots of dQ and dK, sums of shared decays, float32
+// gradients of shared heads.
+struct Back {
+    i64 behind, decays, dots, sums, dq, dk, all;
+};
+
+Back back_of(const AtlasDelta& d) {
+    const Plan p = plan_of(d);
+    Back o{};
+    o.behind = 0;
+    o.decays = o.behind + (p.segments > 1 ? p.heads * p.segments * p.state : 0);
+    o.dots = o.decays + (p.segments > 1 ? p.heads * p.segments : 0);
+    o.sums = o.dots + 2 * p.heads * d.time;
+    o.dq = o.sums + p.heads * p.segments;
+    const i64 shared = d.value_heads > d.heads ? p.heads * d.time * d.key : 0;
+    o.dk = o.dq + shared;
+    o.all = o.dk + shared;
+    return o;
+}
+
+template <bool OUT>
+void launch_scan(const Scan& s, int type, i64 batch, int segments, hipStream_t st) {
+    const dim3 grid((unsigned)segments, (unsigned)s.value_heads, (unsigned)batch);
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        if (s.q.width <= 64 && s.v.width <= 64) scan<T, 64, 1, OUT><<<grid, 256, 0, st>>>(s);
+        else if (s.q.width <= 64) scan<T, 64, 2, OUT><<<grid, 256, 0, st>>>(s);
+        else if (s.v.width <= 64) scan<T, 128, 1, OUT><<<grid, 256, 0, st>>>(s);
+        else scan<T, 128, 2, OUT><<<grid, 256, 0, st>>>(s);
+    });
+}
+
+Tensor tensor_of(const void* data, const int64_t* stride) { return {data, stride[0], stride[1], stride[2]}; }
+
+int check(const AtlasDelta* d, bool chunks, char* err, size_t cap) {
+    if (!d) return fail(err, cap, 7, "null problem");
+    if (d->batch < 1 || d->time < 1 || d->heads < 1 || d->value_heads < 1 || d->value < 1)
+        return fail(err, cap, 7, "every size must be positive");
+    if (d->key < 1 || d->key > MAX_WIDTH || d->value > MAX_WIDTH) return fail(err, cap, 7, "key and value must be 1 to %d", MAX_WIDTH);
+    if (d->value_heads % d->heads) return fail(err, cap, 7, "value_heads must be a multiple of heads");
+    if (d->batch > 65535 || d->value_heads > 65535) return fail(err, cap, 7, "at most 65535 sequences and value heads");
+    if (d->time > ((i64)1 << 29)) return fail(err, cap, 7, "time must be at most 2^29");
+    if (chunks && d->batch * d->value_heads > 65535 * 512) return fail(err, cap, 7, "batch x value_heads must be below 2^25");
+    if (!known_type(d->type) || !known_type(d->log_decay_type)) return fail(err, cap, 7, "unknown type");
+    if (!d->q || !d->k || !d->v) return fail(err, cap, 7, "null tensor");
+    return 0;
+}
+
+Decays decays_of(const AtlasDelta& d) {
+    return {tensor_of(d.log_decay, d.log_decay_stride), d.log_decay_type == ATLAS_OPS_BF16};
+}
+
+Scan scan_of(const AtlasDelta& d, const Plan& p) {
+    Scan s{};
+    s.decay = decays_of(d);
+    s.lengths = d.lengths;
+    s.time = d.time;
+    s.value_heads = (int)d.value_heads;
+    s.chunks = (int)p.chunks;
+    s.per = p.per;
+    s.segments = p.segments;
+    s.write = s.read = 1.0f;
+    return s;
+}
+
+}  // namespace
+}  // namespace atlas_ops
+
+using namespace atlas_ops;
+
+extern "C" {
+
+int atlas_ops_linear_step(const AtlasDelta* d, void* out, float* final_state, void* stream, char* err, size_t cap) {
+    try {
+        if (int rc = check(d, false, err, cap)) return rc;
+        if (!out || !final_state) return fail(err, cap, 7, "null output");
+        const Step s{tensor_of(d->q, d->q_stride), tensor_of(d->k, d->k_stride), tensor_of(d->v, d->v_stride), decays_of(*d), d->state,
+                     d->lengths, d->time, (int)d->value_heads, (int)(d->value_heads / d->heads), (int)d->key, (int)d->value, d->scale};
+        const dim3 grid((unsigned)ceil_div(d->value, 32), (unsigned)d->value_heads, (unsigned)d->batch);
+        with_type(d->type, [&](auto t) {
+            using T = decltype(t);
+            if (d->value % 4 == 0) step_kernel<T, 4><<<grid, 256, 0, (hipStream_t)stream>>>(s, (T*)out, final_state);
+            else step_kernel<T, 1><<<grid, 256, 0, (hipStream_t)stream>>>(s, (T*)out, final_state);
+        });
+        return launched(err, cap, "linear_step");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+int64_t atlas_ops_linear_workspace(const AtlasDelta* d, int train) {
+    char ignored[1];
+    if (check(d, true, ignored, 1)) return 0;
+    return 4 * forward_floats(*d, train != 0) + 16;  // never 0
+}
+
+int atlas_ops_linear_forward(const AtlasDelta* d, int train, void* out, float* final_state, void* workspace, void* stream, char* err,
+                             size_t cap) {
+    try {
+        if (int rc = check(d, true, err, cap)) return rc;
+        if (!out || !final_state || !workspace) return fail(err, cap, 7, "null output or workspace");
+        const Plan p = plan_of(*d);
+        hipStream_t st = (hipStream_t)stream;
+        const int group = (int)(d->value_heads / d->heads);
+        Scan s = scan_of(*d, p);
+        s.q = {tensor_of(d->q, d->q_stride), group, (int)d->key};
+        s.k = {tensor_of(d->k, d->k_stride), group, (int)d->key};
+        s.v = {tensor_of(d->v, d->v_stride), 1, (int)d->value};
+        s.read = d->scale;
+        s.start = d->state;
+        float* starts = (float*)workspace;
+        float* last = starts + (p.segments > 1 ? p.heads * p.segments * (p.state + 1) : 0);
+        if (p.segments > 1) {
+            s.sums = starts;
+            s.decays = starts + p.heads * p.segments * p.state;
+            launch_scan<false>(s, d->type, d->batch, p.segments - 1, st);
+            for (i64 b = 0; b < p.heads; b += 65535)
+                join_states<<<dim3((unsigned)ceil_div(p.state, 256), (unsigned)std::min<i64>(p.heads - b, 65535)), 256, 0, st>>>(
+                    starts + b * p.segments * p.state, s.decays + b * p.segments, d->state ? d->state + b * p.state : nullptr, p.state, p.segments, 0);
+            s.start = starts;
+            s.start_segments = 1;
+        }
+        s.out = out;
+        s.final_state = final_state;
+        s.copy = train ? last : nullptr;
+        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        return launched(err, cap, "linear_forward");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+int64_t atlas_ops_linear_backward_workspace(const AtlasDelta* d) {
+    char ignored[1];
+    if (check(d, true, ignored, 1)) return 0;
+    return 4 * back_of(*d).all;
+}
+
+int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void* grad_out, const int64_t* grad_out_stride,
+                              const float* grad_state, void* dq, void* dk, void* dv, void* dlog_decay, int shared_decay, float* dstate,
+                              void* workspace, void* stream, char* err, size_t cap) {
+    try {
+        if (int rc = check(d, true, err, cap)) return rc;
+        if (!tape || !grad_out || !grad_out_stride || !dq || !dk || !dv || !workspace) return fail(err, cap, 7, "null argument");
+        if (dlog_decay && !d->log_decay) return fail(err, cap, 7, "a gradient of decays that were not given");
+        const Plan p = plan_of(*d);
+        const Back at = back_of(*d);
+        hipStream_t st = (hipStream_t)stream;
+        const int group = (int)(d->value_heads / d->heads);
+        float* base = (float*)workspace;
+        const float* starts = (const float*)tape;
+        const float* last = starts + (p.segments > 1 ? p.heads * p.segments * (p.state + 1) : 0);
+        const Role q{tensor_of(d->q, d->q_stride), group, (int)d->key}, k{tensor_of(d->k, d->k_stride), group, (int)d->key},
+            v{tensor_of(d->v, d->v_stride), 1, (int)d->value}, go{tensor_of(grad_out, grad_out_stride), 1, (int)d->value};
+        float *dots_q = base + at.dots, *dots_k = dots_q + p.heads * d->time;
+        // dQ, forwards
+        Scan s = scan_of(*d, p);
+        s.q = go, s.k = v, s.v = k;
+        s.read = d->scale;
+        s.start = p.segments > 1 ? starts : d->state;
+        s.start_segments = p.segments > 1;
+        s.turned = 1;
+        s.out = group > 1 ? (void*)(base + at.dq) : dq;
+        s.out_f32 = group > 1;
+        s.dot = q;
+        s.dots = dlog_decay ? dots_q : nullptr;
+        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        // T behind the segments
+        s = scan_of(*d, p);
+        s.backwards = 1;
+        s.write = d->scale;
+        s.q = k, s.k = q, s.v = go;
+        s.start = grad_state;
+        if (p.segments > 1) {
+            s.sums = base + at.behind;
+            s.decays = base + at.decays;
+            s.first = 1;
+            launch_scan<false>(s, d->type, d->batch, p.segments - 1, st);
+            s.first = 0;
+            for (i64 b = 0; b < p.heads; b += 65535)
+                join_states<<<dim3((unsigned)ceil_div(p.state, 256), (unsigned)std::min<i64>(p.heads - b, 65535)), 256, 0, st>>>(
+                    s.sums + b * p.segments * p.state, s.decays + b * p.segments, grad_state ? grad_state + b * p.state : nullptr, p.state,
+                    p.segments, 1);
+            s.start = s.sums;
+            s.start_segments = 1;
+        }
+        // dV, backwards
+        s.out = dv;
+        s.final_state = dstate;
+        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        // dK, backwards
+        s.q = v, s.k = go, s.v = q;
+        s.turned = 1;
+        s.final_state = nullptr;
+        s.out = group > 1 ? (void*)(base + at.dk) : dk;
+        s.out_f32 = group > 1;
+        s.dot = k;
+        s.dots = dlog_decay ? dots_k : nullptr;
+        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        if (group > 1) {
+            const i64 count = d->batch * d->time * d->heads * d->key;
+            with_type(d->type, [&](auto t) {
+                using T = decltype(t);
+                const unsigned blocks = (unsigned)std::min<i64>(ceil_div(count, 256), 8192);
+                group_sums<T><<<dim3(blocks), 256, 0, st>>>(base + at.dq, count, (int)d->key, group, (T*)dq);
+                group_sums<T><<<dim3(blocks), 256, 0, st>>>(base + at.dk, count, (int)d->key, group, (T*)dk);
+            });
+        }
+        if (dlog_decay) {
+            DecayGradients g{};
+            g.decay = decays_of(*d);
+            g.other = d->q;
+            g.lengths = d->lengths;
+            g.time = d->time;
+            g.tokens = (i64)p.per * chunk_of(d->type);
+            g.cells = p.state;
+            g.value_heads = (int)d->value_heads;
+            g.segments = p.segments;
+            g.starts = starts;
+            g.last = last;
+            g.behind = p.segments > 1 ? base + at.behind : nullptr;
+            g.grad_state = grad_state;
+            g.dq = dots_q;
+            g.dk = dots_k;
+            g.out = shared_decay ? nullptr : dlog_decay;
+            g.sums = shared_decay ? base + at.sums : nullptr;
+            decay_gradients<<<dim3((unsigned)p.segments, (unsigned)d->value_heads, (unsigned)d->batch), 256, 0, st>>>(g);
+            if (shared_decay)
+                head_sums<<<dim3((unsigned)d->value_heads), 256, 0, st>>>(g.sums, d->batch * p.segments, (int)d->value_heads,
+                                                                         d->log_decay_type == ATLAS_OPS_BF16, dlog_decay);
+        }
+        return launched(err, cap, "linear_backward");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,511 @@
+// The embedding of symbols with its gradient by sorted tokens, and dropout from the simulator's counter
+// generator.  Part of libatlas_ops_hip.so.
+//
+//   out_i = scale table[token_i]            (zeros where the token is no row of the table)
+//   dtable_r = scale sum of grad_i over the i with token_i = r
+//   y_i = residual_i + (draw_i >= p 2^32 ? x_i / (1 - p) : 0)
+//
+// The gradient's sums are taken in the tokens' order: a stable radix sort of (token, place), which starts
+// beside the clearing of the table, brings each row's places together; tiles of sorted places are summed in
+// registers, a run of one row within a tile goes straight to the table, and runs that cross tiles leave
+// partial sums, which a last kernel adds from the first tile to the last.  No atomics in sums: the same bits
+// every time.
+#include <algorithm>
+#include <type_traits>
+
+#include "device/atlas_rows.h"
+
+namespace atlas_ops {
+namespace {
+
+// ------------------------------------------------------------------ lookup
+struct Tokens {
+    const void* data;
+    int wide;  // 64-bit
+    i64 count;
+    __device__ __forceinline__ i64 at(i64 i) const { return wide ? ((const i64*)data)[i] : ((const int32_t*)data)[i]; }
+};
+
+// A group of LANES lanes copies the rows of TOGETHER tokens at a time, all their loads in flight.
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) embed_forward(const T* __restrict__ table, i64 rows, int width, i64 row_stride, Tokens tokens,
+                                                     float scale, T* __restrict__ out) {
+    constexpr int N = Unit<T>::N, GROUPS = 256 / LANES, TOGETHER = 4;
+    const int lane = threadIdx.x % LANES;
+    const i64 stride = (i64)gridDim.x * GROUPS * TOGETHER;
+    for (i64 i = ((i64)blockIdx.x * GROUPS + threadIdx.x / LANES) * TOGETHER; i < tokens.count; i += stride) {
+        i64 row[TOGETHER];
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) row[k] = tokens.at(min(i + k, tokens.count - 1));
+        for (int col = lane * N; col < width; col += LANES * N) {
+            Unit<T> unit[TOGETHER];
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) unit[k].load(table + (row[k] < 0 || row[k] >= rows ? 0 : row[k]) * row_stride, col, width);
+#pragma unroll
+            for (int k = 0; k < TOGETHER; ++k) {
+                if (i + k >= tokens.count) break;
+                float v[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] = row[k] < 0 || row[k] >= rows ? 0.0f : scale * unit[k][e];
+                store_unit<T>(out + (i + k) * width + col, width - col, v);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the stable sort
+constexpr int SORT_TILE = 2048, MAX_BITS = 11, SCANNED = 32;
+
+struct Sort {
+    i64 count, tiles;
+    int rows, shift, bits;  // the key of a token that is no row is `rows`: it sorts behind them
+    __device__ __forceinline__ uint32_t key_of(i64 token) const { return token < 0 || token >= rows ? (uint32_t)rows : (uint32_t)token; }
+    __device__ __forceinline__ uint32_t digit(uint32_t key) const { return (key >> shift) & ((1u << bits) - 1); }
+};
+
+// Digits per tile (blocks below `tiles`); the other blocks clear `size` bytes meanwhile.
+template <bool FIRST>
+__global__ void __launch_bounds__(256) sort_count(Sort s, Tokens tokens, const uint32_t* __restrict__ keys, uint32_t* __restrict__ counts,
+                                                  char* __restrict__ clear, i64 size) {
+    if (blockIdx.x >= s.tiles) {
+        struct __attribute__((packed, aligned(1))) Sixteen { uint32_t word[4]; };
+        const i64 stride = ((i64)gridDim.x - s.tiles) * 256 * 16;
+        for (i64 at = ((blockIdx.x - s.tiles) * 256 + threadIdx.x) * 16; at < size; at += stride) {
+            if (at + 16 <= size) {
+                *(Sixteen*)(clear + at) = Sixteen{};
+            } else {
+                for (i64 b = at; b < size; ++b) clear[b] = 0;
+            }
+        }
+        return;
+    }
+    __shared__ uint32_t bins[1 << MAX_BITS];
+    const int all = 1 << s.bits;
+    for (int b = threadIdx.x; b < all; b += 256) bins[b] = 0;
+    __syncthreads();
+    const i64 start = (i64)blockIdx.x * SORT_TILE;
+#pragma unroll
+    for (int e = 0; e < SORT_TILE / 256; ++e) {
+        const i64 i = start + e * 256 + threadIdx.x;
+        if (i < s.count) atomicAdd(&bins[s.digit(FIRST ? s.key_of(tokens.at(i)) : keys[i])], 1u);
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < all; b += 256) counts[(i64)blockIdx.x * all + b] = bins[b];
+}
+
+// Many tiles: each digit's counts become the counts of the tiles before, and their total goes behind them.
+__global__ void __launch_bounds__(256) sort_scan(Sort s, uint32_t* __restrict__ counts) {
+    const int all = 1 << s.bits, bin = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
+    if (bin >= all) return;
+    uint32_t before = 0;
+    for (i64 base = 0; base < s.tiles; base += 64) {
+        const i64 tile = base + lane;
+        const uint32_t own = tile < s.tiles ? counts[tile * all + bin] : 0;
+        uint32_t sum = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t other = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += other;
+        }
+        if (tile < s.tiles) counts[tile * all + bin] = before + sum - own;
+        before += __shfl(sum, 63, 64);
+    }
+    if (lane == 0) counts[s.tiles * all + bin] = before;
+}
+
+// Places every key of a tile behind those with smaller digits, of earlier tiles and, in the tile, of earlier
+// waves and lanes.  A wave takes 64 neighbouring keys at a time; ballots over the digit's bits find the lanes
+// with the same digit.
+template <bool FIRST, bool PREFIXED>
+__global__ void __launch_bounds__(256) sort_scatter(Sort s, Tokens tokens, const uint32_t* __restrict__ keys,
+                                                    const uint32_t* __restrict__ places, const uint32_t* __restrict__ counts,
+                                                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ places_out) {
+    constexpr int WAVE_KEYS = SORT_TILE / 4, ROUNDS = WAVE_KEYS / 64;
+    __shared__ uint32_t next[4][1 << MAX_BITS];
+    __shared__ uint32_t wave_sums[4];
+    const int all = 1 << s.bits, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const i64 tile = blockIdx.x, start = tile * SORT_TILE + wave * WAVE_KEYS;
+    for (int b = threadIdx.x; b < 4 * all; b += 256) next[b / all][b % all] = 0;
+    __syncthreads();
+    uint32_t key[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const i64 i = start + r * 64 + lane;
+        key[r] = i < s.count ? (FIRST ? s.key_of(tokens.at(i)) : keys[i]) : 0;
+        if (i < s.count) atomicAdd(&next[wave][s.digit(key[r])], 1u);
+    }
+    // each thread: a run of neighbouring digits; what comes before them is scanned over the workgroup
+    const int per = (all + 255) / 256, b0 = min((int)threadIdx.x * per, all), b1 = min(b0 + per, all);
+    uint32_t own = 0;
+    for (int b = b0; b < b1; ++b) {
+        if constexpr (PREFIXED) {
+            own += counts[s.tiles * all + b];
+        } else {
+            for (i64 t = 0; t < s.tiles; ++t) own += counts[t * all + b];
+        }
+    }
+    uint32_t sum = own;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t other = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += other;
+    }
+    if (lane == 63) wave_sums[wave] = sum;
+    __syncthreads();  // the waves' counts and sums are complete
+    uint32_t at = sum - own;
+    for (int w = 0; w < wave; ++w) at += wave_sums[w];
+    for (int b = b0; b < b1; ++b) {
+        uint32_t total = 0, before = 0;
+        if constexpr (PREFIXED) {
+            total = counts[s.tiles * all + b];
+            before = counts[tile * all + b];
+        } else {
+            for (i64 t = 0; t < s.tiles; ++t) {
+                const uint32_t c = counts[t * all + b];
+                total += c;
+                before += t < tile ? c : 0;
+            }
+        }
+        uint32_t place = at + before;
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t c = next[w][b];
+            next[w][b] = place;
+            place += c;
+        }
+        at += total;
+    }
+    __syncthreads();
+    volatile uint32_t* mine = next[wave];  // only this wave reads and writes it from here on, in program order
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const i64 i = start + r * 64 + lane;
+        const bool live = i < s.count;
+        const uint32_t digit = s.digit(key[r]);
+        u64 same = __ballot(live);
+        for (int b = 0; b < s.bits; ++b) {
+            const bool bit = digit >> b & 1;
+            const u64 ones = __ballot(live && bit);
+            same &= bit ? ones : ~ones;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1)), many = __popcll(same);
+        uint32_t place = 0;
+        if (live) place = mine[digit] + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (live && rank == many - 1) mine[digit] = place + 1;
+        __builtin_amdgcn_wave_barrier();
+        if (live) {
+            keys_out[place] = key[r];
+            places_out[place] = FIRST ? (uint32_t)i : places[i];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ the sums
+constexpr int SUM_TILE = 32;  // sorted places that a group sums
+
+// A tile's first run is a part of an earlier tile's row where the key before the tile is the same, its last
+// run of a later one's where the key behind is.  Partial sums: slot 0 of a tile for a run that comes from before,
+// slot 1 for one that starts here and goes on.
+template <typename T, typename O, int LANES>
+__global__ void __launch_bounds__(256) embed_sum(Rows grad, int width, i64 count, int rows, const uint32_t* __restrict__ keys,
+                                                 const uint32_t* __restrict__ places, float scale, O* __restrict__ table,
+                                                 float* __restrict__ partial) {
+    constexpr int N = Unit<T>::N, GROUPS = 256 / LANES, TOGETHER = 8;
+    __shared__ uint32_t key[GROUPS][SUM_TILE + 2], place[GROUPS][SUM_TILE];
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const i64 tile = (i64)blockIdx.x * GROUPS + group, first = tile * SUM_TILE;
+    const int n = first < count ? (int)min((i64)SUM_TILE, count - first) : 0;
+    for (int e = lane; e < SUM_TILE + 2; e += LANES) {
+        const i64 i = first + e - 1;
+        key[group][e] = i >= 0 && i < count ? keys[i] : 0xFFFFFFFFu;  // no row
+    }
+    for (int e = lane; e < n; e += LANES) place[group][e] = places[first + e];
+    __syncthreads();
+    const int col = (blockIdx.y * LANES + lane) * N, left = width - col;
+    if (left <= 0) return;
+    const uint32_t* k = key[group] + 1;
+    float sum[N];
+    int begun = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    for (int e0 = 0; e0 < n; e0 += TOGETHER) {
+        Unit<T> unit[TOGETHER];
+#pragma unroll
+        for (int j = 0; j < TOGETHER; ++j) unit[j].load(grad.at<T>(place[group][min(e0 + j, n - 1)]), col, width);
+#pragma unroll
+        for (int j = 0; j < TOGETHER; ++j) {
+            const int e = e0 + j;
+            if (e >= n || k[e] >= (uint32_t)rows) break;
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += unit[j][i];
+            if (e + 1 < n && k[e + 1] == k[e]) continue;
+            const bool from = begun == 0 && k[-1] == k[e], on = e + 1 == n && k[e + 1] == k[e];
+            if (from || on) {
+                store_unit<float, N>(partial + (2 * tile + (from ? 0 : 1)) * width + col, left, sum);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] *= scale;
+                store_unit<O, N>(table + (i64)k[e] * width + col, left, sum);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+            begun = e + 1;
+        }
+    }
+}
+
+// The row that starts in tile blockIdx.x and goes on behind it: its tiles' partial sums, each group a part of the
+// tiles in order, then the groups in order.
+template <typename O, int LANES, int N>
+__global__ void __launch_bounds__(1024) embed_join(int width, i64 count, int rows, const uint32_t* __restrict__ keys, float scale,
+                                                   O* __restrict__ table, const float* __restrict__ partial) {
+    constexpr int GROUPS = 1024 / LANES;
+    __shared__ float sums[GROUPS][LANES * N];
+    const i64 tile = blockIdx.x, first = tile * SUM_TILE, next = first + SUM_TILE;
+    if (next >= count) return;
+    const uint32_t row = keys[next];
+    if (row >= (uint32_t)rows || keys[next - 1] != row || (keys[first] == row && first > 0 && keys[first - 1] == row)) return;
+    // the tiles behind this one that begin with the row
+    const int lane64 = threadIdx.x % 64;
+    i64 more = 1;
+    for (;;) {
+        const i64 at = (tile + 1 + more + lane64) * SUM_TILE;
+        const u64 others = ~__ballot(at < count && keys[at] == row);
+        if (others) {
+            more += __builtin_ctzll(others);
+            break;
+        }
+        more += 64;
+    }
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    const int col = (blockIdx.y * LANES + lane) * N, left = width - col;
+    const i64 terms = 1 + more, per = (terms + GROUPS - 1) / GROUPS, from = group * per, to = min(terms, from + per);
+    float sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    if (left > 0) {
+#pragma unroll 4
+        for (i64 j = from; j < to; ++j) {
+            float v[N];
+            load_columns<float, N>(partial + (j ? 2 * (tile + j) : 2 * tile + 1) * width, col, width, 0.0f, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) sums[group][lane * N + i] = sum[i];
+    __syncthreads();
+    if (group || left <= 0) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float total = 0.0f;
+        for (int g = 0; g < GROUPS; ++g) total += sums[g][lane * N + i];
+        sum[i] = scale * total;
+    }
+    store_unit<O, N>(table + (i64)row * width + col, left, sum);
+}
+
+struct Plan {
+    Sort sort;
+    int passes, lanes;
+    i64 tiles, counts_at, keys_at, partial_at, bytes;  // tiles of the sums; offsets into the workspace
+};
+
+// What both the workspace and the launch go by.  grad's type sets the lanes: as few as hold a row's units.
+Plan plan_of(i64 count, i64 rows, i64 width, int type) {
+    Plan p{};
+    int bits = 1;
+    while (rows >> bits) ++bits;
+    p.passes = (bits + MAX_BITS - 1) / MAX_BITS;
+    p.sort = Sort{count, ceil_div(count, SORT_TILE), (int)rows, 0, (bits + p.passes - 1) / p.passes};
+    const i64 units = ceil_div(width, type == ATLAS_OPS_F32 ? 4 : 8);
+    p.lanes = 16;
+    while (p.lanes < units && p.lanes < 256) p.lanes *= 2;
+    p.tiles = ceil_div(count, SUM_TILE);
+    p.counts_at = 0;
+    p.keys_at = (p.sort.tiles + 1) * 4 << p.sort.bits;
+    p.partial_at = (p.keys_at + 16 * count + 15) / 16 * 16;
+    p.bytes = p.partial_at + p.tiles * 2 * width * 4;
+    return p;
+}
+
+template <typename F>
+void with_lanes(int lanes, F&& f) {
+    using std::integral_constant;
+    if (lanes == 16) f(integral_constant<int, 16>{});
+    else if (lanes == 32) f(integral_constant<int, 32>{});
+    else if (lanes == 64) f(integral_constant<int, 64>{});
+    else if (lanes == 128) f(integral_constant<int, 128>{});
+    else f(integral_constant<int, 256>{});
+}
+
+template <typename F>
+void with_type(int type, F&& f) {
+    if (type == ATLAS_OPS_F32) f(0.0f);
+    else f(bf16_t{});
+}
+
+// ------------------------------------------------------------------ dropout
+// The simulator's generator: splitmix64's finaliser of seed ^ stream C1 ^ tick C2 ^ draw C3 (executor.rs:190-222).
+// Values 2 n and 2 n + 1 take the low and the high 32 bits of draw n.
+constexpr u64 STREAM = 0x9e3779b97f4a7c15ull, TICK = 0xd1b54a32d192ed03ull, INDEX = 0x94d049bb133111ebull;
+
+__device__ __forceinline__ u64 finalise(u64 v) {
+    v = (v ^ (v >> 30)) * 0xbf58476d1ce4e5b9ull;
+    v = (v ^ (v >> 27)) * 0x94d049bb133111ebull;
+    return v ^ (v >> 31);
+}
+
+template <typename T, bool RESIDUAL>
+__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, i64 count, uint32_t threshold,
+                                                      float factor, u64 base, u64 tick, const i64* __restrict__ tick_at, T* __restrict__ y) {
+    constexpr int N = Unit<T>::N;
+    if (tick_at) tick = (u64)*tick_at;
+    base ^= tick * TICK;
+    const i64 stride = (i64)gridDim.x * 256 * N;
+    for (i64 at = ((i64)blockIdx.x * 256 + threadIdx.x) * N; at < count; at += stride) {
+        const int left = (int)min((i64)N, count - at);
+        Unit<T> v, r;
+        v.load(x + at, 0, left);
+        if constexpr (RESIDUAL) r.load(residual + at, 0, left);
+        u64 index = (u64)(at / 2) * INDEX;
+        float out[N];
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const u64 draw = finalise(base ^ index);
+            index += INDEX;
+            out[i] = (uint32_t)draw >= threshold ? v[i] * factor : 0.0f;
+            out[i + 1] = (uint32_t)(draw >> 32) >= threshold ? v[i + 1] * factor : 0.0f;
+            if constexpr (RESIDUAL) out[i] += r[i], out[i + 1] += r[i + 1];
+        }
+        store_unit<T>(y + at, left, out);
+    }
+}
+
+}  // namespace
+}  // namespace atlas_ops
+
+using namespace atlas_ops;
+
+extern "C" {
+
+int atlas_ops_embedding(const void* table, int64_t rows, int64_t width, int64_t row_stride, int type, const void* tokens, int wide,
+                        int64_t count, float scale, void* out, void* stream, char* err, size_t cap) {
+    try {
+        if (!known_type(type)) return fail(err, cap, 7, "unknown type");
+        if (rows < 1 || width < 1 || width > 0x7FFF0000 || count < 0) return fail(err, cap, 7, "rows and width must be positive, width below 2^31");
+        if (!count) return 0;
+        if (!table || !tokens || !out) return fail(err, cap, 7, "null argument");
+        const int lanes = plan_of(1, 1, width, type).lanes;
+        const i64 blocks = std::min<i64>(ceil_div(count, 4 * (256 / lanes)), 8192);
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            with_lanes(lanes, [&](auto l) {
+                embed_forward<T, l()><<<dim3((unsigned)blocks), 256, 0, (hipStream_t)stream>>>(
+                    (const T*)table, rows, (int)width, row_stride, Tokens{tokens, wide, count}, scale, (T*)out);
+            });
+        });
+        return launched(err, cap, "embedding");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+// Sizes that the sort and the sums' grids take.
+static bool embedding_fits(i64 count, i64 rows, i64 width) {
+    return count >= 0 && count <= (1 << 27) && rows >= 1 && rows < 0x7FFFFFFF && width >= 1 && width <= (1 << 20);
+}
+
+int64_t atlas_ops_embedding_workspace(int64_t count, int64_t rows, int64_t width, int type) {
+    if (!embedding_fits(count, rows, width) || !known_type(type)) return 0;
+    return plan_of(count, rows, width, type).bytes;
+}
+
+int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int wide, int64_t count, int64_t rows, int64_t width, int type,
+                                 int table_type, float scale, void* dtable, void* workspace, void* stream, char* err, size_t cap) {
+    try {
+        if (!known_type(type) || !known_type(table_type)) return fail(err, cap, 7, "unknown type");
+        if (!embedding_fits(count, rows, width)) return fail(err, cap, 7, "at most 2^27 tokens, rows below 2^31 - 1, width up to 2^20, both positive");
+        if (!dtable || (count && (!grad || !grad->data || grad->inner < 1 || !tokens || !workspace)))
+            return fail(err, cap, 7, "null argument");
+        Plan p = plan_of(count, rows, width, type);
+        hipStream_t st = (hipStream_t)stream;
+        const i64 size = rows * width * (table_type == ATLAS_OPS_F32 ? 4 : 2);
+        const i64 clearing = std::min<i64>(ceil_div(size, 256 * 16 * 4), 2048);
+        const Tokens list{tokens, wide, count};
+        char* base = (char*)workspace;
+        uint32_t *counts = (uint32_t*)(base + p.counts_at), *keys[2], *places[2];
+        for (int i = 0; i < 2; ++i) {
+            keys[i] = (uint32_t*)(base + p.keys_at) + 2 * i * count;
+            places[i] = keys[i] + count;
+        }
+        const unsigned tiles = (unsigned)p.sort.tiles;
+        if (!count) {
+            sort_count<true><<<dim3((unsigned)clearing), 256, 0, st>>>(p.sort, list, nullptr, nullptr, (char*)dtable, size);
+            return launched(err, cap, "embedding_backward");
+        }
+        for (int pass = 0; pass < p.passes; ++pass, p.sort.shift += p.sort.bits) {
+            const uint32_t *k = keys[(pass + 1) % 2], *v = places[(pass + 1) % 2];
+            uint32_t *ko = keys[pass % 2], *vo = places[pass % 2];
+            if (pass == 0) sort_count<true><<<dim3((unsigned)(tiles + clearing)), 256, 0, st>>>(p.sort, list, k, counts, (char*)dtable, size);
+            else sort_count<false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, counts, nullptr, 0);
+            const bool scanned = p.sort.tiles > SCANNED;
+            if (scanned) sort_scan<<<dim3((unsigned)ceil_div(1 << p.sort.bits, 4)), 256, 0, st>>>(p.sort, counts);
+            if (pass == 0 && scanned) sort_scatter<true, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
+            else if (pass == 0) sort_scatter<true, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
+            else if (scanned) sort_scatter<false, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
+            else sort_scatter<false, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
+        }
+        const uint32_t *sorted = keys[(p.passes + 1) % 2], *order = places[(p.passes + 1) % 2];
+        float* partial = (float*)(base + p.partial_at);
+        const Rows g{grad->data, grad->inner, grad->outer_stride, grad->inner_stride};
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            constexpr int N = Unit<T>::N;
+            with_type(table_type, [&](auto o) {
+                using O = decltype(o);
+                with_lanes(p.lanes, [&](auto l) {
+                    const unsigned slices = (unsigned)ceil_div(width, l() * N);
+                    embed_sum<T, O, l()><<<dim3((unsigned)ceil_div(p.tiles, 256 / l()), slices), 256, 0, st>>>(
+                        g, (int)width, count, (int)rows, sorted, order, scale, (O*)dtable, partial);
+                    if (p.tiles > 1)
+                        embed_join<O, l(), N><<<dim3((unsigned)(p.tiles - 1), slices), 1024, 0, st>>>(
+                            (int)width, count, (int)rows, sorted, scale, (O*)dtable, partial);
+                });
+            });
+        });
+        return launched(err, cap, "embedding_backward");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+int atlas_ops_dropout(const void* x, const void* residual, int64_t count, int type, double probability, uint64_t seed, uint64_t counter_stream,
+                      uint64_t tick, const int64_t* tick_at, void* y, void* stream, char* err, size_t cap) {
+    try {
+        if (!known_type(type)) return fail(err, cap, 7, "unknown type");
+        if (!(probability >= 0.0 && probability < 1.0)) return fail(err, cap, 7, "probability must be 0 or more and below 1");
+        if (count < 0) return fail(err, cap, 7, "count must not be negative");
+        if (!count) return 0;
+        if (!x || !y) return fail(err, cap, 7, "null argument");
+        const double share = probability * 4294967296.0;
+        const uint32_t threshold = share >= 4294967295.0 ? 0xFFFFFFFFu : (uint32_t)(share + 0.5);
+        const float factor = (float)(1.0 / (1.0 - probability));
+        const u64 base = seed ^ counter_stream * STREAM;
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            const i64 blocks = std::min<i64>(ceil_div(count, 256 * Unit<T>::N), 4096);
+            if (residual)
+                dropout_kernel<T, true><<<dim3((unsigned)blocks), 256, 0, (hipStream_t)stream>>>(
+                    (const T*)x, (const T*)residual, count, threshold, factor, base, tick, tick_at, (T*)y);
+            else
+                dropout_kernel<T, false><<<dim3((unsigned)blocks), 256, 0, (hipStream_t)stream>>>(
+                    (const T*)x, nullptr, count, threshold, factor, base, tick, tick_at, (T*)y);
+        });
+        return launched(err, cap, "dropout");
+    } catch (...) {
+        return fail(err, cap, 7, "host exception");
+    }
+}
+
+}  // extern "C"

@@ -1,6 +1,7 @@
 /*
- * C ABI of the MI355X (gfx950) sequence-layer operators, libatlas_ops_hip.so: layer
- * normalisation, the gated delta rule and the orthogonalised weight update.
+ * C ABI of the MI355X (gfx950) sequence-layer operators, libatlas_ops_hip.so: layer and
+ * root-mean-square normalisation, the gated delta rule, linear attention, the embedding of
+ * symbols, dropout and the orthogonalised weight update.
  *
  * Every pointer is device memory of the current device unless its comment says otherwise, every
  * call enqueues its kernels on `stream` (a hipStream_t) and returns without waiting; nothing is
@@ -120,6 +121,76 @@ int atlas_ops_delta_backward(const AtlasDelta* delta, const void* tape, const vo
                              const int64_t* grad_out_stride, const float* grad_state, void* dq, void* dk, void* dv,
                              void* dlog_decay, void* dbeta, float* dstate, void* workspace, void* stream, char* error,
                              size_t capacity);
+
+/*
+ * Root-mean-square normalisation of a stream: t = x + residual rounded to `type` (t = x where residual is NULL),
+ * y = t rstd weight by row, rstd = 1 / sqrt(mean(t^2) + eps).  y is rows x width, contiguous, of x's type, or,
+ * where scale (f32[rows]) is not NULL, 8-bit e4m3 values of y / scale with scale = max(max |y| / 448, 2^-126).  total
+ * (NULL exactly where residual is) receives t, contiguous; rstd (may be NULL) f32[rows]; weight may be NULL.
+ */
+int atlas_ops_rms_norm(const AtlasRows* x, const AtlasRows* residual, int64_t rows, int64_t width, int type,
+                       const void* weight, int weight_type, float eps, void* y, float* scale, void* total, float* rstd,
+                       void* stream, char* error, size_t capacity);
+
+/* Bytes of workspace that atlas_ops_rms_norm_backward needs for dweight. */
+int64_t atlas_ops_rms_norm_workspace(int64_t rows, int64_t width, int type);
+
+/* The gradient of t (dx, contiguous, of its type), which is that of x and of the residual, from those of y (grad) and of t
+ * itself (grad_total, may be NULL), and, where not NULL, of the weight, summed over the rows in a fixed order. */
+int atlas_ops_rms_norm_backward(const AtlasRows* grad, const AtlasRows* total, const AtlasRows* grad_total, int64_t rows,
+                                int64_t width, int type, const void* weight, int weight_type, const float* rstd, void* dx,
+                                void* dweight, float* workspace, void* stream, char* error, size_t capacity);
+
+/* out_i = scale table[token_i], contiguous, zeros where token_i is no row.  table is rows x width of `type`, its rows
+ * row_stride apart; tokens are `count` contiguous i32, or i64 where wide is not 0. */
+int atlas_ops_embedding(const void* table, int64_t rows, int64_t width, int64_t row_stride, int type, const void* tokens,
+                        int wide, int64_t count, float scale, void* out, void* stream, char* error, size_t capacity);
+
+/* Bytes of the workspace of atlas_ops_embedding_backward: count up to 2^27, rows below 2^31 - 1, width up to 2^20. */
+int64_t atlas_ops_embedding_workspace(int64_t count, int64_t rows, int64_t width, int type);
+
+/* dtable_r = scale times the sum of the rows i of grad (`type`) with token_i = r, in their order: rows x width, contiguous,
+ * of table_type, zeros where there is none.  The same bits on every run. */
+int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int wide, int64_t count, int64_t rows,
+                                 int64_t width, int type, int table_type, float scale, void* dtable, void* workspace,
+                                 void* stream, char* error, size_t capacity);
+
+/*
+ * y_i = residual_i + (kept_i ? x_i / (1 - probability) : 0) of `count` contiguous values; residual may be NULL, y may be x
+ * or residual.  Values 2 n and 2 n + 1 take the low and the high 32 bits of draw n of the simulator's generator, the
+ * finaliser of splitmix64 on seed ^ counter_stream C1 ^ tick C2 ^ n C3 (C1 0x9e3779b97f4a7c15, C2 0xd1b54a32d192ed03,
+ * C3 0x94d049bb133111eb), and are kept where they reach probability 2^32 rounded half up.  tick_at (may be NULL) holds
+ * the tick on the device, read when the kernel runs.
+ */
+int atlas_ops_dropout(const void* x, const void* residual, int64_t count, int type, double probability, uint64_t seed,
+                      uint64_t counter_stream, uint64_t tick, const int64_t* tick_at, void* y, void* stream, char* error,
+                      size_t capacity);
+
+/*
+ * Linear attention with a decay by head.  As the gated delta rule without its correction: by token, with
+ * a = exp(log_decay), S <- a S + k v^T, out = scale S^T q.  The problem is an AtlasDelta whose beta is not
+ * read; log_decay strides may be 0.  Value up to 128 wide, time up to 2^29, batch x value_heads below 2^25 in chunks.
+ */
+int atlas_ops_linear_step(const AtlasDelta* linear, void* out, float* final_state, void* stream, char* error,
+                          size_t capacity);
+
+/* Bytes of the workspace of a forward pass; with train != 0 of one that a backward pass can use. */
+int64_t atlas_ops_linear_workspace(const AtlasDelta* linear, int train);
+
+/* In chunks: out (contiguous, `type`) and final_state.  With train != 0 the workspace is afterwards the tape of
+ * atlas_ops_linear_backward. */
+int atlas_ops_linear_forward(const AtlasDelta* linear, int train, void* out, float* final_state, void* workspace,
+                             void* stream, char* error, size_t capacity);
+
+/* Bytes of the backward pass's own workspace. */
+int64_t atlas_ops_linear_backward_workspace(const AtlasDelta* linear);
+
+/* The gradients as of atlas_ops_delta_backward.  With shared_decay != 0 log_decay is one value by value head, and
+ * dlog_decay, value_heads values, their sum over batch and time. */
+int atlas_ops_linear_backward(const AtlasDelta* linear, const void* tape, const void* grad_out,
+                              const int64_t* grad_out_stride, const float* grad_state, void* dq, void* dk, void* dv,
+                              void* dlog_decay, int shared_decay, float* dstate, void* workspace, void* stream,
+                              char* error, size_t capacity);
 
 #ifdef __cplusplus
 }
