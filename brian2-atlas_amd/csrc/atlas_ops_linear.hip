@@ -26,6 +26,7 @@ namespace atlas_ops {
 namespace {
 
 constexpr int MAX_WIDTH = 128;
+constexpr i64 MAX_STRIDE = 1 << 24;  // from token to token: a chunk's offsets stay below 2^32 bytes
 constexpr float LOWEST = -120.0f;  // the exponential is zero in float32
 
 // Log decays of (batch, time, value head), of any strides.
@@ -203,12 +204,9 @@ struct Scan {
 
 template <typename T>
 struct Cut {
-    static constexpr int N = sizeof(T) == 2 ? 1 : 3;  // bfloat16 pieces of a value
+    static constexpr int N = sizeof(T) == 2 ? 1 : 3;    // bfloat16 pieces of a value
     static constexpr int C = sizeof(T) == 2 ? 64 : 32;  // tokens per chunk
-    static constexpr int QB = C / 16, KB = C / 32;
 };
-
-typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 // Four values of column l % 16, rows quad .. quad + 3 from `at`, the address of row quad + l % 16 / 4, columns 4 (l % 4) ..:
 // the hardware turns 4 x 16 blocks for 16 lanes each.
@@ -219,22 +217,62 @@ __device__ __forceinline__ bf16x4 turned_read(const bf16_t* at) {
 
 __device__ __forceinline__ bf16x8 both(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
-// Workgroup: one segment of one value head.  Wave w holds the state's columns of its NB blocks of 16 in
-// registers, all DK rows.  NB = 2: block n of the wave has columns 32 w + 8 i + 4 n + j (i, j < 4) at lanes 4 i + j, so
-// that a lane's results are eight neighbours; NB = 1: 16 w + l.
-template <typename T, int DK, int NB, bool OUT>
-__global__ void __launch_bounds__(256, 2) scan(Scan d) {
-    constexpr int N = Cut<T>::N, C = Cut<T>::C, QB = Cut<T>::QB, KB = Cut<T>::KB, DV = 64 * NB;
-    constexpr int E = Unit<T>::N, PITCH = DK + 8, VPITCH = DV + (sizeof(T) == 2 ? 8 : 4);
-    constexpr int KU = C * DK / E / 256, VU = C * DV / E / 256;  // units of a chunk per thread
-    constexpr int SCORES = QB == 4 ? 6 : 2;                      // operands of 16 queries x 32 keys that are not zero
+// A thread's share of a chunk's rows, C tokens of up to W values: units of 16 bytes in every STEP-th token.  The loads stand
+// behind no branch: what is no unit of the row or not of a live token reads the chunk's first and becomes zero.  Without
+// WHOLE units the one that the row's end cuts is read as the row's last 16 bytes and shifted down when it is placed.
+template <typename T, int W, int THREADS, int C, bool WHOLE>
+struct Share {
+    static constexpr int E = Unit<T>::N, ACROSS = W / E, STEP = THREADS / ACROSS, COUNT = C / STEP;
+    static_assert(C % STEP == 0, "every thread has the same number of units");
+    Unit<T> unit[COUNT];
+
+    __device__ __forceinline__ static int token(uint32_t thread) { return thread / ACROSS; }
+    __device__ __forceinline__ static int column(uint32_t thread) { return thread % ACROSS * E; }
+    // live: tokens of the chunk that are
+    __device__ __forceinline__ void load(uint32_t thread, const T* chunk, int stride, int width, int live) {
+        const int column = Share::column(thread);
+#pragma unroll
+        for (int u = 0; u < COUNT; ++u) {
+            const int t = token(thread) + u * STEP;
+            if constexpr (WHOLE) {
+                unit[u].memcpy_in(chunk + (uint32_t)(t < live && column < width ? t * stride + column : 0));
+            } else {
+                unit[u].load(chunk + (uint32_t)(t < live ? t * stride : 0), column, width);
+            }
+        }
+    }
+    __device__ __forceinline__ Unit<T> value(uint32_t thread, int u, int width, int live) const {
+        Unit<T> x = unit[u];
+        const bool some = token(thread) + u * STEP < live && column(thread) < width;
+        x.low = some ? x.low : 0;
+        x.high = some ? x.high : 0;
+        return x;
+    }
+};
+
+// The thread's number, from which nothing can be computed ahead of a loop: what is kept for every turn there costs
+// registers that the state needs.
+__device__ __forceinline__ uint32_t thread_here() {
+    uint32_t thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    return thread;
+}
+
+// Workgroup: one segment of one value head.  Wave w holds the state's columns 16 w .. 16 w + 15 in registers, all DK
+// rows.  The tiles lie in LDS token by token, in the order of the recurrence; operands whose sums go over tokens are
+// turned as they are read.
+// WHOLE: both widths are whole units of 16 bytes.
+template <typename T, int DK, int WAVES, bool OUT, bool WHOLE>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2) scan(Scan d) {
+    constexpr int N = Cut<T>::N, C = Cut<T>::C, QB = C / 16, KB = C / 32, THREADS = 64 * WAVES, DV = 16 * WAVES;
+    constexpr int PITCH = DK + 8, VPITCH = DV + (sizeof(T) == 2 ? 8 : 4);
+    constexpr int BLOCKS = QB * (QB + 1) / 2, OPERANDS = QB == 4 ? 6 : 2;  // of scores that are not zero: 16 x 16, 16 queries x 32 keys
     __shared__ __attribute__((aligned(16))) bf16_t qs[OUT ? N * C * PITCH : 8], ks[N * C * PITCH];
     __shared__ __attribute__((aligned(16))) T vs[C * VPITCH];
-    __shared__ __attribute__((aligned(16))) bf16_t scores[OUT ? SCORES * 3 * 512 : 8];
+    __shared__ __attribute__((aligned(16))) bf16_t scores[OUT ? OPERANDS * 3 * 512 : 8];
     __shared__ __attribute__((aligned(16))) float gate_sum[C], gate_rest[C], since[C], rest[C];
-    __shared__ float dot_part[OUT ? 4 : 1][C];
-    const Lane l;
-    const int wave = threadIdx.x / 64;
+    __shared__ float dot_part[OUT ? WAVES : 1][C];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int segment = d.first + blockIdx.x;
     const i64 h = blockIdx.y, b = blockIdx.z, head = b * d.value_heads + h;
     const i64 length = length_of(d.lengths, d.time, b);
@@ -242,64 +280,56 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
     const int used = (int)((length + C - 1) / C);  // chunks with a token
     const int inner = d.q.width, outer = d.v.width;
     const T *qp = d.q.x.at<T>(b, 0, h / d.q.group), *kp = d.k.x.at<T>(b, 0, h / d.k.group), *vp = d.v.x.at<T>(b, 0, h / d.v.group);
-    const int cell = 4 * NB * (l.col / 4) + l.col % 4;  // of block 0 within the wave's columns; block n: + 4 n
-    const int column = 16 * NB * wave + cell;
 
-    // the state: block r of rows 16 r .., block n of columns
-    float4_t s[DK / 16][NB];
+    // the state: block r of rows 16 r ..
+    float4_t s[DK / 16];
 #pragma unroll
-    for (int r = 0; r < DK / 16; ++r)
-#pragma unroll
-        for (int n = 0; n < NB; ++n) s[r][n] = ZERO;
+    for (int r = 0; r < DK / 16; ++r) s[r] = ZERO;
     if (OUT && d.start) {
         const float* from = d.start + (d.start_segments ? head * d.segments + segment : head) * inner * outer;
+        const int down = d.turned ? 1 : outer, across = d.turned ? inner : 1;
+        const Lane l(thread_here());
+        const int column = 16 * wave + l.col, at = min(column, outer - 1) * across;
 #pragma unroll
         for (int r = 0; r < DK / 16; ++r)
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int j = 0; j < 4; ++j) s[r][j] = from[(uint32_t)(min(16 * r + l.quad + j, inner - 1) * down + at)];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = 16 * r + l.quad + j, col = column + 4 * n;
-                    const bool live = row < inner && col < outer;
-                    const float v = from[live ? d.turned ? (i64)col * inner + row : (i64)row * outer + col : 0];
-                    s[r][n][j] = live ? v : 0.0f;
-                }
+        for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[r][j] = 16 * r + l.quad + j < inner && column < outer ? s[r][j] : 0.0f;
     }
+    if constexpr (OUT)  // halves of operands above the diagonal stay zero
+        for (int i = threadIdx.x; i < OPERANDS * 3 * 512 / 2; i += THREADS) ((uint32_t*)scores)[i] = 0;
 
-    Unit<T> qu[OUT ? KU : 1], ku[KU], vu[VU];
+    Share<T, DK, THREADS, C, WHOLE> qu, ku;
+    Share<T, DV, THREADS, C, WHOLE> vu;
     Decays::Raw raw;
-    auto token = [&](int chunk, int row) { return (i64)chunk * C + (d.backwards ? C - 1 - row : row); };
+    // row r of a tile is the chunk's token r, backwards C - 1 - r
+    auto token = [&](int row) { return d.backwards ? C - 1 - row : row; };
     auto fetch = [&](int chunk) {
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const int at = threadIdx.x + 256 * u, row = at / (DK / E), col = at % (DK / E) * E;
-            const i64 t = min(token(chunk, row), d.time - 1);
-            if constexpr (OUT) qu[u].load(qp + t * d.q.x.time, col, inner);
-            ku[u].load(kp + t * d.k.x.time, col, inner);
-        }
-#pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int at = threadIdx.x + 256 * u, row = at / (DV / E), col = at % (DV / E) * E;
-            vu[u].load(vp + min(token(chunk, row), d.time - 1) * d.v.x.time, col, outer);
-        }
-        raw = d.decay.load(qp, b, min(token(chunk, l.id % C) + d.backwards, d.time - 1), h);
+        const i64 t0 = (i64)chunk * C;
+        const int live = (int)min((i64)C, length - t0);
+        const uint32_t thread = thread_here();
+        if constexpr (OUT) qu.load(thread, qp + t0 * d.q.x.time, (int)d.q.x.time, inner, live);
+        ku.load(thread, kp + t0 * d.k.x.time, (int)d.k.x.time, inner, live);
+        vu.load(thread, vp + t0 * d.v.x.time, (int)d.v.x.time, outer, live);
+        raw = d.decay.load(qp, b, min(t0 + token(thread % C) + d.backwards, d.time - 1), h);
     };
-    // splits a unit into the N planes of an LDS tile
-    auto place = [&](bf16_t* tile, const Unit<T>& u, int row, int col, bool live) {
+    // a unit as the N planes of a tile
+    auto place = [&](bf16_t* tile, const Unit<T>& u, int row, int col) {
         bf16_t* p = tile + row * PITCH + col;
         if constexpr (N == 1) {
-            u64* q = (u64*)p;
-            q[0] = live ? u.low : 0;
-            q[1] = live ? u.high : 0;
+            ((u64*)p)[0] = u.low;
+            ((u64*)p)[1] = u.high;
         } else {
-            const float4_t v = {live ? u[0] : 0.0f, live ? u[1] : 0.0f, live ? u[2] : 0.0f, live ? u[3] : 0.0f};
-            const Halves<3> parts = split<3>(v);
+            const Halves<3> parts = split<3>(float4_t{u[0], u[1], u[2], u[3]});
 #pragma unroll
             for (int i = 0; i < 3; ++i) *(bf16x4*)(p + i * C * PITCH) = parts.p[i];
         }
     };
-    // an operand of rows block of a tile, 32 columns from c0
-    auto rows_operand = [&](const bf16_t* tile, int block, int c0) {
+    // operand of a block of 16 rows of a tile, 32 columns from c0
+    auto rows_operand = [&](const Lane& l, const bf16_t* tile, int block, int c0) {
         Pieces<N> r;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -308,17 +338,28 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
         }
         return r;
     };
+    // the values as operands: this wave's column l % 16, sums over 32 tokens
+    auto value_floats = [&](const Lane& l, int kb, float4_t (&x)[2]) {
+        if constexpr (N == 1) {
+            const bf16_t* p = (const bf16_t*)vs + (32 * kb + l.quad + l.col / 4) * VPITCH + 16 * wave + 4 * (l.col % 4);
+            x[0] = widen(turned_read(p)), x[1] = widen(turned_read(p + 16 * VPITCH));
+        } else {
+            const float* p = (const float*)vs + (32 * kb + l.quad) * VPITCH + 16 * wave + l.col;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[0][j] = p[j * VPITCH], x[1][j] = p[(16 + j) * VPITCH];
+        }
+    };
 
     const int steps = high - low;
     double whole = 0.0;  // log decay of the segment's chunks
     if (low < used) fetch(d.backwards ? min(high, used) - 1 : low);
     for (int step = 0; step < steps; ++step) {
         const int chunk = d.backwards ? high - 1 - step : low + step;
+        const i64 t0 = (i64)chunk * C;
         if (chunk >= used) {  // no token: zeros
             if constexpr (OUT) {
-                const i64 t0 = (i64)chunk * C;
                 const int rows = (int)min((i64)C, d.time - t0);
-                for (int at = threadIdx.x; at < rows * outer; at += 256) {
+                for (int at = threadIdx.x; at < rows * outer; at += THREADS) {
                     const i64 o = ((b * d.time + t0 + at / outer) * d.value_heads + h) * outer + at % outer;
                     if (d.out_f32) ((float*)d.out)[o] = 0.0f;
                     else ((T*)d.out)[o] = from_float<T>(0.0f);
@@ -327,26 +368,27 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
             }
             continue;
         }
+        const int live = (int)min((i64)C, length - t0);
+        const uint32_t thread = thread_here();
+        const Lane l(thread);
         // ---- the chunk into LDS, its decays: G as a float and its remainder, in powers of two
 #pragma unroll
-        for (int u = 0; u < KU; ++u) {
-            const int at = threadIdx.x + 256 * u, row = at / (DK / E), col = at % (DK / E) * E;
-            const bool live = token(chunk, row) < length;
-            if constexpr (OUT) place(qs, qu[u], row, col, live);
-            place(ks, ku[u], row, col, live);
+        for (int u = 0; u < ku.COUNT; ++u) {
+            const int row = token(ku.token(thread) + u * ku.STEP);
+            if constexpr (OUT) place(qs, qu.value(thread, u, inner, live), row, qu.column(thread));
+            place(ks, ku.value(thread, u, inner, live), row, ku.column(thread));
         }
 #pragma unroll
-        for (int u = 0; u < VU; ++u) {
-            const int at = threadIdx.x + 256 * u, row = at / (DV / E), col = at % (DV / E) * E;
-            const bool live = token(chunk, row) < length;
-            u64* p = (u64*)(vs + row * VPITCH + col);
-            p[0] = live ? vu[u].low : 0;
-            p[1] = live ? vu[u].high : 0;
+        for (int u = 0; u < vu.COUNT; ++u) {
+            const Unit<T> x = vu.value(thread, u, outer, live);
+            u64* p = (u64*)(vs + token(vu.token(thread) + u * vu.STEP) * VPITCH + vu.column(thread));
+            p[0] = x.low;
+            p[1] = x.high;
         }
         double total;
         {
             const int row = l.id % C;
-            const i64 t = token(chunk, row) + d.backwards;
+            const i64 t = t0 + token(row) + d.backwards;
             double sum = t < length ? (double)d.decay.value(raw) * 1.4426950408889634 : 0.0;
 #pragma unroll
             for (int k = 1; k < C; k *= 2) {
@@ -362,184 +404,126 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
             }
             whole += total;
         }
-        __syncthreads();
+        lds_barrier();
         const int next = d.backwards ? chunk - 1 : chunk + 1;
         if (d.backwards ? next >= low : next < min(high, used)) fetch(next);
-
-        // ---- the values as operands: columns of this wave, sums over tokens
-        float4_t v[KB][NB][2];
-        bf16x8 vb[KB][NB];  // N = 1
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if constexpr (N == 1) {
-                    const bf16_t* p = (const bf16_t*)vs + (32 * kb + l.quad + l.col / 4) * VPITCH + 16 * NB * wave + 4 * NB * (l.col % 4) + 4 * n;
-                    const bf16x4 a = turned_read(p), c = turned_read(p + 16 * VPITCH);
-                    vb[kb][n] = both(a, c);
-                    v[kb][n][0] = widen(a), v[kb][n][1] = widen(c);
-                } else {
-                    const float* p = (const float*)vs + (32 * kb + l.quad) * VPITCH + column + 4 * n;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[kb][n][0][j] = p[j * VPITCH], v[kb][n][1][j] = p[(16 + j) * VPITCH];
-                }
-            }
+        in_order();
 
         if constexpr (OUT) {
-            // ---- decayed scores of this wave's queries, turned: rows are keys
-            for (int qb = wave; qb < QB; qb += 4) {
-                float4_t p[QB];
+            // ---- decayed scores, turned: rows are keys, columns queries
+            for (int block = wave; block < BLOCKS; block += WAVES) {
+                const int qb = block >= 6 ? 3 : block >= 3 ? 2 : block >= 1 ? 1 : 0, kj = block - qb * (qb + 1) / 2;
+                float4_t p = ZERO;
 #pragma unroll
-                for (int kj = 0; kj < QB; ++kj) p[kj] = ZERO;
-#pragma unroll
-                for (int c = 0; c < DK / 32; ++c) {
-                    const Pieces<N> q = rows_operand(qs, qb, 32 * c);
-#pragma unroll
-                    for (int kj = 0; kj < QB; ++kj)
-                        if (kj <= qb) p[kj] = mma(rows_operand(ks, kj, 32 * c), q, p[kj]);
-                }
+                for (int c = 0; c < DK / 32; ++c) p = mma(rows_operand(l, ks, kj, 32 * c), rows_operand(l, qs, qb, 32 * c), p);
                 const int i = 16 * qb + l.col;
                 const float sum = gate_sum[i], remainder = gate_rest[i];
+                const int at = 16 * kj + l.quad;
+                const float4_t sums = *(const float4_t*)(gate_sum + at), remainders = *(const float4_t*)(gate_rest + at);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    if (2 * kb > qb) continue;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float4_t& x = p[2 * kb + half];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int at = 32 * kb + 16 * half + l.quad + j;
-                            const float decay = __builtin_amdgcn_exp2f((sum - gate_sum[at]) + (remainder - gate_rest[at])) * d.write;
-                            x[j] = at <= i ? x[j] * decay : 0.0f;
-                        }
-                    }
-                    const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kb) : qb;
-                    put<3>(scores, operand, l, split<3>(p[2 * kb], p[2 * kb + 1]));
+                for (int j = 0; j < 4; ++j) {  // both selects: a masked decay may be infinite, a masked score anything
+                    const float decay = __builtin_amdgcn_exp2f(at + j <= i ? (sum - sums[j]) + (remainder - remainders[j]) : 0.0f);
+                    p[j] = at + j <= i ? p[j] * decay * d.write : 0.0f;
                 }
+                const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kj / 2) : qb;
+                put_half<3>(scores, operand, kj % 2, l, split<3>(p));
             }
             // ---- what the state answers: rows are columns of the values, columns are queries
-            float4_t o[QB][NB];
+            float4_t o[QB];
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-                for (int n = 0; n < NB; ++n) o[qb][n] = ZERO;
+            for (int qb = 0; qb < QB; ++qb) o[qb] = ZERO;
 #pragma unroll
             for (int c = 0; c < DK / 32; ++c) {
-                Pieces<3> state[NB];
+                const Pieces<3> state = split<3>(s[2 * c], s[2 * c + 1]);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) state[n] = split<3>(s[2 * c][n], s[2 * c + 1][n]);
+                for (int qb = 0; qb < QB; ++qb) o[qb] = mma(state, rows_operand(l, qs, qb, 32 * c), o[qb]);
+                in_order();
+            }
+#pragma unroll
+            for (int qb = 0; qb < QB; ++qb) o[qb] *= since[16 * qb + l.col];
+            lds_barrier();  // the scores are there
+            // ---- the chunk's own tokens.  A NaN or an infinity among the values would reach the tokens before it through
+            // zeros of the scores: it is taken out, and the rows from its column's first on are NaN afterwards
+            int worst = C;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                float4_t x[2];
+                value_floats(l, kb, x);
+                float faulty = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) faulty = fmaf(x[e / 4][e % 4], 0.0f, faulty);
+                if (__ballot(faulty != faulty)) {
+#pragma unroll
+                    for (int e = 7; e >= 0; --e)
+                        if (!(fabsf(x[e / 4][e % 4]) < INFINITY)) {
+                            x[e / 4][e % 4] = 0.0f;
+                            worst = min(worst, 32 * kb + 16 * (e / 4) + l.quad + e % 4);
+                        }
+                }
+                const Pieces<N> value = split<N>(x[0], x[1]);
 #pragma unroll
                 for (int qb = 0; qb < QB; ++qb) {
-                    const Pieces<N> q = rows_operand(qs, qb, 32 * c);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) o[qb][n] = mma(state[n], q, o[qb][n]);
-                }
-            }
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb) {
-                const float g = since[16 * qb + l.col];
-#pragma unroll
-                for (int n = 0; n < NB; ++n) o[qb][n] *= g;
-            }
-            // ---- a NaN or an infinity among the values would reach the tokens before it through zeros of the scores:
-            // it is taken out, and the rows from its column's first on are NaN afterwards
-            float faulty = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) faulty = fmaf(v[kb][n][e / 4][e % 4], 0.0f, faulty);
-            const bool any = __ballot(faulty != faulty) != 0;
-            int worst[NB];  // the first faulty token of block n's column l % 16
-            Pieces<N> value[KB][NB];
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                worst[n] = C;
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    float4_t x[2] = {v[kb][n][0], v[kb][n][1]};
-                    if (any) {
-#pragma unroll
-                        for (int e = 7; e >= 0; --e)
-                            if (!(fabsf(x[e / 4][e % 4]) < INFINITY)) {
-                                x[e / 4][e % 4] = 0.0f;
-                                worst[n] = min(worst[n], 32 * kb + 16 * (e / 4) + l.quad + e % 4);
-                            }
-                    }
-                    if constexpr (N == 1) {
-                        value[kb][n].p[0] = vb[kb][n];
-                        if (any) value[kb][n] = split<1>(x[0], x[1]);
-                    } else {
-                        value[kb][n] = split<3>(x[0], x[1]);
-                    }
-                }
-                if (any) {
-                    worst[n] = min(worst[n], __shfl_xor(worst[n], 16, 64));
-                    worst[n] = min(worst[n], __shfl_xor(worst[n], 32, 64));
-                }
-            }
-            __syncthreads();  // the scores are there
-#pragma unroll
-            for (int qb = 0; qb < QB; ++qb)
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
                     if (2 * kb > qb) continue;
                     const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kb) : qb;
-                    const Pieces<3> p = atlas_ops::fetch<3>(scores, operand, l);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) o[qb][n] = mma(value[kb][n], p, o[qb][n]);
+                    o[qb] = mma(value, atlas_ops::fetch<3>(scores, operand, l), o[qb]);
                 }
-            if (any) {
-#pragma unroll
-                for (int n = 0; n < NB; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int first = __shfl(worst[n], l.quad + j, 64);  // of the results' row
-#pragma unroll
-                        for (int qb = 0; qb < QB; ++qb)
-                            if (16 * qb + l.col >= first) o[qb][n][j] = NAN;
-                    }
+                in_order();
             }
-            // ---- a lane's 4 NB neighbouring columns of one token
-            const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
+            if (__ballot(worst < C)) {
+                worst = min(worst, __shfl_xor(worst, 16, 64));
+                worst = min(worst, __shfl_xor(worst, 32, 64));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int first = __shfl(worst, l.quad + j, 64);  // of the results' row
+#pragma unroll
+                    for (int qb = 0; qb < QB; ++qb)
+                        if (16 * qb + l.col >= first) o[qb][j] = NAN;
+                }
+            }
+            // ---- a lane's four neighbouring columns of one token
+            const int c0 = 16 * wave + l.quad, left = outer - c0;
+            const i64 out0 = ((b * d.time + t0) * d.value_heads + h) * outer + c0;
+            const T* x0 = d.dots ? d.dot.x.at<T>(b, t0, h / d.dot.group) + (left > 0 ? c0 : 0) : nullptr;
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
-                const i64 t = token(chunk, 16 * qb + l.col);
-                float row[4 * NB];
+                const int t = token(16 * qb + l.col);
+                float row[4];
 #pragma unroll
-                for (int e = 0; e < 4 * NB; ++e) row[e] = t < length ? d.read * o[qb][e / 4][e % 4] : 0.0f;
+                for (int e = 0; e < 4; ++e) row[e] = t < live ? d.read * o[qb][e] : 0.0f;
                 if (d.dots) {
                     float dot = 0.0f;
-                    if (t < length && left > 0) {
-                        const T* x = d.dot.x.at<T>(b, t, h / d.dot.group) + c0;
+                    const T* x = x0 + (t < live && left > 0 ? (uint32_t)(t * (int)d.dot.x.time) : 0u);
+                    struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; } four;
+                    if constexpr (WHOLE) {
+                        four = *(const Four*)x;
+                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4 * NB; ++e) dot += e < left ? row[e] * to_float(x[e < left ? e : 0]) : 0.0f;
+                        for (int e = 0; e < 4; ++e) four.v[e] = x[min(e, max(left - 1, 0))];
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dot += e < left && t < live ? row[e] * to_float(four.v[e]) : 0.0f;
                     dot += __shfl_xor(dot, 16, 64);
                     dot += __shfl_xor(dot, 32, 64);
                     if (l.quad == 0) dot_part[wave][16 * qb + l.col] = dot;
                 }
-                if (t < d.time && left > 0) {
-                    const i64 at = ((b * d.time + t) * d.value_heads + h) * outer + c0;
-                    if (d.out_f32) store_unit<float, 4 * NB>((float*)d.out + at, left, row);
-                    else store_unit<T, 4 * NB>((T*)d.out + at, left, row);
+                if (t0 + t < d.time && left > 0) {
+                    const i64 at = out0 + (uint32_t)(t * d.value_heads * outer);
+                    if (d.out_f32) store_unit<float, 4>((float*)d.out + at, WHOLE ? 4 : left, row);
+                    else store_unit<T, 4>((T*)d.out + at, WHOLE ? 4 : left, row);
                 }
             }
+            in_order();
         }
 
         // ---- the state behind the chunk
         const float decayed = __builtin_amdgcn_exp2f((float)total);
 #pragma unroll
-        for (int r = 0; r < DK / 16; ++r)
-#pragma unroll
-            for (int n = 0; n < NB; ++n) s[r][n] *= decayed;
+        for (int r = 0; r < DK / 16; ++r) s[r] *= decayed;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            Pieces<3> written[NB];
-            const float4_t ra = *(const float4_t*)(rest + 32 * kb + l.quad), rb = *(const float4_t*)(rest + 32 * kb + 16 + l.quad);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) written[n] = split<3>(v[kb][n][0] * ra, v[kb][n][1] * rb);
+            float4_t x[2];
+            value_floats(l, kb, x);
+            const Pieces<3> written = split<3>(x[0] * *(const float4_t*)(rest + 32 * kb + l.quad), x[1] * *(const float4_t*)(rest + 32 * kb + 16 + l.quad));
 #pragma unroll
             for (int r = 0; r < DK / 16; ++r) {
                 Pieces<N> k;
@@ -548,16 +532,17 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                     const bf16_t* p = ks + i * C * PITCH + (32 * kb + l.quad + l.col / 4) * PITCH + 16 * r + 4 * (l.col % 4);
                     k.p[i] = both(turned_read(p), turned_read(p + 16 * PITCH));
                 }
-#pragma unroll
-                for (int n = 0; n < NB; ++n) s[r][n] = mma(k, written[n], s[r][n]);
+                s[r] = mma(k, written, s[r]);
+                if (r % 4 == 3) in_order();
             }
         }
-        __syncthreads();  // the tiles are read, the dots written
+        lds_barrier();  // the tiles are read, the dots written
         if constexpr (OUT) {
-            const i64 t = token(chunk, threadIdx.x % C);
-            if (d.dots && threadIdx.x < C && t < d.time) {
-                const int r = threadIdx.x;
-                d.dots[head * d.time + t] = (dot_part[0][r] + dot_part[1][r]) + (dot_part[2][r] + dot_part[3][r]);
+            if (d.dots && thread < C && t0 + token(thread) < d.time) {
+                float dot = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) dot += dot_part[w][thread];
+                d.dots[head * d.time + t0 + token(thread)] = dot;
             }
         }
     }
@@ -575,17 +560,17 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
         if (threadIdx.x == 0) d.decays[head * d.segments + segment] = (float)exp2(whole);
     }
     if (!to) return;
+    const Lane l(thread_here());
+    const int column = 16 * wave + l.col;
 #pragma unroll
     for (int r = 0; r < DK / 16; ++r)
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = 16 * r + l.quad + j, col = column + 4 * n;
-                if (row >= inner || col >= outer) continue;
-                to[(i64)row * outer + col] = factor * s[r][n][j];
-                if (copy) copy[(i64)row * outer + col] = factor * s[r][n][j];
-            }
+        for (int j = 0; j < 4; ++j) {
+            const int row = 16 * r + l.quad + j;
+            if (row >= inner || column >= outer) continue;
+            to[row * outer + column] = factor * s[r][j];
+            if (copy) copy[row * outer + column] = factor * s[r][j];
+        }
 }
 
 // Turns the segments' sums into the states at their starts, in place.  backwards: the last segment's start is `start`.
@@ -757,10 +742,15 @@ void launch_scan(const Scan& s, int type, i64 batch, int segments, hipStream_t s
     const dim3 grid((unsigned)segments, (unsigned)s.value_heads, (unsigned)batch);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        if (s.q.width <= 64 && s.v.width <= 64) scan<T, 64, 1, OUT><<<grid, 256, 0, st>>>(s);
-        else if (s.q.width <= 64) scan<T, 64, 2, OUT><<<grid, 256, 0, st>>>(s);
-        else if (s.v.width <= 64) scan<T, 128, 1, OUT><<<grid, 256, 0, st>>>(s);
-        else scan<T, 128, 2, OUT><<<grid, 256, 0, st>>>(s);
+        constexpr int E = Unit<T>::N;
+        auto widths = [&](auto whole) {
+            if (s.q.width <= 64 && s.v.width <= 64) scan<T, 64, 4, OUT, whole()><<<grid, 256, 0, st>>>(s);
+            else if (s.q.width <= 64) scan<T, 64, 8, OUT, whole()><<<grid, 512, 0, st>>>(s);
+            else if (s.v.width <= 64) scan<T, 128, 4, OUT, whole()><<<grid, 256, 0, st>>>(s);
+            else scan<T, 128, 8, OUT, whole()><<<grid, 512, 0, st>>>(s);
+        };
+        if (s.q.width % E || s.v.width % E) widths(std::false_type{});
+        else widths(std::true_type{});
     });
 }
 
@@ -774,6 +764,8 @@ int check(const AtlasDelta* d, bool chunks, char* err, size_t cap) {
     if (d->value_heads % d->heads) return fail(err, cap, 7, "value_heads must be a multiple of heads");
     if (d->batch > 65535 || d->value_heads > 65535) return fail(err, cap, 7, "at most 65535 sequences and value heads");
     if (d->time > ((i64)1 << 29)) return fail(err, cap, 7, "time must be at most 2^29");
+    for (const int64_t* stride : {d->q_stride, d->k_stride, d->v_stride})
+        if (chunks && (stride[1] < 0 || stride[1] > MAX_STRIDE)) return fail(err, cap, 7, "tokens must be at most 2^24 elements apart");
     if (chunks && d->batch * d->value_heads > 65535 * 512) return fail(err, cap, 7, "batch x value_heads must be below 2^25");
     if (!known_type(d->type) || !known_type(d->log_decay_type)) return fail(err, cap, 7, "unknown type");
     if (!d->q || !d->k || !d->v) return fail(err, cap, 7, "null tensor");

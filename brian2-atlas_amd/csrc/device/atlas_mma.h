@@ -104,7 +104,8 @@ __device__ __forceinline__ void mma2(const Pieces<NA>& a, const Pieces<NB>& b, f
 
 struct Lane {
     int id, col, quad;  // l, l % 16, 4 (l / 16)
-    __device__ __forceinline__ Lane() : id(threadIdx.x % 64), col(threadIdx.x % 16), quad(threadIdx.x % 64 / 16 * 4) {}
+    __device__ __forceinline__ Lane() : Lane(threadIdx.x) {}
+    __device__ __forceinline__ explicit Lane(uint32_t thread) : id(thread % 64), col(thread % 16), quad(thread % 64 / 16 * 4) {}
 };
 
 // Operands in memory: N pieces, 16 bytes per lane each.
