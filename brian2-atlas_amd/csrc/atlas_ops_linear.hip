@@ -33,14 +33,14 @@ constexpr float LOWEST = -120.0f;  // the exponential is zero in float32
 struct Decays {
     Tensor x;
     int bf16;
-    struct Raw { uint16_t low, high; };
+    struct Raw { uint32_t low, high; };  // apart: joined they would be waited for at once
     // with a load that stands behind no branch (of `other` where there are no decays)
     __device__ __forceinline__ Raw load(const void* other, i64 b, i64 t, i64 h) const {
         const uint16_t* p = x.data ? (const uint16_t*)x.data + ((b * x.batch + t * x.time + h * x.head) << (bf16 ? 0 : 1)) : (const uint16_t*)other;
         return {p[0], p[x.data && !bf16 ? 1 : 0]};
     }
     __device__ __forceinline__ float value(Raw r) const {
-        const float g = __uint_as_float(bf16 ? (uint32_t)r.low << 16 : (uint32_t)r.high << 16 | r.low);
+        const float g = __uint_as_float(bf16 ? r.low << 16 : r.high << 16 | r.low);
         return !x.data ? 0.0f : g < LOWEST ? LOWEST : g;  // a NaN stays one
     }
 };
@@ -217,6 +217,22 @@ __device__ __forceinline__ bf16x4 turned_read(const bf16_t* at) {
 
 __device__ __forceinline__ bf16x8 both(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+// Whether any of eight values is a NaN or an infinity: its exponent's bits are all ones.
+__device__ __forceinline__ bool beyond(bf16x8 v) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    const uint4_t bits = __builtin_bit_cast(uint4_t, v);
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, bits[i] & 0x7FFF7FFFu));
+    return max(most[0], most[1]) >= 0x7F80;
+}
+__device__ __forceinline__ bool beyond(float4_t a, float4_t b) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(max(most, __float_as_uint(a[i]) & 0x7FFFFFFFu), __float_as_uint(b[i]) & 0x7FFFFFFFu);
+    return most >= 0x7F800000u;
+}
+
 // A thread's share of a chunk's rows, C tokens of up to W values: units of 16 bytes in every STEP-th token.  The loads stand
 // behind no branch: what is no unit of the row or not of a live token reads the chunk's first and becomes zero.  Without
 // WHOLE units the one that the row's end cuts is read as the row's last 16 bytes and shifted down when it is placed.
@@ -241,8 +257,10 @@ struct Share {
             }
         }
     }
-    __device__ __forceinline__ Unit<T> value(uint32_t thread, int u, int width, int live) const {
+    // all: every unit is one of the row and of a live token
+    __device__ __forceinline__ Unit<T> value(uint32_t thread, int u, int width, int live, bool all) const {
         Unit<T> x = unit[u];
+        if (all) return x;
         const bool some = token(thread) + u * STEP < live && column(thread) < width;
         x.low = some ? x.low : 0;
         x.high = some ? x.high : 0;
@@ -258,19 +276,21 @@ __device__ __forceinline__ uint32_t thread_here() {
     return thread;
 }
 
-// Workgroup: one segment of one value head.  Wave w holds the state's columns 16 w .. 16 w + 15 in registers, all DK
-// rows.  The tiles lie in LDS token by token, in the order of the recurrence; operands whose sums go over tokens are
-// turned as they are read.
-// WHOLE: both widths are whole units of 16 bytes.
-template <typename T, int DK, int WAVES, bool OUT, bool WHOLE>
-__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2) scan(Scan d) {
-    constexpr int N = Cut<T>::N, C = Cut<T>::C, QB = C / 16, KB = C / 32, THREADS = 64 * WAVES, DV = 16 * WAVES;
+// Workgroup: one segment of one value head.  Wave w holds the state's columns of its NB blocks of 16 in
+// registers, all DK rows.  NB = 2: block n of the wave has columns 32 w + 8 i + 4 n + j (i, j < 4) at lanes 4 i + j, so
+// that a lane's results are eight neighbours; NB = 1: 16 w + l.  The tiles lie in LDS token by token, in the order of the
+// recurrence; operands whose sums go over tokens are turned as they are read.  WHOLE: both widths are whole units of 16
+// bytes.
+template <typename T, int DK, int NB, bool OUT, bool WHOLE>
+__global__ void __launch_bounds__(256, 2) scan(Scan d) {
+    constexpr int N = Cut<T>::N, C = Cut<T>::C, QB = C / 16, KB = C / 32, WAVES = 4, THREADS = 64 * WAVES, DV = 16 * NB * WAVES;
     constexpr int PITCH = DK + 8, VPITCH = DV + (sizeof(T) == 2 ? 8 : 4);
     constexpr int BLOCKS = QB * (QB + 1) / 2, OPERANDS = QB == 4 ? 6 : 2;  // of scores that are not zero: 16 x 16, 16 queries x 32 keys
     __shared__ __attribute__((aligned(16))) bf16_t qs[OUT ? N * C * PITCH : 8], ks[N * C * PITCH];
     __shared__ __attribute__((aligned(16))) T vs[C * VPITCH];
     __shared__ __attribute__((aligned(16))) bf16_t scores[OUT ? OPERANDS * 3 * 512 : 8];
-    __shared__ __attribute__((aligned(16))) float gate_sum[C], gate_rest[C], since[C], rest[C];
+    // of two chunks in turn: G as a float and its remainder, the factors of what the state answers and of what is written to it
+    __shared__ __attribute__((aligned(16))) float gate_sum[2][C], gate_rest[2][C], since[2][C], rest[2][C], decays[2];
     __shared__ float dot_part[OUT ? WAVES : 1][C];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int segment = d.first + blockIdx.x;
@@ -280,24 +300,30 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2)
     const int used = (int)((length + C - 1) / C);  // chunks with a token
     const int inner = d.q.width, outer = d.v.width;
     const T *qp = d.q.x.at<T>(b, 0, h / d.q.group), *kp = d.k.x.at<T>(b, 0, h / d.k.group), *vp = d.v.x.at<T>(b, 0, h / d.v.group);
+    auto cell = [&](const Lane& l, int n) { return 16 * NB * wave + 4 * NB * (l.col / 4) + l.col % 4 + 4 * n; };
 
-    // the state: block r of rows 16 r ..
-    float4_t s[DK / 16];
+    // the state: block r of rows 16 r .., block n of columns
+    float4_t s[DK / 16][NB];
 #pragma unroll
-    for (int r = 0; r < DK / 16; ++r) s[r] = ZERO;
+    for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+        for (int n = 0; n < NB; ++n) s[r][n] = ZERO;
     if (OUT && d.start) {
         const float* from = d.start + (d.start_segments ? head * d.segments + segment : head) * inner * outer;
         const int down = d.turned ? 1 : outer, across = d.turned ? inner : 1;
         const Lane l(thread_here());
-        const int column = 16 * wave + l.col, at = min(column, outer - 1) * across;
 #pragma unroll
-        for (int r = 0; r < DK / 16; ++r)
+        for (int n = 0; n < NB; ++n) {
+            const int column = cell(l, n), at = min(column, outer - 1) * across;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[r][j] = from[(uint32_t)(min(16 * r + l.quad + j, inner - 1) * down + at)];
+            for (int r = 0; r < DK / 16; ++r)
 #pragma unroll
-        for (int r = 0; r < DK / 16; ++r)
+                for (int j = 0; j < 4; ++j) s[r][n][j] = from[(uint32_t)(min(16 * r + l.quad + j, inner - 1) * down + at)];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[r][j] = 16 * r + l.quad + j < inner && column < outer ? s[r][j] : 0.0f;
+            for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[r][n][j] = 16 * r + l.quad + j < inner && column < outer ? s[r][n][j] : 0.0f;
+        }
     }
     if constexpr (OUT)  // halves of operands above the diagonal stay zero
         for (int i = threadIdx.x; i < OPERANDS * 3 * 512 / 2; i += THREADS) ((uint32_t*)scores)[i] = 0;
@@ -307,14 +333,16 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2)
     Decays::Raw raw;
     // row r of a tile is the chunk's token r, backwards C - 1 - r
     auto token = [&](int row) { return d.backwards ? C - 1 - row : row; };
-    auto fetch = [&](int chunk) {
+    auto fetch = [&](int chunk, int which) {  // a part at a time: the loads of one after the other would hold the wave up
         const i64 t0 = (i64)chunk * C;
         const int live = (int)min((i64)C, length - t0);
         const uint32_t thread = thread_here();
-        if constexpr (OUT) qu.load(thread, qp + t0 * d.q.x.time, (int)d.q.x.time, inner, live);
-        ku.load(thread, kp + t0 * d.k.x.time, (int)d.k.x.time, inner, live);
-        vu.load(thread, vp + t0 * d.v.x.time, (int)d.v.x.time, outer, live);
-        raw = d.decay.load(qp, b, min(t0 + token(thread % C) + d.backwards, d.time - 1), h);
+        if (which & 1) {
+            raw = d.decay.load(qp, b, min(t0 + token(thread % C) + d.backwards, d.time - 1), h);
+            if constexpr (OUT) qu.load(thread, qp + t0 * d.q.x.time, (int)d.q.x.time, inner, live);
+        }
+        if (which & 2) ku.load(thread, kp + t0 * d.k.x.time, (int)d.k.x.time, inner, live);
+        if (which & 4) vu.load(thread, vp + t0 * d.v.x.time, (int)d.v.x.time, outer, live);
     };
     // a unit as the N planes of a tile
     auto place = [&](bf16_t* tile, const Unit<T>& u, int row, int col) {
@@ -338,21 +366,50 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2)
         }
         return r;
     };
-    // the values as operands: this wave's column l % 16, sums over 32 tokens
-    auto value_floats = [&](const Lane& l, int kb, float4_t (&x)[2]) {
+    // the values as an operand of block n's columns, sums over 32 tokens: as bfloat16, and as floats
+    auto value_raw = [&](const Lane& l, int kb, int n) {
+        const bf16_t* p = (const bf16_t*)vs + (32 * kb + l.quad + l.col / 4) * VPITCH + 16 * NB * wave + 4 * NB * (l.col % 4) + 4 * n;
+        return Halves<2>{turned_read(p), turned_read(p + 16 * VPITCH)};
+    };
+    auto value_floats = [&](const Lane& l, int kb, int n, float4_t (&x)[2]) {
         if constexpr (N == 1) {
-            const bf16_t* p = (const bf16_t*)vs + (32 * kb + l.quad + l.col / 4) * VPITCH + 16 * wave + 4 * (l.col % 4);
-            x[0] = widen(turned_read(p)), x[1] = widen(turned_read(p + 16 * VPITCH));
+            const Halves<2> v = value_raw(l, kb, n);
+            x[0] = widen(v.p[0]), x[1] = widen(v.p[1]);
         } else {
-            const float* p = (const float*)vs + (32 * kb + l.quad) * VPITCH + 16 * wave + l.col;
+            const float* p = (const float*)vs + (32 * kb + l.quad) * VPITCH + cell(l, n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[0][j] = p[j * VPITCH], x[1][j] = p[(16 + j) * VPITCH];
         }
     };
 
+    // a chunk's decays, in powers of two, by the last wave, which has the fewest scores
+    double whole = 0.0;  // log decay of the segment's chunks, in that wave
+    auto gates = [&](int chunk, int turn) {
+        const int lane = thread_here() % 64, row = lane % C;
+        const i64 t = (i64)chunk * C + token(row) + d.backwards;
+        double sum = t < length ? (double)d.decay.value(raw) * 1.4426950408889634 : 0.0;
+#pragma unroll
+        for (int k = 1; k < C; k *= 2) {
+            const double before = __shfl_up(sum, k, C);
+            if (row >= k) sum += before;
+        }
+        const double total = __shfl(sum, C - 1, 64);
+        if (lane < C) {
+            gate_sum[turn][row] = (float)sum;
+            gate_rest[turn][row] = (float)(sum - (double)(float)sum);
+            since[turn][row] = __builtin_amdgcn_exp2f((float)sum) * d.read;
+            rest[turn][row] = __builtin_amdgcn_exp2f((float)(total - sum)) * d.write;
+        }
+        if (lane == 0) decays[turn] = __builtin_amdgcn_exp2f((float)total);
+        whole += total;
+    };
+
     const int steps = high - low;
-    double whole = 0.0;  // log decay of the segment's chunks
-    if (low < used) fetch(d.backwards ? min(high, used) - 1 : low);
+    if (low < used) {
+        const int first = d.backwards ? min(high, used) - 1 : low;
+        fetch(first, 7);
+        if (wave == WAVES - 1) gates(first, (d.backwards ? high - 1 - first : 0) & 1);
+    }
     for (int step = 0; step < steps; ++step) {
         const int chunk = d.backwards ? high - 1 - step : low + step;
         const i64 t0 = (i64)chunk * C;
@@ -371,174 +428,279 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2)
         const int live = (int)min((i64)C, length - t0);
         const uint32_t thread = thread_here();
         const Lane l(thread);
-        // ---- the chunk into LDS, its decays: G as a float and its remainder, in powers of two
+        // ---- the chunk into LDS
+        const bool all_q = live == C && inner == DK, all_v = live == C && outer == DV;
+        const int turn = step & 1;
 #pragma unroll
         for (int u = 0; u < ku.COUNT; ++u) {
             const int row = token(ku.token(thread) + u * ku.STEP);
-            if constexpr (OUT) place(qs, qu.value(thread, u, inner, live), row, qu.column(thread));
-            place(ks, ku.value(thread, u, inner, live), row, ku.column(thread));
+            if constexpr (OUT) place(qs, qu.value(thread, u, inner, live, all_q), row, qu.column(thread));
+            place(ks, ku.value(thread, u, inner, live, all_q), row, ku.column(thread));
         }
 #pragma unroll
         for (int u = 0; u < vu.COUNT; ++u) {
-            const Unit<T> x = vu.value(thread, u, outer, live);
+            const Unit<T> x = vu.value(thread, u, outer, live, all_v);
             u64* p = (u64*)(vs + token(vu.token(thread) + u * vu.STEP) * VPITCH + vu.column(thread));
             p[0] = x.low;
             p[1] = x.high;
         }
-        double total;
-        {
-            const int row = l.id % C;
-            const i64 t = t0 + token(row) + d.backwards;
-            double sum = t < length ? (double)d.decay.value(raw) * 1.4426950408889634 : 0.0;
-#pragma unroll
-            for (int k = 1; k < C; k *= 2) {
-                const double before = __shfl_up(sum, k, C);
-                if (row >= k) sum += before;
-            }
-            total = __shfl(sum, C - 1, 64);
-            if (wave == 0 && l.id < C) {
-                gate_sum[row] = (float)sum;
-                gate_rest[row] = (float)(sum - (double)(float)sum);
-                since[row] = __builtin_amdgcn_exp2f((float)sum);
-                rest[row] = __builtin_amdgcn_exp2f((float)(total - sum)) * d.write;
-            }
-            whole += total;
-        }
         lds_barrier();
         const int next = d.backwards ? chunk - 1 : chunk + 1;
-        if (d.backwards ? next >= low : next < min(high, used)) fetch(next);
+        const bool more = d.backwards ? next >= low : next < min(high, used);
+        if (more) fetch(next, OUT ? 1 : 7);
         in_order();
 
         if constexpr (OUT) {
             // ---- decayed scores, turned: rows are keys, columns queries
-            for (int block = wave; block < BLOCKS; block += WAVES) {
-                const int qb = block >= 6 ? 3 : block >= 3 ? 2 : block >= 1 ? 1 : 0, kj = block - qb * (qb + 1) / 2;
-                float4_t p = ZERO;
+            constexpr int OWN = (BLOCKS + WAVES - 1) / WAVES;  // blocks of a wave, all in flight; what lies beyond the last is not kept
+            float4_t p[OWN];
+            int qbs[OWN], kjs[OWN];
 #pragma unroll
-                for (int c = 0; c < DK / 32; ++c) p = mma(rows_operand(l, ks, kj, 32 * c), rows_operand(l, qs, qb, 32 * c), p);
-                const int i = 16 * qb + l.col;
-                const float sum = gate_sum[i], remainder = gate_rest[i];
-                const int at = 16 * kj + l.quad;
-                const float4_t sums = *(const float4_t*)(gate_sum + at), remainders = *(const float4_t*)(gate_rest + at);
+            for (int m = 0; m < OWN; ++m) {
+                const int block = min(wave + WAVES * m, BLOCKS - 1);
+                qbs[m] = block >= 6 ? 3 : block >= 3 ? 2 : block >= 1 ? 1 : 0;
+                kjs[m] = block - qbs[m] * (qbs[m] + 1) / 2;
+                p[m] = ZERO;
+            }
+            Pieces<N> kn[2][OWN], qn[2][OWN];
+            auto read = [&](int c) {
+#pragma unroll
+                for (int m = 0; m < OWN; ++m) {
+                    kn[c & 1][m] = rows_operand(l, ks, kjs[m], 32 * c);
+                    qn[c & 1][m] = rows_operand(l, qs, qbs[m], 32 * c);
+                }
+                in_order();
+            };
+            read(0);
+#pragma unroll
+            for (int c = 0; c < DK / 32; ++c) {
+                if (c + 1 < DK / 32) read(c + 1);
+                mma_each(kn[c & 1], qn[c & 1], p);
+                in_order();
+            }
+            const float factor = d.write * d.read;
+#pragma unroll
+            for (int m = 0; m < OWN; ++m) {
+                const int qb = qbs[m], kj = kjs[m], i = 16 * qb + l.col, at = 16 * kj + l.quad;
+                const float sum = gate_sum[turn][i], remainder = gate_rest[turn][i];
+                const float4_t sums = *(const float4_t*)(gate_sum[turn] + at), remainders = *(const float4_t*)(gate_rest[turn] + at);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // both selects: a masked decay may be infinite, a masked score anything
                     const float decay = __builtin_amdgcn_exp2f(at + j <= i ? (sum - sums[j]) + (remainder - remainders[j]) : 0.0f);
-                    p[j] = at + j <= i ? p[j] * decay * d.write : 0.0f;
+                    float x = p[m][j] * decay * factor;
+                    asm("" : "+v"(x));  // a select, not a branch
+                    p[m][j] = at + j <= i ? x : 0.0f;
                 }
                 const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kj / 2) : qb;
-                put_half<3>(scores, operand, kj % 2, l, split<3>(p));
+                const Halves<3> parts = split_pairs(p[m]);
+                if (wave + WAVES * m < BLOCKS) put_half<3>(scores, operand, kj % 2, l, parts);
             }
+            if (more) fetch(next, 2);
+            in_order();
             // ---- what the state answers: rows are columns of the values, columns are queries
-            float4_t o[QB];
+            float4_t o[NB][QB];
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) o[qb] = ZERO;
+            for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n][qb] = ZERO;
+            Pieces<N> q[2][QB];
+            auto read_queries = [&](int c) {
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) q[c & 1][qb] = rows_operand(l, qs, qb, 32 * c);
+                in_order();
+            };
+            read_queries(0);
 #pragma unroll
             for (int c = 0; c < DK / 32; ++c) {
-                const Pieces<3> state = split<3>(s[2 * c], s[2 * c + 1]);
+                Pieces<3> state[NB];
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb) o[qb] = mma(state, rows_operand(l, qs, qb, 32 * c), o[qb]);
+                for (int n = 0; n < NB; ++n) state[n] = split_pairs(s[2 * c][n], s[2 * c + 1][n]);
+                if (c + 1 < DK / 32) read_queries(c + 1);
+                mma_grid(state, q[c & 1], o);
                 in_order();
             }
 #pragma unroll
-            for (int qb = 0; qb < QB; ++qb) o[qb] *= since[16 * qb + l.col];
+            for (int qb = 0; qb < QB; ++qb) {
+                const float g = since[turn][16 * qb + l.col];
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n][qb] *= g;
+            }
             lds_barrier();  // the scores are there
+            if (more) fetch(next, 4);
+            in_order();
             // ---- the chunk's own tokens.  A NaN or an infinity among the values would reach the tokens before it through
             // zeros of the scores: it is taken out, and the rows from its column's first on are NaN afterwards
-            int worst = C;
+            constexpr int PAIRS = QB == 4 ? 3 : 1;  // (32 keys, two blocks of queries) that are not zero: (0, 0), (0, 2), (1, 2)
+            Pieces<3> pn[2][2];
+            auto read_scores = [&](int pair) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) pn[pair & 1][i] = atlas_ops::fetch<3>(scores, pair == 0 ? i : 2 * (i + 1) + pair - 1, l);
+                in_order();
+            };
+            int worst[NB];
+            bool any = false;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) worst[n] = C;
+            read_scores(0);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
-                float4_t x[2];
-                value_floats(l, kb, x);
-                float faulty = 0.0f;
+                Pieces<N> value[NB];
+                float4_t x[NB][2];
+                bool faulty = false;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) faulty = fmaf(x[e / 4][e % 4], 0.0f, faulty);
-                if (__ballot(faulty != faulty)) {
-#pragma unroll
-                    for (int e = 7; e >= 0; --e)
-                        if (!(fabsf(x[e / 4][e % 4]) < INFINITY)) {
-                            x[e / 4][e % 4] = 0.0f;
-                            worst = min(worst, 32 * kb + 16 * (e / 4) + l.quad + e % 4);
-                        }
+                for (int n = 0; n < NB; ++n) {
+                    if constexpr (N == 1) {
+                        const Halves<2> v = value_raw(l, kb, n);
+                        value[n].p[0] = both(v.p[0], v.p[1]);
+                        faulty |= beyond(value[n].p[0]);
+                    } else {
+                        value_floats(l, kb, n, x[n]);
+                        faulty |= beyond(x[n][0], x[n][1]);
+                    }
                 }
-                const Pieces<N> value = split<N>(x[0], x[1]);
+                if (__ballot(faulty)) {
+                    any = true;
 #pragma unroll
-                for (int qb = 0; qb < QB; ++qb) {
-                    if (2 * kb > qb) continue;
-                    const int operand = QB == 4 ? (qb < 2 ? qb : 2 * (qb - 1) + kb) : qb;
-                    o[qb] = mma(value, atlas_ops::fetch<3>(scores, operand, l), o[qb]);
+                    for (int n = 0; n < NB; ++n) {
+                        value_floats(l, kb, n, x[n]);
+#pragma unroll
+                        for (int e = 7; e >= 0; --e)
+                            if (!(fabsf(x[n][e / 4][e % 4]) < INFINITY)) {
+                                x[n][e / 4][e % 4] = 0.0f;
+                                worst[n] = min(worst[n], 32 * kb + 16 * (e / 4) + l.quad + e % 4);
+                            }
+                        if constexpr (N == 1) value[n] = split<1>(x[n][0], x[n][1]);
+                    }
                 }
-                in_order();
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+                    if constexpr (N == 3) value[n] = split_pairs(x[n][0], x[n][1]);
+#pragma unroll
+                for (int pair = kb == 0 ? 0 : 2; pair < (kb == 0 ? min(2, PAIRS) : 3); ++pair) {
+                    if (pair + 1 < PAIRS) read_scores(pair + 1);
+                    const int q0 = pair == 0 ? 0 : 2;
+                    float4_t sums[NB][2];
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) sums[n][i] = o[n][q0 + i];
+                    mma_grid(value, pn[pair & 1], sums);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[n][q0 + i] = sums[n][i];
+                    in_order();
+                }
             }
-            if (__ballot(worst < C)) {
-                worst = min(worst, __shfl_xor(worst, 16, 64));
-                worst = min(worst, __shfl_xor(worst, 32, 64));
+            if (any) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int first = __shfl(worst, l.quad + j, 64);  // of the results' row
+                for (int n = 0; n < NB; ++n) {
+                    worst[n] = min(worst[n], __shfl_xor(worst[n], 16, 64));
+                    worst[n] = min(worst[n], __shfl_xor(worst[n], 32, 64));
 #pragma unroll
-                    for (int qb = 0; qb < QB; ++qb)
-                        if (16 * qb + l.col >= first) o[qb][j] = NAN;
+                    for (int j = 0; j < 4; ++j) {
+                        const int first = __shfl(worst[n], l.quad + j, 64);  // of the results' row
+#pragma unroll
+                        for (int qb = 0; qb < QB; ++qb)
+                            if (16 * qb + l.col >= first) o[n][qb][j] = NAN;
+                    }
                 }
             }
-            // ---- a lane's four neighbouring columns of one token
-            const int c0 = 16 * wave + l.quad, left = outer - c0;
+            if (live < C) {
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n)
+                        if (token(16 * qb + l.col) >= live) o[n][qb] = ZERO;
+            }
+            // ---- a lane's 4 NB neighbouring columns of one token
+            constexpr bool FULL = WHOLE && (sizeof(T) == 2 || NB == 1);  // 4 NB columns are there or none
+            const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
             const i64 out0 = ((b * d.time + t0) * d.value_heads + h) * outer + c0;
             const T* x0 = d.dots ? d.dot.x.at<T>(b, t0, h / d.dot.group) + (left > 0 ? c0 : 0) : nullptr;
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 const int t = token(16 * qb + l.col);
-                float row[4];
+                float row[4 * NB];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) row[e] = t < live ? d.read * o[qb][e] : 0.0f;
+                for (int e = 0; e < 4 * NB; ++e) row[e] = o[e / 4][qb][e % 4];
                 if (d.dots) {
                     float dot = 0.0f;
                     const T* x = x0 + (t < live && left > 0 ? (uint32_t)(t * (int)d.dot.x.time) : 0u);
-                    struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; } four;
-                    if constexpr (WHOLE) {
-                        four = *(const Four*)x;
+                    struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[4 * NB]; } few;
+                    if constexpr (FULL) {
+                        few = *(const Few*)x;
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) four.v[e] = x[min(e, max(left - 1, 0))];
+                        for (int e = 0; e < 4 * NB; ++e) few.v[e] = x[min(e, max(left - 1, 0))];
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dot += e < left && t < live ? row[e] * to_float(four.v[e]) : 0.0f;
+                    for (int e = 0; e < 4 * NB; ++e) dot += FULL || e < left ? row[e] * to_float(few.v[e]) : 0.0f;
+                    dot = t < live && left > 0 ? dot : 0.0f;
                     dot += __shfl_xor(dot, 16, 64);
                     dot += __shfl_xor(dot, 32, 64);
                     if (l.quad == 0) dot_part[wave][16 * qb + l.col] = dot;
                 }
                 if (t0 + t < d.time && left > 0) {
                     const i64 at = out0 + (uint32_t)(t * d.value_heads * outer);
-                    if (d.out_f32) store_unit<float, 4>((float*)d.out + at, WHOLE ? 4 : left, row);
-                    else store_unit<T, 4>((T*)d.out + at, WHOLE ? 4 : left, row);
+                    if (d.out_f32) store_unit<float, 4 * NB>((float*)d.out + at, FULL ? 4 * NB : left, row);
+                    else store_unit<T, 4 * NB>((T*)d.out + at, FULL ? 4 * NB : left, row);
                 }
             }
             in_order();
         }
 
         // ---- the state behind the chunk
-        const float decayed = __builtin_amdgcn_exp2f((float)total);
+        const float decayed = decays[turn];
 #pragma unroll
-        for (int r = 0; r < DK / 16; ++r) s[r] *= decayed;
+        for (int r = 0; r < DK / 16; ++r)
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            float4_t x[2];
-            value_floats(l, kb, x);
-            const Pieces<3> written = split<3>(x[0] * *(const float4_t*)(rest + 32 * kb + l.quad), x[1] * *(const float4_t*)(rest + 32 * kb + 16 + l.quad));
+            for (int n = 0; n < NB; ++n) s[r][n] *= decayed;
+        constexpr int R = N == 1 ? 4 : 2, GROUPS = DK / 16 / R;  // blocks of rows at a time
+        Pieces<N> kt[2][R];
+        auto read_keys = [&](int at) {
 #pragma unroll
-            for (int r = 0; r < DK / 16; ++r) {
-                Pieces<N> k;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const bf16_t* p = ks + i * C * PITCH + (32 * kb + l.quad + l.col / 4) * PITCH + 16 * r + 4 * (l.col % 4);
-                    k.p[i] = both(turned_read(p), turned_read(p + 16 * PITCH));
+                    const bf16_t* p = ks + i * C * PITCH + (32 * (at / GROUPS) + l.quad + l.col / 4) * PITCH + 16 * (at % GROUPS * R + r) + 4 * (l.col % 4);
+                    kt[at & 1][r].p[i] = both(turned_read(p), turned_read(p + 16 * PITCH));
                 }
-                s[r] = mma(k, written, s[r]);
-                if (r % 4 == 3) in_order();
+            in_order();
+        };
+        read_keys(0);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            Pieces<3> written[NB];
+            const float4_t first = *(const float4_t*)(rest[turn] + 32 * kb + l.quad), second = *(const float4_t*)(rest[turn] + 32 * kb + 16 + l.quad);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float4_t x[2];
+                value_floats(l, kb, n, x);
+                written[n] = split_pairs(x[0] * first, x[1] * second);
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const int at = kb * GROUPS + g, r0 = g * R;
+                if (at + 1 < KB * GROUPS) read_keys(at + 1);
+                float4_t sums[R][NB];
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) sums[r][n] = s[r0 + r][n];
+                mma_grid(kt[at & 1], written, sums);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) s[r0 + r][n] = sums[r][n];
+                in_order();
             }
         }
+        if (more && wave == WAVES - 1) gates(next, turn ^ 1);
         lds_barrier();  // the tiles are read, the dots written
         if constexpr (OUT) {
-            if (d.dots && thread < C && t0 + token(thread) < d.time) {
+            if (d.dots && thread < C && t0 + token(thread) < d.time)
+{
                 float dot = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) dot += dot_part[w][thread];
@@ -557,20 +719,23 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 ? 4 : DK == 64 ? 3 : 2)
         if (d.backwards && length > 0) factor = expf(d.decay.value(d.decay.load(qp, b, 0, h)));
     } else {
         to = d.sums + (head * d.segments + segment) * inner * outer;
-        if (threadIdx.x == 0) d.decays[head * d.segments + segment] = (float)exp2(whole);
+        if (threadIdx.x == THREADS - 1) d.decays[head * d.segments + segment] = (float)exp2(whole);
     }
     if (!to) return;
     const Lane l(thread_here());
-    const int column = 16 * wave + l.col;
 #pragma unroll
-    for (int r = 0; r < DK / 16; ++r)
+    for (int n = 0; n < NB; ++n) {
+        const int column = cell(l, n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = 16 * r + l.quad + j;
-            if (row >= inner || column >= outer) continue;
-            to[row * outer + column] = factor * s[r][j];
-            if (copy) copy[row * outer + column] = factor * s[r][j];
-        }
+        for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * r + l.quad + j;
+                if (row >= inner || column >= outer) continue;
+                to[row * outer + column] = factor * s[r][n][j];
+                if (copy) copy[row * outer + column] = factor * s[r][n][j];
+            }
+    }
 }
 
 // Turns the segments' sums into the states at their starts, in place.  backwards: the last segment's start is `start`.
@@ -612,7 +777,19 @@ __global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
     const float* grad = d.behind ? d.behind + (head * d.segments + segment) * d.cells : d.grad_state ? d.grad_state + head * d.cells : nullptr;
     double carry = 0.0;
     if (grad) {
-        for (i64 i = threadIdx.x; i < d.cells; i += 256) carry += (double)state[i] * (double)grad[i];
+        double sums[8] = {};
+        for (i64 i = threadIdx.x; i < d.cells; i += 8 * 256) {
+            float x[8], y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const i64 at = min(i + 256 * k, d.cells - 1);
+                x[k] = state[at], y[k] = grad[at];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + 256 * k < d.cells) sums[k] += (double)x[k] * (double)y[k];
+        }
+        carry = ((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7]));
 #pragma unroll
         for (int k = 32; k; k /= 2) carry += __shfl_xor(carry, k, 64);
         if (lane == 0) parts[0][wave] = carry;
@@ -744,10 +921,10 @@ void launch_scan(const Scan& s, int type, i64 batch, int segments, hipStream_t s
         using T = decltype(t);
         constexpr int E = Unit<T>::N;
         auto widths = [&](auto whole) {
-            if (s.q.width <= 64 && s.v.width <= 64) scan<T, 64, 4, OUT, whole()><<<grid, 256, 0, st>>>(s);
-            else if (s.q.width <= 64) scan<T, 64, 8, OUT, whole()><<<grid, 512, 0, st>>>(s);
-            else if (s.v.width <= 64) scan<T, 128, 4, OUT, whole()><<<grid, 256, 0, st>>>(s);
-            else scan<T, 128, 8, OUT, whole()><<<grid, 512, 0, st>>>(s);
+            if (s.q.width <= 64 && s.v.width <= 64) scan<T, 64, 1, OUT, whole()><<<grid, 256, 0, st>>>(s);
+            else if (s.q.width <= 64) scan<T, 64, 2, OUT, whole()><<<grid, 256, 0, st>>>(s);
+            else if (s.v.width <= 64) scan<T, 128, 1, OUT, whole()><<<grid, 256, 0, st>>>(s);
+            else scan<T, 128, 2, OUT, whole()><<<grid, 256, 0, st>>>(s);
         };
         if (s.q.width % E || s.v.width % E) widths(std::false_type{});
         else widths(std::true_type{});

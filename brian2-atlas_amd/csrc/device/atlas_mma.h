@@ -61,6 +61,25 @@ __device__ __forceinline__ Halves<N> split(float4_t v) {
     return h;
 }
 
+// split with one instruction for each remainder: a dot product of two pieces with (-1, 0) or (0, -1), exact as the plain
+// difference is.  The pieces of an infinity's neighbour in a pair become NaNs too, so both must enter the same sums.
+__device__ __forceinline__ Halves<3> split_pairs(float4_t v) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    uint32_t first = 0x0000BF80u, second = 0xBF800000u;
+    asm("" : "+s"(first), "+s"(second));  // in registers: written as a constant, the second reads as another pair
+    const bf16x2 a = __builtin_bit_cast(bf16x2, first), b = __builtin_bit_cast(bf16x2, second);
+    Halves<3> h;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        h.p[i] = __builtin_convertvector(v, bf16x4);
+        if (i == 2) break;
+        const bf16x2 low = __builtin_shufflevector(h.p[i], h.p[i], 0, 1), high = __builtin_shufflevector(h.p[i], h.p[i], 2, 3);
+        v = float4_t{__builtin_amdgcn_fdot2_f32_bf16(low, a, v[0], false), __builtin_amdgcn_fdot2_f32_bf16(low, b, v[1], false),
+                     __builtin_amdgcn_fdot2_f32_bf16(high, a, v[2], false), __builtin_amdgcn_fdot2_f32_bf16(high, b, v[3], false)};
+    }
+    return h;
+}
+
 template <int N>
 __device__ __forceinline__ Pieces<N> join(const Halves<N>& a, const Halves<N>& b) {
     Pieces<N> r;
@@ -74,6 +93,8 @@ __device__ __forceinline__ Pieces<N> split(float4_t a, float4_t b) {
     return join(split<N>(a), split<N>(b));
 }
 
+__device__ __forceinline__ Pieces<3> split_pairs(float4_t a, float4_t b) { return join(split_pairs(a), split_pairs(b)); }
+
 // c + A B: the products of pieces whose order together is below three (below two where no side has
 // three), the smallest first.
 template <int NA, int NB>
@@ -86,6 +107,36 @@ __device__ __forceinline__ float4_t mma(const Pieces<NA>& a, const Pieces<NB>& b
             if (i < NA && order - i < NB)
                 c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[order - i], c, 0, 0, 0);
     return c;
+}
+
+// c[m][n] + A[m] B[n] for a grid of products, as mma: one product of pieces of all of them after the other, since the next
+// on the same sum waits for the one before.
+template <int NA, int NB, int R, int S>
+__device__ __forceinline__ void mma_grid(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[S], float4_t (&c)[R][S]) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB)
+#pragma unroll
+                for (int m = 0; m < R; ++m)
+#pragma unroll
+                    for (int n = 0; n < S; ++n)
+                        c[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[n].p[order - i], c[m][n], 0, 0, 0);
+}
+
+// c[m] + A[m] B[m], in the same order.
+template <int NA, int NB, int R>
+__device__ __forceinline__ void mma_each(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[R], float4_t (&c)[R]) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB)
+#pragma unroll
+                for (int m = 0; m < R; ++m) c[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[m].p[order - i], c[m], 0, 0, 0);
 }
 
 // c + A B in two chains, the smaller products apart from the larger: half the latency of mma.
