@@ -119,13 +119,13 @@ __global__ void __launch_bounds__(256) rms_forward(Rows x, Rows residual, i64 ro
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(v[c][i]));
-            const float scale = fmaxf(group_max<LANES>(most, shared) / LARGEST, SMALLEST_SCALE);
+            const float scale = fmaxf(group_max<LANES>(most, shared) / LARGEST, SMALLEST_SCALE), inverse = 1.0f / scale;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = (lane + c * LANES) * N;
                 if (col >= width) continue;
 #pragma unroll
-                for (int i = 0; i < N; ++i) v[c][i] /= scale;
+                for (int i = 0; i < N; ++i) v[c][i] *= inverse;
                 store_8bit<N>((uint8_t*)out.y + row * width + col, width - col, v[c]);
             }
             if (lane == 0) out.scale[row] = scale;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(256) rms_forward_long(Rows x, Rows residual, i
         for (int i = 0; i < N; ++i) v[i] = v[i] * rstd * w[i];
         if (out.scale) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] /= scale;
+            for (int i = 0; i < N; ++i) v[i] *= 1.0f / scale;
             store_8bit<N>((uint8_t*)out.y + row * width + col, width - col, v);
         } else {
             store_unit<T>((T*)out.y + row * width + col, width - col, v);
@@ -378,7 +378,7 @@ void with_types(int type, int weight_type, F&& f) {
 }
 
 // Workgroups at most: each keeps its columns' weights for all its rows and fetches its next row ahead.
-constexpr i64 FORWARD_BLOCKS = 1024, BACKWARD_BLOCKS = 512;
+constexpr i64 FORWARD_BLOCKS = 2048, BACKWARD_BLOCKS = 768;
 
 // Blocks of the backward pass's rows; the partials stay a small share of the traffic.
 i64 row_blocks(i64 rows, i64 width, int type) {

@@ -8,8 +8,8 @@
 // The gradient's sums are taken in the tokens' order: a stable radix sort of (token, place), which starts
 // beside the clearing of the table, brings each row's places together; tiles of sorted places are summed in
 // registers, a run of one row within a tile goes straight to the table, and runs that cross tiles leave
-// partial sums, which a last kernel adds from the first tile to the last.  No atomics in sums: the same bits
-// every time.
+// partial sums, which a last kernel adds from the first tile to the last.  Atomics count and list, none of them adds
+// values: the same bits every time.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,7 +30,7 @@ struct Tokens {
 template <typename T, int LANES>
 __global__ void __launch_bounds__(256) embed_forward(const T* __restrict__ table, i64 rows, int width, i64 row_stride, Tokens tokens,
                                                      float scale, T* __restrict__ out) {
-    constexpr int N = Unit<T>::N, GROUPS = 256 / LANES, TOGETHER = 4;
+    constexpr int N = Unit<T>::N, GROUPS = 256 / LANES, TOGETHER = 2;
     const int lane = threadIdx.x % LANES;
     const i64 stride = (i64)gridDim.x * GROUPS * TOGETHER;
     for (i64 i = ((i64)blockIdx.x * GROUPS + threadIdx.x / LANES) * TOGETHER; i < tokens.count; i += stride) {
@@ -54,7 +54,10 @@ __global__ void __launch_bounds__(256) embed_forward(const T* __restrict__ table
 }
 
 // ------------------------------------------------------------------ the stable sort
-constexpr int SORT_TILE = 2048, MAX_BITS = 11, SCANNED = 32;
+// Digits of up to 11 bits, the lowest first.  A tile's workgroup needs the digits' counts of the tiles before it: it adds
+// them up itself where there are few tiles, else a kernel between scans them.  The first counts are a kernel's of their
+// own, which clears the table beside; those of a later pass are taken where the keys are placed before it.
+constexpr int SORT_TILE = 1024, MAX_BITS = 11, SCANNED = 32;
 
 struct Sort {
     i64 count, tiles;
@@ -63,32 +66,33 @@ struct Sort {
     __device__ __forceinline__ uint32_t digit(uint32_t key) const { return (key >> shift) & ((1u << bits) - 1); }
 };
 
-// Digits per tile (blocks below `tiles`); the other blocks clear `size` bytes meanwhile.
-template <bool FIRST>
-__global__ void __launch_bounds__(256) sort_count(Sort s, Tokens tokens, const uint32_t* __restrict__ keys, uint32_t* __restrict__ counts,
-                                                  char* __restrict__ clear, i64 size) {
+// The first digit's counts by tile (blocks below `tiles`); the other blocks clear two ranges of memory meanwhile.
+__global__ void __launch_bounds__(256) sort_count(Sort s, Tokens tokens, uint32_t* __restrict__ counts, char* __restrict__ clear, i64 size,
+                                                  char* __restrict__ clear_too, i64 size_too) {
     if (blockIdx.x >= s.tiles) {
         struct __attribute__((packed, aligned(1))) Sixteen { uint32_t word[4]; };
-        const i64 stride = ((i64)gridDim.x - s.tiles) * 256 * 16;
-        for (i64 at = ((blockIdx.x - s.tiles) * 256 + threadIdx.x) * 16; at < size; at += stride) {
+        const i64 stride = ((i64)gridDim.x - s.tiles) * 256 * 16, first = ((blockIdx.x - s.tiles) * 256 + threadIdx.x) * 16;
+        for (i64 at = first; at < size; at += stride) {
             if (at + 16 <= size) {
                 *(Sixteen*)(clear + at) = Sixteen{};
             } else {
                 for (i64 b = at; b < size; ++b) clear[b] = 0;
             }
         }
+        for (i64 at = first; at < size_too; at += stride) *(Sixteen*)(clear_too + at) = Sixteen{};  // a multiple of 16
         return;
     }
     __shared__ uint32_t bins[1 << MAX_BITS];
     const int all = 1 << s.bits;
     for (int b = threadIdx.x; b < all; b += 256) bins[b] = 0;
-    __syncthreads();
+    i64 token[SORT_TILE / 256];
     const i64 start = (i64)blockIdx.x * SORT_TILE;
 #pragma unroll
-    for (int e = 0; e < SORT_TILE / 256; ++e) {
-        const i64 i = start + e * 256 + threadIdx.x;
-        if (i < s.count) atomicAdd(&bins[s.digit(FIRST ? s.key_of(tokens.at(i)) : keys[i])], 1u);
-    }
+    for (int e = 0; e < SORT_TILE / 256; ++e) token[e] = tokens.at(min(start + e * 256 + threadIdx.x, s.count - 1));
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < SORT_TILE / 256; ++e)
+        if (start + e * 256 + threadIdx.x < s.count) atomicAdd(&bins[s.digit(s.key_of(token[e]))], 1u);
     __syncthreads();
     for (int b = threadIdx.x; b < all; b += 256) counts[(i64)blockIdx.x * all + b] = bins[b];
 }
@@ -115,35 +119,59 @@ __global__ void __launch_bounds__(256) sort_scan(Sort s, uint32_t* __restrict__ 
 
 // Places every key of a tile behind those with smaller digits, of earlier tiles and, in the tile, of earlier
 // waves and lanes.  A wave takes 64 neighbouring keys at a time; ballots over the digit's bits find the lanes
-// with the same digit.
+// with the same digit.  next_counts: those of the next digit by the tile of the new place, or null.
 template <bool FIRST, bool PREFIXED>
 __global__ void __launch_bounds__(256) sort_scatter(Sort s, Tokens tokens, const uint32_t* __restrict__ keys,
                                                     const uint32_t* __restrict__ places, const uint32_t* __restrict__ counts,
-                                                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ places_out) {
-    constexpr int WAVE_KEYS = SORT_TILE / 4, ROUNDS = WAVE_KEYS / 64;
+                                                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ places_out,
+                                                    uint32_t* __restrict__ next_counts) {
+    constexpr int WAVE_KEYS = SORT_TILE / 4, ROUNDS = WAVE_KEYS / 64, PER = (1 << MAX_BITS) / 256;
     __shared__ uint32_t next[4][1 << MAX_BITS];
     __shared__ uint32_t wave_sums[4];
     const int all = 1 << s.bits, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const i64 tile = blockIdx.x, start = tile * SORT_TILE + wave * WAVE_KEYS;
-    for (int b = threadIdx.x; b < 4 * all; b += 256) next[b / all][b % all] = 0;
-    __syncthreads();
-    uint32_t key[ROUNDS];
+    uint32_t key[ROUNDS], from[ROUNDS];
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const i64 i = start + r * 64 + lane;
-        key[r] = i < s.count ? (FIRST ? s.key_of(tokens.at(i)) : keys[i]) : 0;
-        if (i < s.count) atomicAdd(&next[wave][s.digit(key[r])], 1u);
+        const i64 i = min(start + r * 64 + lane, s.count - 1);
+        key[r] = FIRST ? s.key_of(tokens.at(i)) : keys[i];
+        from[r] = FIRST ? (uint32_t)i : places[i];
     }
-    // each thread: a run of neighbouring digits; what comes before them is scanned over the workgroup
-    const int per = (all + 255) / 256, b0 = min((int)threadIdx.x * per, all), b1 = min(b0 + per, all);
-    uint32_t own = 0;
-    for (int b = b0; b < b1; ++b) {
-        if constexpr (PREFIXED) {
-            own += counts[s.tiles * all + b];
-        } else {
-            for (i64 t = 0; t < s.tiles; ++t) own += counts[t * all + b];
-        }
+    // each thread: a run of neighbouring digits, their totals and what the tiles before have of them
+    const int per = (all + 255) / 256, b0 = (int)threadIdx.x * per;
+    uint32_t total[PER], before[PER], own = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) total[k] = before[k] = 0;
+    if constexpr (PREFIXED) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (k < per && b0 + k < all) {
+                total[k] = counts[s.tiles * all + b0 + k];
+                before[k] = counts[tile * all + b0 + k];
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            if (k < per && b0 + k < all) {
+                for (int t0 = 0; t0 < (int)s.tiles; t0 += 16) {
+                    uint32_t c[16];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) c[t] = counts[min(t0 + t, (int)s.tiles - 1) * all + b0 + k];
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) {
+                        total[k] += t0 + t < (int)s.tiles ? c[t] : 0;
+                        before[k] += t0 + t < (int)tile ? c[t] : 0;
+                    }
+                }
+            }
     }
+    for (int b = threadIdx.x; b < 4 * all; b += 256) next[b / all][b % all] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r)
+        if (start + r * 64 + lane < s.count) atomicAdd(&next[wave][s.digit(key[r])], 1u);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) own += total[k];
     uint32_t sum = own;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -154,32 +182,22 @@ __global__ void __launch_bounds__(256) sort_scatter(Sort s, Tokens tokens, const
     __syncthreads();  // the waves' counts and sums are complete
     uint32_t at = sum - own;
     for (int w = 0; w < wave; ++w) at += wave_sums[w];
-    for (int b = b0; b < b1; ++b) {
-        uint32_t total = 0, before = 0;
-        if constexpr (PREFIXED) {
-            total = counts[s.tiles * all + b];
-            before = counts[tile * all + b];
-        } else {
-            for (i64 t = 0; t < s.tiles; ++t) {
-                const uint32_t c = counts[t * all + b];
-                total += c;
-                before += t < tile ? c : 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (k < per && b0 + k < all) {
+            uint32_t place = at + before[k];
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t c = next[w][b0 + k];
+                next[w][b0 + k] = place;
+                place += c;
             }
+            at += total[k];
         }
-        uint32_t place = at + before;
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t c = next[w][b];
-            next[w][b] = place;
-            place += c;
-        }
-        at += total;
-    }
     __syncthreads();
     volatile uint32_t* mine = next[wave];  // only this wave reads and writes it from here on, in program order
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const i64 i = start + r * 64 + lane;
-        const bool live = i < s.count;
+        const bool live = start + r * 64 + lane < s.count;
         const uint32_t digit = s.digit(key[r]);
         u64 same = __ballot(live);
         for (int b = 0; b < s.bits; ++b) {
@@ -195,21 +213,45 @@ __global__ void __launch_bounds__(256) sort_scatter(Sort s, Tokens tokens, const
         __builtin_amdgcn_wave_barrier();
         if (live) {
             keys_out[place] = key[r];
-            places_out[place] = FIRST ? (uint32_t)i : places[i];
+            places_out[place] = from[r];
+        }
+        if (next_counts) {
+            // equal keys, which neighbour each other now, are counted together where they lie in one tile
+            const uint32_t after = key[r] >> (s.shift + s.bits) & (all - 1);
+            for (int b = 0; b < s.bits; ++b) {
+                const bool bit = after >> b & 1;
+                const u64 ones = __ballot(live && bit);
+                same &= bit ? ones : ~ones;
+            }
+            const uint32_t to = place / SORT_TILE;
+            const u64 here = same & __ballot(to == (uint32_t)__shfl((int)to, live ? __builtin_ctzll(same) : 0, 64));
+            uint32_t* p = next_counts + (i64)to * all + after;
+            if (live && here == same) {
+                if (lane == __builtin_ctzll(same)) atomicAdd(p, (uint32_t)__popcll(same));
+            } else if (live) {
+                atomicAdd(p, 1u);
+            }
         }
     }
 }
 
 // ------------------------------------------------------------------ the sums
-constexpr int SUM_TILE = 32;  // sorted places that a group sums
-
 // A tile's first run is a part of an earlier tile's row where the key before the tile is the same, its last
 // run of a later one's where the key behind is.  Partial sums: slot 0 of a tile for a run that comes from before,
-// slot 1 for one that starts here and goes on.
-template <typename T, typename O, int LANES>
+// slot 1 for one that starts here and goes on: it goes on a list, of rows that end within SHORT tiles or of longer ones,
+// whose order does not matter, and the tile where it ends is noted by row.
+constexpr int SHORT = 16;
+
+struct Crossing {
+    struct Start { uint32_t tile, row; };
+    uint32_t *counts, *ends;
+    Start* starts[2];
+};
+
+template <typename T, typename O, int LANES, int SUM_TILE>
 __global__ void __launch_bounds__(256) embed_sum(Rows grad, int width, i64 count, int rows, const uint32_t* __restrict__ keys,
                                                  const uint32_t* __restrict__ places, float scale, O* __restrict__ table,
-                                                 float* __restrict__ partial) {
+                                                 float* __restrict__ partial, Crossing crossing) {
     constexpr int N = Unit<T>::N, GROUPS = 256 / LANES, TOGETHER = 8;
     __shared__ uint32_t key[GROUPS][SUM_TILE + 2], place[GROUPS][SUM_TILE];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -242,6 +284,14 @@ __global__ void __launch_bounds__(256) embed_sum(Rows grad, int width, i64 count
             const bool from = begun == 0 && k[-1] == k[e], on = e + 1 == n && k[e + 1] == k[e];
             if (from || on) {
                 store_unit<float, N>(partial + (2 * tile + (from ? 0 : 1)) * width + col, left, sum);
+                if (blockIdx.y == 0 && lane == 0) {
+                    if (!on) crossing.ends[k[e]] = (uint32_t)tile;
+                    if (!from) {
+                        const i64 far = first + (i64)SUM_TILE * SHORT;
+                        const int list = far < count && keys[far] == k[e];
+                        crossing.starts[list][atomicAdd(crossing.counts + list, 1u)] = {(uint32_t)tile, k[e]};
+                    }
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) sum[i] *= scale;
@@ -254,62 +304,76 @@ __global__ void __launch_bounds__(256) embed_sum(Rows grad, int width, i64 count
     }
 }
 
-// The row that starts in tile blockIdx.x and goes on behind it: its tiles' partial sums, each group a part of the
-// tiles in order, then the groups in order.
-template <typename O, int LANES, int N>
-__global__ void __launch_bounds__(1024) embed_join(int width, i64 count, int rows, const uint32_t* __restrict__ keys, float scale,
-                                                   O* __restrict__ table, const float* __restrict__ partial) {
-    constexpr int GROUPS = 1024 / LANES;
-    __shared__ float sums[GROUPS][LANES * N];
-    const i64 tile = blockIdx.x, first = tile * SUM_TILE, next = first + SUM_TILE;
-    if (next >= count) return;
-    const uint32_t row = keys[next];
-    if (row >= (uint32_t)rows || keys[next - 1] != row || (keys[first] == row && first > 0 && keys[first - 1] == row)) return;
-    // the tiles behind this one that begin with the row
-    const int lane64 = threadIdx.x % 64;
-    i64 more = 1;
-    for (;;) {
-        const i64 at = (tile + 1 + more + lane64) * SUM_TILE;
-        const u64 others = ~__ballot(at < count && keys[at] == row);
-        if (others) {
-            more += __builtin_ctzll(others);
-            break;
+// A row's partial sums: those of its tiles from `from` to `to`, in order; slot 1 in its first, 0 behind.
+template <int N>
+__device__ __forceinline__ void add_partials(const float* __restrict__ partial, i64 tile, i64 from, i64 to, int col, int width, float (&sum)[N]) {
+    for (i64 j0 = from; j0 < to; j0 += 8) {
+        float v[8][N];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const i64 j = min(j0 + k, to - 1);
+            load_columns<float, N>(partial + (2 * j + (j == tile)) * width, col, width, 0.0f, v[k]);
         }
-        more += 64;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (j0 + k < to)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += v[k][i];
     }
+}
+
+// The rows that cross tiles, 64 columns per workgroup.  One half of the workgroups takes the list of long ones, each group of
+// 16 lanes a part of a row's tiles in order, then the groups in order; in the other half each group takes short rows of
+// its own.
+
+template <typename O>
+__global__ void __launch_bounds__(1024) embed_join(int width, float scale, O* __restrict__ table, const float* __restrict__ partial,
+                                                   Crossing crossing) {
+    constexpr int LANES = 16, N = 4, GROUPS = 1024 / LANES;
+    __shared__ float sums[GROUPS][LANES * N + 1];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-    const int col = (blockIdx.y * LANES + lane) * N, left = width - col;
-    const i64 terms = 1 + more, per = (terms + GROUPS - 1) / GROUPS, from = group * per, to = min(terms, from + per);
-    float sum[N];
+    const int col0 = blockIdx.y * LANES * N, col = col0 + lane * N, left = width - col;
+    const int half = gridDim.x / 2;
+    const bool is_long = (int)blockIdx.x < half;
+    const i64 rows = crossing.counts[is_long];
+    for (i64 i = is_long ? blockIdx.x : (blockIdx.x - half) * GROUPS + group; i < rows; i += is_long ? half : half * GROUPS) {
+        const Crossing::Start start = crossing.starts[is_long][i];
+        const i64 tile = start.tile, end = (i64)crossing.ends[start.row] + 1;
+        O* out = table + (i64)start.row * width;
+        float sum[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-    if (left > 0) {
-#pragma unroll 4
-        for (i64 j = from; j < to; ++j) {
-            float v[N];
-            load_columns<float, N>(partial + (j ? 2 * (tile + j) : 2 * tile + 1) * width, col, width, 0.0f, v);
+        for (int e = 0; e < N; ++e) sum[e] = 0.0f;
+        if (!is_long) {
+            if (left <= 0) continue;
+            add_partials<N>(partial, tile, tile, end, col, width, sum);
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] += v[i];
+            for (int e = 0; e < N; ++e) sum[e] *= scale;
+            store_unit<O, N>(out + col, left, sum);
+            continue;
+        }
+        const i64 per = (end - tile + GROUPS - 1) / GROUPS, from = tile + group * per;
+        if (left > 0) add_partials<N>(partial, tile, from, min(end, from + per), col, width, sum);
+        __syncthreads();  // the sums of the row before are read
+#pragma unroll
+        for (int e = 0; e < N; ++e) sums[group][lane * N + e] = sum[e];
+        __syncthreads();
+        if (threadIdx.x < LANES * N && col0 + (int)threadIdx.x < width) {
+            float total = 0.0f;
+#pragma unroll 16
+            for (int g = 0; g < GROUPS; ++g) total += sums[g][threadIdx.x];
+            out[col0 + threadIdx.x] = from_float<O>(scale * total);
         }
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) sums[group][lane * N + i] = sum[i];
-    __syncthreads();
-    if (group || left <= 0) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        float total = 0.0f;
-        for (int g = 0; g < GROUPS; ++g) total += sums[g][lane * N + i];
-        sum[i] = scale * total;
-    }
-    store_unit<O, N>(table + (i64)row * width + col, left, sum);
 }
 
 struct Plan {
     Sort sort;
-    int passes, lanes;
-    i64 tiles, counts_at, keys_at, partial_at, bytes;  // tiles of the sums; offsets into the workspace
+    int passes, lanes, sum_tile;  // sorted places that a group sums
+    i64 tiles, counts, lists_at, keys_at, partial_at, bytes;  // tiles of the sums; bytes of a pass's counts; offsets into the workspace
 };
+
+// Short tiles where long ones would leave the chip with fewer lanes than this.
+constexpr i64 SUM_LANES = 256 * 1024;
 
 // What both the workspace and the launch go by.  grad's type sets the lanes: as few as hold a row's units.
 Plan plan_of(i64 count, i64 rows, i64 width, int type) {
@@ -321,9 +385,12 @@ Plan plan_of(i64 count, i64 rows, i64 width, int type) {
     const i64 units = ceil_div(width, type == ATLAS_OPS_F32 ? 4 : 8);
     p.lanes = 16;
     while (p.lanes < units && p.lanes < 256) p.lanes *= 2;
-    p.tiles = ceil_div(count, SUM_TILE);
-    p.counts_at = 0;
-    p.keys_at = (p.sort.tiles + 1) * 4 << p.sort.bits;
+    const i64 slices = ceil_div(units, p.lanes);
+    p.sum_tile = ceil_div(count, 32) * slices * p.lanes >= SUM_LANES ? 32 : 8;
+    p.tiles = ceil_div(count, p.sum_tile);
+    p.counts = ((p.sort.tiles + 1) * 4 << p.sort.bits) + 15 & ~(i64)15;
+    p.lists_at = p.counts * p.passes + 16;  // 16 bytes for the lists' counts, before the second pass's
+    p.keys_at = p.lists_at + 16 * p.tiles + 4 * rows;
     p.partial_at = (p.keys_at + 16 * count + 15) / 16 * 16;
     p.bytes = p.partial_at + p.tiles * 2 * width * 4;
     return p;
@@ -397,7 +464,7 @@ int atlas_ops_embedding(const void* table, int64_t rows, int64_t width, int64_t 
         if (!count) return 0;
         if (!table || !tokens || !out) return fail(err, cap, 7, "null argument");
         const int lanes = plan_of(1, 1, width, type).lanes;
-        const i64 blocks = std::min<i64>(ceil_div(count, 4 * (256 / lanes)), 8192);
+        const i64 blocks = std::min<i64>(ceil_div(count, 2 * (256 / lanes)), 1 << 20);
         with_type(type, [&](auto t) {
             using T = decltype(t);
             with_lanes(lanes, [&](auto l) {
@@ -434,30 +501,31 @@ int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int 
         const i64 clearing = std::min<i64>(ceil_div(size, 256 * 16 * 4), 2048);
         const Tokens list{tokens, wide, count};
         char* base = (char*)workspace;
-        uint32_t *counts = (uint32_t*)(base + p.counts_at), *keys[2], *places[2];
+        uint32_t *counts = (uint32_t*)base, *keys[2], *places[2];
         for (int i = 0; i < 2; ++i) {
             keys[i] = (uint32_t*)(base + p.keys_at) + 2 * i * count;
             places[i] = keys[i] + count;
         }
         const unsigned tiles = (unsigned)p.sort.tiles;
-        if (!count) {
-            sort_count<true><<<dim3((unsigned)clearing), 256, 0, st>>>(p.sort, list, nullptr, nullptr, (char*)dtable, size);
-            return launched(err, cap, "embedding_backward");
-        }
+        sort_count<<<dim3((unsigned)(tiles + clearing)), 256, 0, st>>>(p.sort, list, counts, (char*)dtable, size, base + p.counts,
+                                                                      count ? 16 + p.counts * (p.passes - 1) : 0);
+        if (!count) return launched(err, cap, "embedding_backward");
         for (int pass = 0; pass < p.passes; ++pass, p.sort.shift += p.sort.bits) {
             const uint32_t *k = keys[(pass + 1) % 2], *v = places[(pass + 1) % 2];
             uint32_t *ko = keys[pass % 2], *vo = places[pass % 2];
-            if (pass == 0) sort_count<true><<<dim3((unsigned)(tiles + clearing)), 256, 0, st>>>(p.sort, list, k, counts, (char*)dtable, size);
-            else sort_count<false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, counts, nullptr, 0);
+            uint32_t* after = pass + 1 < p.passes ? (uint32_t*)(base + 16 + (pass + 1) * p.counts) : nullptr;
             const bool scanned = p.sort.tiles > SCANNED;
             if (scanned) sort_scan<<<dim3((unsigned)ceil_div(1 << p.sort.bits, 4)), 256, 0, st>>>(p.sort, counts);
-            if (pass == 0 && scanned) sort_scatter<true, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
-            else if (pass == 0) sort_scatter<true, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
-            else if (scanned) sort_scatter<false, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
-            else sort_scatter<false, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo);
+            if (pass == 0 && scanned) sort_scatter<true, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo, after);
+            else if (pass == 0) sort_scatter<true, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo, after);
+            else if (scanned) sort_scatter<false, true><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo, after);
+            else sort_scatter<false, false><<<dim3(tiles), 256, 0, st>>>(p.sort, list, k, v, counts, ko, vo, after);
+            counts = after;
         }
         const uint32_t *sorted = keys[(p.passes + 1) % 2], *order = places[(p.passes + 1) % 2];
         float* partial = (float*)(base + p.partial_at);
+        Crossing::Start* lists = (Crossing::Start*)(base + p.lists_at);
+        const Crossing crossing{(uint32_t*)(base + p.counts), (uint32_t*)(lists + 2 * p.tiles), {lists, lists + p.tiles}};
         const Rows g{grad->data, grad->inner, grad->outer_stride, grad->inner_stride};
         with_type(type, [&](auto t) {
             using T = decltype(t);
@@ -466,12 +534,17 @@ int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int 
                 using O = decltype(o);
                 with_lanes(p.lanes, [&](auto l) {
                     const unsigned slices = (unsigned)ceil_div(width, l() * N);
-                    embed_sum<T, O, l()><<<dim3((unsigned)ceil_div(p.tiles, 256 / l()), slices), 256, 0, st>>>(
-                        g, (int)width, count, (int)rows, sorted, order, scale, (O*)dtable, partial);
-                    if (p.tiles > 1)
-                        embed_join<O, l(), N><<<dim3((unsigned)(p.tiles - 1), slices), 1024, 0, st>>>(
-                            (int)width, count, (int)rows, sorted, scale, (O*)dtable, partial);
+                    const dim3 grid((unsigned)ceil_div(p.tiles, 256 / l()), slices);
+                    if (p.sum_tile == 32)
+                        embed_sum<T, O, l(), 32><<<grid, 256, 0, st>>>(g, (int)width, count, (int)rows, sorted, order, scale, (O*)dtable, partial, crossing);
+                    else
+                        embed_sum<T, O, l(), 8><<<grid, 256, 0, st>>>(g, (int)width, count, (int)rows, sorted, order, scale, (O*)dtable, partial, crossing);
                 });
+                if (p.tiles > 1) {  // a workgroup to a CU, as its registers allow
+                    const i64 slices = ceil_div(width, 64);
+                    embed_join<O><<<dim3((unsigned)std::max<i64>(256 / slices & ~(i64)1, 2), (unsigned)slices), 1024, 0, st>>>(
+                        (int)width, scale, (O*)dtable, partial, crossing);
+                }
             });
         });
         return launched(err, cap, "embedding_backward");
