@@ -149,6 +149,11 @@ def _last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _near(t):
+    """(batch, time, ...) with tokens as near to one another as linear attention in chunks has them."""
+    return t if t.stride(1) <= 1 << 24 else t.contiguous()
+
+
 def _workspace(size: int, like):
     return torch.empty(size, dtype=torch.uint8, device=like.device)
 
@@ -543,6 +548,8 @@ class _Problem:
             _tensor(lengths, "lengths", device, _I32, (batch,))
             lengths = lengths.contiguous()
         q, k, v = _last(q), _last(k), _last(v)
+        if linear and time_axis:
+            q, k, v = _near(q), _near(k), _near(v)
 
         def strides(t):
             s = t.stride()
@@ -752,7 +759,7 @@ def linear_attention_backward(grad_out, grad_state, tape: LinearTape) -> dict:
     if grad_state is not None:
         _tensor(grad_state, "grad_state", p.device, _F32, (p.batch, p.value_heads, p.key, p.value))
         grad_state = grad_state.contiguous()
-    grad_out = _last(grad_out)
+    grad_out = _near(_last(grad_out))
     grads = {name: None if t is None else _empty(t)
              for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("state", state))}
     if not p.batch or not p.time:

@@ -11,8 +11,11 @@
 //   dQ_t = scale S_t dO_t       forwards:  queries dO, keys v, values k (the state S^T)
 //   dV_t = T_t^T k_t            backwards: queries k,  keys q, values dO
 //   dK_t = T_t v_t              backwards: queries v,  keys dO, values q (the state T^T)
-// The gradient of log a_t is L_t = <T_t, a_t S_{t-1}> with L_t = L_{t+1} + q_t . dQ_t - k_t . dK_t, whose dots
-// the runs take beside their outputs; `decay_gradients` sums them in 64 bits.
+// The gradient of log a_t is L_t = <T_t, a_t S_{t-1}> with L_t = L_{t+1} + q_t . dQ_t - k_t . dK_t.  These dots cancel: with
+// keys nearly orthogonal their parts are far larger than their sum.  So what a chunk's own tokens add, W_ij =
+// scale exp(G_i - G_j) (dO_i . v_j) (q_i . k_j) for j < i, is taken pair by pair, as sums over rows less sums over columns
+// (the dQ run has the first three factors and takes the fourth beside them), only what comes through the states is taken as
+// dots, and every ANCHOR chunks L starts anew from the states themselves.  `decay_gradients` sums in 64 bits.
 //
 // Few sequences are split along time: `scan` first takes the sums of segments from an empty state, `join_states`
 // carries the states through them, and every segment then runs from its own.
@@ -197,10 +200,16 @@ struct Scan {
     int out_f32;                   // float32 whatever T is
     float *final_state, *copy;     // after the last segment; backwards also decayed by the first token; may be null
     float *sums, *decays;          // [batch, value head, segment]: a segment's state from zeros, and its whole decay
-    const void* dot_with;          // (a Role) null, or what each output row is multiplied with
-    Role dot;
-    float* dots;                   // [batch, value head, time]
+    Role dot;                      // what dots and pairs multiply with
+    float* dots;                   // [batch, value head, time] or null: dots with what the states answer
+    float* pairs;                  // [batch, value head, time] or null: by token, sums of W over its row less over its column
+    float* anchors;                // [batch, value head, anchor], or null: backwards the states at the anchors, for
+    double* heights;               // forwards their products with the states there
 };
+
+// Anchors lie behind every ANCHOR-th chunk but the last.
+constexpr int ANCHOR = 8;
+__host__ __device__ inline i64 anchors_of(i64 chunks) { return (chunks - 1) / ANCHOR; }
 
 template <typename T>
 struct Cut {
@@ -231,6 +240,24 @@ __device__ __forceinline__ bool beyond(float4_t a, float4_t b) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) most = max(max(most, __float_as_uint(a[i]) & 0x7FFFFFFFu), __float_as_uint(b[i]) & 0x7FFFFFFFu);
     return most >= 0x7F800000u;
+}
+
+// Four values of a row of `width` from column c0, zeros beyond it.
+template <typename T>
+struct Four { T v[4]; };
+
+template <bool WHOLE, typename T>
+__device__ __forceinline__ Four<T> four(const T* row, int c0, int width) {
+    Four<T> x;
+    if constexpr (WHOLE) {
+        struct __attribute__((packed, aligned(sizeof(T)))) Packed { T v[4]; } raw = *(const Packed*)(row + (c0 < width ? c0 : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = c0 < width ? raw.v[e] : T{};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x.v[e] = c0 + e < width ? row[c0 + e] : T{};
+    }
+    return x;
 }
 
 // A thread's share of a chunk's rows, C tokens of up to W values: units of 16 bytes in every STEP-th token.  The loads stand
@@ -291,7 +318,9 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
     __shared__ __attribute__((aligned(16))) bf16_t scores[OUT ? OPERANDS * 3 * 512 : 8];
     // of two chunks in turn: G as a float and its remainder, the factors of what the state answers and of what is written to it
     __shared__ __attribute__((aligned(16))) float gate_sum[2][C], gate_rest[2][C], since[2][C], rest[2][C], decays[2];
-    __shared__ float dot_part[OUT ? WAVES : 1][C];
+    __shared__ float dot_part[OUT ? WAVES : 1][C], pair_rows[OUT ? BLOCKS : 1][16];
+    __shared__ __attribute__((aligned(16))) float pair_columns[OUT ? BLOCKS : 1][16];
+    __shared__ double height_part[WAVES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int segment = d.first + blockIdx.x;
     const i64 h = blockIdx.y, b = blockIdx.z, head = b * d.value_heads + h;
@@ -422,12 +451,27 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                     else ((T*)d.out)[o] = from_float<T>(0.0f);
                 }
                 if (d.dots && (int)threadIdx.x < rows) d.dots[head * d.time + t0 + threadIdx.x] = 0.0f;
+                if (d.pairs && (int)threadIdx.x < rows) d.pairs[head * d.time + t0 + threadIdx.x] = 0.0f;
             }
             continue;
         }
         const int live = (int)min((i64)C, length - t0);
         const uint32_t thread = thread_here();
         const Lane l(thread);
+        const bool anchored = OUT && d.anchors && (chunk + 1) % ANCHOR == 0 && chunk + 1 < used;
+        float* anchor = anchored ? d.anchors + (head * anchors_of(d.chunks) + (chunk + 1) / ANCHOR - 1) * inner * outer : nullptr;
+        if (anchored && d.backwards) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < DK / 16; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = 16 * r + l.quad + j, column = cell(l, n);
+                        if (row < inner && column < outer) anchor[row * outer + column] = s[r][n][j];
+                    }
+            in_order();
+        }
         // ---- the chunk into LDS
         const bool all_q = live == C && inner == DK, all_v = live == C && outer == DV;
         const int turn = step & 1;
@@ -495,6 +539,45 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                 const Halves<3> parts = split_pairs(p[m]);
                 if (wave + WAVES * m < BLOCKS) put_half<3>(scores, operand, kj % 2, l, parts);
             }
+            if (d.pairs) {
+                // ---- W: the scores times the dots of the other two tensors, a row of `dot` (the queries') and one of the values
+#pragma unroll
+                for (int m = 0; m < OWN; ++m) {
+                    const int qb = qbs[m], kj = kjs[m], t = token(16 * qb + l.col);
+                    const T* row = d.dot.x.at<T>(b, t0 + (t < live ? t : 0), h / d.dot.group);
+                    const T* key = vs + (16 * kj + l.col) * VPITCH;
+                    float4_t w = ZERO;
+#pragma unroll
+                    for (int c = 0; c < DV / 32; ++c) {
+                        const int c0 = 32 * c + l.quad;
+                        Pieces<N> a, x;
+                        if constexpr (N == 1) {
+                            a.p[0] = both(*(const bf16x4*)(key + c0), *(const bf16x4*)(key + c0 + 16));
+                            x.p[0] = both(__builtin_bit_cast(bf16x4, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(bf16x4, four<WHOLE>(row, c0 + 16, outer)));
+                        } else {
+                            a = split<3>(*(const float4_t*)(key + c0), *(const float4_t*)(key + c0 + 16));
+                            x = split<3>(__builtin_bit_cast(float4_t, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(float4_t, four<WHOLE>(row, c0 + 16, outer)));
+                        }
+                        w = mma(a, x, w);
+                    }
+                    const int i = 16 * qb + l.col, at = 16 * kj + l.quad;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        w[j] = at + j < i && t < live ? w[j] * p[m][j] : 0.0f;
+                        sum += w[j];
+                    }
+                    sum += __shfl_xor(sum, 16, 64);
+                    sum += __shfl_xor(sum, 32, 64);
+                    float4_t down;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) down[j] = lane_sum<16>(w[j]);
+                    const int block = wave + WAVES * m;
+                    if (block < BLOCKS && l.quad == 0) pair_rows[block][l.col] = sum;
+                    if (block < BLOCKS && l.col == 0) *(float4_t*)(pair_columns[block] + l.quad) = down;
+                }
+                in_order();
+            }
             if (more) fetch(next, 2);
             in_order();
             // ---- what the state answers: rows are columns of the values, columns are queries
@@ -524,6 +607,30 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                 const float g = since[turn][16 * qb + l.col];
 #pragma unroll
                 for (int n = 0; n < NB; ++n) o[n][qb] *= g;
+            }
+            constexpr bool FULL = WHOLE && (sizeof(T) == 2 || NB == 1);  // a lane's 4 NB neighbouring columns are there or none
+            const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
+            if (d.dots) {
+                const T* x0 = d.dot.x.at<T>(b, t0, h / d.dot.group) + (left > 0 ? c0 : 0);
+#pragma unroll
+                for (int qb = 0; qb < QB; ++qb) {
+                    const int t = token(16 * qb + l.col);
+                    const T* x = x0 + (t < live && left > 0 ? (uint32_t)(t * (int)d.dot.x.time) : 0u);
+                    struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[4 * NB]; } few;
+                    if constexpr (FULL) {
+                        few = *(const Few*)x;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4 * NB; ++e) few.v[e] = x[min(e, max(left - 1, 0))];
+                    }
+                    float dot = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4 * NB; ++e) dot += FULL || e < left ? o[e / 4][qb][e % 4] * to_float(few.v[e]) : 0.0f;
+                    dot = t < live && left > 0 ? dot : 0.0f;
+                    dot += __shfl_xor(dot, 16, 64);
+                    dot += __shfl_xor(dot, 32, 64);
+                    if (l.quad == 0) dot_part[wave][16 * qb + l.col] = dot;
+                }
             }
             lds_barrier();  // the scores are there
             if (more) fetch(next, 4);
@@ -614,33 +721,13 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                         if (token(16 * qb + l.col) >= live) o[n][qb] = ZERO;
             }
             // ---- a lane's 4 NB neighbouring columns of one token
-            constexpr bool FULL = WHOLE && (sizeof(T) == 2 || NB == 1);  // 4 NB columns are there or none
-            const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
             const i64 out0 = ((b * d.time + t0) * d.value_heads + h) * outer + c0;
-            const T* x0 = d.dots ? d.dot.x.at<T>(b, t0, h / d.dot.group) + (left > 0 ? c0 : 0) : nullptr;
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 const int t = token(16 * qb + l.col);
                 float row[4 * NB];
 #pragma unroll
                 for (int e = 0; e < 4 * NB; ++e) row[e] = o[e / 4][qb][e % 4];
-                if (d.dots) {
-                    float dot = 0.0f;
-                    const T* x = x0 + (t < live && left > 0 ? (uint32_t)(t * (int)d.dot.x.time) : 0u);
-                    struct __attribute__((packed, aligned(sizeof(T)))) Few { T v[4 * NB]; } few;
-                    if constexpr (FULL) {
-                        few = *(const Few*)x;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4 * NB; ++e) few.v[e] = x[min(e, max(left - 1, 0))];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4 * NB; ++e) dot += FULL || e < left ? row[e] * to_float(few.v[e]) : 0.0f;
-                    dot = t < live && left > 0 ? dot : 0.0f;
-                    dot += __shfl_xor(dot, 16, 64);
-                    dot += __shfl_xor(dot, 32, 64);
-                    if (l.quad == 0) dot_part[wave][16 * qb + l.col] = dot;
-                }
                 if (t0 + t < d.time && left > 0) {
                     const i64 at = out0 + (uint32_t)(t * d.value_heads * outer);
                     if (d.out_f32) store_unit<float, 4 * NB>((float*)d.out + at, FULL ? 4 * NB : left, row);
@@ -696,15 +783,48 @@ __global__ void __launch_bounds__(256, 2) scan(Scan d) {
                 in_order();
             }
         }
+        if (anchored && !d.backwards) {  // the anchor's rows are this state's columns
+            double height = 0.0;
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < DK / 16; ++r) {
+                    float4_t x;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = 16 * r + l.quad + j, column = cell(l, n);
+                        x[j] = anchor[min(column, outer - 1) * inner + min(row, inner - 1)];
+                        x[j] = row < inner && column < outer ? x[j] : 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) height += (double)x[j] * (double)s[r][n][j];
+                    in_order();
+                }
+#pragma unroll
+            for (int k = 32; k; k /= 2) height += __shfl_xor(height, k, 64);
+            if (l.id == 0) height_part[wave] = height;
+        }
         if (more && wave == WAVES - 1) gates(next, turn ^ 1);
         lds_barrier();  // the tiles are read, the dots written
         if constexpr (OUT) {
-            if (d.dots && thread < C && t0 + token(thread) < d.time)
-{
+            if (anchored && !d.backwards && thread == 0)
+                d.heights[head * anchors_of(d.chunks) + (chunk + 1) / ANCHOR - 1] = (height_part[0] + height_part[1]) + (height_part[2] + height_part[3]);
+            if (d.dots && thread < C && t0 + token(thread) < d.time) {
+                const i64 at = head * d.time + t0 + token(thread);
                 float dot = 0.0f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) dot += dot_part[w][thread];
-                d.dots[head * d.time + t0 + token(thread)] = dot;
+                d.dots[at] = dot;
+                if (d.pairs) {
+                    const int block = thread / 16, in = thread % 16;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < QB; ++k) {
+                        if (k <= block) sum += pair_rows[block * (block + 1) / 2 + k][in];
+                        if (k >= block) sum -= pair_columns[k * (k + 1) / 2 + block][in];
+                    }
+                    d.pairs[at] = sum;
+                }
             }
         }
     }
@@ -754,29 +874,30 @@ __global__ void __launch_bounds__(256) join_states(float* sums, const float* dec
 }
 
 // ------------------------------------------------------------------ gradients of the decays
-// A workgroup takes a segment: L behind its last token from the states there, then back through its tokens.
+// A workgroup takes the tokens between two anchors: L behind its last token, then back through its tokens.
 struct DecayGradients {
     Decays decay;
     const void* other;                      // memory that may be read where there are no decays
     const int32_t* lengths;
-    i64 time, tokens, cells;                // tokens of a segment; cells of a state
-    int value_heads, segments;
-    const float *starts, *last, *behind, *grad_state;  // S at the segments' starts, after the sequence; T behind the segments
-    const float *dq, *dk;                   // the dots, [batch, value head, time]
+    i64 time, tokens, cells, anchors;       // tokens between anchors; cells of a state
+    int value_heads;
+    const float *last, *grad_state;         // S after the sequence and its gradient, which may be null
+    const double* heights;                  // <S, T> at the anchors
+    const float *dq, *dk, *pairs;           // [batch, value head, time]
     void* out;                              // (batch, time, value heads) of the decays' type, or null:
-    float* sums;                            // [batch, segment, value head] sums over the segment's tokens
+    float* sums;                            // [batch, interval, value head] sums over the interval's tokens
 };
 
 __global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
     __shared__ double parts[2][4];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, segment = blockIdx.x;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, interval = blockIdx.x;
     const i64 h = blockIdx.y, b = blockIdx.z, head = b * d.value_heads + h;
-    const i64 length = length_of(d.lengths, d.time, b), first = segment * d.tokens, end = min(first + d.tokens, d.time);
-    // <S, T> behind the segment: sums in 64 bits
-    const float* state = segment + 1 < d.segments ? d.starts + (head * d.segments + segment + 1) * d.cells : d.last + head * d.cells;
-    const float* grad = d.behind ? d.behind + (head * d.segments + segment) * d.cells : d.grad_state ? d.grad_state + head * d.cells : nullptr;
+    const i64 length = length_of(d.lengths, d.time, b), first = interval * d.tokens, end = min(first + d.tokens, d.time);
     double carry = 0.0;
-    if (grad) {
+    if (end < length) {
+        carry = d.heights[head * d.anchors + interval] * exp((double)d.decay.value(d.decay.load(d.other, b, end, h)));
+    } else if (d.grad_state && first < length) {  // sums in 64 bits
+        const float *state = d.last + head * d.cells, *grad = d.grad_state + head * d.cells;
         double sums[8] = {};
         for (i64 i = threadIdx.x; i < d.cells; i += 8 * 256) {
             float x[8], y[8];
@@ -795,7 +916,6 @@ __global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
         if (lane == 0) parts[0][wave] = carry;
         __syncthreads();
         carry = (parts[0][0] + parts[0][1]) + (parts[0][2] + parts[0][3]);
-        if (end < length) carry *= exp((double)d.decay.value(d.decay.load(d.other, b, end, h)));
     }
     double sum = 0.0;
     int turn = 1;
@@ -803,7 +923,7 @@ __global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
         const i64 t = base - 1 - threadIdx.x;
         const bool live = t >= first && t < length;
         const i64 at = head * d.time + (live ? t : first);
-        double x = live ? (double)d.dq[at] - (double)d.dk[at] : 0.0;
+        double x = live ? (double)d.dq[at] - (double)d.dk[at] + (double)d.pairs[at] : 0.0;
 #pragma unroll
         for (int k = 1; k < 64; k *= 2) {
             const double before = __shfl_up(x, k, 64);
@@ -829,7 +949,7 @@ __global__ void __launch_bounds__(256) decay_gradients(DecayGradients d) {
     if (lane == 0) parts[0][wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0)
-        d.sums[(b * d.segments + segment) * d.value_heads + h] = (float)((parts[0][0] + parts[0][1]) + (parts[0][2] + parts[0][3]));
+        d.sums[(b * gridDim.x + interval) * d.value_heads + h] = (float)((parts[0][0] + parts[0][1]) + (parts[0][2] + parts[0][3]));
 }
 
 // Sums over rows of (rows, columns): the gradient of a decay that all sequences share.
@@ -848,15 +968,25 @@ __global__ void __launch_bounds__(256) head_sums(const float* __restrict__ sums,
     else ((float*)out)[column] = total;
 }
 
-// Heads of q and k that `group` value heads share: the sums of their gradients, rows of (value heads x width).
-template <typename T>
-__global__ void __launch_bounds__(256) group_sums(const float* __restrict__ parts, i64 count, int width, int group, T* __restrict__ out) {
-    for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < count; i += (i64)gridDim.x * 256) {
-        const float* p = parts + i / width * group * width + i % width;
-        float sum = 0.0f;
-        for (int g = 0; g < group; ++g) sum += p[(i64)g * width];
-        out[i] = from_float<T>(sum);
-    }
+// Heads of q and k that `group` value heads share: the sums of their gradients, q's and behind them k's (blockIdx.y), whose
+// rows are (head, value head of it, width).  32 lanes take a row's VEC neighbours each.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) group_sums(const float* __restrict__ parts, i64 rows, int width, int group, T* dq, T* dk) {
+    struct Packed { float v[VEC]; };
+    T* out = blockIdx.y ? dk : dq;
+    parts += blockIdx.y * rows * group * width;
+    for (i64 row = (i64)blockIdx.x * 8 + threadIdx.x / 32; row < rows; row += (i64)gridDim.x * 8)
+        for (int c = threadIdx.x % 32 * VEC; c < width; c += 32 * VEC) {
+            const float* p = parts + row * group * width + c;
+            float sum[VEC] = {};
+#pragma unroll 4
+            for (int g = 0; g < group; ++g, p += width) {
+                const Packed x = *(const Packed*)p;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sum[e] += x.v[e];
+            }
+            store_unit<T, VEC>(out + row * width + c, VEC, sum);
+        }
 }
 
 // ------------------------------------------------------------------ plans
@@ -894,20 +1024,22 @@ i64 forward_floats(const AtlasDelta& d, bool train) {
     return starts + (train ? p.heads * p.state : 0);
 }
 
-// Of a backward pass: T behind the segments and their decays, the dots of dQ and dK, sums of shared decays, float32
-// gradients of shared heads.
+// Of a backward pass: T behind the segments and their decays, <S, T> at the anchors and T there, the dots of dQ and dK and the
+// pairs' sums, sums of shared decays, float32 gradients of shared heads.  Without a gradient of decays the middle is empty.
 struct Back {
-    i64 behind, decays, dots, sums, dq, dk, all;
+    i64 heights, behind, decays, anchors, dots, sums, dq, dk, all;
 };
 
 Back back_of(const AtlasDelta& d) {
     const Plan p = plan_of(d);
+    const bool decays = d.log_decay;
     Back o{};
-    o.behind = 0;
+    o.behind = o.heights + (decays ? 2 * p.heads * anchors_of(p.chunks) : 0);
     o.decays = o.behind + (p.segments > 1 ? p.heads * p.segments * p.state : 0);
-    o.dots = o.decays + (p.segments > 1 ? p.heads * p.segments : 0);
-    o.sums = o.dots + 2 * p.heads * d.time;
-    o.dq = o.sums + p.heads * p.segments;
+    o.anchors = o.decays + (p.segments > 1 ? p.heads * p.segments : 0);
+    o.dots = o.anchors + (decays ? p.heads * anchors_of(p.chunks) * p.state : 0);
+    o.sums = o.dots + (decays ? 3 * p.heads * d.time : 0);
+    o.dq = o.sums + (decays ? p.heads * ceil_div(p.chunks, ANCHOR) : 0);
     const i64 shared = d.value_heads > d.heads ? p.heads * d.time * d.key : 0;
     o.dk = o.dq + shared;
     o.all = o.dk + shared;
@@ -1036,7 +1168,7 @@ int atlas_ops_linear_forward(const AtlasDelta* d, int train, void* out, float* f
 int64_t atlas_ops_linear_backward_workspace(const AtlasDelta* d) {
     char ignored[1];
     if (check(d, true, ignored, 1)) return 0;
-    return 4 * back_of(*d).all;
+    return 4 * back_of(*d).all + 16;  // never 0
 }
 
 int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void* grad_out, const int64_t* grad_out_stride,
@@ -1045,6 +1177,7 @@ int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void*
     try {
         if (int rc = check(d, true, err, cap)) return rc;
         if (!tape || !grad_out || !grad_out_stride || !dq || !dk || !dv || !workspace) return fail(err, cap, 7, "null argument");
+        if (grad_out_stride[1] < 0 || grad_out_stride[1] > MAX_STRIDE) return fail(err, cap, 7, "tokens must be at most 2^24 elements apart");
         if (dlog_decay && !d->log_decay) return fail(err, cap, 7, "a gradient of decays that were not given");
         const Plan p = plan_of(*d);
         const Back at = back_of(*d);
@@ -1055,21 +1188,10 @@ int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void*
         const float* last = starts + (p.segments > 1 ? p.heads * p.segments * (p.state + 1) : 0);
         const Role q{tensor_of(d->q, d->q_stride), group, (int)d->key}, k{tensor_of(d->k, d->k_stride), group, (int)d->key},
             v{tensor_of(d->v, d->v_stride), 1, (int)d->value}, go{tensor_of(grad_out, grad_out_stride), 1, (int)d->value};
-        float *dots_q = base + at.dots, *dots_k = dots_q + p.heads * d->time;
-        // dQ, forwards
-        Scan s = scan_of(*d, p);
-        s.q = go, s.k = v, s.v = k;
-        s.read = d->scale;
-        s.start = p.segments > 1 ? starts : d->state;
-        s.start_segments = p.segments > 1;
-        s.turned = 1;
-        s.out = group > 1 ? (void*)(base + at.dq) : dq;
-        s.out_f32 = group > 1;
-        s.dot = q;
-        s.dots = dlog_decay ? dots_q : nullptr;
-        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        float *dots_q = base + at.dots, *dots_k = dots_q + p.heads * d->time, *pairs = dots_k + p.heads * d->time;
+        float* anchors = dlog_decay ? base + at.anchors : nullptr;
         // T behind the segments
-        s = scan_of(*d, p);
+        Scan s = scan_of(*d, p);
         s.backwards = 1;
         s.write = d->scale;
         s.q = k, s.k = q, s.v = go;
@@ -1087,26 +1209,43 @@ int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void*
             s.start = s.sums;
             s.start_segments = 1;
         }
+        const Scan behind = s;
         // dV, backwards
         s.out = dv;
         s.final_state = dstate;
+        s.anchors = anchors;
+        launch_scan<true>(s, d->type, d->batch, p.segments, st);
+        // dQ, forwards
+        s = scan_of(*d, p);
+        s.q = go, s.k = v, s.v = k;
+        s.read = d->scale;
+        s.start = p.segments > 1 ? starts : d->state;
+        s.start_segments = p.segments > 1;
+        s.turned = 1;
+        s.out = group > 1 ? (void*)(base + at.dq) : dq;
+        s.out_f32 = group > 1;
+        s.dot = q;
+        s.dots = dlog_decay ? dots_q : nullptr;
+        s.pairs = dlog_decay ? pairs : nullptr;
+        s.anchors = anchors;
+        s.heights = (double*)(base + at.heights);
         launch_scan<true>(s, d->type, d->batch, p.segments, st);
         // dK, backwards
+        s = behind;
         s.q = v, s.k = go, s.v = q;
         s.turned = 1;
-        s.final_state = nullptr;
         s.out = group > 1 ? (void*)(base + at.dk) : dk;
         s.out_f32 = group > 1;
         s.dot = k;
         s.dots = dlog_decay ? dots_k : nullptr;
         launch_scan<true>(s, d->type, d->batch, p.segments, st);
         if (group > 1) {
-            const i64 count = d->batch * d->time * d->heads * d->key;
+            const i64 rows = d->batch * d->time * d->heads;
             with_type(d->type, [&](auto t) {
                 using T = decltype(t);
-                const unsigned blocks = (unsigned)std::min<i64>(ceil_div(count, 256), 8192);
-                group_sums<T><<<dim3(blocks), 256, 0, st>>>(base + at.dq, count, (int)d->key, group, (T*)dq);
-                group_sums<T><<<dim3(blocks), 256, 0, st>>>(base + at.dk, count, (int)d->key, group, (T*)dk);
+                const dim3 grid((unsigned)std::min<i64>(ceil_div(rows, 8), 4096), 2);
+                auto* sums = d->key % 4 == 0 ? group_sums<T, 4> : group_sums<T, 1>;
+                sums<<<grid, 256, 0, st>>>(base + at.dq, rows, (int)d->key, group, (T*)dq, (T*)dk);
             });
         }
         if (dlog_decay) {
@@ -1115,21 +1254,22 @@ int atlas_ops_linear_backward(const AtlasDelta* d, const void* tape, const void*
             g.other = d->q;
             g.lengths = d->lengths;
             g.time = d->time;
-            g.tokens = (i64)p.per * chunk_of(d->type);
+            g.tokens = (i64)ANCHOR * chunk_of(d->type);
             g.cells = p.state;
+            g.anchors = anchors_of(p.chunks);
             g.value_heads = (int)d->value_heads;
-            g.segments = p.segments;
-            g.starts = starts;
             g.last = last;
-            g.behind = p.segments > 1 ? base + at.behind : nullptr;
             g.grad_state = grad_state;
+            g.heights = (const double*)(base + at.heights);
             g.dq = dots_q;
             g.dk = dots_k;
+            g.pairs = pairs;
             g.out = shared_decay ? nullptr : dlog_decay;
             g.sums = shared_decay ? base + at.sums : nullptr;
-            decay_gradients<<<dim3((unsigned)p.segments, (unsigned)d->value_heads, (unsigned)d->batch), 256, 0, st>>>(g);
+            const i64 intervals = ceil_div(p.chunks, ANCHOR);
+            decay_gradients<<<dim3((unsigned)intervals, (unsigned)d->value_heads, (unsigned)d->batch), 256, 0, st>>>(g);
             if (shared_decay)
-                head_sums<<<dim3((unsigned)d->value_heads), 256, 0, st>>>(g.sums, d->batch * p.segments, (int)d->value_heads,
+                head_sums<<<dim3((unsigned)d->value_heads), 256, 0, st>>>(g.sums, d->batch * intervals, (int)d->value_heads,
                                                                          d->log_decay_type == ATLAS_OPS_BF16, dlog_decay);
         }
         return launched(err, cap, "linear_backward");

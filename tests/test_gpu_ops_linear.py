@@ -198,6 +198,25 @@ def test_gradients_of_strided_results():
     assert all(torch.equal(one[n], same[n]) for n in one)
 
 
+def test_tokens_far_apart():
+    """More than 2^24 elements from token to token: the results are those of a contiguous copy, bit by bit."""
+    T, far = 18, (1 << 24) + 8
+    memory = torch.zeros((T - 1) * far + 64, dtype=BF16, device="cuda")
+    spread = memory.as_strided((2, T, 2, 8), (32, far, 8, 1))
+    case = make(2, T, 2, 2, 8, 8, BF16)
+    gs = torch.randn(2, 2, 8, 8, device="cuda")
+    want = ops.linear_attention(**case, tape=True)
+    go = torch.randn(want[0].shape, device="cuda").to(BF16)
+    grads = ops.linear_attention_backward(go, gs, want[2])
+    for name in ("q", "v"):
+        spread.copy_(case[name])
+        got = ops.linear_attention(**dict(case, **{name: spread}), tape=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    spread.copy_(go)
+    again = ops.linear_attention_backward(spread, gs, want[2])
+    assert all(torch.equal(again[n], grads[n]) for n in grads)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_a_fault_reaches_its_own_and_later_tokens(dtype):
     print(f"case: linear attention faults {dtype}", flush=True)

@@ -193,6 +193,10 @@ def test_the_abi_refuses_linear_attention(refused):
     refused("atlas_ops_linear_forward", many, 0, P, P, P, text="2^25")
     without = ops._DELTA.pack(P, P, P, 0, 0, *([4] * 15), 0, 0, 1, 1, 1, 1, 4, 4, 0, 0, 0, 1.0)
     refused("atlas_ops_linear_backward", without, P, P, ops.struct.pack("@3q", 4, 4, 4), P, P, P, P, P, 0, P, P, text="decays")
+    far = ops.struct.pack("@3q", 4, (1 << 24) + 1, 4)
+    refused("atlas_ops_linear_backward", linear(), P, P, far, P, P, P, P, P, 0, P, P, text="2^24")
+    apart = ops._DELTA.pack(P, P, P, P, 0, *([4, (1 << 24) + 1, 4] * 5), 0, 0, 1, 1, 1, 1, 4, 4, 0, 0, 0, 1.0)
+    refused("atlas_ops_linear_forward", apart, 0, P, P, P, text="2^24")
     assert 0 < lib.atlas_ops_linear_workspace(linear(time=1000), 0) < lib.atlas_ops_linear_workspace(linear(time=1000), 1)
 
 
