@@ -192,10 +192,10 @@ __global__ void __launch_bounds__(256) rms_forward_long(Rows x, Rows residual, i
 
 // Group j of the grid visits rows j, j + groups, ...; partials: block b's sums of dw at partial[b * width].
 template <typename T, typename W, int LANES, int CH, bool STREAM>
-__global__ void __launch_bounds__(256, 2) rms_backward(Rows grad, Rows total, Rows grad_total, i64 rows, int width,
+__global__ void __launch_bounds__(LANES > 256 ? LANES : 256, 2) rms_backward(Rows grad, Rows total, Rows grad_total, i64 rows, int width,
                                                        const W* __restrict__ weight, const float* __restrict__ rstd_in,
                                                        T* __restrict__ dx, float* __restrict__ partial) {
-    constexpr int N = Unit<T>::N, GROUPS = 256 / LANES;
+    constexpr int N = Unit<T>::N, GROUPS = LANES > 256 ? 1 : 256 / LANES;
     __shared__ float shared[12];
     extern __shared__ float columns[];  // GROUPS > 1: the groups' column sums, one group after the other
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -344,7 +344,12 @@ __global__ void __launch_bounds__(1024) rms_reduce(i64 blocks, i64 width, const 
     }
 }
 
-// The layout of a row by its units of 16 bytes, as few lanes as hold it in registers.
+// The layout of a row by its units of 16 bytes, as few lanes as hold it in registers: a wider group waits for its sum with less
+// to load.  Forward and backward with the layout taken and with the next one:
+//   32768 x 64 float32     16 lanes 8.1 and 9.8 us,             64 lanes 13.1 and 18.9
+//   32768 x 512 float32    64 lanes of two units 46.8 and 46.3, 256 lanes 55 and 76
+//   4096 x 4096 float32    256 lanes of four 54.6 and 62.5,     as long rows 59.5 and 93.7
+//   4096 x 8192 bfloat16   backward 512 lanes of two 76 us (four units of 256 lanes spill: 126), as long rows 111
 struct Shape {
     int lanes, chunks;  // chunks 0: long rows
 };
@@ -355,7 +360,7 @@ Shape shape_of(i64 width, int type, bool backward) {
     for (int c : {1, 2})
         if (units <= 64 * c) return {64, c};
     for (int c : {1, 2, 4})
-        if (units <= 256 * c && !(backward && c == 4 && type == ATLAS_OPS_BF16)) return {256, c};
+        if (units <= 256 * c) return backward && c == 4 && type == ATLAS_OPS_BF16 ? Shape{512, 2} : Shape{256, c};
     return {256, 0};
 }
 
@@ -365,9 +370,10 @@ void with_shape(Shape s, F&& f) {
     if (s.lanes == 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
     else if (s.lanes == 64 && s.chunks == 1) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (s.lanes == 64) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-    else if (s.chunks == 1) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (s.chunks == 2) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if constexpr (!BACKWARD || sizeof(T) == 4) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else if (s.lanes == 256 && s.chunks == 1) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (s.lanes == 256 && s.chunks == 2) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if constexpr (BACKWARD && sizeof(T) == 2) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    else f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
 }
 
 template <typename F>
@@ -377,14 +383,18 @@ void with_types(int type, int weight_type, F&& f) {
     else f(bf16_t{}, bf16_t{});
 }
 
-// Workgroups at most: each keeps its columns' weights for all its rows and fetches its next row ahead.
-constexpr i64 FORWARD_BLOCKS = 2048, BACKWARD_BLOCKS = 768;
+// Workgroups at most: each keeps its columns' weights for all its rows and fetches its next row ahead.  Forward 1024 are within
+// 8 % either way, 4096 up to 18 % slower (4096 x 4096 float32 64 us instead of 54.6).
+constexpr i64 FORWARD_BLOCKS = 2048;
 
-// Blocks of the backward pass's rows; the partials stay a small share of the traffic.
+// Blocks of the backward pass's rows: as many as its registers let stay on 256 CUs, so that none waits for a second turn.
+// 8192 x 4096 bfloat16: 768 in 64 us, 512 in 75, 1024 in 91; of four units 4096 x 4096 float32: 512 in 62.5, 768 in 82.  The
+// partials stay a small share of the traffic.
 i64 row_blocks(i64 rows, i64 width, int type) {
     const Shape s = shape_of(width, type, true);
     if (s.chunks == 0) return std::min<i64>(rows, 64);
-    return std::min<i64>(ceil_div(rows, 256 / s.lanes), BACKWARD_BLOCKS);
+    if (s.lanes == 512) return std::min<i64>(rows, 256);
+    return std::min<i64>(ceil_div(rows, 256 / s.lanes), s.chunks == 4 ? 512 : 768);
 }
 
 // A long row is a workgroup of its own.
@@ -482,7 +492,7 @@ int atlas_ops_rms_norm_backward(const AtlasRows* grad, const AtlasRows* total, c
                     }
                     with_shape<T, true>(shape, [&](auto lanes, auto chunks) {
                         const size_t lds = lanes() < 256 ? 256 * chunks() * Unit<T>::N * sizeof(float) : 0;
-                        rms_backward<T, W, lanes(), chunks(), added()><<<dim3((unsigned)blocks), 256, lds, st>>>(
+                        rms_backward<T, W, lanes(), chunks(), added()><<<dim3((unsigned)blocks), std::max(256, lanes()), lds, st>>>(
                             g, in, s, rows, (int)width, (const W*)weight, rstd, (T*)dx, dweight ? workspace : nullptr);
                     });
                 });

@@ -86,7 +86,7 @@ struct Rows {
     }
 };
 
-// Sums of K values over a row's group: LANES lanes of one wave, or (LANES = 256) the workgroup.
+// Sums of K values over a row's group: LANES lanes of one wave, or (LANES = 256 or 512) the workgroup.
 template <int LANES, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* shared) {
 #pragma unroll
@@ -95,11 +95,15 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* shared) {
         __syncthreads();  // the previous use of `shared` is read
         if (threadIdx.x % 64 == 0) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) shared[4 * k + threadIdx.x / 64] = v[k];
+            for (int k = 0; k < K; ++k) shared[LANES / 64 * k + threadIdx.x / 64] = v[k];
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = (shared[4 * k] + shared[4 * k + 1]) + (shared[4 * k + 2] + shared[4 * k + 3]);
+        for (int k = 0; k < K; ++k) {
+            const float* part = shared + LANES / 64 * k;
+            v[k] = (part[0] + part[1]) + (part[2] + part[3]);
+            if constexpr (LANES == 512) v[k] += (part[4] + part[5]) + (part[6] + part[7]);
+        }
     }
 }
 
