@@ -207,7 +207,8 @@ struct Scan {
     double* heights;               // forwards their products with the states there
 };
 
-// Anchors lie behind every ANCHOR-th chunk but the last.
+// Anchors lie behind every ANCHOR-th chunk but the last: an error of the dots reaches as far back.  Training on 16384 tokens of 8
+// heads of 128: 4, 8 or 16 take 393, 383 or 378 us.
 constexpr int ANCHOR = 8;
 __host__ __device__ inline i64 anchors_of(i64 chunks) { return (chunks - 1) / ANCHOR; }
 
@@ -998,7 +999,10 @@ void with_type(int type, F&& f) {
 
 int chunk_of(int type) { return type == ATLAS_OPS_F32 ? Cut<float>::C : Cut<bf16_t>::C; }
 
-// Segments: as many as give every CU two workgroups, of at least two chunks each.
+// Segments: as many as give every CU its two workgroups, one chunk each if need be; two chunks are not worth two launches
+// more.  1 x 16384 of 8 heads of 128 bfloat16, training: 512 workgroups 383 us, 256 432, 1024 511.  500 tokens of 8 heads of
+// 64 float32: a segment for each chunk 19 us, for every two 21.5, for every four 30.6; 64 tokens (two chunks) of 4 heads 14.4,
+// 11.9 in one segment.
 struct Plan {
     i64 chunks, heads;  // of a sequence; batch x value heads
     int per, segments;
@@ -1010,7 +1014,7 @@ Plan plan_of(const AtlasDelta& d) {
     p.chunks = ceil_div(d.time, chunk_of(d.type));
     p.heads = d.batch * d.value_heads;
     p.state = d.key * d.value;
-    const i64 wanted = std::max<i64>(1, std::min<i64>(512 / p.heads, p.chunks / 2));
+    const i64 wanted = std::max<i64>(1, std::min<i64>(512 / p.heads, p.chunks > 2 ? p.chunks : 1));
     p.per = (int)ceil_div(p.chunks, wanted);
     p.segments = (int)ceil_div(p.chunks, p.per);
     return p;
@@ -1046,6 +1050,9 @@ Back back_of(const AtlasDelta& d) {
     return o;
 }
 
+// The narrowest kernel that holds both widths: 64 x 64 float32, training on 8 x 1000 tokens of 8 heads, 162 us, in the one for
+// 128 x 128 277.  Whole units of 16 bytes where both widths have them: 16384 tokens of 8 heads of 128 bfloat16, forward 105 us
+// and training 378, without that knowledge 128 and 544.
 template <bool OUT>
 void launch_scan(const Scan& s, int type, i64 batch, int segments, hipStream_t st) {
     const dim3 grid((unsigned)segments, (unsigned)s.value_heads, (unsigned)batch);

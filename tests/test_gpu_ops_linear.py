@@ -258,9 +258,10 @@ def test_steps_continue_a_sequence(B, H, Hv, dk, dv, dtype):
             assert state._version > version
         close(torch.stack(outs, 1), want, size, 80, "out")
         close(state, last, size_last, 80, "state")
-        short = {n: t[:, :12] if n in "qkv" or n == "log_decay" and decay == "token" else t for n, t in case.items()}
+        most = ops.SHORT_LINEAR
+        short = {n: t[:, :most] if n in "qkv" or n == "log_decay" and decay == "token" else t for n, t in case.items()}
         out, final = ops.linear_attention(**short)
-        assert torch.equal(out, torch.stack(outs[:12], 1)), "the same kernel"
+        assert torch.equal(out, torch.stack(outs[:most], 1)), "the same kernel"
 
 
 def test_bfloat16_outputs_round_once():
