@@ -69,6 +69,14 @@ def test_gradient(count, rows, width, kind, dtype):
     check_gradient(make((count, width), dtype, 1), drawn((count,), rows, kind), rows, 0.5)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,kind", [(9, "often"), (5000, "even"), (1, "one")])
+def test_gradient_of_wide_rows(rows, kind, dtype):
+    """So many lanes that float32 takes its longest tiles, bfloat16 the next."""
+    print(f"case: embedding gradient of wide rows {rows} {kind} {dtype}", flush=True)
+    check_gradient(make((17003, 1030), dtype, 1), drawn((17003,), rows, kind), rows, 0.5)
+
+
 @pytest.mark.parametrize("dtype,out", [(F32, BF16), (BF16, F32), (BF16, BF16)])
 def test_gradient_types_and_strides(dtype, out):
     print(f"case: embedding gradient {dtype} to {out}", flush=True)
