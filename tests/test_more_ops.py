@@ -156,7 +156,7 @@ def test_the_abi_refuses_streams_and_symbols(refused):
     refused(norm, rows, None, 1 << 24, 4100, 0, None, 0, 1e-5, P, None, None, None, text="2^24")
     refused(back, rows, rows, None, 4, 8, 0, None, 0, None, P, None, None, text="null")
     refused(back, rows, rows, None, 4, 8, 0, None, 0, P, P, P, None, text="null")
-    refused(back, rows, rows, None, 1 << 24, 4100, 1, None, 0, P, P, P, P, text="2^24")
+    refused(back, rows, rows, None, 1 << 24, 8200, 1, None, 0, P, P, P, P, text="2^24")
     look, sums = "atlas_ops_embedding", "atlas_ops_embedding_backward"
     refused(look, P, 0, 8, 8, 0, P, 0, 4, 1.0, P, text="positive")
     refused(look, P, 4, 0, 8, 0, P, 0, 4, 1.0, P, text="positive")
