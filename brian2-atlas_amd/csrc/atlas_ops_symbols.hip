@@ -5,16 +5,15 @@
 //   dtable_r = scale sum of grad_i over the i with token_i = r
 //   y_i = residual_i + (draw_i >= p 2^32 ? x_i / (1 - p) : 0)
 //
-// The gradient's sums are taken in the tokens' order: a stable radix sort of (token, place), which starts
-// beside the clearing of the table, brings each row's places together; tiles of sorted places are summed in
-// registers, a run of one row within a tile goes straight to the table, and runs that cross tiles leave
-// partial sums, which a last kernel adds from the first tile to the last.  Atomics count and list, none of them adds
-// values: the same bits every time.
+// The gradient's sums are taken in an order that the tokens alone set.  Few symbols are looked for by every row's
+// workgroup.  Else a stable radix sort of (token, place), which starts beside the clearing of the table, brings each row's
+// places together; tiles of sorted places are summed in registers, a run of one row within a tile goes straight to the
+// table, and runs that cross tiles leave partial sums, which a last kernel adds from the first tile to the last.  Atomics
+// count and list, none of them adds values: the same bits every time.
 //
 // Memory bounds the large ones: 32752 symbols of 50000 rows of 1024 bfloat16 values looked up in 28 us (4.8 TB/s); their
-// gradient in 80: the first counts with the clearing 19 (5.4 TB/s), placing 13.5 and 9, sums 20, crossing rows 8.  Small ones
-// are a chain of launches: 12288 symbols of 32 rows of 128 float32 values 25 us in four kernels.  Dropout of 12289 x 4099
-// bfloat16 values with a residual 59 us (5.1 TB/s).
+// gradient in 75: the first counts with the clearing 19 (5.4 TB/s), placing 13.5 and 9, sums 19, crossing rows 8.  Dropout of
+// 12289 x 4099 bfloat16 values with a residual 59 us (5.1 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -374,6 +373,77 @@ __global__ void __launch_bounds__(1024) embed_join(int width, float scale, O* __
     }
 }
 
+// ------------------------------------------------------------------ few symbols
+// A workgroup for each row and 8 units of its columns: it finds the row's places among all tokens, in their order, 128 groups of
+// 8 lanes add a part of them each, and the groups are added in a fixed order.  One launch; what bounds it is its chain of
+// tokens, places, gradients and two sums: 12288 symbols of 32 rows of 128 float32 values 12 us with cold caches, 9 with warm
+// ones.  TURNS: tokens of a lane; with 2 rather than 16 turns 2000 tokens take 6.5 us instead of 8.6.
+constexpr int FEW_TOKENS = 16384;
+
+template <typename T, typename O, int TURNS>
+__global__ void __launch_bounds__(1024) embed_few(Rows grad, int width, Tokens tokens, float scale, O* __restrict__ table) {
+    constexpr int N = Unit<T>::N, LANES = 8, GROUPS = 1024 / LANES, WAVES = 16, TOGETHER = 8;
+    __shared__ uint16_t list[TURNS * 1024];
+    __shared__ int found[WAVES];
+    __shared__ float sums[WAVES][LANES * N];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const i64 row = blockIdx.x;
+    const int count = (int)tokens.count, turns = (count + 1023) / 1024, first = wave * turns * 64 + lane;
+    i64 token[TURNS];
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) token[k] = tokens.at(min(first + k * 64, count - 1));
+    u64 met[TURNS];
+    int own = 0;
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        met[k] = __ballot(k < turns && first + k * 64 < count && token[k] == row);
+        own += __popcll(met[k]);
+    }
+    if (lane == 0) found[wave] = own;
+    __syncthreads();
+    int at = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        at += w < wave ? found[w] : 0;
+        n += found[w];
+    }
+#pragma unroll
+    for (int k = 0; k < TURNS; ++k) {
+        if (met[k] >> lane & 1) list[at + __popcll(met[k] & ((1ull << lane) - 1))] = (uint16_t)(first + k * 64);
+        at += __popcll(met[k]);
+    }
+    __syncthreads();
+    const int group = threadIdx.x / LANES, from = n * group / GROUPS, to = n * (group + 1) / GROUPS;
+    const int col0 = blockIdx.y * LANES * N, col = col0 + threadIdx.x % LANES * N;
+    float sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    for (int e0 = from; e0 < to; e0 += TOGETHER) {
+        Unit<T> unit[TOGETHER];
+#pragma unroll
+        for (int j = 0; j < TOGETHER; ++j) unit[j].load(grad.at<T>(list[min(e0 + j, to - 1)]), col, width);
+#pragma unroll
+        for (int j = 0; j < TOGETHER; ++j)
+            if (e0 + j < to)
+#pragma unroll
+                for (int i = 0; i < N; ++i) sum[i] += unit[j][i];
+    }
+#pragma unroll
+    for (int k = LANES; k < 64; k *= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] += __shfl_xor(sum[i], k, 64);
+    if (lane < LANES)
+#pragma unroll
+        for (int i = 0; i < N; ++i) sums[wave][lane * N + i] = sum[i];
+    __syncthreads();
+    if (threadIdx.x < LANES * N && col0 + (int)threadIdx.x < width) {
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) total += sums[w][threadIdx.x];
+        table[row * width + col0 + threadIdx.x] = from_float<O>(scale * total);
+    }
+}
+
 struct Plan {
     Sort sort;
     int passes, lanes, sum_tile;  // sorted places that a group sums
@@ -384,6 +454,16 @@ struct Plan {
 // 65536 x 512 float32 (32 taken) 84, 98 and 85 us; 32752 x 1024 bfloat16 (16 taken) 70, 69 and 75, by Zipf's law 53, 54 and 66;
 // 16384 x 512 float32 (8 taken) 43 with 32 and 38.5 with 8.
 constexpr i64 SUM_LANES = 250000;  // about a thousand to a CU
+
+// embed_few takes few symbols: its workgroups all find a place at once, and no row has very many places unless nearly all
+// symbols are one.  Whole gradient by it and by sorting: 12288 x 128 float32 of 32 rows 9 and 19 us, by Zipf's law 13 and 23;
+// 16000 x 256 of 16 rows by Zipf's law 25 and 24; 16000 x 128 of one row 41 and 31; 16000 x 128 of 500 rows (2000 workgroups)
+// 52 and 28, 2000 x 128 of 400 rows (1600) 28 and 23.
+i64 few_slices(i64 width, int type) { return ceil_div(width, 8 * (type == ATLAS_OPS_F32 ? 4 : 8)); }
+constexpr i64 FEW_BLOCKS = 512;
+bool is_few(i64 count, i64 rows, i64 width, int type) {
+    return count && count <= std::min<i64>(FEW_TOKENS, std::max<i64>(4096, 1024 * rows)) && rows * few_slices(width, type) <= FEW_BLOCKS;
+}
 
 // What both the workspace and the launch go by.  grad's type sets the lanes: as few as hold a row's units.
 Plan plan_of(i64 count, i64 rows, i64 width, int type) {
@@ -496,7 +576,7 @@ static bool embedding_fits(i64 count, i64 rows, i64 width) {
 
 int64_t atlas_ops_embedding_workspace(int64_t count, int64_t rows, int64_t width, int type) {
     if (!embedding_fits(count, rows, width) || !known_type(type)) return 0;
-    return plan_of(count, rows, width, type).bytes;
+    return is_few(count, rows, width, type) ? 16 : plan_of(count, rows, width, type).bytes;
 }
 
 int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int wide, int64_t count, int64_t rows, int64_t width, int type,
@@ -506,8 +586,20 @@ int atlas_ops_embedding_backward(const AtlasRows* grad, const void* tokens, int 
         if (!embedding_fits(count, rows, width)) return fail(err, cap, 7, "at most 2^27 tokens, rows below 2^31 - 1, width up to 2^20, both positive");
         if (!dtable || (count && (!grad || !grad->data || grad->inner < 1 || !tokens || !workspace)))
             return fail(err, cap, 7, "null argument");
-        Plan p = plan_of(count, rows, width, type);
         hipStream_t st = (hipStream_t)stream;
+        if (is_few(count, rows, width, type)) {
+            const Rows g{grad->data, grad->inner, grad->outer_stride, grad->inner_stride};
+            const dim3 grid((unsigned)rows, (unsigned)few_slices(width, type));
+            with_type(type, [&](auto t) {
+                with_type(table_type, [&](auto o) {
+                    using O = decltype(o);
+                    auto* few = count <= 2048 ? embed_few<decltype(t), O, 2> : embed_few<decltype(t), O, FEW_TOKENS / 1024>;
+                    few<<<grid, 1024, 0, st>>>(g, (int)width, Tokens{tokens, wide, count}, scale, (O*)dtable);
+                });
+            });
+            return launched(err, cap, "embedding_backward");
+        }
+        Plan p = plan_of(count, rows, width, type);
         const i64 size = rows * width * (table_type == ATLAS_OPS_F32 ? 4 : 2);
         const i64 clearing = std::min<i64>(ceil_div(size, 256 * 16 * 4), 2048);
         const Tokens list{tokens, wide, count};

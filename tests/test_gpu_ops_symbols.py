@@ -77,6 +77,17 @@ def test_gradient_of_wide_rows(rows, kind, dtype):
     check_gradient(make((17003, 1030), dtype, 1), drawn((17003,), rows, kind), rows, 0.5)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["even", "often", "one", "beyond"])
+def test_gradient_of_few_symbols(kind, dtype):
+    """On both sides of what one launch takes, of 2 and 16 tokens a lane, and of a slice's columns."""
+    for count, rows, width in ((1, 3, 5), (63, 512, 8), (64, 513, 8), (1023, 7, 31), (2047, 5, 33), (2049, 11, 64), (4096, 1, 65), (4097, 1, 40),
+                               (5119, 5, 129), (5121, 5, 130), (16384, 16, 24), (16385, 17, 24), (9001, 100, 100)):
+        print(f"case: embedding gradient of few {count} tokens {rows} x {width} {kind} {dtype}", flush=True)
+        grad = make((count, 2 * width), dtype, 1)[:, :width]
+        check_gradient(grad, drawn((count,), rows, kind, dtype=torch.int32), rows, -1.5)
+
+
 @pytest.mark.parametrize("dtype,out", [(F32, BF16), (BF16, F32), (BF16, BF16)])
 def test_gradient_types_and_strides(dtype, out):
     print(f"case: embedding gradient {dtype} to {out}", flush=True)
