@@ -110,6 +110,16 @@ def test_one_segment(dtype):
     check(make(33, 150, 16, 16, 16, 20, dtype, decay="head"), lengths=[150, 0, 1] + [7 * i % 151 for i in range(30)])
 
 
+@pytest.mark.parametrize("dtype,T", [(F32, 650), (BF16, 1290)])
+@pytest.mark.parametrize("dk,dv", [(20, 24), (68, 12)])
+def test_segments_of_several_chunks(dk, dv, dtype, T):
+    """Segments of three chunks each, which end between the places where a decay's gradient starts anew; widths that one kernel
+    holds both ways round and widths that take two."""
+    print(f"case: linear attention segments {T} tokens {dk} x {dv} {dtype}", flush=True)
+    check(make(9, T, 4, 8, dk, dv, dtype), lengths=[T, 0, 1, T - 1, T // 2, 192, 193, 40, T // 3])
+    check(make(9, T, 8, 8, dk, dv, dtype, decay="head", state=False), grad_state=False)
+
+
 @pytest.mark.parametrize("decay", [None, "token", "head"])
 @pytest.mark.parametrize("lengths", [[70, 33, 0], [1, 64, 200], [200, 199, -3], [65, 300, 32]])
 def test_lengths(lengths, decay):
