@@ -516,14 +516,14 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
         if constexpr (OUT) {
             // ---- decayed scores, turned: rows are keys, columns queries
             constexpr int OWN = (BLOCKS + WAVES - 1) / WAVES;  // blocks of a wave, all in flight; what lies beyond the last is not kept
-            float4_t p[OWN];
+            float4_t p[OWN], p_small[OWN];
             int qbs[OWN], kjs[OWN];
 #pragma unroll
             for (int m = 0; m < OWN; ++m) {
                 const int block = min(wave + WAVES * m, BLOCKS - 1);
                 qbs[m] = block >= 6 ? 3 : block >= 3 ? 2 : block >= 1 ? 1 : 0;
                 kjs[m] = block - qbs[m] * (qbs[m] + 1) / 2;
-                p[m] = ZERO;
+                p[m] = p_small[m] = ZERO;
             }
             Pieces<N> kn[2][OWN], qn[2][OWN];
             auto read = [&](int c) {
@@ -538,9 +538,12 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
 #pragma unroll
             for (int c = 0; c < DK / 32; ++c) {
                 if (c + 1 < DK / 32) read(c + 1);
-                mma_each(kn[c & 1], qn[c & 1], p);
+                mma_each(kn[c & 1], qn[c & 1], p, p_small);
                 in_order();
             }
+            if constexpr (N > 1)
+#pragma unroll
+                for (int m = 0; m < OWN; ++m) p[m] += p_small[m];
             const float factor = d.write * d.read;
 #pragma unroll
             for (int m = 0; m < OWN; ++m) {
@@ -565,32 +568,33 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
                     const int qb = qbs[m], kj = kjs[m], t = token(16 * qb + l.col);
                     const T* row = d.dot.x.at<T>(b, t0 + (t < live ? t : 0), h / d.dot.group);
                     const T* key = vs + (16 * kj + l.col) * VPITCH;
-                    float4_t w = ZERO;
+                    float4_t w[1] = {ZERO}, w_small[1] = {ZERO};
 #pragma unroll
                     for (int c = 0; c < DV / 32; ++c) {
                         const int c0 = 32 * c + l.quad;
-                        Pieces<N> a, x;
+                        Pieces<N> a[1], x[1];
                         if constexpr (N == 1) {
-                            a.p[0] = both(*(const bf16x4*)(key + c0), *(const bf16x4*)(key + c0 + 16));
-                            x.p[0] = both(__builtin_bit_cast(bf16x4, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(bf16x4, four<WHOLE>(row, c0 + 16, outer)));
+                            a[0].p[0] = both(*(const bf16x4*)(key + c0), *(const bf16x4*)(key + c0 + 16));
+                            x[0].p[0] = both(__builtin_bit_cast(bf16x4, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(bf16x4, four<WHOLE>(row, c0 + 16, outer)));
                         } else {
-                            a = split<3>(*(const float4_t*)(key + c0), *(const float4_t*)(key + c0 + 16));
-                            x = split<3>(__builtin_bit_cast(float4_t, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(float4_t, four<WHOLE>(row, c0 + 16, outer)));
+                            a[0] = split<3>(*(const float4_t*)(key + c0), *(const float4_t*)(key + c0 + 16));
+                            x[0] = split<3>(__builtin_bit_cast(float4_t, four<WHOLE>(row, c0, outer)), __builtin_bit_cast(float4_t, four<WHOLE>(row, c0 + 16, outer)));
                         }
-                        w = mma(a, x, w);
+                        mma_each(a, x, w, w_small);
                     }
+                    if constexpr (N > 1) w[0] += w_small[0];
                     const int i = 16 * qb + l.col, at = 16 * kj + l.quad;
                     float sum = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        w[j] = at + j < i && t < live ? w[j] * p[m][j] : 0.0f;
-                        sum += w[j];
+                        w[0][j] = at + j < i && t < live ? w[0][j] * p[m][j] : 0.0f;
+                        sum += w[0][j];
                     }
                     sum += __shfl_xor(sum, 16, 64);
                     sum += __shfl_xor(sum, 32, 64);
                     float4_t down;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) down[j] = lane_sum<16>(w[j]);
+                    for (int j = 0; j < 4; ++j) down[j] = lane_sum<16>(w[0][j]);
                     const int block = wave + WAVES * m;
                     if (block < BLOCKS && l.quad == 0) pair_rows[block][l.col] = sum;
                     if (block < BLOCKS && l.col == 0) *(float4_t*)(pair_columns[block] + l.quad) = down;
@@ -600,11 +604,14 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
             if (more) fetch(next, 2);
             in_order();
             // ---- what the state answers: rows are columns of the values, columns are queries
-            float4_t o[NB][QB];
+            float4_t o[NB][QB], o_small[N > 1 ? NB : 1][N > 1 ? QB : 1];
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[n][qb] = ZERO;
+                for (int n = 0; n < NB; ++n) {
+                    o[n][qb] = ZERO;
+                    if constexpr (N > 1) o_small[n][qb] = ZERO;
+                }
             Pieces<N> q[2][QB];
             auto read_queries = [&](int c) {
 #pragma unroll
@@ -618,14 +625,18 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) state[n] = split_pairs(s[2 * c][n], s[2 * c + 1][n]);
                 if (c + 1 < DK / 32) read_queries(c + 1);
-                mma_grid(state, q[c & 1], o);
+                if constexpr (N > 1) mma_grid(state, q[c & 1], o, o_small);
+                else mma_grid(state, q[c & 1], o);
                 in_order();
             }
 #pragma unroll
             for (int qb = 0; qb < QB; ++qb) {
                 const float g = since[turn][16 * qb + l.col];
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[n][qb] *= g;
+                for (int n = 0; n < NB; ++n) {
+                    if constexpr (N > 1) o[n][qb] += o_small[n][qb];
+                    o[n][qb] *= g;
+                }
             }
             constexpr bool FULL = WHOLE && (sizeof(T) == 2 || NB == 1);  // a lane's 4 NB neighbouring columns are there or none
             const int c0 = 16 * NB * wave + NB * l.quad, left = outer - c0;
@@ -756,12 +767,13 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
             in_order();
         }
 
-        // ---- the state behind the chunk
+        // ---- the state behind the chunk; of float32 the chunk's share is summed alone, and the state rounded once
         const float decayed = decays[turn];
+        if constexpr (KB > 1)
 #pragma unroll
-        for (int r = 0; r < DK / 16; ++r)
+            for (int r = 0; r < DK / 16; ++r)
 #pragma unroll
-            for (int n = 0; n < NB; ++n) s[r][n] *= decayed;
+                for (int n = 0; n < NB; ++n) s[r][n] *= decayed;
         constexpr int R = N == 1 ? 4 : 2, GROUPS = DK / 16 / R;  // blocks of rows at a time
         Pieces<N> kt[2][R];
         auto read_keys = [&](int at) {
@@ -793,12 +805,12 @@ __global__ void __launch_bounds__(256, 2) scan(Runs) {
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) sums[r][n] = s[r0 + r][n];
+                    for (int n = 0; n < NB; ++n) sums[r][n] = KB > 1 ? s[r0 + r][n] : ZERO;
                 mma_grid(kt[at & 1], written, sums);
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) s[r0 + r][n] = sums[r][n];
+                    for (int n = 0; n < NB; ++n) s[r0 + r][n] = KB > 1 ? sums[r][n] : decayed * s[r0 + r][n] + sums[r][n];
                 in_order();
             }
         }

@@ -139,6 +139,40 @@ __device__ __forceinline__ void mma_each(const Pieces<NA> (&a)[R], const Pieces<
                 for (int m = 0; m < R; ++m) c[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[m].p[order - i], c[m], 0, 0, 0);
 }
 
+// The same with the first pieces' products in `c` alone, the others in `small`: a sum over many operands is then rounded at its
+// full size once for each of them, not once for each product of pieces.
+template <int NA, int NB, int R, int S>
+__device__ __forceinline__ void mma_grid(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[S], float4_t (&c)[R][S], float4_t (&small)[R][S]) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB)
+#pragma unroll
+                for (int m = 0; m < R; ++m)
+#pragma unroll
+                    for (int n = 0; n < S; ++n) {
+                        float4_t& sum = order ? small[m][n] : c[m][n];
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[n].p[order - i], sum, 0, 0, 0);
+                    }
+}
+
+template <int NA, int NB, int R>
+__device__ __forceinline__ void mma_each(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[R], float4_t (&c)[R], float4_t (&small)[R]) {
+    constexpr int ORDERS = NA > NB ? NA : NB;
+#pragma unroll
+    for (int order = ORDERS - 1; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i <= order; ++i)
+            if (i < NA && order - i < NB)
+#pragma unroll
+                for (int m = 0; m < R; ++m) {
+                    float4_t& sum = order ? small[m] : c[m];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[m].p[order - i], sum, 0, 0, 0);
+                }
+}
+
 // c + A B in two chains, the smaller products apart from the larger: half the latency of mma.
 template <int NA, int NB>
 __device__ __forceinline__ void mma2(const Pieces<NA>& a, const Pieces<NB>& b, float4_t& large, float4_t& small) {
