@@ -151,7 +151,13 @@ def _last(t):
 
 def _near(t):
     """(batch, time, ...) with tokens as near to one another as linear attention in chunks has them."""
-    return t if t.stride(1) <= 1 << 24 else t.contiguous()
+    return t if t.stride(1) <= 1 << 24 or t.shape[1] == 1 else t.contiguous()
+
+
+def _token_strides(t):
+    """Of the first three axes of (batch, time, ...); a single token, whose stride may be anything, is nowhere near another."""
+    s = t.stride()
+    return s[:3] if t.shape[1] > 1 else (s[0], 0, s[2])
 
 
 def _workspace(size: int, like):
@@ -552,8 +558,10 @@ class _Problem:
             q, k, v = _near(q), _near(k), _near(v)
 
         def strides(t):
+            if time_axis:
+                return _token_strides(t)
             s = t.stride()
-            return s[:3] if time_axis else (s[0], 0, s[1])
+            return s[0], 0, s[1]
 
         self.device, self.batch, self.time, self.heads, self.value_heads = device, batch, time, heads, value_heads
         self.key, self.value, self.type = key, value, q.dtype
@@ -780,6 +788,6 @@ def linear_attention_backward(grad_out, grad_state, tape: LinearTape) -> dict:
     workspace = _workspace(lib.atlas_ops_linear_backward_workspace(p.packed), v)
     dq, dk, dv, decay, dstate = (None if g is None else g.data_ptr() for g in grads.values())
     _call(p.device, lib.atlas_ops_linear_backward, p.packed, tape.memory.data_ptr(), grad_out.data_ptr(),
-          struct.pack("@3q", *grad_out.stride()[:3]), None if grad_state is None else grad_state.data_ptr(), dq, dk, dv, decay,
+          struct.pack("@3q", *_token_strides(grad_out)), None if grad_state is None else grad_state.data_ptr(), dq, dk, dv, decay,
           int(log_decay is not None and log_decay.dim() == 1), dstate, workspace.data_ptr())
     return grads

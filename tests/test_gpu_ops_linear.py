@@ -323,3 +323,22 @@ def test_refusals():
             call()
     with torch.no_grad():
         ops.linear_attention(q.clone().requires_grad_(), k, v, g)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_single_token_of_any_stride(dtype):
+    """One token has no distance to the next: (time, batch, ...) turned, whose time stride passes 2^24 elements."""
+    print(f"case: linear attention single token {dtype}", flush=True)
+    far = lambda t: t.as_strided(t.shape, (t.stride(0), 1 << 25, *t.stride()[2:]))  # noqa: E731
+    case = make(2, 1, 2, 2, 8, 8, dtype)
+    want = ops.linear_attention(**case, tape=True)
+    go, gs = torch.randn(want[0].shape, device="cuda").to(dtype), torch.randn(want[1].shape, device="cuda")
+    grads = ops.linear_attention_backward(go, gs, want[2])
+    turned = {n: far(t) if n in ("q", "k", "v", "log_decay") else t for n, t in case.items()}
+    assert all(turned[n].is_contiguous() and turned[n].stride(1) == 1 << 25 for n in ("q", "k", "v"))
+    out, final, tape = ops.linear_attention(**turned, tape=True)
+    assert torch.equal(out, want[0]) and torch.equal(final, want[1])
+    got = ops.linear_attention_backward(far(go), gs, tape)
+    assert all(torch.equal(got[n], grads[n]) for n in grads)
+    out, final = ops.linear_attention(**turned)
+    assert torch.equal(out, ops.linear_attention(**case)[0])
