@@ -290,7 +290,7 @@ def rms_norm(x, weight=None, residual=None, *, eps: float = 1e-5, statistics: bo
 
     x: float32 or bfloat16; residual: of x's shape and type; weight: float32 or x's type.  Returns y, or (y, total) with a
     residual, both contiguous and of x's type; ``statistics`` adds rstd at the end, float32 of x's leading shape, which
-    ``rms_norm_backward`` takes."""
+    ``rms_norm_backward`` takes.  The squares are summed in float32: where that is infinite, rstd is 0."""
     device, width, rows, weight, code = _rms_arguments(x, weight, residual)
     y = _empty(x)
     total = None if residual is None else _empty(x)
@@ -305,8 +305,9 @@ def rms_norm(x, weight=None, residual=None, *, eps: float = 1e-5, statistics: bo
 def rms_norm_8bit(x, weight=None, residual=None, *, eps: float = 1e-5):
     """``rms_norm`` for a product of 8 bits: (values, scale), or (values, scale, total) with a residual.
 
-    values: float8_e4m3fn, the norm's result over its row's scale, rounded once; scale: float32 of x's leading shape, the
-    row's largest magnitude / 448, at least 2^-126.  A NaN has no part in the scale; an infinity makes it infinite."""
+    values: float8_e4m3fn, the norm's result over its row's scale, computed in float32 and then rounded; scale: float32 of x's
+    leading shape, the row's largest magnitude / 448, at least 2^-126.  A NaN has no part in the scale.  The scale is infinite
+    where the row's largest magnitude or its sum of squares in float32 is: an infinity, or values above about 1e19."""
     device, width, rows, weight, code = _rms_arguments(x, weight, residual)
     values = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)

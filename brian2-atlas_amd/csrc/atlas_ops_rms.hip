@@ -4,7 +4,7 @@
 //   t = x + r (rounded to the rows' type, as the next layer reads it),  z = t rstd,  y = z w,
 //   rstd = 1 / sqrt(mean(t^2) + eps)
 //   dt = rstd (h - z mean(h z)) + g_t,  h = g w,  which is the gradient of x and of r;   dw = sum_rows g z
-//   8 bits: scale = max(max |y| / 448, 2^-126),  value = y / scale as e4m3
+//   8 bits: scale = max(max |y| / 448, 2^-126),  value = y / scale as e4m3; infinite where the sum of squares is
 //
 // Memory bounds all of it.  A row is read once into registers, summed, written; the next row's loads are in
 // flight meanwhile.  16384 x 4096 bfloat16 with a residual: forward 94 us (5.7 TB/s over four passes), backward 135 us (4.0: its
@@ -19,6 +19,11 @@ namespace atlas_ops {
 namespace {
 
 constexpr float LARGEST = 448.0f, SMALLEST_SCALE = 0x1p-126f;  // of e4m3; a zero row's scale
+
+// Of a row of 8 bits.  rstd is 0 where the sum of squares passes float32 and every value is lost: an infinite scale says so.
+__device__ __forceinline__ float scale_of(float most, float rstd) {
+    return rstd == 0.0f ? INFINITY : fmaxf(most / LARGEST, SMALLEST_SCALE);
+}
 
 template <int LANES>
 __device__ __forceinline__ float group_max(float v, float* shared) {
@@ -120,7 +125,7 @@ __global__ void __launch_bounds__(256) rms_forward(Rows x, Rows residual, i64 ro
             for (int c = 0; c < CH; ++c)
 #pragma unroll
                 for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(v[c][i]));
-            const float scale = fmaxf(group_max<LANES>(most, shared) / LARGEST, SMALLEST_SCALE), inverse = 1.0f / scale;
+            const float scale = scale_of(group_max<LANES>(most, shared), rstd), inverse = 1.0f / scale;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int col = (lane + c * LANES) * N;
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(256) rms_forward_long(Rows x, Rows residual, i
 #pragma unroll
             for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(v[i] * rstd * w[i]));
         }
-        scale = fmaxf(group_max<256>(most, shared) / LARGEST, SMALLEST_SCALE);
+        scale = scale_of(group_max<256>(most, shared), rstd);
         if (threadIdx.x == 0) out.scale[row] = scale;
     }
     for (int col = threadIdx.x * N; col < width; col += 256 * N) {

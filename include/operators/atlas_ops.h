@@ -125,8 +125,9 @@ int atlas_ops_delta_backward(const AtlasDelta* delta, const void* tape, const vo
 /*
  * Root-mean-square normalisation of a stream: t = x + residual rounded to `type` (t = x where residual is NULL),
  * y = t rstd weight by row, rstd = 1 / sqrt(mean(t^2) + eps).  y is rows x width, contiguous, of x's type, or,
- * where scale (f32[rows]) is not NULL, 8-bit e4m3 values of y / scale with scale = max(max |y| / 448, 2^-126).  total
- * (NULL exactly where residual is) receives t, contiguous; rstd (may be NULL) f32[rows]; weight may be NULL.
+ * where scale (f32[rows]) is not NULL, 8-bit e4m3 values of y / scale with scale = max(max |y| / 448, 2^-126), infinite
+ * where the sum of t^2 is (rstd is 0 there).  total (NULL exactly where residual is) receives t, contiguous; rstd (may be
+ * NULL) f32[rows]; weight may be NULL.
  */
 int atlas_ops_rms_norm(const AtlasRows* x, const AtlasRows* residual, int64_t rows, int64_t width, int type,
                        const void* weight, int weight_type, float eps, void* y, float* scale, void* total, float* rstd,

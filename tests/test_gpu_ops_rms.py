@@ -191,3 +191,29 @@ def test_offsets_beyond_32_bits():
     far = memory.as_strided((2, 64), (1 << 31, 1))
     far.copy_(make((2, 64), BF16, 7))
     check(far, None, far, make((2, 64), BF16, 8), far)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [20, 96, 300, 1000, 1500, 4000, 9000])
+def test_8bit_rows_beyond_float32(width, dtype):
+    """Rows whose squares pass float32 have an infinite scale in every layout: an infinity of either sign, one that the residual
+    brings, and finite values too large.  So has a row with an infinite weight; their neighbours keep theirs."""
+    print(f"case: rms norm 8 bits beyond float32, {width} {dtype}", flush=True)
+    x = make((6, width), dtype)
+    clean = ops.rms_norm_8bit(x)
+    dirty, residual = x.clone(), torch.zeros_like(x)
+    dirty[1, width // 2], dirty[2, 0], residual[3, width - 1], dirty[4] = float("inf"), -float("inf"), float("inf"), 3e19
+    values, scale, total = ops.rms_norm_8bit(dirty, None, residual)
+    assert torch.isinf(scale[1:5]).all() and (scale[1:5] > 0).all()
+    for row in (0, 5):
+        assert scale[row] == clean[1][row] and torch.equal(values[row].float(), clean[0][row].float())
+    assert torch.isnan(values[1, width // 2].float()) and torch.isnan(values[2, 0].float()) and torch.isnan(values[3, width - 1].float())
+    assert (values[4].float() == 0).all() and (values[1].float() == 0).sum() == width - 1
+    dirty = x.clone()
+    dirty[1, 3] = float("nan")   # of a NaN no scale knows: the values are NaN
+    values, scale = ops.rms_norm_8bit(dirty)
+    assert torch.isnan(values[1].float()).all() and scale[1] == 2.0 ** -126
+    weight = torch.ones(width, device="cuda")
+    weight[5] = float("inf")
+    values, scale = ops.rms_norm_8bit(x, weight)
+    assert torch.isinf(scale).all()
