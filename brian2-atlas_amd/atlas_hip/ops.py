@@ -125,7 +125,7 @@ def _tensor(t, name: str, device=None, types=TYPES, shape=None):
     return index
 
 
-_F32, _I32, _I64 = {torch.float32: 0}, {torch.int32: 0}, {torch.int64: 0}
+_F32, _I32, _I64, _U8 = {torch.float32: 0}, {torch.int32: 0}, {torch.int64: 0}, {torch.uint8: 0}
 _SAME = {t: {t: 0} for t in TYPES}
 
 
@@ -522,7 +522,7 @@ def muon_update(weight, gradient, momentum, *, learning_rate: float, factor: flo
 class _Problem:
     """The checked arguments of a delta rule, or of linear attention: sizes, the packed AtlasDelta and the tensors behind it."""
 
-    __slots__ = ("device", "batch", "time", "heads", "value_heads", "key", "value", "type", "packed", "tensors")
+    __slots__ = ("device", "batch", "time", "heads", "value_heads", "key", "value", "type", "scale", "packed", "tensors")
 
     def __init__(self, q, k, v, log_decay, beta, state, lengths, scale, time_axis: bool, linear: bool = False):
         device = _tensor(q, "q")
@@ -565,7 +565,7 @@ class _Problem:
             return s[0], 0, s[1]
 
         self.device, self.batch, self.time, self.heads, self.value_heads = device, batch, time, heads, value_heads
-        self.key, self.value, self.type = key, value, q.dtype
+        self.key, self.value, self.type, self.scale = key, value, q.dtype, scale
         self.tensors = (q, k, v, log_decay, beta, state, lengths)
         self.packed = _DELTA.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if log_decay is None else log_decay.data_ptr(),
@@ -602,14 +602,41 @@ def delta_rule_step(q, k, v, log_decay, beta, state, *, scale: float | None = No
 SHORT = 12
 
 
-class DeltaTape:
-    """What ``delta_rule_backward`` needs of a forward pass: its inputs and the chunks' states.  The inputs
-    must not change before the backward pass has run."""
-
+class _Tape:
     __slots__ = ("problem", "memory", "stream")
 
     def __init__(self, problem, memory, stream):
         self.problem, self.memory, self.stream = problem, memory, stream
+
+    def split(self):
+        """(tensors, rest): all that the tape holds on the GPU, some None, as autograd's saved tensors take it, and what ``join``
+        needs besides.  Hold no other reference to the tape to let its memory go with theirs."""
+        return (*self.problem.tensors, self.memory), (self.stream, self.problem.scale)
+
+    @classmethod
+    def join(cls, tensors, rest):
+        """The tape of ``split``, whose tensors may have moved in the meantime, or been laid out anew."""
+        if len(tensors) != 8:
+            raise ValueError("tensors must be those of a tape's split()")
+        *inputs, state, lengths, memory = tensors
+        stream, scale = rest
+        if isinstance(state, torch.Tensor):
+            state = state.contiguous()
+        problem = _Problem(*inputs, state, lengths, scale, True, cls is LinearTape)
+        if problem.batch and problem.time:
+            _tensor(memory, "the tape's memory", problem.device, _U8)
+            lib = library()
+            if memory.numel() != (lib.atlas_ops_linear_workspace if cls is LinearTape else lib.atlas_ops_delta_workspace)(problem.packed, True):
+                raise ValueError("the tape's memory is not that of these tensors")
+            memory = memory.contiguous() if memory.data_ptr() % 16 == 0 else memory.clone(memory_format=torch.contiguous_format)
+        return cls(problem, memory, stream)
+
+
+class DeltaTape(_Tape):
+    """What ``delta_rule_backward`` needs of a forward pass: its inputs and the chunks' states.  The inputs
+    must not change before the backward pass has run."""
+
+    __slots__ = ()
 
 
 def delta_rule(q, k, v, log_decay, beta, state=None, *, lengths=None, scale: float | None = None, tape: bool = False):
@@ -712,14 +739,11 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale: float | None = No
 SHORT_LINEAR = 5
 
 
-class LinearTape:
+class LinearTape(_Tape):
     """What ``linear_attention_backward`` needs of a forward pass: its inputs and the segments' states.  The inputs must
     not change before the backward pass has run."""
 
-    __slots__ = ("problem", "memory", "stream")
-
-    def __init__(self, problem, memory, stream):
-        self.problem, self.memory, self.stream = problem, memory, stream
+    __slots__ = ()
 
 
 def linear_attention(q, k, v, log_decay=None, state=None, *, lengths=None, scale: float | None = None, tape: bool = False):

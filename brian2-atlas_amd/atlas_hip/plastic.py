@@ -45,13 +45,15 @@ class DeltaRule(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay, beta):
-        out, _, ctx.tape = ops.delta_rule(q, k, v, log_decay, beta, scale=1.0, tape=True)
+        out, _, tape = ops.delta_rule(q, k, v, log_decay, beta, scale=1.0, tape=True)
+        tensors, ctx.rest = tape.split()
+        ctx.save_for_backward(*tensors)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        grads = ops.delta_rule_backward(grad, None, ctx.tape)
+        grads = ops.delta_rule_backward(grad, None, ops.DeltaTape.join(ctx.saved_tensors, ctx.rest))
         return tuple(grads[name] for name in ("q", "k", "v", "log_decay", "beta"))
 
 
@@ -76,13 +78,15 @@ class LinearAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, log_decay):
-        out, _, ctx.tape = ops.linear_attention(q, k, v, log_decay, scale=1.0, tape=True)
+        out, _, tape = ops.linear_attention(q, k, v, log_decay, scale=1.0, tape=True)
+        tensors, ctx.rest = tape.split()
+        ctx.save_for_backward(*tensors)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        grads = ops.linear_attention_backward(grad, None, ctx.tape)
+        grads = ops.linear_attention_backward(grad, None, ops.LinearTape.join(ctx.saved_tensors, ctx.rest))
         return tuple(grads[name] for name in ("q", "k", "v", "log_decay"))
 
 
@@ -102,18 +106,21 @@ class Embedding(torch.autograd.Function):
 
 
 class Dropout(torch.autograd.Function):
-    """``ops.dropout`` for torch's autograd; the tick must not change before the backward pass."""
+    """``ops.dropout`` for torch's autograd; a tick on the GPU must not change before the backward pass, which refuses it then."""
 
     @staticmethod
     def forward(ctx, x, probability, seed, stream, tick):
-        ctx.arguments = probability, seed, stream, tick
+        held = isinstance(tick, torch.Tensor)
+        ctx.arguments = probability, seed, stream, None if held else tick
+        ctx.save_for_backward(tick if held else None)
         return ops.dropout(x, probability, seed, stream=stream, tick=tick)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         probability, seed, stream, tick = ctx.arguments
-        return ops.dropout(grad, probability, seed, stream=stream, tick=tick), None, None, None, None
+        held, = ctx.saved_tensors
+        return ops.dropout(grad, probability, seed, stream=stream, tick=tick if held is None else held), None, None, None, None
 
 
 class PlasticLayer:
