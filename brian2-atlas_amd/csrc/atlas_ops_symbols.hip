@@ -514,9 +514,10 @@ __device__ __forceinline__ u64 finalise(u64 v) {
     return v ^ (v >> 31);
 }
 
+// y may be x or residual: a thread reads its values before it writes them, and no other reads them.
 template <typename T, bool RESIDUAL>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, i64 count, uint32_t threshold,
-                                                      float factor, u64 base, u64 tick, const i64* __restrict__ tick_at, T* __restrict__ y) {
+__global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, i64 count, uint32_t threshold, float factor, u64 base,
+                                                      u64 tick, const i64* tick_at, T* y) {
     constexpr int N = Unit<T>::N;
     if (tick_at) tick = (u64)*tick_at;
     base ^= tick * TICK;

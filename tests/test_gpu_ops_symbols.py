@@ -242,3 +242,21 @@ def test_dropout_empty_and_refused():
                  lambda: ops.dropout(x, 0.5, 0, residual=x.bfloat16()), lambda: ops.dropout(x.clone().requires_grad_(), 0.5, 0), lambda: ops.dropout(None, 0.5, 0)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("count", [1, 7, 4096, 8 * 256 * 4096 + 24581])
+def test_dropout_in_place(count, dtype):
+    """Through the C ABI, whose result may be its input or its residual: the same bits as in memory of its own."""
+    print(f"case: dropout in place, {count} {dtype}", flush=True)
+    x, residual = make((count,), dtype), make((count,), dtype, 1)
+    for added in (None, residual):
+        want = ops.dropout(x, 0.3, 5, stream=2, tick=9, residual=added)
+        for name in ("x", "residual"):
+            if name == "residual" and added is None:
+                continue
+            given = {"x": x.clone(), "residual": None if added is None else added.clone()}
+            y = given[name]
+            ops._call(0, ops.library().atlas_ops_dropout, given["x"].data_ptr(), None if added is None else given["residual"].data_ptr(), count,
+                      ops.TYPES[dtype], 0.3, 5, 2, 9, None, y.data_ptr())
+            assert torch.equal(y, want), name

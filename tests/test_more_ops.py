@@ -209,3 +209,10 @@ def test_tensors_on_the_cpu_are_refused():
                  lambda: ops.linear_attention_step(x[:, 0], x[:, 0], x[:, 0], gate[:, 0], torch.zeros(2, 2, 4, 4))):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_what_may_share_memory_is_not_declared_apart():
+    """Dropout's result may be its input or its residual: none of the kernel's pointers may promise otherwise."""
+    source = (ops.LIBRARY.parent / "csrc" / "atlas_ops_symbols.hip").read_text()
+    start = source.index("dropout_kernel(")
+    assert "__restrict__" not in source[start:source.index("{", start)]
