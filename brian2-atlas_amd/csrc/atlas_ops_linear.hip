@@ -55,6 +55,9 @@ __device__ __forceinline__ i64 length_of(const int32_t* lengths, i64 time, i64 b
 }
 
 // ------------------------------------------------------------------ token by token
+// 16 bytes in one access wherever a caller's floats start: a state need not lie on 16 bytes, and gfx950 takes any.
+typedef float4_t float4_any_t __attribute__((aligned(4)));
+
 struct Step {
     Tensor q, k, v;
     Decays decay;
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(256) step_kernel(Step d, T* __restrict__ out, 
     for (int r = 0; r < PER; ++r) {
         const float* p = from + (i64)min(row + r * ROWS, d.key - 1) * d.value;
         if constexpr (VEC == 4) {  // value is a multiple of 4
-            const float4_t v = *(const float4_t*)p;
+            const float4_t v = *(const float4_any_t*)p;
 #pragma unroll
             for (int c = 0; c < VEC; ++c) s[r][c] = v[c];
         } else {
@@ -168,7 +171,7 @@ __global__ void __launch_bounds__(256) step_kernel(Step d, T* __restrict__ out, 
             float4_t v;
 #pragma unroll
             for (int c = 0; c < VEC; ++c) v[c] = s[r][c];
-            *(float4_t*)p = v;
+            *(float4_any_t*)p = v;
         } else {
             *p = s[r][0];
         }

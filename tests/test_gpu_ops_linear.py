@@ -342,3 +342,25 @@ def test_a_single_token_of_any_stride(dtype):
     assert all(torch.equal(got[n], grads[n]) for n in grads)
     out, final = ops.linear_attention(**turned)
     assert torch.equal(out, ops.linear_attention(**case)[0])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_states_off_16_bytes(dtype):
+    """A contiguous state that starts anywhere a float may: the same bits as in a state of its own."""
+    print(f"case: linear attention state alignment {dtype}", flush=True)
+    for width in (64, 20):
+        case = make(3, 4, 2, 4, 24, width, dtype)
+        token = {n: t[:, 0].contiguous() if n != "state" else t for n, t in case.items()}
+        own = case["state"].clone()
+        want = ops.linear_attention_step(**dict(token, state=own))
+        for start in (1, 2, 3):
+            memory = torch.full((case["state"].numel() + 8,), 7.0, device="cuda")
+            state = memory[start:start + case["state"].numel()].view(case["state"].shape)
+            state.copy_(case["state"])
+            out = ops.linear_attention_step(**dict(token, state=state))
+            assert torch.equal(out, want) and torch.equal(state, own)
+            assert (memory[:start] == 7.0).all() and (memory[start + state.numel():] == 7.0).all()
+            state.copy_(case["state"])
+            for tape in (False, True):
+                got, expected = (ops.linear_attention(**dict(case, state=s), tape=tape) for s in (state, case["state"]))
+                assert torch.equal(got[0], expected[0]) and torch.equal(got[1], expected[1])
