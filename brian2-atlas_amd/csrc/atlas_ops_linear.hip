@@ -30,7 +30,9 @@ namespace {
 
 constexpr int MAX_WIDTH = 128;
 constexpr i64 MAX_STRIDE = 1 << 24;  // from token to token: a chunk's offsets stay below 2^32 bytes
-constexpr float LOWEST = -120.0f;  // the exponential is zero in float32
+// Log decays are held from below, since differences of infinite sums are none.  No growth that float32 holds (e^88) brings back
+// what this has emptied, and 64 of them still leave a chunk's sums, as a float and its remainder, to 2^-28.
+constexpr float LOWEST = -16384.0f;
 
 // Log decays of (batch, time, value head), of any strides.
 struct Decays {

@@ -364,3 +364,21 @@ def test_states_off_16_bytes(dtype):
             for tape in (False, True):
                 got, expected = (ops.linear_attention(**dict(case, state=s), tape=tape) for s in (state, case["state"]))
                 assert torch.equal(got[0], expected[0]) and torch.equal(got[1], expected[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [5, 100, 700])
+@pytest.mark.parametrize("reset", [-float("inf"), -300.0])
+def test_an_emptied_state_stays_empty_while_it_grows(reset, T, dtype):
+    """Log decays that grow behind one of -inf, or one whose exponential is zero in float32: nothing from before it returns.  No
+    later token writes, so answers and state are zeros (e^-220 of what was, which float32 does not hold)."""
+    print(f"case: linear attention growth behind {reset}, {T} tokens {dtype}", flush=True)
+    case, at = make(2, T, 1, 2, 20, 24, dtype), T // 2
+    case["log_decay"][:, at] = reset
+    case["log_decay"][:, at + 1:at + 3] = 40.0
+    case["k"][:, at:] = 0.0
+    for tape in (False, True):
+        out, final, *_ = ops.linear_attention(**case, tape=tape)
+        assert (out[:, at:] == 0).all() and (final == 0).all()
+        assert (out[:, :at] != 0).any()
+    check(case, train=False)
