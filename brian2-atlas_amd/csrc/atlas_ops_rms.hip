@@ -334,7 +334,7 @@ template <typename W>
 __global__ void __launch_bounds__(1024) rms_reduce(i64 blocks, i64 width, const float* __restrict__ partial, W* __restrict__ dweight) {
     __shared__ float sums[32][33];
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    const i64 col = (i64)blockIdx.x * 32 + lane;
+    const i64 col = first_column() + lane;
     float total = 0.0f;
     if (col < width) {
 #pragma unroll 8
@@ -503,7 +503,7 @@ int atlas_ops_rms_norm_backward(const AtlasRows* grad, const AtlasRows* total, c
                     });
                 });
             if (dweight)
-                rms_reduce<W><<<dim3((unsigned)ceil_div(width, 32)), 1024, 0, st>>>(blocks, width, workspace, (W*)dweight);
+                rms_reduce<W><<<column_grid(ceil_div(width, 32)), 1024, 0, st>>>(blocks, width, workspace, (W*)dweight);
         });
         return launched(err, cap, "rms_norm_backward");
     } catch (...) {

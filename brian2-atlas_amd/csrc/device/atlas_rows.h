@@ -76,6 +76,14 @@ __device__ __forceinline__ void load_columns(const W* p, int col, int width, flo
     for (int i = 0; i < N; ++i) out[i] = units[i / PER][i % PER];
 }
 
+// A grid of `groups` workgroups for 32 columns each, 1024 threads, of which along x no more than a launch may have; the first
+// column of a workgroup of it.
+inline dim3 column_grid(i64 groups) {
+    const i64 across = groups < THREADS / 1024 ? groups : THREADS / 1024 - 1;
+    return dim3((unsigned)across, (unsigned)ceil_div(groups, across));
+}
+__device__ __forceinline__ i64 first_column() { return ((i64)blockIdx.y * gridDim.x + blockIdx.x) * 32; }
+
 struct Rows {
     const void* data;
     i64 inner, outer_stride, inner_stride;

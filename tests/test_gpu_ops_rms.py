@@ -217,3 +217,17 @@ def test_8bit_rows_beyond_float32(width, dtype):
     weight[5] = float("inf")
     values, scale = ops.rms_norm_8bit(x, weight)
     assert torch.isinf(scale).all()
+
+
+@pytest.mark.parametrize("width", [(1 << 27) - 32, (1 << 27) + 40])
+def test_column_sums_of_the_widest_rows(width):
+    """On both sides of 2^27 columns, where a workgroup of 1024 threads for 32 columns would pass 2^32 threads."""
+    print(f"case: rms norm column sums of {width}", flush=True)
+    x = torch.ones(1, width, dtype=BF16, device="cuda")
+    x[0, ::3] = 2.0
+    y, rstd = ops.rms_norm(x, statistics=True)
+    dx, dw = ops.rms_norm_backward(x, x, None, rstd)
+    square = float((x[0, :3].double() ** 2).sum() / 3)
+    assert abs(rstd.item() - square ** -0.5) <= 1e-3 * square ** -0.5
+    want = x[0].float() * (x[0].float() * rstd[0])
+    assert torch.equal(dw, want), "one row: the sum is its product"
