@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(1024) norm_reduce(i64 blocks, i64 width, const
                                                     W* __restrict__ dweight, W* __restrict__ dbias) {
     __shared__ float sums[32][33];
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
-    const i64 col = (i64)blockIdx.x * 32 + lane;
+    const i64 col = first_column() + lane;
     float total = 0.0f;
     if (col < 2 * width) {
 #pragma unroll 8
@@ -478,7 +478,7 @@ int atlas_ops_layer_norm_backward(const AtlasRows* grad, const AtlasRows* x, int
                 }
             }
             if (sums)
-                norm_reduce<W><<<dim3((unsigned)ceil_div(2 * width, 32)), 1024, 0, st>>>(
+                norm_reduce<W><<<column_grid(ceil_div(2 * width, 32)), 1024, 0, st>>>(
                     blocks, width, workspace, (W*)dweight, (W*)dbias);
         });
         return launched(err, cap, "layer_norm_backward");

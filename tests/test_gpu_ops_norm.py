@@ -188,3 +188,16 @@ def test_several_rows_in_each_place(rows, width, dtype):
     print(f"case: layer norm rows {rows} x {width} {dtype}", flush=True)
     x, grad = make((rows, width), dtype, 4), make((rows, width), dtype, 5, 0.1)
     check(x, make(width, F32, 2, 1.0), make(width, F32, 3, 0.0), grad)
+
+
+@pytest.mark.parametrize("width", [(1 << 26) - 16, (1 << 26) + 40])
+def test_column_sums_of_the_widest_rows(width):
+    """On both sides of 2^26 columns, where a workgroup of 1024 threads for 32 of both sums' columns would pass 2^32 threads."""
+    print(f"case: layer norm column sums of {width}", flush=True)
+    # half of the values 2, half 1: a mean of 1.5.  From there six roundings of 2^-24 of at most 2 x 2 x 2.
+    x = torch.ones(1, width, dtype=BF16, device="cuda")
+    x[0, ::2] = 2.0
+    _, mean, rstd = ops.layer_norm(x, statistics=True)
+    dx, dweight, dbias = ops.layer_norm_backward(x, x, None, mean, rstd)
+    want = x[0].float() * ((x[0].float() - 1.5) * rstd[0])
+    assert (dweight - want).abs().max() <= 48 * 2.0 ** -24 and torch.equal(dbias, x[0].float()), "one row: the sum is its product"
