@@ -82,7 +82,7 @@ inline dim3 column_grid(i64 groups) {
     const i64 across = groups < THREADS / 1024 ? groups : THREADS / 1024 - 1;
     return dim3((unsigned)across, (unsigned)ceil_div(groups, across));
 }
-__device__ __forceinline__ i64 first_column() { return ((i64)blockIdx.y * gridDim.x + blockIdx.x) * 32; }
+__device__ __forceinline__ i64 first_column() { return (i64)(blockIdx.y * gridDim.x + blockIdx.x) * 32; }
 
 struct Rows {
     const void* data;
