@@ -26,7 +26,6 @@ struct Tensor {
 // are their columns.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float float8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
@@ -126,19 +125,6 @@ __device__ __forceinline__ void mma_grid(const Pieces<NA> (&a)[R], const Pieces<
                         c[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[n].p[order - i], c[m][n], 0, 0, 0);
 }
 
-// c[m] + A[m] B[m], in the same order.
-template <int NA, int NB, int R>
-__device__ __forceinline__ void mma_each(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[R], float4_t (&c)[R]) {
-    constexpr int ORDERS = NA > NB ? NA : NB;
-#pragma unroll
-    for (int order = ORDERS - 1; order >= 0; --order)
-#pragma unroll
-        for (int i = 0; i <= order; ++i)
-            if (i < NA && order - i < NB)
-#pragma unroll
-                for (int m = 0; m < R; ++m) c[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[m].p[i], b[m].p[order - i], c[m], 0, 0, 0);
-}
-
 // The same with the first pieces' products in `c` alone, the others in `small`: a sum over many operands is then rounded at its
 // full size once for each of them, not once for each product of pieces.
 template <int NA, int NB, int R, int S>
@@ -158,6 +144,7 @@ __device__ __forceinline__ void mma_grid(const Pieces<NA> (&a)[R], const Pieces<
                     }
 }
 
+// c[m] + A[m] B[m], likewise.
 template <int NA, int NB, int R>
 __device__ __forceinline__ void mma_each(const Pieces<NA> (&a)[R], const Pieces<NB> (&b)[R], float4_t (&c)[R], float4_t (&small)[R]) {
     constexpr int ORDERS = NA > NB ? NA : NB;
