@@ -1,9 +1,10 @@
 """Embedding, its gradient and dropout on the GPU against the float64 reference (oracle/ops_oracle.py).
 
 Tolerances.  A looked-up value is one product, rounded once: equal to the same product in float32, rounded to the table's
-type.  A row of the gradient adds up to 32 values one after the other in a tile, then the tiles' sums in up to 64 parts in
-order, and those: with n tokens at most 32 + n / 32 + 64 roundings of 2^-24 of the sum of magnitudes, one for the scale, and one
-to the table's type (bfloat16 2^-8).  Dropout keeps exactly what the reference keeps; a value is one product and, with a residual,
+type.  A row of the gradient adds up to 32 values one after the other in a tile of 8 to 32 places, then the tiles' sums in up to
+64 parts in order, and those: 32 + n / 512 + 64 for its n tokens.  Where one launch takes few symbols, 128 groups add n / 128
+values each, and 3 + 16 sums join them.  Either is below 96 + n / 32 roundings of 2^-24 of the sum of magnitudes; one more for the
+scale, and one to the table's type (bfloat16 2^-8).  Dropout keeps exactly what the reference keeps; a value is one product and, with a residual,
 one sum: 2 roundings.
 """
 import numpy as np
@@ -56,8 +57,8 @@ def drawn(shape, rows, kind, seed=0, dtype=torch.int64):
     return tokens.clamp(max=rows + 1).to(dtype).cuda()
 
 
-# counts around a tile of the sums (32) and of the sort (2048), with scanned counts beyond 32 of them; rows of one,
-# two and three passes; widths of every number of lanes, beyond a slice, odd
+# counts around 32 places and around two tiles of the sort (1024 each), with scanned counts beyond 32 of them; rows of one,
+# two and three passes; widths of every number of lanes, beyond a slice, odd.  Of few rows and tokens one launch takes care
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("count,rows,width,kind", [
     (1, 1, 1, "even"), (1, 5, 7, "one"), (31, 3, 64, "even"), (32, 1, 33, "one"), (33, 2, 128, "even"), (64, 64, 20, "one"),
@@ -260,3 +261,65 @@ def test_dropout_in_place(count, dtype):
             ops._call(0, ops.library().atlas_ops_dropout, given["x"].data_ptr(), None if added is None else given["residual"].data_ptr(), count,
                       ops.TYPES[dtype], 0.3, 5, 2, 9, None, y.data_ptr())
             assert torch.equal(y, want), name
+
+
+# ------------------------------------------------------------- the gradient by sorting, whatever the tokens' number
+# 601 rows are more than one launch takes, so few tokens are sorted too: counts around a tile of the sums (8 places, beyond
+# 32 of them a list of its own) and of the sort (1024)
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("count", [1, 2, 7, 8, 9, 31, 32, 33, 64, 65, 127, 129, 255, 257, 1023, 1024, 1025, 2049, 3000])
+def test_gradient_by_sorting(count, dtype, out):
+    print(f"case: sorted gradient of {count} tokens {dtype} to {out}", flush=True)
+    for kind, width in (("one", 33), ("often", 20), ("even", 130), ("beyond", 7)):
+        check_gradient(make((count, width), dtype, 1), drawn((count,), 601, kind), 601, -1.5, out)
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, BF16), (BF16, F32), (BF16, BF16)])
+def test_gradient_by_sorting_of_strides(dtype, out):
+    print(f"case: sorted gradient strides {dtype} to {out}", flush=True)
+    grad = make((6, 50, 2, 40), dtype, 2)
+    for view, lead in ((lambda t: t[:, :, 0], (6, 50)), (lambda t: t[:, ::2, 1].transpose(0, 1), (25, 6)), (lambda t: t[0, 0, 0].expand(7, 40), (7,)),
+                       (lambda t: t[1:2, 3:4, 0], (1, 1)), (lambda t: t[:, 0, 0, :].t(), (40,))):
+        check_gradient(view(grad), drawn(lead, 700, "often", 3, torch.int32), 700, -1.5, out)
+    flat = make(300 * 40 + 1, dtype, 3)
+    check_gradient(flat[1:].view(300, 40), drawn((600,), 700, "beyond", 4)[::2], 700, 1.0, out)
+
+
+@pytest.mark.parametrize("dtype,count,rows,width", [(BF16, 32752, 50000, 1024), (F32, 9001, 50000, 512), (F32, 270001, 900, 8), (BF16, 520001, 900, 8)])
+def test_gradient_by_sorting_in_each_length_of_tile(dtype, count, rows, width):
+    """Tiles of 16 places with 128 lanes and with 16, of 8 with 128, of 32 with 16."""
+    print(f"case: sorted gradient {count} tokens of {rows} x {width} {dtype}", flush=True)
+    check_gradient(make((count, width), dtype, 1), drawn((count,), rows, "often"), rows, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_special_values_in_sorted_rows(dtype):
+    """Non-finite values of rows within a tile, of rows that cross a few tiles and of one that crosses many."""
+    print(f"case: sorted gradient special values {dtype}", flush=True)
+    tokens = torch.cat([torch.full((n,), r) for r, n in ((2, 3), (5, 50), (9, 600), (300, 1), (600, 13))])
+    tokens = tokens[torch.randperm(len(tokens), generator=torch.Generator().manual_seed(1))].cuda()
+    grad = make((len(tokens), 24), dtype)
+    clean = ops.embedding_backward(grad, tokens, 601)
+    for row in (2, 5, 9, 300, 600):
+        places = (tokens == row).nonzero().flatten().tolist()
+        for at in (places[0], places[len(places) // 2], places[-1]):
+            dirty = grad.clone()
+            dirty[at, 3], dirty[at, 4] = float("nan"), -float("inf")
+            got = ops.embedding_backward(dirty, tokens, 601)
+            bad = ~torch.isfinite(got)
+            assert torch.isnan(got[row, 3]) and got[row, 4] == -float("inf") and bad.sum() == 2 and torch.equal(got[~bad], clean[~bad])
+    dirty = grad.clone()
+    dirty[tokens == 9] = float("nan")
+    gone = torch.where(tokens == 9, 601, tokens)   # no row any more: its gradients are not looked at
+    got = ops.embedding_backward(dirty, gone, 601)
+    assert (got[9] == 0).all() and torch.isfinite(got).all()
+
+
+def test_sorted_tokens_of_64_bits():
+    """Tokens whose lower 32 bits would be a row."""
+    print("case: sorted wide tokens", flush=True)
+    tokens = torch.tensor([1, (1 << 32) + 1, -(1 << 32) + 1, -(1 << 63), 2, 600, (1 << 33) + 600, 601, -1] * 40, device="cuda")
+    got = ops.embedding_backward(torch.ones(len(tokens), 8, device="cuda"), tokens, 601)
+    want = torch.zeros(601, device="cuda")
+    want[[1, 2, 600]] = 40.0
+    assert torch.equal(got, want[:, None].expand(601, 8))

@@ -4,7 +4,7 @@ which the kernels sum anew from the states every eight chunks (256 tokens of flo
 Tolerances, relative to the norm of what is expected.  A state passes T / C chunks (C = 32 in float32, 64 in bfloat16) and is
 rounded at most 14 times in each, relative to its own norm; what else a result passes (pieces, decays, a chunk's own products)
 is within 20 more.  Independent roundings add as the root of the sum of their squares, and four standard deviations are allowed:
-TOL = 4 sqrt(14 T / C + 20) 2^-24, 3 to 6 e-6.  A gradient takes two such states: twice that.  The sum of n tokens' gradients errs by
+TOL = 4 sqrt(14 T / C + 20) 2^-24, 2e-6 to 6e-6.  A gradient takes two such states: twice that.  The sum of n tokens' gradients errs by
 no more than sqrt(n) times the norm of their errors (Cauchy-Schwarz), whether they cancel or not.  Results of bfloat16 add
 half a step of each value, 2^-8 of the norm.
 """
