@@ -321,10 +321,11 @@ __device__ __forceinline__ uint32_t thread_here() {
 // bytes.
 //
 // Products are to 24 bits: a float32 operand is the sum of three bfloat16 pieces (six matrix instructions for a product), the
-// state and the decayed scores are so in either type.  16384 tokens of 16 heads of 128 bfloat16 in 32 segments: 106 us, 512
-// workgroups at two to a CU (their registers); 256 x 100 tokens of 4 heads of 64 float32: 54 us, their three gradients 140.
-// Vector instructions take half of the time, LDS 45 %, matrix instructions 29 %: what bounds it is the chain of a chunk's
-// stages with 8 to 12 waves on a CU.
+// state and the decayed scores are so in either type.  16384 tokens of 16 heads of 128 bfloat16 in 32 segments: 105 us, 512
+// workgroups at two to a CU, which 253 registers and 75 KB of LDS allow alike; 256 x 100 tokens of 4 heads of 64 float32: 49 us,
+// their three gradients 145, three to a CU by 135 registers and 44 KB.  Vector instructions take 48 % of the first's time, LDS 37 %,
+// matrix instructions 29 %, of the others 45 to 57 %, 41 to 47 % and 18 to 21 %: what bounds it is the chain of a chunk's stages with 8
+// to 12 waves on a CU.
 template <typename T, int DK, int NB, bool OUT, bool WHOLE>
 __global__ void __launch_bounds__(256, 2) scan(Runs) {
     // the launch's argument, where it lies: an index into a copy would need memory
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(256) join_states(float* sums, const float* dec
 
 // ------------------------------------------------------------------ gradients of the decays
 // A workgroup takes the tokens between two anchors: L behind its last token, then back through its tokens.  A launch's chain of
-// loads and barriers, 9 to 10 us for 1024 sequences of 100 tokens or 32 of 4099.
+// loads and barriers, 9 us for 1024 sequences of 100 tokens, 12 for 32 of 4099.
 struct DecayGradients {
     Decays decay;
     const void* other;                      // memory that may be read where there are no decays

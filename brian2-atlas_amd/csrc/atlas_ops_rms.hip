@@ -7,10 +7,10 @@
 //   8 bits: scale = max(max |y| / 448, 2^-126),  value = y / scale as e4m3; infinite where the sum of squares is
 //
 // Memory bounds all of it.  A row is read once into registers, summed, written; the next row's loads are in
-// flight meanwhile.  16384 x 4096 bfloat16 with a residual: forward 94 us (5.7 TB/s over four passes), backward 135 us (4.0: its
-// registers leave 12 waves to a CU); 2048 x 4096 to 8 bits 16.5 us.  The backward pass keeps the column sums of dw in registers over the rows that a group
-// visits, adds the groups of a workgroup in LDS and writes one row of partial sums per workgroup, which a
-// second kernel adds in a fixed order.
+// flight meanwhile.  16384 x 4096 bfloat16 with a residual: forward 94 us (5.7 TB/s over four passes), backward 137 us (3.9: its
+// registers leave 12 waves to a CU); 2048 x 4096 to 8 bits 16.7 us.  The backward pass keeps the column sums of dw in registers
+// over the rows that a group visits, adds the groups of a workgroup in LDS and writes one row of partial sums per workgroup,
+// which a second kernel adds in a fixed order.
 #include <algorithm>
 
 #include "device/atlas_rows.h"
