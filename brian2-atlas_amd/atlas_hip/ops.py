@@ -154,12 +154,6 @@ def _near(t):
     return t if t.stride(1) <= 1 << 24 or t.shape[1] == 1 else t.contiguous()
 
 
-def _token_strides(t):
-    """Of the first three axes of (batch, time, ...); a single token, whose stride may be anything, is nowhere near another."""
-    s = t.stride()
-    return s[:3] if t.shape[1] > 1 else (s[0], 0, s[2])
-
-
 def _workspace(size: int, like):
     return torch.empty(size, dtype=torch.uint8, device=like.device)
 
@@ -558,11 +552,9 @@ class _Problem:
         if linear and time_axis:
             q, k, v = _near(q), _near(k), _near(v)
 
-        def strides(t):
-            if time_axis:
-                return _token_strides(t)
+        def strides(t):  # a single token, whose stride may be anything, is nowhere near another
             s = t.stride()
-            return s[0], 0, s[1]
+            return s[:3] if time > 1 else (s[0], 0, s[2]) if time_axis else (s[0], 0, s[1])
 
         self.device, self.batch, self.time, self.heads, self.value_heads = device, batch, time, heads, value_heads
         self.key, self.value, self.type, self.scale = key, value, q.dtype, scale
@@ -795,6 +787,7 @@ def linear_attention_backward(grad_out, grad_state, tape: LinearTape) -> dict:
         _tensor(grad_state, "grad_state", p.device, _F32, (p.batch, p.value_heads, p.key, p.value))
         grad_state = grad_state.contiguous()
     grad_out = _near(_last(grad_out))
+    go = grad_out.stride()
     grads = {name: None if t is None else _empty(t)
              for name, t in (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("state", state))}
     if not p.batch or not p.time:
@@ -813,6 +806,6 @@ def linear_attention_backward(grad_out, grad_state, tape: LinearTape) -> dict:
     workspace = _workspace(lib.atlas_ops_linear_backward_workspace(p.packed), v)
     dq, dk, dv, decay, dstate = (None if g is None else g.data_ptr() for g in grads.values())
     _call(p.device, lib.atlas_ops_linear_backward, p.packed, tape.memory.data_ptr(), grad_out.data_ptr(),
-          struct.pack("@3q", *_token_strides(grad_out)), None if grad_state is None else grad_state.data_ptr(), dq, dk, dv, decay,
+          struct.pack("@3q", go[0], go[1] if p.time > 1 else 0, go[2]), None if grad_state is None else grad_state.data_ptr(), dq, dk, dv, decay,
           int(log_decay is not None and log_decay.dim() == 1), dstate, workspace.data_ptr())
     return grads
